@@ -19,7 +19,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.environ.get("FALKON_B200_LIB") or os.path.join(_HERE, "libfalkon_b200.so")
 
-FLK_F32, FLK_F64 = 0, 1
+FLK_F32, FLK_F64, FLK_BF16, FLK_F16 = 0, 1, 2, 3
 FLK_GAUSSIAN, FLK_LAPLACIAN, FLK_MATERN15, FLK_MATERN25 = 0, 1, 2, 3
 FLAG_FORCE_SIMT, FLAG_FORCE_TC, FLAG_FP64_MATH, FLAG_NO_FOLD, FLAG_ACCUMULATE = 1, 2, 4, 8, 16
 FLAG_KEEP_X1, FLAG_KEEP_X2 = 32, 64
@@ -30,8 +30,9 @@ FLK_ERR_CUDA, FLK_ERR_UNSUPPORTED, FLK_ERR_DEVICE, FLK_ERR_TIMEOUT = -4, -5, -6,
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v",
+    "-Xcompiler", "-fPIC", "-Xptxas", "-v",
 ]
+LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared"]
 PTXAS_REPORT = LIB_PATH + ".ptxas.txt"
 # The tensor-core sweeps read their accumulators with asynchronous tcgen05.ld: a register that such a load is still
 # to fill must never be spilled, so the resident kernel has to compile without any spill.  It re-partitions
@@ -58,14 +59,53 @@ def _up_to_date() -> bool:
     return os.path.getmtime(LIB_PATH) >= max(os.path.getmtime(s) for s in sources())
 
 
+def _includes(path: str, seen=None):
+    """The file and every header of this repository that it includes, directly or not."""
+    seen = set() if seen is None else seen
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#include\s+"([^"]+)"', f.read(), flags=re.M):
+                _includes(os.path.normpath(os.path.join(os.path.dirname(path), name)), seen)
+    return seen
+
+
+def _compile(unit: str, flags, force: bool, verbose: bool):
+    """(object file, ptxas report) of one translation unit; both are kept in csrc/ and made again when a source that
+    the unit includes, or the command, has changed."""
+    obj = unit[:-3] + ".o"
+    report = obj + ".ptxas.txt"
+    cmd = [os.environ.get("NVCC", "nvcc")] + flags + ["-c", unit]
+    head = "# " + " ".join(cmd) + "\n"
+    if not force and os.path.exists(obj) and os.path.exists(report):
+        with open(report) as f:
+            text = f.read()
+        if text.startswith(head) and os.path.getmtime(obj) >= max(os.path.getmtime(s) for s in _includes(unit)):
+            return obj, text[len(head):]
+    tmp = f"{obj}.{os.getpid()}.tmp.o"
+    if verbose:
+        print(" ".join(cmd + ["-o", obj]))
+    res = subprocess.run(cmd + ["-o", tmp], capture_output=True, text=True)
+    if res.returncode != 0:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+        raise RuntimeError(f"nvcc failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, obj)
+    with open(report, "w") as f:
+        f.write(head + res.stderr)
+    return obj, res.stderr
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles csrc/flk_api.cu into libfalkon_b200.so (nvcc cross-compiles without a GPU).
+    """Compiles the translation units in csrc/ (one nvcc each, side by side) and links them into libfalkon_b200.so
+    (nvcc cross-compiles without a GPU).
 
     Safe when several processes (one per GPU) start at once: the build runs under an exclusive file lock,
     writes to a temporary name and is moved into place atomically, and a process that waited for the lock
     finds the library up to date and does not build again."""
     if not force and _up_to_date():
         return LIB_PATH
+    import concurrent.futures
     import fcntl
 
     with open(LIB_PATH + ".lock", "w") as lock:
@@ -74,23 +114,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if not force and _up_to_date():
                 return LIB_PATH
             tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
-            nvcc = os.environ.get("NVCC", "nvcc")
             extra = os.environ.get("FALKON_B200_NVCC_EXTRA", "").split()  # e.g. -D tuning macros of the kernels
-            cmd = [nvcc] + NVCC_FLAGS + extra + ["-o", tmp, os.path.join(_CSRC, "flk_api.cu")]
-            if verbose:
-                print(" ".join(cmd))
-            res = subprocess.run(cmd, capture_output=True, text=True)
-            if res.returncode != 0:
-                if os.path.exists(tmp):
-                    os.remove(tmp)
-                raise RuntimeError(f"nvcc failed:\n{res.stdout}\n{res.stderr}")
-            table = parse_ptxas(res.stderr)
+            units = [s for s in sources() if s.endswith(".cu")]
+            with concurrent.futures.ThreadPoolExecutor(len(units)) as pool:
+                done = list(pool.map(lambda u: _compile(u, NVCC_FLAGS + extra, force, verbose), units))
+            table = sorted(row for _, text in done for row in parse_ptxas(text))
             problems = check_ptxas(table)
             with open(PTXAS_REPORT, "w") as f:
                 f.write(format_ptxas(table))
             if problems:
-                os.remove(tmp)
                 raise RuntimeError("register check of the tensor-core kernels failed:\n" + "\n".join(problems))
+            cmd = [os.environ.get("NVCC", "nvcc")] + LINK_FLAGS + ["-o", tmp] + [obj for obj, _ in done]
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            if res.returncode != 0:
+                if os.path.exists(tmp):
+                    os.remove(tmp)
+                raise RuntimeError(f"linking failed:\n{res.stdout}\n{res.stderr}")
             os.replace(tmp, LIB_PATH)
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
@@ -150,6 +189,33 @@ _dp = ctypes.POINTER(ctypes.c_double)
 
 _MAT = [_vp, _i64, _i64, _i64]  # pointer, rows, row stride, col stride
 
+
+
+class Tensor4(ctypes.Structure):
+    """flk_tensor4: data pointer and the strides of batch, rows and heads, in elements."""
+    _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_n", _i64), ("stride_h", _i64)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """flk_attention_args."""
+    _fields_ = [(n, _i64) for n in ("dtype", "batch", "nq", "nk", "hq", "hk", "d", "causal", "flags")]
+    _fields_ += [("scale", ctypes.c_double), ("softcap", ctypes.c_double)]
+    _fields_ += [(n, Tensor4) for n in ("q", "k", "v", "out")]
+    _fields_ += [(n, _vp) for n in ("lse", "slopes", "prefix_lens", "kv_lens", "q_starts")]
+    _fields_ += [("q_documents", _vp), ("q_documents_stride", _i64), ("k_documents", _vp), ("k_documents_stride", _i64)]
+    _fields_ += [(n, Tensor4) for n in ("dout", "dq", "dk", "dv")]
+    _fields_ += [("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+class LayerNormArgs(ctypes.Structure):
+    """flk_layer_norm_args."""
+    _fields_ = [(n, _i64) for n in ("dtype", "wdtype", "n", "d")] + [("eps", ctypes.c_double), ("x", _vp)]
+    _fields_ += [(n, _i64) for n in ("x_inner", "x_outer_stride", "x_inner_stride")]
+    _fields_ += [(n, _vp) for n in ("weight", "bias", "y", "mean", "rstd", "dy")]
+    _fields_ += [(n, _i64) for n in ("dy_inner", "dy_outer_stride", "dy_inner_stride")]
+    _fields_ += [(n, _vp) for n in ("dx", "dweight", "dbias", "workspace")] + [("workspace_bytes", _i64)]
+
+
 _SIGNATURES = {
     "flk_version": (_int, []),
     "flk_last_error": (ctypes.c_char_p, []),
@@ -174,6 +240,13 @@ _SIGNATURES = {
     # dtype, kernel, X1(4), X2(4), d, out ptr + strides(3), sigma, len, ws, bytes, flags, stream
     "flk_kgrad": (_int, [_int, _int] + _MAT + _MAT + [_i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _dp, _i64, _vp, _i64, _int, _vp]),
     "flk_fmm": (_int, [_int, _int] + _MAT + _MAT + [_i64, _vp, _i64, _i64, _dp, _i64, _vp, _i64, _int, _vp]),
+    # struct, backward / stream
+    "flk_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionArgs), _int]),
+    "flk_attention_forward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
+    "flk_attention_backward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
+    "flk_layer_norm_workspace_bytes": (_i64, [ctypes.POINTER(LayerNormArgs)]),
+    "flk_layer_norm_forward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
+    "flk_layer_norm_backward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
     "flk_tc_status": (_int, [_vp, _vp, ctypes.POINTER(_int)]),
     "flk_range_flag": (_int, [_vp, _vp, ctypes.POINTER(_int)]),
     "flk_probe_mufu": (_int, [_int, _vp, ctypes.POINTER(_i64), _vp]),
@@ -613,6 +686,40 @@ def call_square_norm(X, sigma=None, out=None):
     del keep
     raise_for_status(status)
     return out
+
+
+_ROW_TYPES = {torch.float32: FLK_F32, torch.bfloat16: FLK_BF16, torch.float16: FLK_F16}
+
+
+def row_dtype_code(dtype: torch.dtype) -> int:
+    """Data types of attention and layer norm."""
+    code = _ROW_TYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"attention and layer_norm take float32, bfloat16 and float16 data, not {dtype}")
+    return code
+
+
+def call_struct(name: str, args: ctypes.Structure, device: torch.device, *query):
+    """Calls the entry point ``flk_<name>`` on ``args`` with the device's current stream.  Its workspace comes from torch's
+    caching allocator and belongs to this call alone, so that calls on several streams, and captured graphs, share none
+    (``query``: name of the workspace query, and its further arguments)."""
+    lib = load()
+    ref = ctypes.byref(args)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call_struct(name, args, device, *query)
+    ws = None
+    if query:
+        need = getattr(lib, query[0])(ref, *query[1:])
+        if need < 0:
+            raise_for_status(int(need))
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            args.workspace = ws.data_ptr()
+            args.workspace_bytes = need
+    status = getattr(lib, "flk_" + name)(ref, torch.cuda.current_stream(device).cuda_stream)
+    if status != 0:
+        raise_for_status(status)
 
 
 def tc_status(device: torch.device) -> int:

@@ -1,6 +1,5 @@
 // extern "C" entry points of libfalkon_b200: argument checks, workspace planning, dispatch.
 #include <algorithm>
-#include <atomic>
 #include <vector>
 
 #include "flk_common.cuh"
@@ -15,11 +14,6 @@
 #include "flk_wide.cuh"
 
 namespace flk {
-
-static std::atomic<int64_t> g_launches{0};
-static inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
-
-constexpr int kNumSMs = 148;  // B200
 
 // Optional per-sweep timing (CUDA events recorded on the caller's stream around the dominant
 // kernel of each sweep).  Off by default; bench.py turns it on to measure the kernel live.

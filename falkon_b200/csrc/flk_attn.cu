@@ -1,0 +1,176 @@
+// extern "C" entry points of attention: argument checks, workspace, choice of kernel.
+#include "flk_attn.cuh"
+#include "flk_attn_simt.cuh"
+
+namespace flk {
+namespace attn {
+
+static int esize_of(int64_t dtype) { return dtype == FLK_F32 ? 4 : 2; }
+
+static int check_sizes(const flk_attention_args* p) {
+  if (p == nullptr) return fail(FLK_ERR_BAD_ARG, "args: null pointer");
+  if (p->dtype != FLK_F32 && p->dtype != FLK_BF16 && p->dtype != FLK_F16)
+    return fail(FLK_ERR_BAD_ARG, "attention takes fp32, bf16 or fp16 data, not dtype %lld", (long long)p->dtype);
+  if (p->batch < 0 || p->nq < 0 || p->nk < 0 || p->hq < 1 || p->hk < 1 || p->d < 1)
+    return fail(FLK_ERR_BAD_ARG, "negative or empty sizes");
+  if (p->batch > 65535 || p->hq > 65535 || p->nq > (1 << 29) || p->nk > (1 << 29))
+    return fail(FLK_ERR_UNSUPPORTED, "at most 65535 sequences and heads, and 2^29 rows");
+  if (p->hq % p->hk != 0)
+    return fail(FLK_ERR_BAD_ARG, "%lld query heads cannot share %lld key heads", (long long)p->hq, (long long)p->hk);
+  const int unit = p->dtype == FLK_F32 ? 4 : 8;
+  if (p->d > kMaxHeadDim || p->d % unit != 0)
+    return fail(FLK_ERR_UNSUPPORTED, "head dimension %lld: a multiple of %d up to %d", (long long)p->d, unit, kMaxHeadDim);
+  if (!(p->softcap >= 0) || p->softcap > 1e30 || !(p->scale > -1e30 && p->scale < 1e30))
+    return fail(FLK_ERR_BAD_ARG, "scale must be finite, softcap finite and not negative");
+  if ((p->q_documents == nullptr) != (p->k_documents == nullptr))
+    return fail(FLK_ERR_BAD_ARG, "q_documents and k_documents are given together");
+  if (p->prefix_lens != nullptr && p->causal == 0) return fail(FLK_ERR_BAD_ARG, "prefix_lens needs causal");
+  return FLK_OK;
+}
+
+static int check_tensor(const char* name, const flk_tensor4& t, int64_t b, int64_t n, int64_t h, int es) {
+  if (b == 0 || n == 0) return FLK_OK;
+  if (t.data == nullptr) return fail(FLK_ERR_BAD_ARG, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(t.data) % 16 != 0 || (b > 1 && t.stride_b * es % 16 != 0) || (n > 1 && t.stride_n * es % 16 != 0) ||
+      (h > 1 && t.stride_h * es % 16 != 0))
+    return fail(FLK_ERR_LAYOUT, "%s: address and strides must be multiples of 16 bytes", name);
+  return FLK_OK;
+}
+
+struct Workspace {
+  int64_t qdocs, kdocs, qtab, ktab, delta, total;
+};
+static int64_t pad_rows(int64_t n) { return round_up(n, kTile); }
+static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
+  Workspace w{};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  if (p->q_documents != nullptr) {
+    w.qdocs = take(p->batch * pad_rows(p->nq) * 4);
+    w.kdocs = take(p->batch * pad_rows(p->nk) * 4);
+    w.qtab = take(p->batch * pad_rows(p->nq) / kTile * 8);
+    w.ktab = take(p->batch * pad_rows(p->nk) / kTile * 8);
+  }
+  if (backward) w.delta = take(p->batch * p->hq * p->nq * 4);
+  w.total = at;
+  return w;
+}
+
+static Tensor4 tensor_of(const flk_tensor4& t) { return Tensor4{t.data, t.stride_b, t.stride_n, t.stride_h}; }
+
+// Device arguments, and the tables of documents in the workspace.
+static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaStream_t st) {
+  const Workspace w = plan_workspace(p, backward);
+  if (w.total > 0 && (p->workspace == nullptr || p->workspace_bytes < w.total || reinterpret_cast<uintptr_t>(p->workspace) % 256 != 0))
+    return fail(FLK_ERR_WORKSPACE, "attention needs %lld bytes of 256-byte aligned workspace", (long long)w.total);
+  char* ws = reinterpret_cast<char*>(p->workspace);
+  a = Args{};
+  a.b = (int)p->batch, a.nq = (int)p->nq, a.nk = (int)p->nk, a.hq = (int)p->hq, a.hk = (int)p->hk;
+  a.grp = (int)(p->hq / p->hk), a.d = (int)p->d, a.causal = p->causal != 0;
+  a.scale_raw = (float)p->scale;
+  a.scale = (float)(p->softcap > 0 ? p->scale / p->softcap : p->scale * 1.4426950408889634);
+  a.cap2 = (float)(p->softcap * 1.4426950408889634);
+  a.slopes = p->slopes, a.prefix = p->prefix_lens, a.kv_lens = p->kv_lens, a.q_starts = p->q_starts;
+  a.nq_pad = (int)pad_rows(p->nq), a.nk_pad = (int)pad_rows(p->nk);
+  a.q = tensor_of(p->q), a.k = tensor_of(p->k), a.v = tensor_of(p->v), a.o = tensor_of(p->out);
+  a.lse = p->lse;
+  if (backward) {
+    a.dout = tensor_of(p->dout), a.dq = tensor_of(p->dq), a.dk = tensor_of(p->dk), a.dv = tensor_of(p->dv);
+    a.delta = reinterpret_cast<float*>(ws + w.delta);
+  }
+  if (p->q_documents != nullptr) {
+    int *qd = reinterpret_cast<int*>(ws + w.qdocs), *kd = reinterpret_cast<int*>(ws + w.kdocs);
+    int2 *qt = reinterpret_cast<int2*>(ws + w.qtab), *kt = reinterpret_cast<int2*>(ws + w.ktab);
+    a.qdocs = qd, a.kdocs = kd, a.qtab = qt, a.ktab = kt;
+    if (p->nq > 0) {
+      documents_kernel<<<dim3((unsigned)ceil_div(a.nq_pad / kTile, 4), a.b), 128, 0, st>>>(
+          p->q_documents, p->q_documents_stride, a.nq, nullptr, -2, a.nq_pad, qd, qt);
+      count_launch();
+    }
+    if (p->nk > 0) {
+      documents_kernel<<<dim3((unsigned)ceil_div(a.nk_pad / kTile, 4), a.b), 128, 0, st>>>(
+          p->k_documents, p->k_documents_stride, a.nk, p->kv_lens, -1, a.nk_pad, kd, kt);
+      count_launch();
+    }
+  }
+  return FLK_OK;
+}
+
+template <typename T>
+static int simt_forward(const Args& a, cudaStream_t st) {
+  return a.d <= 64 ? simt::launch_forward<T, 64>(a, st) : simt::launch_forward<T, 128>(a, st);
+}
+template <typename T>
+static int simt_backward(const Args& a, cudaStream_t st) {
+  if (a.nq > 0) {
+    simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a);
+    count_launch();
+  }
+  return a.d <= 64 ? simt::launch_backward<T, 64>(a, st) : simt::launch_backward<T, 128>(a, st);
+}
+
+}  // namespace attn
+}  // namespace flk
+
+using namespace flk;
+
+extern "C" {
+
+int64_t flk_attention_workspace_bytes(const flk_attention_args* p, int backward) {
+  const int s = attn::check_sizes(p);
+  if (s != FLK_OK) return s;
+  return attn::plan_workspace(p, backward != 0).total;
+}
+
+int flk_attention_forward(const flk_attention_args* p, void* stream) {
+  FLK_TRY(attn::check_sizes(p));
+  const int es = attn::esize_of(p->dtype);
+  FLK_TRY(attn::check_tensor("q", p->q, p->batch, p->nq, p->hq, es));
+  FLK_TRY(attn::check_tensor("k", p->k, p->batch, p->nk, p->hk, es));
+  FLK_TRY(attn::check_tensor("v", p->v, p->batch, p->nk, p->hk, es));
+  FLK_TRY(attn::check_tensor("out", p->out, p->batch, p->nq, p->hq, es));
+  if (p->batch == 0 || p->nq == 0) return FLK_OK;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  attn::Args a;
+  FLK_TRY(attn::make_args(p, false, a, st));
+  if (p->dtype == FLK_F32) FLK_TRY(attn::simt_forward<float>(a, st));
+  else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_forward<__nv_bfloat16>(a, st));
+  else FLK_TRY(attn::simt_forward<__half>(a, st));
+  FLK_CUDA_TRY(cudaGetLastError());
+  return FLK_OK;
+}
+
+int flk_attention_backward(const flk_attention_args* p, void* stream) {
+  FLK_TRY(attn::check_sizes(p));
+  const int es = attn::esize_of(p->dtype);
+  FLK_TRY(attn::check_tensor("q", p->q, p->batch, p->nq, p->hq, es));
+  FLK_TRY(attn::check_tensor("k", p->k, p->batch, p->nk, p->hk, es));
+  FLK_TRY(attn::check_tensor("v", p->v, p->batch, p->nk, p->hk, es));
+  FLK_TRY(attn::check_tensor("out", p->out, p->batch, p->nq, p->hq, es));
+  FLK_TRY(attn::check_tensor("dout", p->dout, p->batch, p->nq, p->hq, es));
+  if ((p->dk.data == nullptr) != (p->dv.data == nullptr) && p->nk > 0)
+    return fail(FLK_ERR_BAD_ARG, "dk and dv are given together");
+  if (p->dq.data != nullptr) FLK_TRY(attn::check_tensor("dq", p->dq, p->batch, p->nq, p->hq, es));
+  if (p->dk.data != nullptr) {
+    FLK_TRY(attn::check_tensor("dk", p->dk, p->batch, p->nk, p->hk, es));
+    FLK_TRY(attn::check_tensor("dv", p->dv, p->batch, p->nk, p->hk, es));
+  }
+  if (p->batch == 0) return FLK_OK;
+  if (p->nq > 0 && p->lse == nullptr) return fail(FLK_ERR_BAD_ARG, "lse: null pointer");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  attn::Args a;
+  FLK_TRY(attn::make_args(p, true, a, st));
+  if (a.nq == 0) a.dq.p = nullptr;
+  if (a.nk == 0) a.dk.p = a.dv.p = nullptr;
+  if (p->dtype == FLK_F32) FLK_TRY(attn::simt_backward<float>(a, st));
+  else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_backward<__nv_bfloat16>(a, st));
+  else FLK_TRY(attn::simt_backward<__half>(a, st));
+  FLK_CUDA_TRY(cudaGetLastError());
+  return FLK_OK;
+}
+
+}  // extern "C"

@@ -6,6 +6,8 @@
 #include <stdio.h>
 #include <stdarg.h>
 
+#include <atomic>
+
 #include "../../include/falkon_b200.h"
 
 namespace flk {
@@ -40,6 +42,12 @@ inline int fail(int code, const char* fmt, ...) {
     int _s = (expr);             \
     if (_s != FLK_OK) return _s; \
   } while (0)
+
+// Kernels launched by this process (all translation units).
+inline std::atomic<int64_t> g_launches{0};
+inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
+constexpr int kNumSMs = 148;  // B200
 
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t ceil_div(int64_t x, int64_t m) { return (x + m - 1) / m; }

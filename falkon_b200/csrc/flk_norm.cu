@@ -1,0 +1,533 @@
+// Layer norm of the rows of a matrix, forward and backward, and its C entry points.
+//
+//   mu = mean(x), var = mean((x - mu)^2), r = 1 / sqrt(var + eps), xh = (x - mu) r
+//   forward    y = xh * w + b                        (mu and r are kept for the backward pass, in fp32)
+//   backward   g = dy * w,   dx = r (g - mean(g) - xh mean(g xh)),   dw = sum_rows dy xh,   db = sum_rows dy
+//
+// Both passes are bound by HBM: forward moves 2 row lengths per row, backward 3.  A row is therefore read once, kept in
+// registers by the group of threads that owns it, and every statistic is taken from those registers (the variance from
+// the centred values, so a large mean costs no digits).  The grid is persistent: a group walks over rows, holds its
+// slice of w (and, backward, its partial sums of dw and db) in registers all along, and issues the loads of its next row
+// before it reduces the present one.  dw and db: every block adds up its groups in a fixed order and writes one partial
+// row; a second kernel adds the partial rows, also in a fixed order, so results do not depend on timing.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "flk_common.cuh"
+
+namespace flk {
+namespace norm {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// VEC values that are loaded and stored at once (16 bytes, or a single value where rows are not 16-byte aligned)
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+// Rows of a matrix whose row index has two levels (the heads of a packed projection): offset of row r
+struct Rows {
+  int64_t inner, s_outer, s_inner;
+  __device__ __forceinline__ int64_t at(int64_t r) const {
+    if (inner == 1) return r * s_outer;
+    if (r < (1ll << 31) && inner < (1ll << 31)) {
+      const uint32_t o = (uint32_t)r / (uint32_t)inner;
+      return (int64_t)o * s_outer + (int64_t)((uint32_t)r - o * (uint32_t)inner) * s_inner;
+    }
+    const int64_t o = r / inner;
+    return o * s_outer + (r - o * inner) * s_inner;
+  }
+};
+
+struct Args {
+  int64_t n;   // rows
+  int d;       // row length
+  int tpr;     // threads per row (a power of two)
+  int wdtype;  // data type of w and b
+  float eps, inv_d;
+  const void *x, *dy, *w, *b;
+  void *y, *dx;
+  Rows xr, dyr;  // y and dx are dense
+  float *mean, *rstd;
+  float* part;  // [blocks][2][d] partial sums of dw, db
+};
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == FLK_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == FLK_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
+  if (dtype == FLK_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == FLK_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// Sum of one or two values over the tpr threads of a row group; every thread of the group gets the result.  `red`
+// is a 2 x 32 x K shared array: calls alternate between its halves (`flip`), so one barrier per call is enough.
+template <int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float* red, int& flip) {
+  const int lanes = tpr < 32 ? tpr : 32;
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
+  if (tpr <= 32) return;
+  float* buf = red + flip * (32 * K);
+  flip ^= 1;
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) buf[warp * K + k] = v[k];
+  }
+  __syncthreads();
+  const int warps = tpr >> 5, first = warp / warps * warps;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float s = 0.f;
+    for (int i = 0; i < warps; ++i) s += buf[(first + i) * K + k];
+    v[k] = s;
+  }
+}
+
+template <typename T, int VEC, int V>
+__device__ __forceinline__ void load_row(Pack<T, VEC> (&raw)[V], const T* row, int lane, int tpr, int packs) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int p = lane + i * tpr;
+    if (p < packs) raw[i] = *reinterpret_cast<const Pack<T, VEC>*>(row + (int64_t)p * VEC);
+  }
+}
+
+// Rows of up to tpr * V * VEC values.
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(1024 / (V * VEC > 16 ? 2 : 1)) forward_kernel(const Args a) {
+  __shared__ float red[2 * 32];
+  const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr;
+  const int packs = a.d / VEC;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  T* y = reinterpret_cast<T*>(a.y);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int flip = 0;
+  float w[V][VEC], b[V][VEC];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (lane + i * a.tpr) * VEC + j;
+      w[i][j] = a.w != nullptr && c < a.d ? load_any(a.w, a.wdtype, c) : 1.f;
+      b[i][j] = a.b != nullptr && c < a.d ? load_any(a.b, a.wdtype, c) : 0.f;
+    }
+  Pack<T, VEC> next[V];
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+  if (row < a.n) load_row<T, VEC, V>(next, x + a.xr.at(row), lane, a.tpr, packs);
+  // every group makes the same number of turns, so that the barriers inside the sums match
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.n; r0 += step, row += step) {
+    const bool on = row < a.n;
+    float v[V][VEC];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = lane + i * a.tpr < packs && on ? to_f<T>(next[i].v[j]) : 0.f;
+        s[0] += v[i][j];
+      }
+    if (row + step < a.n) load_row<T, VEC, V>(next, x + a.xr.at(row + step), lane, a.tpr, packs);
+    group_sum<1>(s, a.tpr, red, flip);
+    const float mu = s[0] * a.inv_d;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = lane + i * a.tpr < packs ? v[i][j] - mu : 0.f;
+        s[0] = fmaf(v[i][j], v[i][j], s[0]);
+      }
+    group_sum<1>(s, a.tpr, red, flip);
+    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    if (on) {
+      if (lane == 0 && a.mean != nullptr) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int p = lane + i * a.tpr;
+        if (p >= packs) continue;
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out.v[j] = from_f<T>(fmaf(v[i][j] * r, w[i][j], b[i][j]));
+        *reinterpret_cast<Pack<T, VEC>*>(y + row * a.d + (int64_t)p * VEC) = out;
+      }
+    }
+  }
+}
+
+// One block per row, rows of any length; the row is read three times (from L2 after the first).
+template <typename T>
+__global__ void __launch_bounds__(1024) forward_long_kernel(const Args a) {
+  __shared__ float red[2 * 32];
+  int flip = 0;
+  T* y = reinterpret_cast<T*>(a.y);
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.x) + a.xr.at(row);
+    float s[1] = {0.f};
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) s[0] += to_f<T>(x[c]);
+    group_sum<1>(s, blockDim.x, red, flip);
+    const float mu = s[0] * a.inv_d;
+    s[0] = 0.f;
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      const float v = to_f<T>(x[c]) - mu;
+      s[0] = fmaf(v, v, s[0]);
+    }
+    group_sum<1>(s, blockDim.x, red, flip);
+    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    if (threadIdx.x == 0 && a.mean != nullptr) {
+      a.mean[row] = mu;
+      a.rstd[row] = r;
+    }
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      const float w = a.w != nullptr ? load_any(a.w, a.wdtype, c) : 1.f, b = a.b != nullptr ? load_any(a.b, a.wdtype, c) : 0.f;
+      y[row * a.d + c] = from_f<T>(fmaf((to_f<T>(x[c]) - mu) * r, w, b));
+    }
+  }
+}
+
+template <typename T, int VEC, int V>
+__global__ void __launch_bounds__(V * VEC > 16 ? 256 : (V * VEC > 8 ? 512 : 1024)) backward_kernel(const Args a) {
+  extern __shared__ float sums[];  // [groups][d] when a block has several groups, used once at the end
+  __shared__ float red[2 * 32 * 2];
+  const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr;
+  const int packs = a.d / VEC;
+  const T *x = reinterpret_cast<const T*>(a.x), *dy = reinterpret_cast<const T*>(a.dy);
+  T* dx = reinterpret_cast<T*>(a.dx);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int flip = 0;
+  float w[V][VEC], dw[V][VEC], db[V][VEC];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (lane + i * a.tpr) * VEC + j;
+      w[i][j] = a.w != nullptr && c < a.d ? load_any(a.w, a.wdtype, c) : 1.f;
+      dw[i][j] = db[i][j] = 0.f;
+    }
+  Pack<T, VEC> nx[V], ng[V];
+  float nmu = 0.f, nr = 0.f;
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+  if (row < a.n) {
+    load_row<T, VEC, V>(nx, x + a.xr.at(row), lane, a.tpr, packs);
+    load_row<T, VEC, V>(ng, dy + a.dyr.at(row), lane, a.tpr, packs);
+    nmu = a.mean[row];
+    nr = a.rstd[row];
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.n; r0 += step, row += step) {
+    const bool on = row < a.n;
+    Pack<T, VEC> cx[V], cg[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      cx[i] = nx[i];
+      cg[i] = ng[i];
+    }
+    const float mu = nmu, r = nr;
+    if (row + step < a.n) {
+      load_row<T, VEC, V>(nx, x + a.xr.at(row + step), lane, a.tpr, packs);
+      load_row<T, VEC, V>(ng, dy + a.dyr.at(row + step), lane, a.tpr, packs);
+      nmu = a.mean[row + step];
+      nr = a.rstd[row + step];
+    }
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (lane + i * a.tpr >= packs || !on) continue;
+        const float g0 = to_f<T>(cg[i].v[j]), xh = (to_f<T>(cx[i].v[j]) - mu) * r, g = g0 * w[i][j];
+        s[0] += g;
+        s[1] = fmaf(g, xh, s[1]);
+        dw[i][j] = fmaf(g0, xh, dw[i][j]);
+        db[i][j] += g0;
+      }
+    group_sum<2>(s, a.tpr, red, flip);
+    const float m1 = s[0] * a.inv_d, m2 = s[1] * a.inv_d;
+    if (on && dx != nullptr) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int p = lane + i * a.tpr;
+        if (p >= packs) continue;
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float xh = (to_f<T>(cx[i].v[j]) - mu) * r;
+          out.v[j] = from_f<T>((to_f<T>(cg[i].v[j]) * w[i][j] - m1 - xh * m2) * r);
+        }
+        *reinterpret_cast<Pack<T, VEC>*>(dx + row * a.d + (int64_t)p * VEC) = out;
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.d;
+  if (groups == 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int c = (lane + i * a.tpr) * VEC + j;
+        if (c < a.d) {
+          part[c] = dw[i][j];
+          part[a.d + c] = db[i][j];
+        }
+      }
+    return;
+  }
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int c = (lane + i * a.tpr) * VEC + j;
+        if (c < a.d) sums[group * a.d + c] = which == 0 ? dw[i][j] : db[i][j];
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      float t = 0.f;
+      for (int g = 0; g < groups; ++g) t += sums[g * a.d + c];
+      part[which * a.d + c] = t;
+    }
+  }
+}
+
+// One block per row, rows of any length.  The partial sums live in the block's row of the workspace.
+template <typename T>
+__global__ void __launch_bounds__(1024) backward_long_kernel(const Args a) {
+  __shared__ float red[2 * 32 * 2];
+  int flip = 0;
+  T* dx = reinterpret_cast<T*>(a.dx);
+  float* part = a.part == nullptr ? nullptr : a.part + (int64_t)blockIdx.x * 2 * a.d;
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.x) + a.xr.at(row);
+    const T* dy = reinterpret_cast<const T*>(a.dy) + a.dyr.at(row);
+    const float mu = a.mean[row], r = a.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      const float g0 = to_f<T>(dy[c]), xh = (to_f<T>(x[c]) - mu) * r;
+      const float g = g0 * (a.w != nullptr ? load_any(a.w, a.wdtype, c) : 1.f);
+      s[0] += g;
+      s[1] = fmaf(g, xh, s[1]);
+      if (part != nullptr) {
+        const bool first = row == blockIdx.x;
+        part[c] = fmaf(g0, xh, first ? 0.f : part[c]);
+        part[a.d + c] = (first ? 0.f : part[a.d + c]) + g0;
+      }
+    }
+    group_sum<2>(s, blockDim.x, red, flip);
+    const float m1 = s[0] * a.inv_d, m2 = s[1] * a.inv_d;
+    if (dx != nullptr)
+      for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+        const float xh = (to_f<T>(x[c]) - mu) * r;
+        const float g = to_f<T>(dy[c]) * (a.w != nullptr ? load_any(a.w, a.wdtype, c) : 1.f);
+        dx[row * a.d + c] = from_f<T>((g - m1 - xh * m2) * r);
+      }
+  }
+}
+
+// dw, db = sums of the blocks' partial rows: 32 columns per block, 8 slices of partial rows added side by side and then
+// in order.
+__global__ void __launch_bounds__(256) reduce_kernel(const float* part, int64_t blocks, int d, void* dw, void* db, int wdtype) {
+  __shared__ float buf[8][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5, which = blockIdx.y;
+  float s = 0.f;
+  if (c < d)
+    for (int64_t i = slice; i < blocks; i += 8) s += part[(i * 2 + which) * d + c];
+  buf[slice][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (slice == 0 && c < d) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += buf[i][threadIdx.x & 31];
+    void* out = which == 0 ? dw : db;
+    if (out != nullptr) store_any(out, wdtype, c, s);
+  }
+}
+
+// How a call is laid out: values per load, loads per thread, threads per row and per block, blocks.
+struct Plan {
+  int vec, v, tpr, threads;
+  bool is_long;
+  int64_t blocks;
+};
+
+// Threads per row: the fewest (a power of two) whose registers hold the row; short rows share a block of 256 threads.
+// `most` is the number of values a thread may hold (its registers hold them once forward, up to four times backward).
+static Plan make_plan(int esize, int64_t n, int64_t d, bool aligned, bool backward) {
+  Plan p{};
+  const int full = 16 / esize;
+  p.vec = aligned && d % full == 0 ? full : 1;
+  const int64_t packs = d / p.vec;
+  const int choices_vec[3] = {1, 2, 4}, choices_one[3] = {2, 8, 16};
+  p.is_long = true;
+  for (int i = 0; i < 3 && p.is_long; ++i) {
+    p.v = p.vec == 1 ? choices_one[i] : choices_vec[i];
+    const int values = p.v * p.vec;
+    const int limit = backward ? (values > 16 ? 256 : values > 8 ? 512 : 1024) : (values > 16 ? 512 : 1024);
+    int tpr = 4;
+    while ((int64_t)tpr * p.v < packs) tpr <<= 1;
+    // two 16-byte loads per thread and array keep enough bytes in flight; one would not
+    if (tpr <= limit && (i > 0 || tpr <= 32)) {
+      p.tpr = tpr;
+      p.is_long = false;
+    }
+  }
+  if (p.is_long) p.tpr = 1024, p.v = 1, p.vec = 1;
+  p.threads = p.tpr < 256 ? 256 : p.tpr;
+  const int64_t groups = p.threads / p.tpr;
+  int64_t resident = 2048 / p.threads;
+  if (backward) resident = p.threads >= 1024 ? 1 : (p.v * p.vec > 8 ? 512 : 1024) / p.threads;
+  if (resident < 1) resident = 1;
+  const int64_t need = ceil_div(n, groups);
+  p.blocks = need < kNumSMs * resident ? need : kNumSMs * resident;
+  if (p.blocks < 1) p.blocks = 1;
+  return p;
+}
+
+static bool is_aligned(const void* p, int64_t s0, int64_t s1, int esize) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 * esize % 16 == 0 && s1 * esize % 16 == 0;
+}
+
+#define FLK_NORM_LAUNCH(KERNEL, VECFULL, SMEM)                                                                          \
+  if (p.is_long) KERNEL##_long_kernel<T><<<(unsigned)p.blocks, p.threads, 0, st>>>(a);                                  \
+  else if (p.vec > 1 && p.v == 1) KERNEL##_kernel<T, VECFULL, 1><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);       \
+  else if (p.vec > 1 && p.v == 2) KERNEL##_kernel<T, VECFULL, 2><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);       \
+  else if (p.vec > 1) KERNEL##_kernel<T, VECFULL, 4><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                   \
+  else if (p.v == 2) KERNEL##_kernel<T, 1, 2><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                          \
+  else if (p.v == 8) KERNEL##_kernel<T, 1, 8><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                          \
+  else KERNEL##_kernel<T, 1, 16><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);
+
+template <typename T>
+static void launch_forward(const Args& a, const Plan& p, cudaStream_t st) {
+  FLK_NORM_LAUNCH(forward, (16 / (int)sizeof(T)), 0)
+  count_launch();
+}
+
+// Several groups share a block only up to 128 threads per row, at most 64 * 32 * 64 ... values: the sums of a block's
+// groups take threads * V * VEC floats, 32 KB at most.
+template <typename T>
+static void launch_backward(const Args& a, const Plan& p, cudaStream_t st) {
+  const int groups = p.threads / p.tpr;
+  const size_t smem = groups > 1 ? (size_t)groups * a.d * 4 : 0;
+  FLK_NORM_LAUNCH(backward, (16 / (int)sizeof(T)), smem)
+  count_launch();
+}
+
+static int esize_of(int dtype) { return dtype == FLK_F32 ? 4 : 2; }
+
+static int check(const flk_layer_norm_args* p) {
+  if (p == nullptr) return fail(FLK_ERR_BAD_ARG, "args: null pointer");
+  if (p->dtype != FLK_F32 && p->dtype != FLK_BF16 && p->dtype != FLK_F16)
+    return fail(FLK_ERR_BAD_ARG, "layer norm takes fp32, bf16 or fp16 data, not dtype %lld", (long long)p->dtype);
+  if (p->wdtype != p->dtype && p->wdtype != FLK_F32)
+    return fail(FLK_ERR_BAD_ARG, "weight and bias have the data's type or fp32");
+  if (p->n < 0 || p->d < 1 || p->d > (1ll << 24) || p->n > (1ll << 40))
+    return fail(FLK_ERR_BAD_ARG, "bad sizes n = %lld, d = %lld (1 <= d <= 2^24)", (long long)p->n, (long long)p->d);
+  if (p->x_inner < 1) return fail(FLK_ERR_BAD_ARG, "x_inner must be at least 1");
+  if (!(p->eps >= 0)) return fail(FLK_ERR_BAD_ARG, "eps must not be negative");
+  return FLK_OK;
+}
+
+static Plan plan_of(const flk_layer_norm_args* p, bool backward) {
+  const int es = esize_of((int)p->dtype);
+  bool al = is_aligned(p->x, p->x_outer_stride, p->x_inner_stride, es);
+  if (backward)
+    al = al && is_aligned(p->dy, p->dy_outer_stride, p->dy_inner_stride, es) && is_aligned(p->dx, 0, 0, es);
+  else
+    al = al && is_aligned(p->y, 0, 0, es);
+  return make_plan(es, p->n, p->d, al, backward);
+}
+
+}  // namespace norm
+}  // namespace flk
+
+using namespace flk;
+
+extern "C" {
+
+int flk_layer_norm_forward(const flk_layer_norm_args* p, void* stream) {
+  FLK_TRY(norm::check(p));
+  if (p->n == 0) return FLK_OK;
+  if (p->x == nullptr || p->y == nullptr) return fail(FLK_ERR_BAD_ARG, "x / y: null pointer");
+  if ((p->mean == nullptr) != (p->rstd == nullptr)) return fail(FLK_ERR_BAD_ARG, "mean and rstd are given together");
+  norm::Args a{};
+  a.n = p->n, a.d = (int)p->d, a.wdtype = (int)p->wdtype, a.eps = (float)p->eps, a.inv_d = (float)(1.0 / (double)p->d);
+  a.x = p->x, a.w = p->weight, a.b = p->bias, a.y = p->y, a.mean = p->mean, a.rstd = p->rstd;
+  a.xr = {p->x_inner, p->x_outer_stride, p->x_inner_stride};
+  const norm::Plan plan = norm::plan_of(p, false);
+  a.tpr = plan.tpr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p->dtype == FLK_F32) norm::launch_forward<float>(a, plan, st);
+  else if (p->dtype == FLK_BF16) norm::launch_forward<__nv_bfloat16>(a, plan, st);
+  else norm::launch_forward<__half>(a, plan, st);
+  FLK_CUDA_TRY(cudaGetLastError());
+  return FLK_OK;
+}
+
+int64_t flk_layer_norm_workspace_bytes(const flk_layer_norm_args* p) {
+  const int s = norm::check(p);
+  if (s != FLK_OK) return s;
+  if (p->dweight == nullptr && p->dbias == nullptr) return 0;
+  return norm::plan_of(p, true).blocks * 2 * p->d * 4;
+}
+
+int flk_layer_norm_backward(const flk_layer_norm_args* p, void* stream) {
+  FLK_TRY(norm::check(p));
+  const bool sums = p->dweight != nullptr || p->dbias != nullptr;
+  if (p->n == 0 && !sums) return FLK_OK;
+  if (p->dy_inner < 1) return fail(FLK_ERR_BAD_ARG, "dy_inner must be at least 1");
+  if (p->n > 0 && (p->x == nullptr || p->dy == nullptr || p->mean == nullptr || p->rstd == nullptr))
+    return fail(FLK_ERR_BAD_ARG, "x, dy, mean and rstd are needed");
+  norm::Args a{};
+  a.n = p->n, a.d = (int)p->d, a.wdtype = (int)p->wdtype, a.eps = (float)p->eps, a.inv_d = (float)(1.0 / (double)p->d);
+  a.x = p->x, a.dy = p->dy, a.w = p->weight, a.dx = p->dx, a.mean = p->mean, a.rstd = p->rstd;
+  a.xr = {p->x_inner, p->x_outer_stride, p->x_inner_stride};
+  a.dyr = {p->dy_inner, p->dy_outer_stride, p->dy_inner_stride};
+  const norm::Plan plan = norm::plan_of(p, true);
+  a.tpr = plan.tpr;
+  if (sums) {
+    const int64_t need = plan.blocks * 2 * p->d * 4;
+    if (p->workspace == nullptr || p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16 != 0)
+      return fail(FLK_ERR_WORKSPACE, "layer norm needs %lld bytes of 16-byte aligned workspace", (long long)need);
+    a.part = reinterpret_cast<float*>(p->workspace);
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p->n > 0) {
+    if (p->dtype == FLK_F32) norm::launch_backward<float>(a, plan, st);
+    else if (p->dtype == FLK_BF16) norm::launch_backward<__nv_bfloat16>(a, plan, st);
+    else norm::launch_backward<__half>(a, plan, st);
+  }
+  if (sums) {
+    norm::reduce_kernel<<<dim3((unsigned)ceil_div(p->d, 32), 2), 256, 0, st>>>(a.part, p->n > 0 ? plan.blocks : 0, a.d,
+                                                                               p->dweight, p->dbias, a.wdtype);
+    count_launch();
+  }
+  FLK_CUDA_TRY(cudaGetLastError());
+  return FLK_OK;
+}
+
+}  // extern "C"

@@ -43,7 +43,8 @@ typedef enum flk_status {
   FLK_ERR_TIMEOUT = -7       /* a bounded device-side wait gave up (tensor-core kernel)     */
 } flk_status;
 
-typedef enum flk_dtype { FLK_F32 = 0, FLK_F64 = 1 } flk_dtype;
+/* The kernel-matrix products take FLK_F32 and FLK_F64; attention and layer norm FLK_F32, FLK_BF16 and FLK_F16. */
+typedef enum flk_dtype { FLK_F32 = 0, FLK_F64 = 1, FLK_BF16 = 2, FLK_F16 = 3 } flk_dtype;
 
 /* Matern with nu = 0.5 is FLK_LAPLACIAN and nu = inf is FLK_GAUSSIAN, as in
  * falkon/kernels/distance_kernel.py:235-238. */
@@ -248,6 +249,86 @@ int flk_kgrad(int dtype, int kernel,
               void* out, int64_t out_rs, int64_t out_cs,
               const double* sigma_host, int64_t sigma_len,
               void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
+/*
+ * Attention: the row-normalised product with exp(scores), next to the products with a kernel matrix above.  (No
+ * counterpart in the reference.)
+ *
+ *   r_ij = scale q_i . k_j ;   s_ij = softcap tanh(r_ij / softcap)  (softcap == 0: r_ij)  -  slope_h |p_i - j|
+ *   out_i = sum_j softmax_j(s_ij) v_j  over the keys j that query i may see ;   lse_i = log sum_j exp(s_ij)
+ *
+ * Query i of sequence b stands at position p_i = q_starts[b] + i (default: the last query at the last key, that is
+ * kv_len_b - nq + i) and sees key j when
+ *      j < kv_lens[b] (default nk)  and  (causal == 0  or  j <= p_i  or  j < prefix_lens[b])
+ *      and  (no documents  or  q_documents[b][i] == k_documents[b][j] >= 0).
+ * A query that sees nothing gets out = 0 and lse = -inf, and passes no gradient.  Keys and values at or behind
+ * kv_lens[b], and rows whose document is negative, may hold anything (NaN included).  A value or key that is not finite
+ * and that some query may see reaches the outputs of the queries that share a tile with that one.
+ *
+ * Types FLK_F32, FLK_BF16, FLK_F16; 1 <= d <= 128, d a multiple of 8 (of 4 with FLK_F32); hq a multiple of hk (query
+ * head h reads key head h / (hq / hk)).  Tensors are (batch, rows, heads, d) with unit stride over d, the other strides
+ * in elements; base addresses and strides are multiples of 16 bytes.  kv_lens, prefix_lens, q_starts: int32 device
+ * arrays of one entry per sequence (values outside [0, nk], and positions beyond 2^29, are clamped); documents: int32, one row per
+ * sequence with the given stride; slopes: fp32, one per query head.  All of them may be NULL.
+ *
+ * flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
+ * v, out, lse and dout and writes dq, dk, dv (dk and dv are given together; dq.data or both may be NULL).  Sums run in
+ * an order fixed by the sizes: results are the same from run to run.  The workspace query takes the same struct
+ * (pointers other than the documents' are not looked at).
+ */
+typedef struct flk_tensor4 {
+  void* data;
+  int64_t stride_b, stride_n, stride_h;
+} flk_tensor4;
+
+typedef struct flk_attention_args {
+  int64_t dtype, batch, nq, nk, hq, hk, d, causal, flags;
+  double scale, softcap;
+  flk_tensor4 q, k, v, out;
+  float* lse;
+  const float* slopes;
+  const int32_t *prefix_lens, *kv_lens, *q_starts;
+  const int32_t* q_documents;
+  int64_t q_documents_stride;
+  const int32_t* k_documents;
+  int64_t k_documents_stride;
+  flk_tensor4 dout, dq, dk, dv;
+  void* workspace;
+  int64_t workspace_bytes;
+} flk_attention_args;
+
+int64_t flk_attention_workspace_bytes(const flk_attention_args* args, int backward);
+int flk_attention_forward(const flk_attention_args* args, void* stream);
+int flk_attention_backward(const flk_attention_args* args, void* stream);
+
+/*
+ * Layer norm of rows (no counterpart in the reference):
+ *      y = (x - mean) / sqrt(var + eps) * weight + bias,   var = mean((x - mean)^2).
+ * x has n rows of d values (unit stride) at x + (r / x_inner) x_outer_stride + (r % x_inner) x_inner_stride: rows of
+ * a matrix (x_inner = 1), or the heads of a packed projection.  y and dx are dense.  Types FLK_F32, FLK_BF16, FLK_F16;
+ * weight and bias (either may be NULL) and their gradients have type wdtype: the data's, or FLK_F32.
+ * Forward writes y and, unless NULL, mean and rstd (n entries each, fp32), which backward reads; backward writes dx,
+ * dweight and dbias where they are not NULL.  Only the sums over rows need a workspace.  Results are the same from run
+ * to run.
+ */
+typedef struct flk_layer_norm_args {
+  int64_t dtype, wdtype, n, d;
+  double eps;
+  const void* x;
+  int64_t x_inner, x_outer_stride, x_inner_stride;
+  const void *weight, *bias;
+  void* y;
+  float *mean, *rstd;
+  const void* dy;
+  int64_t dy_inner, dy_outer_stride, dy_inner_stride;
+  void *dx, *dweight, *dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+} flk_layer_norm_args;
+
+int64_t flk_layer_norm_workspace_bytes(const flk_layer_norm_args* args);
+int flk_layer_norm_forward(const flk_layer_norm_args* args, void* stream);
+int flk_layer_norm_backward(const flk_layer_norm_args* args, void* stream);
 
 /*
  * Counters for the calling process: number of kernels this library has launched and the status
