@@ -38,7 +38,9 @@ PTXAS_REPORT = LIB_PATH + ".ptxas.txt"
 # to fill must never be spilled, so the resident kernel has to compile without any spill.  It re-partitions
 # registers between its warp roles and relies on being launched with exactly this many per thread:
 TC_LAUNCH_REGISTERS = 80
-# A few instantiations of the K-loop kernel still spill one or two 32-bit values that are stored once before the
+# Registers per thread that the attention kernels (12 warps) are launched with and re-partition:
+ATTENTION_LAUNCH_REGISTERS = 168
+# A few instantiations of the K-loop kernel and of the attention kernels still spill one or two 32-bit values that are stored once before the
 # warp roles split (none inside a tile loop); the build tolerates up to this many bytes of spill stores / loads
 # there and fails beyond (a regression guard, not an endorsement).
 TCK_SPILL_ALLOWANCE = (16, 48)
@@ -171,6 +173,11 @@ def check_ptxas(table):
                 problems.append(f"{name}: {st} bytes of spill stores, {ld} of spill loads (must be 0)")
             if regs != TC_LAUNCH_REGISTERS:
                 problems.append(f"{name}: launched with {regs} registers per thread, {TC_LAUNCH_REGISTERS} assumed")
+        elif re.search(r"attn::(fwd|bwd)::kernel", name):
+            if st > TCK_SPILL_ALLOWANCE[0] or ld > TCK_SPILL_ALLOWANCE[1]:
+                problems.append(f"{name}: {st} / {ld} bytes of spill stores / loads exceed the allowance")
+            if regs != ATTENTION_LAUNCH_REGISTERS:
+                problems.append(f"{name}: launched with {regs} registers per thread, {ATTENTION_LAUNCH_REGISTERS} assumed")
         elif "tck::kmv_tck_kernel" in name and (st > TCK_SPILL_ALLOWANCE[0] or ld > TCK_SPILL_ALLOWANCE[1]):
             problems.append(f"{name}: {st} / {ld} bytes of spill stores / loads exceed the allowance")
     if table and not seen_tc:
@@ -201,7 +208,7 @@ class AttentionArgs(ctypes.Structure):
     _fields_ = [(n, _i64) for n in ("dtype", "batch", "nq", "nk", "hq", "hk", "d", "causal", "flags")]
     _fields_ += [("scale", ctypes.c_double), ("softcap", ctypes.c_double)]
     _fields_ += [(n, Tensor4) for n in ("q", "k", "v", "out")]
-    _fields_ += [(n, _vp) for n in ("lse", "slopes", "prefix_lens", "kv_lens", "q_starts")]
+    _fields_ += [(n, _vp) for n in ("out_lo", "lse", "slopes", "prefix_lens", "kv_lens", "q_starts")]
     _fields_ += [("q_documents", _vp), ("q_documents_stride", _i64), ("k_documents", _vp), ("k_documents_stride", _i64)]
     _fields_ += [(n, Tensor4) for n in ("dout", "dq", "dk", "dv")]
     _fields_ += [("workspace", _vp), ("workspace_bytes", _i64)]
@@ -244,6 +251,7 @@ _SIGNATURES = {
     "flk_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionArgs), _int]),
     "flk_attention_forward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
     "flk_attention_backward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
+    "flk_attention_status": (_int, [_vp, ctypes.POINTER(_int)]),
     "flk_layer_norm_workspace_bytes": (_i64, [ctypes.POINTER(LayerNormArgs)]),
     "flk_layer_norm_forward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
     "flk_layer_norm_backward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
@@ -720,6 +728,15 @@ def call_struct(name: str, args: ctypes.Structure, device: torch.device, *query)
     status = getattr(lib, "flk_" + name)(ref, torch.cuda.current_stream(device).cuda_stream)
     if status != 0:
         raise_for_status(status)
+
+
+def attention_status(device: torch.device) -> int:
+    """1 when a bounded wait of an attention kernel gave up on this device since the library was loaded, else 0."""
+    out = ctypes.c_int(0)
+    with torch.cuda.device(device):
+        stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+        raise_for_status(load().flk_attention_status(stream, ctypes.byref(out)))
+    return out.value
 
 
 def tc_status(device: torch.device) -> int:

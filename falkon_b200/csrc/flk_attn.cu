@@ -1,9 +1,42 @@
 // extern "C" entry points of attention: argument checks, workspace, choice of kernel.
 #include "flk_attn.cuh"
+#include "flk_attn_fwd.cuh"
 #include "flk_attn_simt.cuh"
 
 namespace flk {
 namespace attn {
+
+int forward_bf16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
+int forward_f16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
+int forward_status_bf16(cudaStream_t st, int* out);
+int forward_status_f16(cudaStream_t st, int* out);
+
+// The tables of documents: labels padded to whole tiles, -1 (keys) / -2 (queries) where nothing may be seen, and the
+// smallest and largest label of each tile (an empty tile: a range that meets no other).  One warp per tile.
+__global__ void __launch_bounds__(128) documents_kernel(const int* docs, int64_t sb, int n, const int* lens, int none, int n_pad,
+                                                        int* out, int4* tab) {
+  const int b = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (tile * kTile >= n_pad) return;
+  const int len = lens != nullptr ? min(max(lens[b], 0), n) : n;
+  int lo = INT32_MAX, hi = INT32_MIN, bad = 0;
+  for (int r = lane; r < kTile; r += 32) {
+    const int i = tile * kTile + r;
+    const int id = i < len ? docs[b * sb + i] : -1;
+    if (id >= 0) {
+      lo = min(lo, id);
+      hi = max(hi, id);
+    } else {
+      bad = 1;
+    }
+    out[(int64_t)b * n_pad + i] = id >= 0 ? id : none;
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) tab[(int64_t)b * (n_pad / kTile) + tile] = make_int4(lo, hi, bad, 0);
+}
 
 static int esize_of(int64_t dtype) { return dtype == FLK_F32 ? 4 : 2; }
 
@@ -37,8 +70,16 @@ static int check_tensor(const char* name, const flk_tensor4& t, int64_t b, int64
   return FLK_OK;
 }
 
+// The tensor-core kernels take 16-bit data; without keys there is nothing for them to do.
+static bool on_tensor_cores(const flk_attention_args* p) {
+  return p->dtype != FLK_F32 && p->nk > 0 && (p->flags & FLK_FLAG_FORCE_SIMT) == 0;
+}
+static fwd::Plan forward_plan(const flk_attention_args* p) {
+  return fwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk);
+}
+
 struct Workspace {
-  int64_t qdocs, kdocs, qtab, ktab, delta, total;
+  int64_t qdocs, kdocs, qtab, ktab, delta, part_o, part_lse, total;
 };
 static int64_t pad_rows(int64_t n) { return round_up(n, kTile); }
 static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
@@ -52,10 +93,15 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
   if (p->q_documents != nullptr) {
     w.qdocs = take(p->batch * pad_rows(p->nq) * 4);
     w.kdocs = take(p->batch * pad_rows(p->nk) * 4);
-    w.qtab = take(p->batch * pad_rows(p->nq) / kTile * 8);
-    w.ktab = take(p->batch * pad_rows(p->nk) / kTile * 8);
+    w.qtab = take(p->batch * pad_rows(p->nq) / kTile * 16);
+    w.ktab = take(p->batch * pad_rows(p->nk) / kTile * 16);
   }
   if (backward) w.delta = take(p->batch * p->hq * p->nq * 4);
+  if (!backward && on_tensor_cores(p) && p->batch > 0 && p->nq > 0) {
+    const int64_t rows = fwd::partial_rows(forward_plan(p), (int)p->batch);
+    w.part_o = take(rows * p->d * 4);
+    w.part_lse = take(rows * 4);
+  }
   w.total = at;
   return w;
 }
@@ -77,14 +123,14 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
   a.slopes = p->slopes, a.prefix = p->prefix_lens, a.kv_lens = p->kv_lens, a.q_starts = p->q_starts;
   a.nq_pad = (int)pad_rows(p->nq), a.nk_pad = (int)pad_rows(p->nk);
   a.q = tensor_of(p->q), a.k = tensor_of(p->k), a.v = tensor_of(p->v), a.o = tensor_of(p->out);
-  a.lse = p->lse;
+  a.lse = p->lse, a.o_lo = p->dtype == FLK_F32 ? nullptr : p->out_lo;
   if (backward) {
     a.dout = tensor_of(p->dout), a.dq = tensor_of(p->dq), a.dk = tensor_of(p->dk), a.dv = tensor_of(p->dv);
     a.delta = reinterpret_cast<float*>(ws + w.delta);
   }
   if (p->q_documents != nullptr) {
     int *qd = reinterpret_cast<int*>(ws + w.qdocs), *kd = reinterpret_cast<int*>(ws + w.kdocs);
-    int2 *qt = reinterpret_cast<int2*>(ws + w.qtab), *kt = reinterpret_cast<int2*>(ws + w.ktab);
+    int4 *qt = reinterpret_cast<int4*>(ws + w.qtab), *kt = reinterpret_cast<int4*>(ws + w.ktab);
     a.qdocs = qd, a.kdocs = kd, a.qtab = qt, a.ktab = kt;
     if (p->nq > 0) {
       documents_kernel<<<dim3((unsigned)ceil_div(a.nq_pad / kTile, 4), a.b), 128, 0, st>>>(
@@ -133,14 +179,33 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
   FLK_TRY(attn::check_tensor("k", p->k, p->batch, p->nk, p->hk, es));
   FLK_TRY(attn::check_tensor("v", p->v, p->batch, p->nk, p->hk, es));
   FLK_TRY(attn::check_tensor("out", p->out, p->batch, p->nq, p->hq, es));
+  if (reinterpret_cast<uintptr_t>(p->out_lo) % 16 != 0) return fail(FLK_ERR_LAYOUT, "out_lo: not 16-byte aligned");
   if (p->batch == 0 || p->nq == 0) return FLK_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   attn::Args a;
   FLK_TRY(attn::make_args(p, false, a, st));
-  if (p->dtype == FLK_F32) FLK_TRY(attn::simt_forward<float>(a, st));
+  if (attn::on_tensor_cores(p)) {
+    attn::TcArgs t{};
+    t.a = a;
+    const attn::Workspace w = attn::plan_workspace(p, false);
+    char* ws = reinterpret_cast<char*>(p->workspace);
+    t.part_o = reinterpret_cast<float*>(ws + w.part_o), t.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
+    const attn::fwd::Plan plan = attn::forward_plan(p);
+    FLK_TRY(p->dtype == FLK_BF16 ? attn::forward_bf16(t, plan, st) : attn::forward_f16(t, plan, st));
+  } else if (p->dtype == FLK_F32) FLK_TRY(attn::simt_forward<float>(a, st));
   else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_forward<__nv_bfloat16>(a, st));
   else FLK_TRY(attn::simt_forward<__half>(a, st));
   FLK_CUDA_TRY(cudaGetLastError());
+  return FLK_OK;
+}
+
+int flk_attention_status(void* stream, int* out) {
+  if (out == nullptr) return fail(FLK_ERR_BAD_ARG, "status_out: null pointer");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int x = 0, y = 0;
+  FLK_TRY(attn::forward_status_bf16(st, &x));
+  FLK_TRY(attn::forward_status_f16(st, &y));
+  *out = x | y;
   return FLK_OK;
 }
 
@@ -151,6 +216,7 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
   FLK_TRY(attn::check_tensor("k", p->k, p->batch, p->nk, p->hk, es));
   FLK_TRY(attn::check_tensor("v", p->v, p->batch, p->nk, p->hk, es));
   FLK_TRY(attn::check_tensor("out", p->out, p->batch, p->nq, p->hq, es));
+  if (reinterpret_cast<uintptr_t>(p->out_lo) % 16 != 0) return fail(FLK_ERR_LAYOUT, "out_lo: not 16-byte aligned");
   FLK_TRY(attn::check_tensor("dout", p->dout, p->batch, p->nq, p->hq, es));
   if ((p->dk.data == nullptr) != (p->dv.data == nullptr) && p->nk > 0)
     return fail(FLK_ERR_BAD_ARG, "dk and dv are given together");

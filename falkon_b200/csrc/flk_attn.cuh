@@ -33,9 +33,10 @@ struct Args {
   const float* slopes;  // per query head, or null
   const int *prefix, *kv_lens, *q_starts;
   const int *qdocs, *kdocs;  // padded tables of the workspace ([b][nq_pad], [b][nk_pad]; -2 / -1 where nothing is seen), or null
-  const int2 *qtab, *ktab;   // smallest and largest label of every tile of 128 ([b][nq_pad / 128], ...)
+  const int4 *qtab, *ktab;   // of every tile of 128: smallest, largest label, whether a row has none ([b][nq_pad / 128], ...)
   int nq_pad, nk_pad;
   Tensor4 q, k, v, o, dout, dq, dk, dv;
+  void* o_lo;    // what rounding took from `o` (16-bit types; strides of o), or null
   float* lse;    // (b, hq, nq), natural logarithm; -inf for rows that see nothing
   float* delta;  // (b, hq, nq)
 };
@@ -75,30 +76,6 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 constexpr float kLn2 = 0.6931471805599453f;
-
-// The tables of documents: labels padded to whole tiles, -1 (keys) / -2 (queries) where nothing may be seen, and the
-// smallest and largest label of each tile (an empty tile: a range that meets no other).  One warp per tile.
-__global__ void __launch_bounds__(128) documents_kernel(const int* docs, int64_t sb, int n, const int* lens, int none, int n_pad,
-                                                        int* out, int2* tab) {
-  const int b = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (tile * kTile >= n_pad) return;
-  const int len = lens != nullptr ? min(max(lens[b], 0), n) : n;
-  int lo = INT32_MAX, hi = INT32_MIN;
-  for (int r = lane; r < kTile; r += 32) {
-    const int i = tile * kTile + r;
-    const int id = i < len ? docs[b * sb + i] : -1;
-    if (id >= 0) {
-      lo = min(lo, id);
-      hi = max(hi, id);
-    }
-    out[(int64_t)b * n_pad + i] = id >= 0 ? id : none;
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (lane == 0) tab[(int64_t)b * (n_pad / kTile) + tile] = make_int2(lo, hi);
-}
 
 }  // namespace attn
 }  // namespace flk

@@ -1,0 +1,528 @@
+// Forward attention on tcgen05: out, and the log-sum-exp of every row.
+//
+// A block has 12 warps: two softmax warpgroups (a thread owns one packed query row), a warp that issues the matrix products
+// and one that issues the copies.  Tensor memory holds two score tiles of 128 x 128 and two accumulators of 128 x DP, all
+// 512 columns.  The two warpgroups take turns on the tensor cores: while one turns its scores into weights, the products
+// of the other run.
+//   PAIR   two row tiles (256 rows) against the same key tiles, for prompts and training
+//   !PAIR  one row tile; the warpgroups take the even and the odd key tiles, and end with a partial result each: few
+//          rows over a long key axis (single tokens)
+// Weights are exp2(s - m) with a maximum m that follows the running one only when that has grown by more than 8: weights
+// stay below 2^8, and the accumulator is rescaled a few times in a row's life instead of once per tile.  The sum of the
+// weights is taken before they are rounded to the data's 16 bits (a relative error of half a step per weight, which is what the
+// result itself is rounded by); it, the maximum and the accumulators are fp32.
+// Where blocks are fewer than SMs, the key axis is cut into parts, whose normalised fp32 results a second kernel joins.
+#pragma once
+
+#include "flk_attn_tc.cuh"
+
+namespace flk {
+namespace attn {
+namespace fwd {
+
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// registers: 384 threads are launched with 168 each (64512); two warpgroups of 216 and one of 72 make the same sum
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * 168, "registers");
+
+template <int DP, bool PAIR>
+struct Layout {
+  static constexpr uint32_t kTileBytes = DP / 64 * kBlockBytes;
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kRing = (PAIR ? 2 : 1) * kTileBytes;
+  static constexpr int kStages = (int)((224 * 1024 - kRing) / kTileBytes) < 8 ? (int)((224 * 1024 - kRing) / kTileBytes) : 8;
+  static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
+  static constexpr uint32_t kBytes = kBars + 384 + 1024;  // barriers and slots, and room to align the tiles to 1024 bytes
+};
+static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
+
+// packed head, sequence, part of the key axis, first row of the block
+__device__ __forceinline__ int4 get_place(uint32_t at) {
+  int4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// Turns the raw scores of one row into scores in base 2 (where the kernel keeps them raw, CAP and BIAS being off, nothing).
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void transform(uint32_t (&s)[4][32], const Args& a, float slope2, float d0) {
+  if constexpr (CAP || BIAS) {
+    const float f = CAP ? a.scale * (2.f * kLog2e) : a.scale, cap2 = a.cap2;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        float x = __uint_as_float(s[p][c]) * f;
+        if constexpr (CAP) x = fmaf(-2.f * cap2, rcp_approx(1.f + ex2_approx(x)), cap2);  // cap tanh, tanh(x) = 1 - 2 / (1 + e^2x)
+        if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
+        s[p][c] = __float_as_uint(x);
+      }
+  }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const TcArgs t) {
+  using L = Layout<DP, PAIR>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t raw[];
+  const Args& a = t.a;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const uint32_t bars = base + L::kBars;
+  auto full = [&](int s) { return bars + s * 8; };
+  auto empty = [&](int s) { return bars + 64 + s * 8; };
+  auto sfull = [&](int w) { return bars + 128 + w * 8; };
+  auto pfull = [&](int w) { return bars + 144 + w * 8; };
+  auto odone = [&](int w) { return bars + 160 + w * 8; };
+  const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320;
+  const int warp = threadIdx.x >> 5;
+
+  // block -> (row block, part of the key axis, sequence, packed head); late row blocks have the most keys under a causal
+  // mask and start first
+  int64_t id = blockIdx.x;
+  const int hp = (int)(id % t.hp);
+  id /= t.hp;
+  const int b = (int)(id % a.b);
+  id /= a.b;
+  const int split = (int)(id % t.splits);
+  const int rb = t.blocks - 1 - (int)(id / t.splits);
+  constexpr int kRows = PAIR ? 256 : 128;
+  const int row0 = rb * kRows, hk = hp * t.pg / a.grp;
+  const int i0 = row0 >> t.pg_shift, i1 = min(a.nq, (row0 + kRows) >> t.pg_shift);  // queries of this block
+  const Limits lim = limits_of(a, b);
+  const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
+  const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
+  const int4* ktab = kd ? a.ktab + (int64_t)b * (a.nk_pad / kTile) : nullptr;
+  const int tiles = (lim.row_end(i1 - 1, a.causal) + kTile - 1) / kTile;
+  const int first = (int)((int64_t)tiles * split / t.splits), last = (int)((int64_t)tiles * (split + 1) / t.splits);
+  LabelRange lab{0, 0, false};
+  if (kd) lab = labels_of(qd, i0, i1);
+  const int steps = count_tiles(ktab, first, last, lab.lo, lab.hi);
+
+  if (warp == kMmaWarp) {
+    if (elect_one()) {
+      for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+      for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 4), mbar_init(odone(w), 1);
+      mbar_init(qfull, 1);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place + 16), "r"(lim.len), "r"(lim.start), "r"(lim.prefix), "r"(0) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(hp), "r"(b), "r"(split), "r"(row0) : "memory");
+      tc::fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+  auto ts = [&](int w) { return tmem + (uint32_t)w * kTile; };                  // scores, then weights
+  auto to = [&](int w) { return tmem + 2 * kTile + (uint32_t)w * DP; };  // accumulators
+
+  if (warp >= 8) {
+    tc::reg_release<kRegsOther>();
+    if (warp == kLoadWarp) {
+      TileWalk walk(ktab, first, last, lab.lo, lab.hi);
+      bool ok = true;
+      if (steps > 0 && elect_one()) {
+        mbar_expect_tx(qfull, (PAIR ? 2 : 1) * L::kTileBytes);
+#pragma unroll
+        for (int r = 0; r < (PAIR ? 2 : 1); ++r)
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c)
+            tma_load(base + r * L::kTileBytes + c * kBlockBytes, &tq, c * 64, hp * t.pg, (row0 + r * kTile) >> t.pg_shift, b, qfull);
+      }
+      __syncwarp();
+      int n = 0;  // copies issued
+      for (int step = 0; step < steps && ok; ++step) {
+        const Tile e = walk.next();
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int s = n % kStages;
+          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (!ok) break;
+          if (elect_one()) {
+            if (kv == 0) put_tile(slots, step, e);
+            mbar_expect_tx(full(s), L::kTileBytes);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+              tma_load(base + L::kRing + s * L::kTileBytes + c * kBlockBytes, kv == 0 ? &tk : &tv, c * 64, hk, e.at * kTile, b, full(s));
+          }
+          __syncwarp();
+          ++n;
+        }
+      }
+      // no copy may land after the block has gone
+      if (steps > 0) wait_bar(qfull, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+    } else if (warp == kMmaWarp) {
+      bool ok = steps == 0 || wait_bar(qfull, 0);
+      auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
+      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      auto clean = [&](int step) {
+        const Tile e = get_tile(slots, step);
+        if (e.dirty || (e.at + 1) * kTile > lim.len) clean_tile<DP>(stage(2 * step + 1), e.at * kTile, lim.len, kd);
+      };
+      // copy 2 i is the key tile, copy 2 i + 1 the value tile of step i
+      if (steps > 0) {
+        ok = ok && ready(0);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          issue_scores<T, DP>(ts(0), base, stage(0));
+          mma_commit(sfull(0));
+          if constexpr (PAIR) {
+            issue_scores<T, DP>(ts(1), base + L::kTileBytes, stage(0));
+            mma_commit(sfull(1));
+          }
+          mma_commit(empty(0));
+        }
+        __syncwarp();
+      }
+      for (int i = 0; i < steps && ok; ++i) {
+        const bool more = i + 1 < steps;
+        if constexpr (PAIR) {
+          ok = ready(2 * i + 1);
+          if (ok) clean(i);
+          for (int w = 0; w < 2 && ok; ++w) {
+            ok = wait_bar(pfull(w), (uint32_t)i & 1);
+            if (ok && w == 0 && more) ok = ready(2 * i + 2);
+            tc_fence_after();
+            if (ok && elect_one()) {
+              issue_weighted<T, DP>(to(w), ts(w), stage(2 * i + 1), i > 0);
+              if (w == 1) mma_commit(empty((2 * i + 1) % kStages));
+              if (more) {
+                issue_scores<T, DP>(ts(w), base + w * L::kTileBytes, stage(2 * i + 2));
+                mma_commit(sfull(w));
+                if (w == 1) mma_commit(empty((2 * i + 2) % kStages));
+              }
+            }
+            __syncwarp();
+          }
+        } else {
+          // step i belongs to warpgroup i & 1: its scores are issued one step ahead of the weighted sum
+          const int w = i & 1;
+          if (more) {
+            ok = ready(2 * i + 2);
+            tc_fence_after();
+            // the other score tile was consumed by the weighted sum of step i - 1, issued before
+            if (ok && elect_one()) {
+              issue_scores<T, DP>(ts(w ^ 1), base, stage(2 * i + 2));
+              mma_commit(sfull(w ^ 1));
+              mma_commit(empty((2 * i + 2) % kStages));
+            }
+            __syncwarp();
+          }
+          ok = ok && ready(2 * i + 1);
+          if (ok) clean(i);
+          ok = ok && wait_bar(pfull(w), (uint32_t)(i >> 1) & 1);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            issue_weighted<T, DP>(to(w), ts(w), stage(2 * i + 1), i > 1);
+            mma_commit(empty((2 * i + 1) % kStages));
+          }
+          __syncwarp();
+        }
+      }
+      if (steps > 0 && ok && elect_one()) {
+        mma_commit(odone(0));
+        mma_commit(odone(1));
+      }
+      __syncwarp();
+      // no arrival may come after the block has gone
+      if (steps > 0 && ok) {
+        wait_bar(odone(0), 0);
+        wait_bar(odone(1), 0);
+      }
+    }
+  } else {
+    tc::reg_claim<kRegsSoftmax>();
+    const int w = warp >> 2, lane_row = threadIdx.x & 127;
+    const uint32_t lane_at = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in bits 16 and up
+    const int r = row0 + (PAIR ? w * kTile : 0) + lane_row;  // packed row
+    const bool live = (r & ~31) < t.rows;                     // some row of this warp exists
+    const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+    const bool exists = r < t.rows;
+    const int my = qd && exists ? qd[i] : -2;
+    const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+    const int pos = lim.start + i;
+    // keys before this bound are visible to every row of the warpgroup's tile that exists
+    const int tile_i0 = (row0 + (PAIR ? w * kTile : 0)) >> t.pg_shift;
+    const int all_before = lim.row_end(min(tile_i0, a.nq - 1), a.causal);
+    int only = -1;  // the one label of its queries
+    if (kd) {
+      const LabelRange mine = labels_of(qd, min(tile_i0, a.nq), min(a.nq, (tile_i0 + (kTile >> t.pg_shift))));
+      if (!mine.bad && mine.lo == mine.hi) only = mine.lo;
+    }
+    const float f2 = a.scale;  // raw score -> base 2, where nothing else is done to it
+    float m = -INFINITY;       // of the weights, base 2
+    float l = 0.f;
+    bool ok = true;
+    int turn = 0;
+    for (int step = PAIR ? 0 : w; step < steps && ok; step += PAIR ? 1 : 2) {
+      ok = wait_bar(sfull(w), (uint32_t)turn & 1);
+      ++turn;
+      if (!ok) break;
+      if (!live) {  // the weights of rows that do not exist reach nothing
+        if (elect_one()) mbar_arrive(pfull(w));
+        __syncwarp();
+        continue;
+      }
+      tc_fence_after();
+      const Tile e = get_tile(slots, step);
+      const int k0 = e.at * kTile;
+      const bool whole = k0 + kTile <= all_before && (a.kdocs == nullptr || (e.label >= 0 && e.label == only));
+      uint32_t s[4][32];
+      const uint32_t at = ts(w) + lane_at;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) tmem_ld32(at + 32 * p, s[p]);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) tmem_ld_wait_on(s[p]);
+      transform<CAP, BIAS>(s, a, slope2, (float)(pos - k0));
+      if (!whole) {
+        const int4 x = get_place(place + 16);
+        const int r = row0 + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
+        const int end = r < t.rows ? Limits{x.x, x.y, x.z}.row_end(r >> t.pg_shift, a.causal) : 0;
+        const int* labels = a.kdocs == nullptr ? nullptr : a.kdocs + (int64_t)get_place(place).y * a.nk_pad + k0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) hide_columns(s[p], seen_columns(end - k0 - 32 * p, labels == nullptr ? nullptr : labels + 32 * p, my));
+      }
+      float top[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        top[p] = __uint_as_float(s[p][0]);
+#pragma unroll
+        for (int c = 1; c < 31; c += 2) top[p] = fmaxf(fmaxf(top[p], __uint_as_float(s[p][c])), __uint_as_float(s[p][c + 1]));
+        top[p] = fmaxf(top[p], __uint_as_float(s[p][31]));
+      }
+      float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if constexpr (!CAP && !BIAS) mt *= f2;
+      const bool grow = mt > m + 8.f || (m == -INFINITY && mt != -INFINITY);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float mn = grow ? mt : m;
+        const float f = m == mn ? 1.f : ex2_approx(m - mn);
+        if (step > (PAIR ? 0 : 1)) {
+          // s_full of this step says that the weighted sums before it are done
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tc::tmem_ld16(to(w) + lane_at + c, o);
+            tmem_ld_wait_on(o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(to(w) + lane_at + c, o);
+          }
+        }
+        l *= f;
+        m = mn;
+      }
+      const float mb = m == -INFINITY ? 0.f : m;
+      const uint64_t f2v = tc::pack2(f2, f2), mv = tc::pack2(-mb, -mb);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const uint32_t s0 = s[p][c], s1 = s[p][c + 1];
+          const uint64_t v = tc::pack2(__uint_as_float(s0), __uint_as_float(s1));
+          const uint64_t x = CAP || BIAS ? tc::add2(v, mv) : tc::fma2(v, f2v, mv);
+          float x0, x1, p0, p1;
+          tc::unpack2(x, x0, x1);
+          p0 = ex2_approx(x0);
+          p1 = ex2_approx(x1);
+          sum[(c / 2) & 1] = tc::add2(sum[(c / 2) & 1], tc::pack2(p0, p1));
+          o[c / 2] = pack16<T>(p0, p1);
+        }
+        tmem_st16(at + 16 * p, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (elect_one()) mbar_arrive(pfull(w));
+      __syncwarp();
+      float u0, u1;
+      tc::unpack2(tc::add2(sum[0], sum[1]), u0, u1);
+      l += u0 + u1;
+    }
+    // ---- results
+    const bool worked = turn > 0;
+    if (worked && ok) ok = wait_bar(odone(w), 0);
+    tc_fence_after();
+    const bool none = m == -INFINITY;
+    const float inv = none ? 0.f : 1.0f / l, lse2 = none ? -INFINITY : m + log2f(l);
+    if (live && ok) {
+      // read again instead of held in registers through the loop above
+      const int4 at = get_place(place);
+      const int hp = at.x, b = at.y, split = at.z, r = at.w + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
+      const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+      const bool exists = r < t.rows;
+      const bool parts = !PAIR || t.splits > 1;
+      const int part = PAIR ? split : 2 * split + w;
+      const int64_t prow = (((int64_t)part * a.b + b) * t.hp + hp) * t.rows + r;
+      if (exists) {
+        if (parts)
+          t.part_lse[prow] = lse2;
+        else if (a.lse != nullptr)
+          a.lse[((int64_t)b * a.hq + h) * a.nq + i] = lse2 * kLn2;
+      }
+      T* out = reinterpret_cast<T*>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
+      T* lo = a.o_lo == nullptr ? nullptr : reinterpret_cast<T*>(a.o_lo) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (worked) {
+          tmem_ld32(to(w) + lane_at + c, o);
+          tmem_ld_wait_on(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+        if (parts) {
+          if (exists && !none) {  // the joining kernel does not read empty rows
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < a.d) *reinterpret_cast<uint4*>(t.part_o + prow * a.d + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        } else if (exists) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (c + e < a.d) {
+              uint32_t v[4], x[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float y0 = __uint_as_float(o[e + 2 * q]), y1 = __uint_as_float(o[e + 2 * q + 1]);
+                v[q] = pack16<T>(y0, y1);
+                x[q] = pack16<T>(y0 - to_f<T>(from_f<T>(y0)), y1 - to_f<T>(from_f<T>(y1)));
+              }
+              *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+              if (lo != nullptr) *reinterpret_cast<uint4*>(lo + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the key axis: out = sum_p w_p o_p with w_p = 2^(lse_p - max) / sum.  A warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
+  const Args& a = t.a;
+  const int64_t n = (int64_t)a.b * t.hp * t.rows, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= n) return;
+  const int r = (int)(row % t.rows), hp = (int)(row / t.rows % t.hp), b = (int)(row / t.rows / t.hp);
+  const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+  float top = -INFINITY;
+  for (int p = lane; p < parts; p += 32) top = fmaxf(top, t.part_lse[p * n + row]);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+  if (top != -INFINITY)
+    for (int p = lane; p < parts; p += 32) sum += exp2f(t.part_lse[p * n + row] - top);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = top == -INFINITY ? 0.f : 1.0f / sum;
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.hq + h) * a.nq + i] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+  const int c = lane * 4;
+  if (c >= a.d) return;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (top != -INFINITY)
+    for (int p = 0; p < parts; ++p) {
+      const float e = t.part_lse[p * n + row];
+      if (e == -INFINITY) continue;
+      const float w = exp2f(e - top) * inv;
+      const float4 v = *reinterpret_cast<const float4*>(t.part_o + (p * n + row) * a.d + c);
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+  const int64_t at = b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh + c;
+  const uint2 v = make_uint2(pack16<T>(acc.x, acc.y), pack16<T>(acc.z, acc.w));
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o.p) + at) = v;
+  if (a.o_lo != nullptr) {
+    const uint2 x = make_uint2(pack16<T>(acc.x - to_f<T>(from_f<T>(acc.x)), acc.y - to_f<T>(from_f<T>(acc.y))),
+                               pack16<T>(acc.z - to_f<T>(from_f<T>(acc.z)), acc.w - to_f<T>(from_f<T>(acc.w))));
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o_lo) + at) = x;
+  }
+}
+
+// Parts of the key axis.  With PAIR, one part where the blocks fill the SMs; else the number with the lowest
+// max(waves) x (tiles of a part + 3 tiles' time for a block's start and end).
+struct Plan {
+  bool pair;
+  int pg, pg_shift, hp, rows, blocks, splits, parts;
+};
+inline Plan make_plan(int b, int nq, int nk, int hq, int hk) {
+  Plan p{};
+  const int grp = hq / hk;
+  p.pg = (grp & (grp - 1)) == 0 && grp <= 64 ? grp : 1;
+  while ((1 << p.pg_shift) < p.pg) ++p.pg_shift;
+  p.hp = hq / p.pg;
+  p.rows = nq * p.pg;
+  p.pair = p.rows > 128;
+  p.blocks = (int)ceil_div(p.rows, p.pair ? 256 : 128);
+  const int64_t blocks = (int64_t)p.blocks * p.hp * b, tiles = ceil_div(nk, kTile);
+  p.splits = 1;
+  double best = 1e300;
+  const int64_t least = p.pair ? 4 : 2;  // key tiles of a part
+  for (int64_t s = 1; s <= 64 && (s == 1 || s * least <= tiles); ++s) {
+    const double cost = (double)ceil_div(blocks * s, kNumSMs) * ((double)ceil_div(tiles, s) + 3) + (s > 1 || !p.pair ? 0.05 * s : 0.0);
+    if (cost < best * 0.97) best = cost, p.splits = (int)s;
+  }
+  p.parts = p.pair ? p.splits : 2 * p.splits;
+  return p;
+}
+inline int64_t partial_rows(const Plan& p, int b) { return p.parts > 1 ? (int64_t)p.parts * b * p.hp * p.rows : 0; }
+
+template <typename T, int DP, bool CAP, bool BIAS, bool PAIR>
+inline int launch_one(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcArgs& t, cudaStream_t st) {
+  auto* fn = kernel<T, DP, CAP, BIAS, PAIR>;
+  constexpr int kBytes = (int)Layout<DP, PAIR>::kBytes;
+  FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  const int64_t grid = (int64_t)t.blocks * t.splits * t.a.b * t.hp;
+  if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many row blocks");
+  fn<<<(unsigned)grid, kThreads, kBytes, st>>>(tq, tk, tv, t);
+  count_launch();
+  return FLK_OK;
+}
+template <typename T, int DP, bool PAIR>
+inline int launch_some(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcArgs& t, cudaStream_t st) {
+  const bool cap = t.a.cap2 != 0.f;
+  // without a cap and a bias the maximum is taken of the raw scores, which needs a positive factor
+  const bool bias = t.a.slopes != nullptr || (!cap && !(t.a.scale > 0.f));
+  if (cap) return bias ? launch_one<T, DP, true, true, PAIR>(tq, tk, tv, t, st) : launch_one<T, DP, true, false, PAIR>(tq, tk, tv, t, st);
+  return bias ? launch_one<T, DP, false, true, PAIR>(tq, tk, tv, t, st) : launch_one<T, DP, false, false, PAIR>(tq, tk, tv, t, st);
+}
+
+template <typename T>
+inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
+  const Args& a = t.a;
+  const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
+  t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.blocks, t.splits = p.splits;
+  CUtensorMap tq, tk, tv;
+  FLK_TRY(make_map(&tq, a.q, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
+  FLK_TRY(make_map(&tk, a.k, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
+  FLK_TRY(make_map(&tv, a.v, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
+  if (a.d <= 64)
+    FLK_TRY((p.pair ? launch_some<T, 64, true>(tq, tk, tv, t, st) : launch_some<T, 64, false>(tq, tk, tv, t, st)));
+  else
+    FLK_TRY((p.pair ? launch_some<T, 128, true>(tq, tk, tv, t, st) : launch_some<T, 128, false>(tq, tk, tv, t, st)));
+  if (p.parts > 1) {
+    join_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * t.hp * t.rows, 8), 256, 0, st>>>(t, p.parts);
+    count_launch();
+  }
+  return FLK_OK;
+}
+
+}  // namespace fwd
+}  // namespace attn
+}  // namespace flk

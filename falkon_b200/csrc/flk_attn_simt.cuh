@@ -93,7 +93,7 @@ __device__ __forceinline__ void outer(float (&acc)[4][DM / 16], const float* W, 
 
 template <typename T, int DM>
 __device__ __forceinline__ void store_rows(T* dst, int64_t sn, int r0, int n, int d, const float (&acc)[4][DM / 16], const float (&f)[4],
-                                           int ty, int tx) {
+                                           int ty, int tx, T* lo = nullptr) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + 4 * ty + i;
@@ -103,7 +103,10 @@ __device__ __forceinline__ void store_rows(T* dst, int64_t sn, int r0, int n, in
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int col = 4 * tx + 64 * c + e;
-        if (col < d) dst[(int64_t)r * sn + col] = from_f<T>(acc[i][4 * c + e] * f[i]);
+        if (col >= d) continue;
+        const float y = acc[i][4 * c + e] * f[i];
+        dst[(int64_t)r * sn + col] = from_f<T>(y);
+        if (lo != nullptr) lo[(int64_t)r * sn + col] = from_f<T>(y - to_f<T>(from_f<T>(y)));
       }
   }
 }
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   for (int k0 = 0; k0 < last; k0 += kT) {
     if (kd != nullptr) {  // no label in common: nothing to see
-      const int2 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
       if (x.y < y.x || y.y < x.x) continue;
     }
     __syncthreads();
@@ -200,7 +203,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
     if (tx == 0 && r < a.nq && a.lse != nullptr)
       a.lse[((int64_t)b * a.hq + h) * a.nq + r] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
-  store_rows<T, DM>((T*)a.o.p + b * a.o.sb + h * a.o.sh, a.o.sn, q0, a.nq, a.d, acc, f, ty, tx);
+  store_rows<T, DM>((T*)a.o.p + b * a.o.sb + h * a.o.sh, a.o.sn, q0, a.nq, a.d, acc, f, ty, tx,
+                    a.o_lo == nullptr ? nullptr : (T*)a.o_lo + b * a.o.sb + h * a.o.sh);
 }
 
 // delta_i = dO_i . O_i, a group of 16 lanes per row of one head
@@ -223,6 +227,11 @@ __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
     *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(y + c);
 #pragma unroll
     for (int e = 0; e < kVec; ++e) s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
+    if (a.o_lo != nullptr) {
+      *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>((const T*)a.o_lo + (y - (const T*)a.o.p) + c);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
+    }
   }
   // all 16 lanes of the group are here; the mask names them alone, so that groups behind the last row may be gone
   const unsigned mask = 0xffffu << (threadIdx.x & 16);
@@ -255,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
     for (int q0 = 0; q0 < a.nq; q0 += kT) {
       if (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) <= k0) continue;
       if (kd != nullptr) {
-        const int2 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+        const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
         if (x.y < y.x || y.y < x.x) continue;
       }
       __syncthreads();
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   for (int k0 = 0; k0 < last; k0 += kT) {
     if (kd != nullptr) {
-      const int2 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
       if (x.y < y.x || y.y < x.x) continue;
     }
     float s[4][4] = {}, dp[4][4] = {};

@@ -1,0 +1,318 @@
+// What the tensor-core attention kernels share: tensor maps, tcgen05 wrappers, the walk over key tiles, the scores.
+//
+// Operands reach shared memory as tiles of 128 rows by TMA, in blocks of 64 columns (128-byte rows, 128-byte swizzle; head
+// dimensions are filled up to 64 or 128 with zeros by the copy itself).  Such a tile serves tcgen05.mma in two ways:
+// K-major, where the product runs along d (scores), and MN-major, where it runs along the rows (weights times rows).  The
+// weights are the A operand of the second kind and never leave tensor memory: a thread owns one row (TMEM lane) of a score
+// tile, reads it, and writes the 16-bit weights back over it.
+//
+// Heads that share a key head are packed into the rows of one tile where their number is a power of two: packed row r is
+// query r / pg of head r % pg.  A key tile then meets pg times as many rows, and the triangle of a causal mask is cut in
+// steps pg times as fine.
+//
+// Every wait on a barrier is bounded; when one gives up, the block records a code, stops issuing work, lets its copies
+// land, frees its tensor memory and returns.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "flk_attn.cuh"
+#include "flk_ptx.cuh"
+
+namespace flk {
+namespace attn {
+
+using tc::elect_one;
+using tc::mbar_arrive;
+using tc::mbar_expect_tx;
+using tc::mbar_init;
+using tc::mbar_try_wait;
+using tc::mma_commit;
+using tc::smem_u32;
+using tc::tc_fence_after;
+using tc::tc_fence_before;
+using tc::tmem_alloc;
+using tc::tmem_dealloc;
+using tc::tmem_ld32;
+using tc::tmem_ld_wait_on;
+using tc::tmem_relinquish;
+
+constexpr uint32_t kBlockBytes = kTile * 128;  // 128 rows x 64 columns of 16 bits
+
+// Set by a kernel whose bounded wait gave up (one word per translation unit).
+static __device__ int g_wait_status;
+
+// A waiting warp looks again without sleeping: the other roles of the block wait for what it does next.
+static __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t t0 = tc::timer_lo_ns();
+  for (uint32_t it = 0; it < (1u << 28); ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 15) == 15 && tc::timer_lo_ns() - t0 > 1000000000u) break;
+  }
+  atomicExch(&g_wait_status, 1);
+  return false;
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+
+// Shared-memory matrix descriptors of a 128-byte-swizzled tile (8-row groups of 1024 bytes).
+__device__ __forceinline__ uint64_t desc_base(uint32_t lead_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)(lead_bytes >> 4) << 16;  // MN-major: from one block of 64 columns to the next; K-major: unused
+  d |= (uint64_t)(1024 >> 4) << 32;        // from one group of 8 rows to the next
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;  // SWIZZLE_128B
+  return d;
+}
+__device__ __forceinline__ uint64_t desc_at(uint64_t base, uint32_t addr) { return base | (uint64_t)((addr >> 4) & 0x3FFF); }
+
+template <typename T>
+__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
+  const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// A from tensor memory (16-bit values, two per column), B from shared memory
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// scores: D[128 x 128] = A B^T along DP columns
+template <typename T, int DP>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a, uint32_t b) {
+  const uint64_t base = desc_base(16);
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    const uint32_t off = (ks / 4) * kBlockBytes + (ks % 4) * 32;
+    tc::mma_f16(d_tmem, desc_at(base, a + off), desc_at(base, b + off), instr_desc<T>(kTile, false), ks > 0);
+  }
+}
+// accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B
+template <typename T, int DP>
+__device__ __forceinline__ void issue_weighted(uint32_t d_tmem, uint32_t w_tmem, uint32_t b, bool accumulate) {
+  const uint64_t base = desc_base(kBlockBytes);
+#pragma unroll
+  for (int ks = 0; ks < kTile / 16; ++ks)
+    mma_ts(d_tmem, w_tmem + ks * 8, desc_at(base, b + ks * 2048), instr_desc<T>(DP, true), accumulate || ks > 0);
+}
+
+#define FLK_R32_IN(r)                                                                                                    \
+  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),          \
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),        \
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),        \
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      FLK_R32_IN(r)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What the tensor-core kernels need on top of Args.
+struct TcArgs {
+  Args a;
+  int pg, pg_shift;  // heads packed into the rows of a tile (a power of two), its logarithm
+  int hp, rows;      // hq / pg, nq * pg
+  int blocks;        // row blocks per (sequence, packed head)
+  int splits;        // parts of the key axis
+  float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
+  float* part_lse;   // [split][b][hp][rows], base 2
+  void* o_lo;        // what rounding took from `out` (same type, strides of out), or null
+  const uint32_t* amax;  // largest |dout| as bits, or null
+};
+
+// The tiles of [first, last) that a block has to look at: all of them or, with documents, those whose labels overlap [lo, hi].
+// `tab` has the smallest and largest label of every tile and whether one of its rows has none.  Used by whole warps.
+struct Tile {
+  int at;     // index, -1 behind the last
+  int label;  // the one label of all its rows, -1 where there is no such
+  bool dirty; // it holds rows that nobody may see
+};
+struct TileWalk {
+  const int4* tab;
+  int at, last, lo, hi;
+  uint32_t mask;
+  int4 mine;
+  int base;
+  __device__ __forceinline__ TileWalk(const int4* table, int first, int end, int l, int h)
+      : tab(table), at(first), last(end), lo(l), hi(h), mask(0), mine(make_int4(0, 0, 0, 0)), base(first - 32) {}
+  __device__ __forceinline__ Tile next() {
+    if (tab == nullptr) return Tile{at < last ? at++ : -1, -1, false};
+    while (mask == 0) {
+      base += 32;
+      if (base >= last) return Tile{-1, -1, false};
+      const int t = base + (int)(threadIdx.x & 31);
+      mine = t < last ? __ldg(tab + t) : make_int4(1, 0, 0, 0);
+      mask = __ballot_sync(0xffffffffu, mine.x <= hi && lo <= mine.y && mine.x <= mine.y);
+    }
+    const int b = __ffs(mask) - 1;
+    mask &= mask - 1;
+    const bool dirty = __shfl_sync(0xffffffffu, mine.z, b) != 0;
+    const int x = __shfl_sync(0xffffffffu, mine.x, b), y = __shfl_sync(0xffffffffu, mine.y, b);
+    return Tile{base + b, !dirty && x == y ? x : -1, dirty};
+  }
+};
+// how many tiles such a walk visits
+__device__ __forceinline__ int count_tiles(const int4* tab, int first, int last, int lo, int hi) {
+  if (tab == nullptr) return max(last - first, 0);
+  int n = 0;
+  for (int t0 = first; t0 < last; t0 += 32) {
+    const int t = t0 + (int)(threadIdx.x & 31);
+    const int4 r = t < last ? __ldg(tab + t) : make_int4(1, 0, 0, 0);
+    n += __popc(__ballot_sync(0xffffffffu, r.x <= hi && lo <= r.y && r.x <= r.y));
+  }
+  return n;
+}
+// The loading warp tells the others which tile a step works on through a ring of 16 slots; it is never that many steps ahead
+// of them, its copies having fewer stages.
+constexpr int kSlots = 16;
+__device__ __forceinline__ void put_tile(uint32_t slots, int step, const Tile& t) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(slots + (step % kSlots) * 8), "r"(t.at | (t.dirty ? 1 << 30 : 0)), "r"(t.label) : "memory");
+}
+__device__ __forceinline__ Tile get_tile(uint32_t slots, int step) {
+  int x, y;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(slots + (step % kSlots) * 8) : "memory");
+  return Tile{x & ~(1 << 30), y, (x >> 30 & 1) != 0};
+}
+
+// Writes zeros over the rows of a 128-row operand tile that nobody may see (row index >= end, or label < 0), so that what
+// they hold meets no product.  One warp.
+template <int DP>
+__device__ __forceinline__ void clean_tile(uint32_t tile, int r0, int end, const int* docs) {
+  for (int r = threadIdx.x & 31; r < kTile; r += 32) {
+    if (r0 + r < end && (docs == nullptr || __ldg(docs + r0 + r) >= 0)) continue;
+#pragma unroll
+    for (int b = 0; b < DP / 64; ++b)
+#pragma unroll
+      for (int c = 0; c < 128; c += 16)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + b * kBlockBytes + r * 128 + c), "r"(0) : "memory");
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// Bit c: column c of 32 lies before `stop` and has the label `my` (`labels`: 32 of them, 16-byte aligned, or null)
+__device__ __forceinline__ uint32_t seen_columns(int stop, const int* labels, int my) {
+  uint32_t seen = stop >= 32 ? 0xffffffffu : stop <= 0 ? 0u : (1u << stop) - 1u;
+  if (labels != nullptr) {
+    uint32_t bits = 0;
+#pragma unroll 1
+    for (int c = 0; c < 32; c += 4) {
+      const int4 v = __ldg(reinterpret_cast<const int4*>(labels + c));
+      bits |= ((uint32_t)(v.x == my) | (uint32_t)(v.y == my) << 1 | (uint32_t)(v.z == my) << 2 | (uint32_t)(v.w == my) << 3) << c;
+    }
+    seen &= bits;
+  }
+  return seen;
+}
+// -infinity in the columns whose bit is not set
+__device__ __forceinline__ void hide_columns(uint32_t (&s)[32], uint32_t seen) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %1, 0;\n\t@p mov.b32 %0, 0xff800000;\n\t}" : "+r"(s[c]) : "r"(seen & (1u << c)));
+}
+
+// smallest and largest label of the queries [i0, i1), and whether one of them has none; a whole warp
+struct LabelRange {
+  int lo, hi;
+  bool bad;
+};
+__device__ __forceinline__ LabelRange labels_of(const int* docs, int i0, int i1) {
+  LabelRange r{INT32_MAX, INT32_MIN, false};
+  for (int i = i0 + (int)(threadIdx.x & 31); i < i1; i += 32) {
+    const int id = __ldg(docs + i);
+    if (id >= 0) {
+      r.lo = min(r.lo, id);
+      r.hi = max(r.hi, id);
+    } else {
+      r.bad = true;
+    }
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    r.lo = min(r.lo, __shfl_xor_sync(0xffffffffu, r.lo, o));
+    r.hi = max(r.hi, __shfl_xor_sync(0xffffffffu, r.hi, o));
+  }
+  r.bad = __any_sync(0xffffffffu, r.bad);
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess) p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// (d, heads, rows, batch), boxes of 64 columns x `heads_box` heads x `rows_box` rows
+inline int make_map(CUtensorMap* m, const Tensor4& t, int dtype, int d, int h, int n, int b, int heads_box, int rows_box) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) return fail(FLK_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)h, (cuuint64_t)n, (cuuint64_t)b};
+  // the stride of a dimension of one entry is never used, but has to be valid
+  const cuuint64_t one = (cuuint64_t)round_up(d * 2, 16);
+  const cuuint64_t strides[3] = {h > 1 ? (cuuint64_t)t.sh * 2 : one, n > 1 ? (cuuint64_t)t.sn * 2 : one, b > 1 ? (cuuint64_t)t.sb * 2 : one};
+  const cuuint32_t box[4] = {64, (cuuint32_t)heads_box, (cuuint32_t)rows_box, 1}, unit[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, dtype == FLK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.p, dims, strides, box,
+                        unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FLK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FLK_OK;
+}
+
+// The status word of this translation unit's kernels; waits for the stream.
+static int read_wait_status(cudaStream_t st, int* out) {
+  FLK_CUDA_TRY(cudaMemcpyFromSymbolAsync(out, g_wait_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  FLK_CUDA_TRY(cudaStreamSynchronize(st));
+  return FLK_OK;
+}
+
+}  // namespace attn
+}  // namespace flk

@@ -40,31 +40,34 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _fill(q, k, v, out, lse, opts, grads=(None, None, None, None)):
+def _fill(q, k, v, out, out_lo, lse, opts, grads=(None, None, None, None)):
     scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs, flags = opts
     b, nq, hq, d = q.shape
     return _lib.AttentionArgs(
         _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, 1 if causal else 0, flags, scale, softcap,
-        _t4(q), _t4(k), _t4(v), _t4(out), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens), _ptr(q_starts),
+        _t4(q), _t4(k), _t4(v), _t4(out), _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens), _ptr(q_starts),
         _ptr(q_docs), 0 if q_docs is None else q_docs.stride(0), _ptr(k_docs), 0 if k_docs is None else k_docs.stride(0),
         *(_t4(g) for g in grads), None, 0)
 
 
-def _forward(q, k, v, opts, with_lse):
+def _forward(q, k, v, opts, with_lse, with_lo=False):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out_lo = torch.empty_like(out) if with_lo and q.dtype != torch.float32 else None
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if with_lse else None
-    args = _fill(q, k, v, out, lse, opts)
+    args = _fill(q, k, v, out, out_lo, lse, opts)
     _lib.call_struct("attention_forward", args, q.device, "flk_attention_workspace_bytes", 0)
-    return out, lse
+    return out, out_lo, lse
 
 
 class AttentionFn(torch.autograd.Function):
-    """``attention`` with a backward pass for q, k and v (the log-sum-exp that it also returns passes no gradient)."""
+    """``attention`` with a backward pass for q, k and v (the log-sum-exp that it also returns passes no gradient).  With
+    16-bit data it also keeps what rounding took from ``out``, as large as ``out``: the backward pass subtracts
+    ``dout . out`` from every weight's gradient, and the rounding would be the largest error of dq and dk."""
 
     @staticmethod
     def forward(ctx, q, k, v, opts):
-        out, lse = _forward(q, k, v, opts, True)
-        ctx.save_for_backward(q, k, v, out, lse, *(t for t in opts if isinstance(t, torch.Tensor)))
+        out, out_lo, lse = _forward(q, k, v, opts, True, True)
+        ctx.save_for_backward(q, k, v, out, out_lo, lse, *(t for t in opts if isinstance(t, torch.Tensor)))
         ctx.opts = tuple(None if isinstance(t, torch.Tensor) else t for t in opts)
         ctx.held = tuple(isinstance(t, torch.Tensor) for t in opts)
         ctx.mark_non_differentiable(lse)
@@ -73,7 +76,7 @@ class AttentionFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, out, lse, *kept = ctx.saved_tensors
+        q, k, v, out, out_lo, lse, *kept = ctx.saved_tensors
         kept = iter(kept)
         opts = tuple(next(kept) if held else t for t, held in zip(ctx.opts, ctx.held))
         need_q, need_k, need_v, _ = ctx.needs_input_grad
@@ -83,7 +86,7 @@ class AttentionFn(torch.autograd.Function):
             dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
             dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         dout = _strided(dout)
-        args = _fill(q, k, v, out, lse, opts, (dout, dq, dk, dv))
+        args = _fill(q, k, v, out, out_lo, lse, opts, (dout, dq, dk, dv))
         _lib.call_struct("attention_backward", args, q.device, "flk_attention_workspace_bytes", 1)
         return dq, dk if need_k else None, dv if need_v else None, None
 
@@ -197,7 +200,7 @@ def attention(
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = AttentionFn.apply(q, k, v, opts)
     else:
-        out, lse = _forward(q, k, v, opts, return_lse)
+        out, _, lse = _forward(q, k, v, opts, return_lse)
     if pad:
         out = out[..., :d]
     return (out, lse) if return_lse else out

@@ -275,6 +275,8 @@ int flk_kgrad(int dtype, int kernel,
  * v, out, lse and dout and writes dq, dk, dv (dk and dv are given together; dq.data or both may be NULL).  Sums run in
  * an order fixed by the sizes: results are the same from run to run.  The workspace query takes the same struct
  * (pointers other than the documents' are not looked at).
+ * out_lo (16-bit types; strides of out; may be NULL): forward stores there what rounding took from out, and backward,
+ * which needs dout_i . out_i, adds it back; without it that sum carries the rounding of out into dq and dk.
  */
 typedef struct flk_tensor4 {
   void* data;
@@ -285,6 +287,7 @@ typedef struct flk_attention_args {
   int64_t dtype, batch, nq, nk, hq, hk, d, causal, flags;
   double scale, softcap;
   flk_tensor4 q, k, v, out;
+  void* out_lo;
   float* lse;
   const float* slopes;
   const int32_t *prefix_lens, *kv_lens, *q_starts;
@@ -300,6 +303,10 @@ typedef struct flk_attention_args {
 int64_t flk_attention_workspace_bytes(const flk_attention_args* args, int backward);
 int flk_attention_forward(const flk_attention_args* args, void* stream);
 int flk_attention_backward(const flk_attention_args* args, void* stream);
+
+/* 0, or 1 when a bounded wait of a tensor-core attention kernel has given up on the current device since the library was
+ * loaded (the results of that call are not valid).  Synchronises the stream. */
+int flk_attention_status(void* stream, int* status_out);
 
 /*
  * Layer norm of rows (no counterpart in the reference):
