@@ -1,5 +1,6 @@
 // extern "C" entry points of attention: argument checks, workspace, choice of kernel.
 #include "flk_attn.cuh"
+#include "flk_attn_bwd.cuh"
 #include "flk_attn_fwd.cuh"
 #include "flk_attn_simt.cuh"
 
@@ -10,32 +11,39 @@ int forward_bf16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
 int forward_f16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
 int forward_status_bf16(cudaStream_t st, int* out);
 int forward_status_f16(cudaStream_t st, int* out);
+int backward_bf16(const TcArgs& t, const bwd::Plan& p, cudaStream_t st);
+int backward_f16(const TcArgs& t, const bwd::Plan& p, cudaStream_t st);
+int backward_status_bf16(cudaStream_t st, int* out);
+int backward_status_f16(cudaStream_t st, int* out);
 
-// The tables of documents: labels padded to whole tiles, -1 (keys) / -2 (queries) where nothing may be seen, and the
-// smallest and largest label of each tile (an empty tile: a range that meets no other).  One warp per tile.
-__global__ void __launch_bounds__(128) documents_kernel(const int* docs, int64_t sb, int n, const int* lens, int none, int n_pad,
+// The tables of documents: labels padded to whole tiles, `none` (-1 for keys, -2 for queries) where nothing may be seen, and,
+// for every tile of `per` rows (a power of two up to 128), the smallest and largest label and whether a row has none (a tile
+// of none: a range that meets no other).  One warp per 128 rows.
+__global__ void __launch_bounds__(128) documents_kernel(const int* docs, int64_t sb, int n, const int* lens, int none, int n_pad, int per,
                                                         int* out, int4* tab) {
-  const int b = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (tile * kTile >= n_pad) return;
+  const int b = blockIdx.y, r0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * kTile, lane = threadIdx.x & 31;
+  if (r0 >= n_pad) return;
   const int len = lens != nullptr ? min(max(lens[b], 0), n) : n;
-  int lo = INT32_MAX, hi = INT32_MIN, bad = 0;
-  for (int r = lane; r < kTile; r += 32) {
-    const int i = tile * kTile + r;
-    const int id = i < len ? docs[b * sb + i] : -1;
-    if (id >= 0) {
-      lo = min(lo, id);
-      hi = max(hi, id);
-    } else {
-      bad = 1;
+  for (int t = 0; t < kTile; t += per) {
+    int lo = INT32_MAX, hi = INT32_MIN, bad = 0;
+    for (int r = lane; r < per; r += 32) {
+      const int i = r0 + t + r;
+      const int id = i < len ? docs[b * sb + i] : -1;
+      if (id >= 0) {
+        lo = min(lo, id);
+        hi = max(hi, id);
+      } else {
+        bad = 1;
+      }
+      out[(int64_t)b * n_pad + i] = id >= 0 ? id : none;
     }
-    out[(int64_t)b * n_pad + i] = id >= 0 ? id : none;
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) tab[(int64_t)b * (n_pad / per) + (r0 + t) / per] = make_int4(lo, hi, bad, 0);
   }
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  bad = __any_sync(0xffffffffu, bad);
-  if (lane == 0) tab[(int64_t)b * (n_pad / kTile) + tile] = make_int4(lo, hi, bad, 0);
 }
 
 static int esize_of(int64_t dtype) { return dtype == FLK_F32 ? 4 : 2; }
@@ -78,8 +86,14 @@ static fwd::Plan forward_plan(const flk_attention_args* p) {
   return fwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk);
 }
 
+static bwd::Plan backward_plan(const flk_attention_args* p) {
+  return bwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk);
+}
+// Queries of a tile of the documents' table: those of a tile of 128 packed rows.
+static int query_rows(const flk_attention_args* p) { return on_tensor_cores(p) ? kTile / forward_plan(p).pg : kTile; }
+
 struct Workspace {
-  int64_t qdocs, kdocs, qtab, ktab, delta, part_o, part_lse, total;
+  int64_t qdocs, kdocs, qtab, ktab, delta, amax, part_o, part_lse, total;
 };
 static int64_t pad_rows(int64_t n) { return round_up(n, kTile); }
 static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
@@ -93,10 +107,14 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
   if (p->q_documents != nullptr) {
     w.qdocs = take(p->batch * pad_rows(p->nq) * 4);
     w.kdocs = take(p->batch * pad_rows(p->nk) * 4);
-    w.qtab = take(p->batch * pad_rows(p->nq) / kTile * 16);
+    w.qtab = take(p->batch * pad_rows(p->nq) / query_rows(p) * 16);
     w.ktab = take(p->batch * pad_rows(p->nk) / kTile * 16);
   }
-  if (backward) w.delta = take(p->batch * p->hq * p->nq * 4);
+  if (backward) {
+    w.delta = take(p->batch * p->hq * p->nq * 4);
+    w.amax = take(8);
+    if (on_tensor_cores(p)) w.part_o = take(bwd::partial_floats(backward_plan(p), p->batch, p->nk, p->hk, p->d) * 4);
+  }
   if (!backward && on_tensor_cores(p) && p->batch > 0 && p->nq > 0) {
     const int64_t rows = fwd::partial_rows(forward_plan(p), (int)p->batch);
     w.part_o = take(rows * p->d * 4);
@@ -121,7 +139,7 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
   a.scale = (float)(p->softcap > 0 ? p->scale / p->softcap : p->scale * 1.4426950408889634);
   a.cap2 = (float)(p->softcap * 1.4426950408889634);
   a.slopes = p->slopes, a.prefix = p->prefix_lens, a.kv_lens = p->kv_lens, a.q_starts = p->q_starts;
-  a.nq_pad = (int)pad_rows(p->nq), a.nk_pad = (int)pad_rows(p->nk);
+  a.q_rows = query_rows(p), a.nq_pad = (int)pad_rows(p->nq), a.nk_pad = (int)pad_rows(p->nk);
   a.q = tensor_of(p->q), a.k = tensor_of(p->k), a.v = tensor_of(p->v), a.o = tensor_of(p->out);
   a.lse = p->lse, a.o_lo = p->dtype == FLK_F32 ? nullptr : p->out_lo;
   if (backward) {
@@ -134,12 +152,12 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
     a.qdocs = qd, a.kdocs = kd, a.qtab = qt, a.ktab = kt;
     if (p->nq > 0) {
       documents_kernel<<<dim3((unsigned)ceil_div(a.nq_pad / kTile, 4), a.b), 128, 0, st>>>(
-          p->q_documents, p->q_documents_stride, a.nq, nullptr, -2, a.nq_pad, qd, qt);
+          p->q_documents, p->q_documents_stride, a.nq, nullptr, -2, a.nq_pad, a.q_rows, qd, qt);
       count_launch();
     }
     if (p->nk > 0) {
       documents_kernel<<<dim3((unsigned)ceil_div(a.nk_pad / kTile, 4), a.b), 128, 0, st>>>(
-          p->k_documents, p->k_documents_stride, a.nk, p->kv_lens, -1, a.nk_pad, kd, kt);
+          p->k_documents, p->k_documents_stride, a.nk, p->kv_lens, -1, a.nk_pad, kTile, kd, kt);
       count_launch();
     }
   }
@@ -153,10 +171,24 @@ static int simt_forward(const Args& a, cudaStream_t st) {
 template <typename T>
 static int simt_backward(const Args& a, cudaStream_t st) {
   if (a.nq > 0) {
-    simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a);
+    simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a, nullptr);
     count_launch();
   }
   return a.d <= 64 ? simt::launch_backward<T, 64>(a, st) : simt::launch_backward<T, 128>(a, st);
+}
+
+// delta, and for fp16 the largest magnitudes that the scale of dS is taken from
+template <typename T>
+static int prepare_backward(const Args& a, uint32_t* amax, cudaStream_t st) {
+  if (amax != nullptr) {
+    FLK_CUDA_TRY(cudaMemsetAsync(amax, 0, 8, st));
+    const int64_t packs = (int64_t)a.b * a.nk * a.hk * a.d / 8, blocks = ceil_div(packs, 256 * 8);
+    simt::largest_value_kernel<T><<<(unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 256, 0, st>>>(a, amax + 1);
+    count_launch();
+  }
+  simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a, amax);
+  count_launch();
+  return FLK_OK;
 }
 
 }  // namespace attn
@@ -202,10 +234,12 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
 int flk_attention_status(void* stream, int* out) {
   if (out == nullptr) return fail(FLK_ERR_BAD_ARG, "status_out: null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  int x = 0, y = 0;
-  FLK_TRY(attn::forward_status_bf16(st, &x));
-  FLK_TRY(attn::forward_status_f16(st, &y));
-  *out = x | y;
+  int x[4] = {0, 0, 0, 0};
+  FLK_TRY(attn::forward_status_bf16(st, &x[0]));
+  FLK_TRY(attn::forward_status_f16(st, &x[1]));
+  FLK_TRY(attn::backward_status_bf16(st, &x[2]));
+  FLK_TRY(attn::backward_status_f16(st, &x[3]));
+  *out = x[0] | x[1] | x[2] | x[3];
   return FLK_OK;
 }
 
@@ -232,7 +266,23 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
   FLK_TRY(attn::make_args(p, true, a, st));
   if (a.nq == 0) a.dq.p = nullptr;
   if (a.nk == 0) a.dk.p = a.dv.p = nullptr;
-  if (p->dtype == FLK_F32) FLK_TRY(attn::simt_backward<float>(a, st));
+  if (attn::on_tensor_cores(p) && a.nq > 0) {
+    attn::TcArgs t{};
+    t.a = a;
+    const attn::Workspace w = attn::plan_workspace(p, true);
+    char* ws = reinterpret_cast<char*>(p->workspace);
+    t.part_o = reinterpret_cast<float*>(ws + w.part_o);
+    const attn::bwd::Plan plan = attn::backward_plan(p);
+    if (p->dtype == FLK_BF16) {
+      FLK_TRY(attn::prepare_backward<__nv_bfloat16>(a, nullptr, st));
+      FLK_TRY(attn::backward_bf16(t, plan, st));
+    } else {
+      uint32_t* amax = reinterpret_cast<uint32_t*>(ws + w.amax);
+      t.amax = amax;
+      FLK_TRY(attn::prepare_backward<__half>(a, amax, st));
+      FLK_TRY(attn::backward_f16(t, plan, st));
+    }
+  } else if (p->dtype == FLK_F32) FLK_TRY(attn::simt_backward<float>(a, st));
   else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_backward<__nv_bfloat16>(a, st));
   else FLK_TRY(attn::simt_backward<__half>(a, st));
   FLK_CUDA_TRY(cudaGetLastError());

@@ -33,7 +33,8 @@ struct Args {
   const float* slopes;  // per query head, or null
   const int *prefix, *kv_lens, *q_starts;
   const int *qdocs, *kdocs;  // padded tables of the workspace ([b][nq_pad], [b][nk_pad]; -2 / -1 where nothing is seen), or null
-  const int4 *qtab, *ktab;   // of every tile of 128: smallest, largest label, whether a row has none ([b][nq_pad / 128], ...)
+  const int4 *qtab, *ktab;   // of every tile: smallest, largest label, whether a row has none ([b][nq_pad / q_rows], [b][nk_pad / 128])
+  int q_rows;                // queries of a tile of qtab
   int nq_pad, nk_pad;
   Tensor4 q, k, v, o, dout, dq, dk, dv;
   void* o_lo;    // what rounding took from `o` (16-bit types; strides of o), or null

@@ -1,0 +1,851 @@
+// Backward attention on tcgen05: two kernels, one for dK and dV, one for dQ.  No atomics: every gradient is summed by one block
+// in a fixed order (or by a few, whose fp32 partial results a last kernel adds in order).  Forming the weights twice costs two
+// of seven products; adding dQ up over the blocks of all key tiles instead would cost atomics on fp32, and results that depend
+// on their order.
+//
+//   keys kernel     a block owns 128 keys and walks over the query tiles:  S^T = K Q^T, dP^T = V dO^T  (rows are keys),
+//                   P = exp2(S - lse), dV += P^T dO, dS = P (dP - delta), dK += dS^T Q.
+//                   Tensor memory: S, dP, dV, dK, 128 columns each.  P and dS replace the scores they were made from.
+//                   The tensor cores run dV(i), S(i+1) while dS(i) is being made and dK(i), dP(i+1) while P(i+1) is.
+//   queries kernel  a block owns 128 packed query rows and walks over the key tiles:  S = Q K^T (two buffers), dP = dO V^T,
+//                   dQ += dS K.
+// Both have 12 warps: two warpgroups that turn scores into weights (a thread owns one row and half of the columns), a warp that
+// issues products, one that issues copies, and in the keys kernel one that gathers what the columns need (lse, delta, ...).
+//
+// P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass.  In fp16 they would
+// leave its range: weights are held times 2^12, and dS times a power of two that 2 d max|dO| max|V|, a bound of every
+// |dP - delta|, takes to at most 2^15.
+#pragma once
+
+#include "flk_attn_tc.cuh"
+
+namespace flk {
+namespace attn {
+namespace bwd {
+
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kStatWarp = 10;
+// registers of the two working warpgroups, and of the third; the block is launched with 384 x 168
+template <bool KEYS>
+struct Regs {
+  static constexpr int kWork = KEYS ? 216 : 208, kOther = KEYS ? 72 : 88;
+  static_assert(2 * 128 * kWork + 128 * kOther <= kThreads * 168, "registers");
+};
+
+// what the columns (queries) of a tile bring into the keys kernel
+enum { kLse = 0, kDelta = 128, kSlope = 256, kPos = 384, kEnd = 512, kLabel = 640, kStatWords = 768 };
+constexpr int kStatSlots = 4;
+
+template <int DP, bool KEYS>
+struct Layout {
+  static constexpr uint32_t kTileBytes = DP / 64 * kBlockBytes;
+  static constexpr uint32_t kOwn = 0;  // K, V (keys kernel) or Q, dO
+  static constexpr uint32_t kRing = 2 * kTileBytes;
+  static constexpr uint32_t kStats = KEYS ? kStatSlots * kStatWords * 4 : 0;
+  static constexpr int kFit = (int)((224 * 1024 - kRing - kStats) / kTileBytes);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr uint32_t kStatAt = kRing + kStages * kTileBytes;
+  static constexpr uint32_t kBars = kStatAt + kStats;
+  static constexpr uint32_t kBytes = kBars + 512 + 1024;
+};
+static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
+static_assert(Layout<128, true>::kStages >= 4 && Layout<128, false>::kStages >= 5, "stages");
+
+// Factors of the data's type: weights are exp2(s - lse + kWeightShift)
+template <typename T>
+struct Scales {
+  static constexpr bool kHalf = !std::is_same<T, __nv_bfloat16>::value;
+  static constexpr float kShift = kHalf ? 12.f : 0.f;
+  static constexpr float kUnshift = kHalf ? 1.f / 4096.f : 1.f;
+  // what the weights of the keys kernel carry and dS is not to: 2^shift, and the quarter that the slope of the cap is taken with
+  template <bool CAP>
+  static __device__ __forceinline__ float per_weight() { return kUnshift * (CAP ? 4.f : 1.f); }
+  // the factor that dS is held with, a power of two
+  static __device__ __forceinline__ float ds(const TcArgs& t) {
+    if (!kHalf) return 1.f;
+    const float bound = 2.f * (float)t.a.d * __uint_as_float(t.amax[0]) * __uint_as_float(t.amax[1]);
+    if (!(bound > 0.f && bound < 1e30f)) return 1.f;
+    const int e = (int)(__float_as_uint(bound) >> 23) - 127;  // 2^e <= bound < 2^(e+1)
+    return __uint_as_float((uint32_t)(127 + min(max(14 - e, -100), 100)) << 23);
+  }
+};
+
+// Raw scores -> scores in base 2 of 32 columns, and, with a cap, the slope r (1 - r) = (1 - tanh^2) / 4 of it in `slope`
+template <bool CAP>
+__device__ __forceinline__ float base2(float raw, const Args& a, float f, float& slope) {
+  float x = raw * f;
+  if constexpr (CAP) {
+    const float r = rcp_approx(1.f + ex2_approx(x));
+    slope = fmaf(-r, r, r);
+    x = fmaf(-2.f * a.cap2, r, a.cap2);
+  }
+  return x;
+}
+template <bool CAP>
+__device__ __forceinline__ float base2_factor(const Args& a) { return CAP ? a.scale * (2.f * kLog2e) : a.scale; }
+
+// accumulator half (DP / 2 columns from c0) times f -> a row of 16-bit values, or of fp32 partial results
+template <typename T, int DP>
+__device__ __forceinline__ void store_half(uint32_t acc, int c0, float f, bool exists, bool zero, int d, T* row, float* part) {
+#pragma unroll
+  for (int c = 0; c < DP / 2; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(acc + c0 + c, o);
+    tmem_ld_wait_on(o);
+    if (exists) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        const int col = c0 + c + e;
+        if (col < d) {
+          if (part != nullptr) {
+            *reinterpret_cast<uint4*>(part + col) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            *reinterpret_cast<uint4*>(part + col + 4) = make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+          } else {
+            uint32_t v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = pack16<T>(__uint_as_float(o[e + 2 * q]), __uint_as_float(o[e + 2 * q + 1]));
+            *reinterpret_cast<uint4*>(row + col) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void store_zeros(int c0, bool exists, int d, T* row, float* part) {
+  if (!exists) return;
+  for (int c = c0; c < c0 + DP / 2 && c < d; c += 8) {
+    if (part != nullptr)
+      *reinterpret_cast<uint4*>(part + c) = *reinterpret_cast<uint4*>(part + c + 4) = make_uint4(0, 0, 0, 0);
+    else
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// The steps of the keys kernel: query tiles of each packed head in turn, from step `skip` on.
+struct StepWalk {
+  const int4* tab;
+  int first, last, lo, hi, head;
+  TileWalk walk;
+  __device__ __forceinline__ StepWalk(const int4* table, int f, int l, int a, int b, int per_head, int skip)
+      : tab(table), first(f), last(l), lo(a), hi(b), head(per_head > 0 ? skip / per_head : 0), walk(table, f, l, a, b) {
+    int rest = per_head > 0 ? skip % per_head : 0;
+    if (tab == nullptr)
+      walk.at += rest;
+    else
+      for (; rest > 0; --rest) walk.next();
+  }
+  __device__ __forceinline__ Tile next() {
+    Tile t = walk.next();
+    if (t.at < 0) {
+      ++head;
+      walk = TileWalk(tab, first, last, lo, hi);
+      t = walk.next();
+    }
+    return t;
+  }
+};
+
+struct Maps {
+  CUtensorMap q, dout, k, v;
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dK, dV
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant__ Maps maps, const TcArgs t) {
+  using L = Layout<DP, true>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t raw[];
+  const Args& a = t.a;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, bars = base + L::kBars;
+  auto full = [&](int s) { return bars + s * 8; };
+  auto empty = [&](int s) { return bars + 64 + s * 8; };
+  const uint32_t own = bars + 128, sfull = bars + 136, pfull = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176;
+  auto statfull = [&](int s) { return bars + 192 + s * 8; };
+  auto statempty = [&](int s) { return bars + 224 + s * 8; };
+  const uint32_t slots = bars + 256;
+  const int warp = threadIdx.x >> 5;
+
+  int64_t id = blockIdx.x;
+  const int hk = (int)(id % a.hk);
+  id /= a.hk;
+  const int b = (int)(id % a.b);
+  id /= a.b;
+  const int split = (int)(id % t.splits), k0 = (int)(id / t.splits) * kTile;
+  const Limits lim = limits_of(a, b);
+  const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
+  const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
+  const int4* qtab = qd ? a.qtab + (int64_t)b * (a.nq_pad / a.q_rows) : nullptr;
+  // query tiles that may see one of these keys
+  int first = 0, last = (t.rows + kTile - 1) / kTile;
+  if (k0 >= lim.len) last = 0;
+  if (a.causal && lim.prefix <= k0) {
+    const int64_t i = (int64_t)k0 - lim.start;  // the first query that stands at key k0 or behind it
+    first = i <= 0 ? 0 : i >= a.nq ? last : (int)((i << t.pg_shift) / kTile);
+  }
+  LabelRange lab{0, 0, false};
+  if (kd) lab = labels_of(kd, k0, k0 + kTile);
+  const int heads = a.grp >> t.pg_shift;
+  const int per_head = count_tiles(qtab, first, last, lab.lo, lab.hi);
+  const int64_t total = (int64_t)per_head * heads;
+  const int skip = (int)(total * split / t.splits), steps = (int)(total * (split + 1) / t.splits) - skip;
+
+  if (warp == kMmaWarp) {
+    if (elect_one()) {
+      for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+      mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 8), mbar_init(dpfull, 1), mbar_init(dsfull, 8), mbar_init(done, 1);
+      for (int s = 0; s < kStatSlots; ++s) mbar_init(statfull(s), 1), mbar_init(statempty(s), 8);
+      tc::fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+  const uint32_t ts = tmem, tp = tmem + 128, tdv = tmem + 256, tdk = tmem + 256 + DP;
+
+  if (warp >= 8) {
+    tc::reg_release<Regs<true>::kOther>();
+    if (warp == kLoadWarp) {
+      bool ok = true;
+      if (steps > 0 && elect_one()) {
+        mbar_expect_tx(own, 2 * L::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          tma_load(base + c * kBlockBytes, &maps.k, c * 64, hk, k0, b, own);
+          tma_load(base + L::kTileBytes + c * kBlockBytes, &maps.v, c * 64, hk, k0, b, own);
+        }
+      }
+      __syncwarp();
+      StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
+      int n = 0;
+      for (int step = 0; step < steps && ok; ++step) {
+        const Tile e = walk.next();
+        const int h = hk * a.grp + walk.head * t.pg;
+#pragma unroll
+        for (int qo = 0; qo < 2; ++qo) {
+          const int s = n % kStages;
+          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (!ok) break;
+          if (elect_one()) {
+            if (qo == 0) put_tile(slots, step, e);
+            mbar_expect_tx(full(s), L::kTileBytes);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+              tma_load(base + L::kRing + s * L::kTileBytes + c * kBlockBytes, qo == 0 ? &maps.q : &maps.dout, c * 64, h, (e.at * kTile) >> t.pg_shift, b, full(s));
+          }
+          __syncwarp();
+          ++n;
+        }
+      }
+      if (steps > 0) wait_bar(own, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+    } else if (warp == kStatWarp) {
+      bool ok = true;
+      StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
+      const float g = Scales<T>::ds(t) * Scales<T>::template per_weight<CAP>();
+      for (int step = 0; step < steps && ok; ++step) {
+        const Tile e = walk.next();
+        const int slot = step % kStatSlots;
+        if (step >= kStatSlots) ok = wait_bar(statempty(slot), (uint32_t)(step / kStatSlots - 1) & 1);
+        if (!ok) break;
+        const uint32_t at = base + L::kStatAt + slot * kStatWords * 4;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int c = (threadIdx.x & 31) + 32 * x, r = e.at * kTile + c, i = r >> t.pg_shift;
+          const int h = hk * a.grp + walk.head * t.pg + (r & (t.pg - 1));
+          float lse = -INFINITY, delta = 0.f;
+          int end = 0, label = -2;
+          if (r < t.rows) {
+            const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
+            lse = a.lse[row];
+            delta = a.delta[row];
+            end = lim.row_end(i, a.causal);
+            if (qd) label = qd[i];
+          }
+          // rows that see nothing: weights exp2(s - inf) = 0, and no delta, which may be NaN there
+          const bool none = lse == -INFINITY;
+          auto put = [&](int word, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + (word + c) * 4), "r"(v) : "memory"); };
+          put(kLse, __float_as_uint(none ? -INFINITY : fmaf(-lse, kLog2e, Scales<T>::kShift)));  // added to the score
+          put(kDelta, __float_as_uint(none ? 0.f : -delta * g));
+          if constexpr (BIAS) {
+            put(kSlope, __float_as_uint(a.slopes == nullptr ? 0.f : -a.slopes[h] * kLog2e));
+            put(kPos, __float_as_uint((float)(lim.start + i - k0)));
+          }
+          put(kEnd, (uint32_t)(end - k0));
+          put(kLabel, (uint32_t)label);
+        }
+        __syncwarp();
+        if (elect_one()) mbar_arrive(statfull(slot));
+        __syncwarp();
+      }
+    } else if (warp == kMmaWarp) {
+      bool ok = steps == 0 || wait_bar(own, 0);
+      auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
+      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      // queries without a label may hold anything; their weights are zero, and they must be
+      auto arrived = [&](int n) {
+        if (!ready(n)) return false;
+        if (qd != nullptr) {
+          const Tile e = get_tile(slots, n / 2);
+          if (e.dirty) {
+            // packed row r is query r >> pg_shift
+            const int lane = threadIdx.x & 31;
+            for (int r = lane; r < kTile; r += 32) {
+              const int i = (e.at * kTile + r) >> t.pg_shift;
+              if (i < a.nq && __ldg(qd + i) >= 0) continue;
+#pragma unroll
+              for (int blk = 0; blk < DP / 64; ++blk)
+#pragma unroll
+                for (int c = 0; c < 128; c += 16)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage(n) + blk * kBlockBytes + r * 128 + c), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+        return true;
+      };
+      if (steps > 0 && ok) {
+        ok = arrived(0);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          issue_scores<T, DP>(ts, base, stage(0));
+          mma_commit(sfull);
+        }
+        __syncwarp();
+        ok = ok && arrived(1);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          issue_scores<T, DP>(tp, base + L::kTileBytes, stage(1));
+          mma_commit(dpfull);
+        }
+        __syncwarp();
+      }
+      for (int i = 0; i < steps && ok; ++i) {
+        const bool more = i + 1 < steps;
+        ok = wait_bar(pfull, (uint32_t)i & 1);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          issue_weighted<T, DP, true>(tdv, ts, stage(2 * i + 1), i > 0);
+          mma_commit(empty((2 * i + 1) % kStages));
+        }
+        __syncwarp();
+        if (more) {
+          ok = ok && arrived(2 * i + 2);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            issue_scores<T, DP>(ts, base, stage(2 * i + 2));
+            mma_commit(sfull);
+          }
+          __syncwarp();
+        }
+        ok = ok && wait_bar(dsfull, (uint32_t)i & 1);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          issue_weighted<T, DP, true>(tdk, tp, stage(2 * i), i > 0);
+          mma_commit(empty((2 * i) % kStages));
+        }
+        __syncwarp();
+        if (more) {
+          ok = ok && arrived(2 * i + 3);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            issue_scores<T, DP>(tp, base + L::kTileBytes, stage(2 * i + 3));
+            mma_commit(dpfull);
+          }
+          __syncwarp();
+        }
+      }
+      if (steps > 0 && ok) {
+        if (elect_one()) mma_commit(done);
+        __syncwarp();
+        wait_bar(done, 0);
+      }
+    }
+  } else {
+    tc::reg_claim<Regs<true>::kWork>();
+    const int w = warp >> 2;
+    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, half = 64 * w;
+    const int key = k0 + (int)(threadIdx.x & 127);
+    const float mine = (float)(threadIdx.x & 127);  // key - k0
+    const int my = kd ? kd[key] : 0;
+    int only = -1;
+    if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
+    const float f = base2_factor<CAP>(a);
+    const float gs = Scales<T>::ds(t), g = gs * Scales<T>::template per_weight<CAP>();
+    bool ok = true;
+    for (int i = 0; i < steps && ok; ++i) {
+      const int slot = i % kStatSlots;
+      const uint32_t st = base + L::kStatAt + slot * kStatWords * 4 + half * 4;
+      ok = wait_bar(statfull(slot), (uint32_t)(i / kStatSlots) & 1);
+      ok = ok && wait_bar(sfull, (uint32_t)i & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const Tile e = get_tile(slots, i);
+      const bool whole = k0 + kTile <= lim.row_end((e.at * kTile) >> t.pg_shift, a.causal) && (kd == nullptr || (e.label >= 0 && e.label == only));
+      uint32_t s[2][32];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld32(ts + lane_at + half + 32 * p, s[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const uint32_t at = st + (32 * p + c) * 4;
+          float x[4], add[4], slope[4];
+          tc::ld_shared_f4(at + kLse * 4, add[0], add[1], add[2], add[3]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) slope[q] = 1.f;
+          if constexpr (!CAP && !BIAS) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[p][c + q]), f, add[q]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = base2<CAP>(__uint_as_float(s[p][c + q]), a, f, slope[q]);
+            if constexpr (BIAS) {
+              float sl[4], ps[4];
+              tc::ld_shared_f4(at + kSlope * 4, sl[0], sl[1], sl[2], sl[3]);
+              tc::ld_shared_f4(at + kPos * 4, ps[0], ps[1], ps[2], ps[3]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) x[q] = fmaf(sl[q], fabsf(ps[q] - mine), x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] += add[q];
+          }
+          if (!whole) {
+            int en[4], lb[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(at + kEnd * 4) : "memory");
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(lb[0]), "=r"(lb[1]), "=r"(lb[2]), "=r"(lb[3]) : "r"(at + kLabel * 4) : "memory");
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (key - k0 >= en[q] || (kd != nullptr && lb[q] != my)) x[q] = -INFINITY;
+          }
+          float pr[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            pr[q] = ex2_approx(x[q]);
+            s[p][c + q] = __float_as_uint(CAP ? pr[q] * slope[q] : pr[q]);
+          }
+          o[c / 2] = pack16<T>(pr[0], pr[1]);
+          o[c / 2 + 1] = pack16<T>(pr[2], pr[3]);
+        }
+        tmem_st16(ts + lane_at + half + 16 * p, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (elect_one()) mbar_arrive(pfull);
+      __syncwarp();
+      ok = wait_bar(dpfull, (uint32_t)i & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t d[2][32];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld32(tp + lane_at + half + 32 * p, d[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(d[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          float dl[4], y[4];
+          tc::ld_shared_f4(st + (kDelta + 32 * p + c) * 4, dl[0], dl[1], dl[2], dl[3]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float pr = __uint_as_float(s[p][c + q]);
+            y[q] = pr * fmaf(__uint_as_float(d[p][c + q]), g, dl[q]);
+          }
+          o[c / 2] = pack16<T>(y[0], y[1]);
+          o[c / 2 + 1] = pack16<T>(y[2], y[3]);
+        }
+        tmem_st16(tp + lane_at + half + 16 * p, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (elect_one()) {
+        mbar_arrive(dsfull);
+        mbar_arrive(statempty(slot));
+      }
+      __syncwarp();
+    }
+    if (steps > 0 && ok) ok = wait_bar(done, 0);
+    tc_fence_after();
+    if (ok) {
+      const bool exists = key < a.nk;
+      const bool zero = key >= lim.len || (kd != nullptr && my < 0);  // keys that nobody sees
+      const int c0 = w * (DP / 2);
+      T* rk = reinterpret_cast<T*>(a.dk.p) + b * a.dk.sb + (int64_t)key * a.dk.sn + hk * a.dk.sh;
+      T* rv = reinterpret_cast<T*>(a.dv.p) + b * a.dv.sb + (int64_t)key * a.dv.sn + hk * a.dv.sh;
+      float *pk = nullptr, *pv = nullptr;
+      if (t.splits > 1) {
+        const int64_t n = (int64_t)a.b * a.nk * a.hk * a.d, at = (((int64_t)b * a.nk + key) * a.hk + hk) * a.d;
+        pk = t.part_o + (int64_t)split * 2 * n + at;
+        pv = pk + n;
+      }
+      if (steps > 0) {
+        store_half<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, exists, zero, a.d, rk, pk);
+        store_half<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, exists, zero, a.d, rv, pv);
+      } else {
+        store_zeros<T, DP>(c0, exists, a.d, rk, pk);
+        store_zeros<T, DP>(c0, exists, a.d, rv, pv);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds the partial results of dK and dV: four values per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const TcArgs t) {
+  const Args& a = t.a;
+  const int64_t n = (int64_t)a.b * a.nk * a.hk * a.d, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  const int c = (int)(at % a.d);
+  const int64_t row = at / a.d;
+  const int hk = (int)(row % a.hk), j = (int)(row / a.hk % a.nk), b = (int)(row / a.hk / a.nk);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < t.splits; ++p) {
+      const float4 v = *reinterpret_cast<const float4*>(t.part_o + ((int64_t)p * 2 + which) * n + at);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const Tensor4& o = which == 0 ? a.dk : a.dv;
+    T* out = reinterpret_cast<T*>(o.p) + b * o.sb + (int64_t)j * o.sn + hk * o.sh + c;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(s.x, s.y), pack16<T>(s.z, s.w));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dQ
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_constant__ Maps maps, const TcArgs t) {
+  using L = Layout<DP, false>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t raw[];
+  const Args& a = t.a;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, bars = base + L::kBars;
+  auto full = [&](int s) { return bars + s * 8; };
+  auto empty = [&](int s) { return bars + 64 + s * 8; };
+  auto sfull = [&](int s) { return bars + 128 + s * 8; };
+  const uint32_t own = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, slots = bars + 256;
+  const int warp = threadIdx.x >> 5;
+
+  int64_t id = blockIdx.x;
+  const int hp = (int)(id % t.hp);
+  id /= t.hp;
+  const int b = (int)(id % a.b);
+  const int row0 = (t.blocks - 1 - (int)(id / a.b)) * kTile, hk = hp * t.pg / a.grp;
+  const int i0 = row0 >> t.pg_shift, i1 = min(a.nq, (row0 + kTile) >> t.pg_shift);
+  const Limits lim = limits_of(a, b);
+  const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
+  const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
+  const int4* ktab = kd ? a.ktab + (int64_t)b * (a.nk_pad / kTile) : nullptr;
+  const int last = (lim.row_end(i1 - 1, a.causal) + kTile - 1) / kTile;
+  LabelRange lab{0, 0, false};
+  if (kd) lab = labels_of(qd, i0, i1);
+  const int steps = count_tiles(ktab, 0, last, lab.lo, lab.hi);
+
+  if (warp == kMmaWarp) {
+    if (elect_one()) {
+      for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+      mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 8), mbar_init(done, 1);
+      tc::fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+  auto ts = [&](int i) { return tmem + (uint32_t)(i & 1) * 128; };
+  const uint32_t tp = tmem + 256, tdq = tmem + 384;
+
+  if (warp >= 8) {
+    tc::reg_release<Regs<false>::kOther>();
+    if (warp == kLoadWarp) {
+      bool ok = true;
+      if (steps > 0 && elect_one()) {
+        mbar_expect_tx(own, 2 * L::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          tma_load(base + c * kBlockBytes, &maps.q, c * 64, hp * t.pg, i0, b, own);
+          tma_load(base + L::kTileBytes + c * kBlockBytes, &maps.dout, c * 64, hp * t.pg, i0, b, own);
+        }
+      }
+      __syncwarp();
+      TileWalk walk(ktab, 0, last, lab.lo, lab.hi);
+      int n = 0;
+      for (int step = 0; step < steps && ok; ++step) {
+        const Tile e = walk.next();
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int s = n % kStages;
+          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (!ok) break;
+          if (elect_one()) {
+            if (kv == 0) put_tile(slots, step, e);
+            mbar_expect_tx(full(s), L::kTileBytes);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+              tma_load(base + L::kRing + s * L::kTileBytes + c * kBlockBytes, kv == 0 ? &maps.k : &maps.v, c * 64, hk, e.at * kTile, b, full(s));
+          }
+          __syncwarp();
+          ++n;
+        }
+      }
+      if (steps > 0) wait_bar(own, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+    } else if (warp == kMmaWarp) {
+      bool ok = steps == 0 || wait_bar(own, 0);
+      auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
+      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      // keys that nobody may see: dQ takes dS K, and their dS is zero, so K has to be finite there
+      auto scores = [&](int i) {
+        if (!ready(2 * i)) return false;
+        const Tile e = get_tile(slots, i);
+        if (e.dirty || (e.at + 1) * kTile > lim.len) clean_tile<DP>(stage(2 * i), e.at * kTile, lim.len, kd);
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<T, DP>(ts(i), base, stage(2 * i));
+          mma_commit(sfull(i & 1));
+        }
+        __syncwarp();
+        return true;
+      };
+      auto products = [&](int i) {
+        if (!ready(2 * i + 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<T, DP>(tp, base + L::kTileBytes, stage(2 * i + 1));
+          mma_commit(dpfull);
+          mma_commit(empty((2 * i + 1) % kStages));
+        }
+        __syncwarp();
+        return true;
+      };
+      if (steps > 0) ok = ok && scores(0) && products(0) && (steps == 1 || scores(1));
+      for (int i = 0; i < steps && ok; ++i) {
+        ok = wait_bar(dsfull, (uint32_t)i & 1);
+        tc_fence_after();
+        if (i + 1 < steps) ok = ok && products(i + 1);
+        if (ok && elect_one()) {
+          issue_weighted<T, DP, true>(tdq, ts(i), stage(2 * i), i > 0);
+          mma_commit(empty((2 * i) % kStages));
+        }
+        __syncwarp();
+        if (i + 2 < steps) ok = ok && scores(i + 2);
+      }
+      if (steps > 0 && ok) {
+        if (elect_one()) mma_commit(done);
+        __syncwarp();
+        wait_bar(done, 0);
+      }
+    }
+  } else {
+    tc::reg_claim<Regs<false>::kWork>();
+    const int w = warp >> 2;
+    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, half = 64 * w;
+    const int r = row0 + (int)(threadIdx.x & 127), i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+    const bool exists = r < t.rows;
+    const int end = exists ? lim.row_end(i, a.causal) : 0;
+    const int my = qd && exists ? qd[i] : -2;
+    const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+    const int pos = lim.start + i;
+    const int all_before = lim.row_end(i0, a.causal);
+    int only = -1;
+    if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
+    const float f = base2_factor<CAP>(a), gs = Scales<T>::ds(t);
+    float add = -INFINITY, nd = 0.f;  // of a row that sees nothing
+    if (exists) {
+      const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
+      const float lse = a.lse[row];
+      if (lse != -INFINITY) {
+        add = -lse * kLog2e;
+        nd = -a.delta[row] * gs * (CAP ? 4.f : 1.f);
+      }
+    }
+    const float g = gs * (CAP ? 4.f : 1.f);
+    bool ok = true;
+    for (int step = 0; step < steps && ok; ++step) {
+      ok = wait_bar(sfull(step & 1), (uint32_t)(step >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const Tile e = get_tile(slots, step);
+      const int k0 = e.at * kTile;
+      const bool whole = k0 + kTile <= all_before && (kd == nullptr || (e.label >= 0 && e.label == only));
+      uint32_t s[2][32];
+      const uint32_t at = ts(step) + lane_at + half;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld32(at + 32 * p, s[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
+      const float d0 = (float)(pos - k0 - (int)half);
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+      if (!whole) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          seen[p] = seen_columns(end - k0 - (int)half - 32 * p, kd == nullptr ? nullptr : kd + k0 + half + 32 * p, my);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          float slope = 1.f, x;
+          if constexpr (!CAP && !BIAS) {
+            x = fmaf(__uint_as_float(s[p][c]), f, add);
+          } else {
+            x = base2<CAP>(__uint_as_float(s[p][c]), a, f, slope);
+            if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
+            x += add;
+          }
+          if (!whole && (seen[p] >> c & 1) == 0) x = -INFINITY;
+          x = ex2_approx(x);
+          s[p][c] = __float_as_uint(CAP ? x * slope : x);
+        }
+      ok = wait_bar(dpfull, (uint32_t)step & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t d[2][32];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld32(tp + lane_at + half + 32 * p, d[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(d[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float y[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            y[q] = __uint_as_float(s[p][c + q]) * fmaf(__uint_as_float(d[p][c + q]), g, nd);
+            // V rows that nobody may see are not cleaned here: their products may be anything
+            if (!whole && (seen[p] >> (c + q) & 1) == 0) y[q] = 0.f;
+          }
+          o[c / 2] = pack16<T>(y[0], y[1]);
+        }
+        tmem_st16(at + 16 * p, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (elect_one()) mbar_arrive(dsfull);
+      __syncwarp();
+    }
+    if (steps > 0 && ok) ok = wait_bar(done, 0);
+    tc_fence_after();
+    if (ok) {
+      T* row = reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.sn + h * a.dq.sh;
+      const int c0 = w * (DP / 2);
+      if (steps > 0)
+        store_half<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, exists, add == -INFINITY, a.d, row, nullptr);
+      else
+        store_zeros<T, DP>(c0, exists, a.d, row, nullptr);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+struct Plan {
+  int pg, pg_shift, hp, rows, q_blocks, splits;
+};
+inline Plan make_plan(int b, int nq, int nk, int hq, int hk) {
+  Plan p{};
+  const int grp = hq / hk;
+  p.pg = (grp & (grp - 1)) == 0 && grp <= 64 ? grp : 1;
+  while ((1 << p.pg_shift) < p.pg) ++p.pg_shift;
+  p.hp = hq / p.pg;
+  p.rows = nq * p.pg;
+  p.q_blocks = (int)ceil_div(p.rows, kTile);
+  // parts of a key tile's query tiles: few key tiles would leave SMs without work.  Blocks per SM, rounded up, times the steps
+  // of a block with 4 steps' time for its start and end and, with parts, the time of writing and adding them
+  const int64_t blocks = ceil_div(nk, kTile) * hk * b, steps = (int64_t)p.q_blocks * (grp / p.pg);
+  p.splits = 1;
+  double best = 1e300;
+  for (int64_t s = 1; s <= 32 && (s == 1 || s * 4 <= steps); ++s) {
+    const double cost = (double)ceil_div(blocks * s, kNumSMs) * ((double)ceil_div(steps, s) + 4 + (s > 1 ? 2 : 0)) + (s > 1 ? 4 + 0.02 * (double)(blocks * s) : 0.0);
+    if (cost < best * 0.97) best = cost, p.splits = (int)s;
+  }
+  return p;
+}
+inline int64_t partial_floats(const Plan& p, int64_t b, int64_t nk, int64_t hk, int64_t d) { return p.splits > 1 ? 2 * p.splits * b * nk * hk * d : 0; }
+
+template <typename T, int DP, bool CAP, bool BIAS>
+inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
+  const Args& a = t.a;
+  if (a.dk.p != nullptr) {
+    auto* fn = kernel_keys<T, DP, CAP, BIAS>;
+    constexpr int kBytes = (int)Layout<DP, true>::kBytes;
+    FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    const int64_t grid = ceil_div(a.nk, kTile) * t.splits * a.b * a.hk;
+    if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many key blocks");
+    fn<<<(unsigned)grid, kThreads, kBytes, st>>>(m, t);
+    count_launch();
+    if (t.splits > 1) {
+      add_parts_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nk * a.hk * a.d / 4, 256), 256, 0, st>>>(t);
+      count_launch();
+    }
+  }
+  if (a.dq.p != nullptr) {
+    auto* fn = kernel_queries<T, DP, CAP, BIAS>;
+    constexpr int kBytes = (int)Layout<DP, false>::kBytes;
+    FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    const int64_t grid = (int64_t)t.blocks * a.b * t.hp;
+    if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many row blocks");
+    fn<<<(unsigned)grid, kThreads, kBytes, st>>>(m, t);
+    count_launch();
+  }
+  return FLK_OK;
+}
+
+template <typename T>
+inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
+  const Args& a = t.a;
+  const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
+  t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.q_blocks, t.splits = p.splits;
+  Maps m;
+  FLK_TRY(make_map(&m.q, a.q, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
+  FLK_TRY(make_map(&m.dout, a.dout, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
+  FLK_TRY(make_map(&m.k, a.k, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
+  FLK_TRY(make_map(&m.v, a.v, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
+  const bool cap = a.cap2 != 0.f, bias = a.slopes != nullptr;
+  if (a.d <= 64) {
+    if (cap) return bias ? launch_one<T, 64, true, true>(m, t, st) : launch_one<T, 64, true, false>(m, t, st);
+    return bias ? launch_one<T, 64, false, true>(m, t, st) : launch_one<T, 64, false, false>(m, t, st);
+  }
+  if (cap) return bias ? launch_one<T, 128, true, true>(m, t, st) : launch_one<T, 128, true, false>(m, t, st);
+  return bias ? launch_one<T, 128, false, true>(m, t, st) : launch_one<T, 128, false, false>(m, t, st);
+}
+
+}  // namespace bwd
+}  // namespace attn
+}  // namespace flk

@@ -1,0 +1,11 @@
+// Backward attention kernels of f16 data.
+#include "flk_attn_bwd.cuh"
+
+namespace flk {
+namespace attn {
+
+int backward_f16(const TcArgs& t, const bwd::Plan& p, cudaStream_t st) { return bwd::launch<__half>(t, p, st); }
+int backward_status_f16(cudaStream_t st, int* out) { return read_wait_status(st, out); }
+
+}  // namespace attn
+}  // namespace flk

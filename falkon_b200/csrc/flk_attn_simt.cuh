@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   for (int k0 = 0; k0 < last; k0 += kT) {
     if (kd != nullptr) {  // no label in common: nothing to see
-      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
       if (x.y < y.x || y.y < x.x) continue;
     }
     __syncthreads();
@@ -207,9 +207,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
                     a.o_lo == nullptr ? nullptr : (T*)a.o_lo + b * a.o.sb + h * a.o.sh);
 }
 
-// delta_i = dO_i . O_i, a group of 16 lanes per row of one head
+// delta_i = dO_i . O_i, a group of 16 lanes per row of one head, and the largest |dO| of the rows that see something (`amax`, as
+// bits, unless null; a maximum does not depend on the order it is taken in)
 template <typename T>
-__global__ void __launch_bounds__(256) delta_kernel(const Args a) {
+__global__ void __launch_bounds__(256) delta_kernel(const Args a, uint32_t* amax) {
   const int lane = threadIdx.x & 15;
   const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i, h), h fastest
   const int64_t n = (int64_t)a.b * a.nq * a.hq;
@@ -219,14 +220,17 @@ __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
   const int i = (int)(bi % a.nq), b = (int)(bi / a.nq);
   const T* x = (const T*)a.dout.p + b * a.dout.sb + i * a.dout.sn + h * a.dout.sh;
   const T* y = (const T*)a.o.p + b * a.o.sb + i * a.o.sn + h * a.o.sh;
-  float s = 0.f;
+  float s = 0.f, top = 0.f;
   constexpr int kVec = 16 / sizeof(T);
   for (int c = lane * kVec; c < a.d; c += 16 * kVec) {
     T u[kVec], w[kVec];
     *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(x + c);
     *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(y + c);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
+    for (int e = 0; e < kVec; ++e) {
+      s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
+      top = fmaxf(top, fabsf(to_f<T>(u[e])));
+    }
     if (a.o_lo != nullptr) {
       *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>((const T*)a.o_lo + (y - (const T*)a.o.p) + c);
 #pragma unroll
@@ -236,7 +240,33 @@ __global__ void __launch_bounds__(256) delta_kernel(const Args a) {
   // all 16 lanes of the group are here; the mask names them alone, so that groups behind the last row may be gone
   const unsigned mask = 0xffffu << (threadIdx.x & 16);
   for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
-  if (lane == 0) a.delta[((int64_t)b * a.hq + h) * a.nq + i] = s;
+  const int64_t at = ((int64_t)b * a.hq + h) * a.nq + i;
+  if (lane == 0) a.delta[at] = s;
+  if (amax != nullptr) {
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+    if (lane == 0 && a.lse[at] != -INFINITY && __float_as_uint(top) > *reinterpret_cast<volatile uint32_t*>(amax)) atomicMax(amax, __float_as_uint(top));
+  }
+}
+
+// Largest |v| of the rows that may be seen, as bits.
+template <typename T>
+__global__ void __launch_bounds__(256) largest_value_kernel(const Args a, uint32_t* amax) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int packs = a.d / kVec;
+  const int64_t n = (int64_t)a.b * a.nk * a.hk * packs;
+  float top = 0.f;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+    const int c = (int)(e % packs) * kVec;
+    const int64_t row = e / packs;
+    const int h = (int)(row % a.hk), j = (int)(row / a.hk % a.nk), b = (int)(row / a.hk / a.nk);
+    if (j >= (a.kv_lens != nullptr ? a.kv_lens[b] : a.nk) || (a.kdocs != nullptr && a.kdocs[(int64_t)b * a.nk_pad + j] < 0)) continue;
+    T u[kVec];
+    *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>((const T*)a.v.p + b * a.v.sb + j * a.v.sn + h * a.v.sh + c);
+#pragma unroll
+    for (int x = 0; x < kVec; ++x) top = fmaxf(top, fabsf(to_f<T>(u[x])));
+  }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) atomicMax(amax, __float_as_uint(top));
 }
 
 // Gradients of 64 keys and values: loops over the query heads that share them and over their query tiles.
@@ -264,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
     for (int q0 = 0; q0 < a.nq; q0 += kT) {
       if (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) <= k0) continue;
       if (kd != nullptr) {
-        const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+        const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
         if (x.y < y.x || y.y < x.x) continue;
       }
       __syncthreads();
@@ -339,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   for (int k0 = 0; k0 < last; k0 += kT) {
     if (kd != nullptr) {
-      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / kTile) + q0 / kTile], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
+      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
       if (x.y < y.x || y.y < x.x) continue;
     }
     float s[4][4] = {}, dp[4][4] = {};

@@ -101,12 +101,13 @@ __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a, uint32
   }
 }
 // accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B
-template <typename T, int DP>
+// (HALVES: the weights of rows 64 and up lie 64 columns behind those of rows 0 to 63, in place of 32)
+template <typename T, int DP, bool HALVES>
 __device__ __forceinline__ void issue_weighted(uint32_t d_tmem, uint32_t w_tmem, uint32_t b, bool accumulate) {
   const uint64_t base = desc_base(kBlockBytes);
 #pragma unroll
   for (int ks = 0; ks < kTile / 16; ++ks)
-    mma_ts(d_tmem, w_tmem + ks * 8, desc_at(base, b + ks * 2048), instr_desc<T>(DP, true), accumulate || ks > 0);
+    mma_ts(d_tmem, w_tmem + ks * 8 + (HALVES && ks >= 4 ? 32 : 0), desc_at(base, b + ks * 2048), instr_desc<T>(DP, true), accumulate || ks > 0);
 }
 
 #define FLK_R32_IN(r)                                                                                                    \
@@ -157,7 +158,7 @@ struct TcArgs {
   float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
   float* part_lse;   // [split][b][hp][rows], base 2
   void* o_lo;        // what rounding took from `out` (same type, strides of out), or null
-  const uint32_t* amax;  // largest |dout| as bits, or null
+  const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
 };
 
 // The tiles of [first, last) that a block has to look at: all of them or, with documents, those whose labels overlap [lo, hi].
