@@ -17,33 +17,55 @@ int backward_status_bf16(cudaStream_t st, int* out);
 int backward_status_f16(cudaStream_t st, int* out);
 
 // The tables of documents: labels padded to whole tiles, `none` (-1 for keys, -2 for queries) where nothing may be seen, and,
-// for every tile of `per` rows (a power of two up to 128), the smallest and largest label and whether a row has none (a tile
-// of none: a range that meets no other).  One warp per 128 rows.
-__global__ void __launch_bounds__(128) documents_kernel(const int* docs, int64_t sb, int n, const int* lens, int none, int n_pad, int per,
-                                                        int* out, int4* tab) {
+// for every tile of `per` rows (a power of two from 2 to 128), the smallest and largest label and whether a row has none (a tile
+// of none: a range that meets no other).  One warp per 128 rows, four rows per lane.
+struct DocTable {
+  const int* docs;
+  int64_t sb;
+  const int* lens;
+  int n, n_pad, none, per;
+  int* out;
+  int4* tab;
+};
+struct DocTables {
+  DocTable of[2];  // queries, keys
+};
+__global__ void __launch_bounds__(128) documents_kernel(const DocTables both) {
+  const DocTable& a = both.of[blockIdx.z];
   const int b = blockIdx.y, r0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * kTile, lane = threadIdx.x & 31;
-  if (r0 >= n_pad) return;
-  const int len = lens != nullptr ? min(max(lens[b], 0), n) : n;
-  for (int t = 0; t < kTile; t += per) {
-    int lo = INT32_MAX, hi = INT32_MIN, bad = 0;
-    for (int r = lane; r < per; r += 32) {
-      const int i = r0 + t + r;
-      const int id = i < len ? docs[b * sb + i] : -1;
-      if (id >= 0) {
-        lo = min(lo, id);
-        hi = max(hi, id);
-      } else {
-        bad = 1;
-      }
-      out[(int64_t)b * n_pad + i] = id >= 0 ? id : none;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) tab[(int64_t)b * (n_pad / per) + (r0 + t) / per] = make_int4(lo, hi, bad, 0);
+  if (r0 >= a.n_pad) return;
+  const int len = a.lens != nullptr ? min(max(a.lens[b], 0), a.n) : a.n;
+  int id[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int i = r0 + 4 * lane + e;
+    id[e] = i < len ? a.docs[b * a.sb + i] : -1;
   }
+  int lo[2], hi[2], bad[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int x = id[2 * e], y = id[2 * e + 1];
+    lo[e] = min(x >= 0 ? x : INT32_MAX, y >= 0 ? y : INT32_MAX);
+    hi[e] = max(x >= 0 ? x : INT32_MIN, y >= 0 ? y : INT32_MIN);
+    bad[e] = x < 0 || y < 0;
+  }
+  int4* tab = a.tab + (int64_t)b * (a.n_pad / a.per);
+  *reinterpret_cast<int4*>(a.out + (int64_t)b * a.n_pad + r0 + 4 * lane) =
+      make_int4(id[0] >= 0 ? id[0] : a.none, id[1] >= 0 ? id[1] : a.none, id[2] >= 0 ? id[2] : a.none, id[3] >= 0 ? id[3] : a.none);
+  if (a.per == 2) {
+    tab[r0 / 2 + 2 * lane] = make_int4(lo[0], hi[0], bad[0], 0);
+    tab[r0 / 2 + 2 * lane + 1] = make_int4(lo[1], hi[1], bad[1], 0);
+    return;
+  }
+  lo[0] = min(lo[0], lo[1]);
+  hi[0] = max(hi[0], hi[1]);
+  bad[0] |= bad[1];
+  for (int o = a.per / 8; o > 0; o >>= 1) {
+    lo[0] = min(lo[0], __shfl_xor_sync(0xffffffffu, lo[0], o));
+    hi[0] = max(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], o));
+    bad[0] |= __shfl_xor_sync(0xffffffffu, bad[0], o);
+  }
+  if (4 * lane % a.per == 0) tab[(r0 + 4 * lane) / a.per] = make_int4(lo[0], hi[0], bad[0], 0);
 }
 
 static int esize_of(int64_t dtype) { return dtype == FLK_F32 ? 4 : 2; }
@@ -56,6 +78,7 @@ static int check_sizes(const flk_attention_args* p) {
     return fail(FLK_ERR_BAD_ARG, "negative or empty sizes");
   if (p->batch > 65535 || p->hq > 65535 || p->nq > (1 << 29) || p->nk > (1 << 29))
     return fail(FLK_ERR_UNSUPPORTED, "at most 65535 sequences and heads, and 2^29 rows");
+  if (p->nq * p->hq > INT32_MAX || p->nk * p->hk > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "at most 2^31 - 1 rows of all heads of a sequence");
   if (p->hq % p->hk != 0)
     return fail(FLK_ERR_BAD_ARG, "%lld query heads cannot share %lld key heads", (long long)p->hq, (long long)p->hk);
   const int unit = p->dtype == FLK_F32 ? 4 : 8;
@@ -83,14 +106,15 @@ static bool on_tensor_cores(const flk_attention_args* p) {
   return p->dtype != FLK_F32 && p->nk > 0 && (p->flags & FLK_FLAG_FORCE_SIMT) == 0;
 }
 static fwd::Plan forward_plan(const flk_attention_args* p) {
-  return fwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk);
+  return fwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d, p->causal != 0, p->q_documents != nullptr,
+                        p->kv_lens != nullptr);
 }
 
 static bwd::Plan backward_plan(const flk_attention_args* p) {
-  return bwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk);
+  return bwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d, p->causal != 0, p->q_documents != nullptr);
 }
 // Queries of a tile of the documents' table: those of a tile of 128 packed rows.
-static int query_rows(const flk_attention_args* p) { return on_tensor_cores(p) ? kTile / forward_plan(p).pg : kTile; }
+static int query_rows(const flk_attention_args* p) { return on_tensor_cores(p) ? kTile / fwd::packed_heads((int)p->hq, (int)p->hk) : kTile; }
 
 struct Workspace {
   int64_t qdocs, kdocs, qtab, ktab, delta, amax, part_o, part_lse, total;
@@ -150,14 +174,12 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
     int *qd = reinterpret_cast<int*>(ws + w.qdocs), *kd = reinterpret_cast<int*>(ws + w.kdocs);
     int4 *qt = reinterpret_cast<int4*>(ws + w.qtab), *kt = reinterpret_cast<int4*>(ws + w.ktab);
     a.qdocs = qd, a.kdocs = kd, a.qtab = qt, a.ktab = kt;
-    if (p->nq > 0) {
-      documents_kernel<<<dim3((unsigned)ceil_div(a.nq_pad / kTile, 4), a.b), 128, 0, st>>>(
-          p->q_documents, p->q_documents_stride, a.nq, nullptr, -2, a.nq_pad, a.q_rows, qd, qt);
-      count_launch();
-    }
-    if (p->nk > 0) {
-      documents_kernel<<<dim3((unsigned)ceil_div(a.nk_pad / kTile, 4), a.b), 128, 0, st>>>(
-          p->k_documents, p->k_documents_stride, a.nk, p->kv_lens, -1, a.nk_pad, kTile, kd, kt);
+    DocTables tables;
+    tables.of[0] = {p->q_documents, p->q_documents_stride, nullptr, a.nq, a.nq_pad, -2, a.q_rows, qd, qt};
+    tables.of[1] = {p->k_documents, p->k_documents_stride, p->kv_lens, a.nk, a.nk_pad, -1, kTile, kd, kt};
+    const int most = a.nq_pad > a.nk_pad ? a.nq_pad : a.nk_pad;
+    if (most > 0) {
+      documents_kernel<<<dim3((unsigned)ceil_div(most / kTile, 4), a.b, 2), 128, 0, st>>>(tables);
       count_launch();
     }
   }
@@ -171,8 +193,7 @@ static int simt_forward(const Args& a, cudaStream_t st) {
 template <typename T>
 static int simt_backward(const Args& a, cudaStream_t st) {
   if (a.nq > 0) {
-    simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a, nullptr);
-    count_launch();
+    FLK_TRY(simt::launch_delta<T>(a, nullptr, st));
   }
   return a.d <= 64 ? simt::launch_backward<T, 64>(a, st) : simt::launch_backward<T, 128>(a, st);
 }
@@ -186,9 +207,7 @@ static int prepare_backward(const Args& a, uint32_t* amax, cudaStream_t st) {
     simt::largest_value_kernel<T><<<(unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 256, 0, st>>>(a, amax + 1);
     count_launch();
   }
-  simt::delta_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * a.nq * a.hq, 16), 256, 0, st>>>(a, amax);
-  count_launch();
-  return FLK_OK;
+  return simt::launch_delta<T>(a, amax, st);
 }
 
 }  // namespace attn

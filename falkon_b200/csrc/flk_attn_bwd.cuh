@@ -17,7 +17,7 @@
 // |dP - delta|, takes to at most 2^15.
 #pragma once
 
-#include "flk_attn_tc.cuh"
+#include "flk_attn_fwd.cuh"
 
 namespace flk {
 namespace attn {
@@ -57,9 +57,6 @@ struct Scales {
   static constexpr bool kHalf = !std::is_same<T, __nv_bfloat16>::value;
   static constexpr float kShift = kHalf ? 12.f : 0.f;
   static constexpr float kUnshift = kHalf ? 1.f / 4096.f : 1.f;
-  // what the weights of the keys kernel carry and dS is not to: 2^shift, and the quarter that the slope of the cap is taken with
-  template <bool CAP>
-  static __device__ __forceinline__ float per_weight() { return kUnshift * (CAP ? 4.f : 1.f); }
   // the factor that dS is held with, a power of two
   static __device__ __forceinline__ float ds(const TcArgs& t) {
     if (!kHalf) return 1.f;
@@ -69,20 +66,6 @@ struct Scales {
     return __uint_as_float((uint32_t)(127 + min(max(14 - e, -100), 100)) << 23);
   }
 };
-
-// Raw scores -> scores in base 2 of 32 columns, and, with a cap, the slope r (1 - r) = (1 - tanh^2) / 4 of it in `slope`
-template <bool CAP>
-__device__ __forceinline__ float base2(float raw, const Args& a, float f, float& slope) {
-  float x = raw * f;
-  if constexpr (CAP) {
-    const float r = rcp_approx(1.f + ex2_approx(x));
-    slope = fmaf(-r, r, r);
-    x = fmaf(-2.f * a.cap2, r, a.cap2);
-  }
-  return x;
-}
-template <bool CAP>
-__device__ __forceinline__ float base2_factor(const Args& a) { return CAP ? a.scale * (2.f * kLog2e) : a.scale; }
 
 // accumulator half (DP / 2 columns from c0) times f -> a row of 16-bit values, or of fp32 partial results
 template <typename T, int DP>
@@ -252,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     } else if (warp == kStatWarp) {
       bool ok = true;
       StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
-      const float g = Scales<T>::ds(t) * Scales<T>::template per_weight<CAP>();
+      const float g = Scales<T>::ds(t) * Scales<T>::kUnshift;
       for (int step = 0; step < steps && ok; ++step) {
         const Tile e = walk.next();
         const int slot = step % kStatSlots;
@@ -381,8 +364,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     const int my = kd ? kd[key] : 0;
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
-    const float f = base2_factor<CAP>(a);
-    const float gs = Scales<T>::ds(t), g = gs * Scales<T>::template per_weight<CAP>();
+    const float f = CAP ? a.cap2 : a.scale;  // raw score, or its tanh -> base 2
+    const float gs = Scales<T>::ds(t), g = gs * Scales<T>::kUnshift;
     bool ok = true;
     for (int i = 0; i < steps && ok; ++i) {
       const int slot = i % kStatSlots;
@@ -398,32 +381,24 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       for (int p = 0; p < 2; ++p) tmem_ld32(ts + lane_at + half + 32 * p, s[p]);
 #pragma unroll
       for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
+      if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         uint32_t o[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           const uint32_t at = st + (32 * p + c) * 4;
-          float x[4], add[4], slope[4];
+          float x[4], add[4];
           tc::ld_shared_f4(at + kLse * 4, add[0], add[1], add[2], add[3]);
+          if constexpr (BIAS) {
+            float sl[4], ps[4];
+            tc::ld_shared_f4(at + kSlope * 4, sl[0], sl[1], sl[2], sl[3]);
+            tc::ld_shared_f4(at + kPos * 4, ps[0], ps[1], ps[2], ps[3]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) slope[q] = 1.f;
-          if constexpr (!CAP && !BIAS) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[p][c + q]), f, add[q]);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] = base2<CAP>(__uint_as_float(s[p][c + q]), a, f, slope[q]);
-            if constexpr (BIAS) {
-              float sl[4], ps[4];
-              tc::ld_shared_f4(at + kSlope * 4, sl[0], sl[1], sl[2], sl[3]);
-              tc::ld_shared_f4(at + kPos * 4, ps[0], ps[1], ps[2], ps[3]);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) x[q] = fmaf(sl[q], fabsf(ps[q] - mine), x[q]);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] += add[q];
+            for (int q = 0; q < 4; ++q) add[q] = fmaf(sl[q], fabsf(ps[q] - mine), add[q]);
           }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[p][c + q]), f, add[q]);
           if (!whole) {
             int en[4], lb[4];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(at + kEnd * 4) : "memory");
@@ -436,7 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             pr[q] = ex2_approx(x[q]);
-            s[p][c + q] = __float_as_uint(CAP ? pr[q] * slope[q] : pr[q]);
+            // with a cap, the weight times 1 - tanh^2
+            s[p][c + q] = __float_as_uint(CAP ? pr[q] * fmaf(-__uint_as_float(s[p][c + q]), __uint_as_float(s[p][c + q]), 1.f) : pr[q]);
           }
           o[c / 2] = pack16<T>(pr[0], pr[1]);
           o[c / 2 + 1] = pack16<T>(pr[2], pr[3]);
@@ -678,17 +654,16 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     const int all_before = lim.row_end(i0, a.causal);
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
-    const float f = base2_factor<CAP>(a), gs = Scales<T>::ds(t);
+    const float f = CAP ? a.cap2 : a.scale, gs = Scales<T>::ds(t);
     float add = -INFINITY, nd = 0.f;  // of a row that sees nothing
     if (exists) {
       const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
       const float lse = a.lse[row];
       if (lse != -INFINITY) {
         add = -lse * kLog2e;
-        nd = -a.delta[row] * gs * (CAP ? 4.f : 1.f);
+        nd = -a.delta[row] * gs;
       }
     }
-    const float g = gs * (CAP ? 4.f : 1.f);
     bool ok = true;
     for (int step = 0; step < steps && ok; ++step) {
       ok = wait_bar(sfull(step & 1), (uint32_t)(step >> 1) & 1);
@@ -710,21 +685,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         for (int p = 0; p < 2; ++p)
           seen[p] = seen_columns(end - k0 - (int)half - 32 * p, kd == nullptr ? nullptr : kd + k0 + half + 32 * p, my);
       }
+      if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          float slope = 1.f, x;
-          if constexpr (!CAP && !BIAS) {
-            x = fmaf(__uint_as_float(s[p][c]), f, add);
-          } else {
-            x = base2<CAP>(__uint_as_float(s[p][c]), a, f, slope);
-            if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
-            x += add;
-          }
+          const float raw = __uint_as_float(s[p][c]);
+          float x = fmaf(raw, f, add);
+          if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
           if (!whole && (seen[p] >> c & 1) == 0) x = -INFINITY;
           x = ex2_approx(x);
-          s[p][c] = __float_as_uint(CAP ? x * slope : x);
+          s[p][c] = __float_as_uint(CAP ? x * fmaf(-raw, raw, 1.f) : x);
         }
       ok = wait_bar(dpfull, (uint32_t)step & 1);
       if (!ok) break;
@@ -742,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
           float y[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            y[q] = __uint_as_float(s[p][c + q]) * fmaf(__uint_as_float(d[p][c + q]), g, nd);
+            y[q] = __uint_as_float(s[p][c + q]) * fmaf(__uint_as_float(d[p][c + q]), gs, nd);
             // V rows that nobody may see are not cleaned here: their products may be anything
             if (!whole && (seen[p] >> (c + q) & 1) == 0) y[q] = 0.f;
           }
@@ -778,22 +749,26 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
 struct Plan {
   int pg, pg_shift, hp, rows, q_blocks, splits;
 };
-inline Plan make_plan(int b, int nq, int nk, int hq, int hk) {
+inline Plan make_plan(int b, int nq, int nk, int hq, int hk, int d, bool causal, bool documents) {
   Plan p{};
   const int grp = hq / hk;
-  p.pg = (grp & (grp - 1)) == 0 && grp <= 64 ? grp : 1;
+  p.pg = fwd::packed_heads(hq, hk);
   while ((1 << p.pg_shift) < p.pg) ++p.pg_shift;
   p.hp = hq / p.pg;
   p.rows = nq * p.pg;
   p.q_blocks = (int)ceil_div(p.rows, kTile);
-  // parts of a key tile's query tiles: few key tiles would leave SMs without work.  Blocks per SM, rounded up, times the steps
-  // of a block with 4 steps' time for its start and end and, with parts, the time of writing and adding them
+  // parts of a key tile's query tiles: few or uneven key tiles would leave SMs without work.  The lowest estimate, the
+  // traffic of the partial results included; a step takes about 1.6 us with heads of 128, 1 us with heads of 64
   const int64_t blocks = ceil_div(nk, kTile) * hk * b, steps = (int64_t)p.q_blocks * (grp / p.pg);
+  const double step = d <= 64 ? 1.0 : 1.6, added = (double)b * nk * hk * d * 16.0 / 5e6;
+  double mean = (double)steps;
+  if (causal) mean *= 0.5;
+  if (documents) mean *= 0.5;
   p.splits = 1;
   double best = 1e300;
   for (int64_t s = 1; s <= 32 && (s == 1 || s * 4 <= steps); ++s) {
-    const double cost = (double)ceil_div(blocks * s, kNumSMs) * ((double)ceil_div(steps, s) + 4 + (s > 1 ? 2 : 0)) + (s > 1 ? 4 + 0.02 * (double)(blocks * s) : 0.0);
-    if (cost < best * 0.97) best = cost, p.splits = (int)s;
+    const double cost = fwd::time_of(blocks, s, (double)steps, mean, step, causal || documents) + (s > 1 ? 3 + s * added : 0);
+    if (cost < best * 0.98) best = cost, p.splits = (int)s;
   }
   return p;
 }

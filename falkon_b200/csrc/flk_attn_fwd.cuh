@@ -33,7 +33,7 @@ struct Layout {
   static constexpr uint32_t kRing = (PAIR ? 2 : 1) * kTileBytes;
   static constexpr int kStages = (int)((224 * 1024 - kRing) / kTileBytes) < 8 ? (int)((224 * 1024 - kRing) / kTileBytes) : 8;
   static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
-  static constexpr uint32_t kBytes = kBars + 384 + 1024;  // barriers and slots, and room to align the tiles to 1024 bytes
+  static constexpr uint32_t kBytes = kBars + 512 + 1024;  // barriers and slots, and room to align the tiles to 1024 bytes
 };
 static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
 
@@ -42,23 +42,6 @@ __device__ __forceinline__ int4 get_place(uint32_t at) {
   int4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
-}
-
-// Turns the raw scores of one row into scores in base 2 (where the kernel keeps them raw, CAP and BIAS being off, nothing).
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void transform(uint32_t (&s)[4][32], const Args& a, float slope2, float d0) {
-  if constexpr (CAP || BIAS) {
-    const float f = CAP ? a.scale * (2.f * kLog2e) : a.scale, cap2 = a.cap2;
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        float x = __uint_as_float(s[p][c]) * f;
-        if constexpr (CAP) x = fmaf(-2.f * cap2, rcp_approx(1.f + ex2_approx(x)), cap2);  // cap tanh, tanh(x) = 1 - 2 / (1 + e^2x)
-        if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
-        s[p][c] = __float_as_uint(x);
-      }
-  }
 }
 
 template <typename T, int DP, bool CAP, bool BIAS, bool PAIR>
@@ -244,25 +227,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool live = (r & ~31) < t.rows;                     // some row of this warp exists
     const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
     const bool exists = r < t.rows;
-    const int my = qd && exists ? qd[i] : -2;
     const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
     const int pos = lim.start + i;
-    // keys before this bound are visible to every row of the warpgroup's tile that exists
-    const int tile_i0 = (row0 + (PAIR ? w * kTile : 0)) >> t.pg_shift;
-    const int all_before = lim.row_end(min(tile_i0, a.nq - 1), a.causal);
-    int only = -1;  // the one label of its queries
-    if (kd) {
-      const LabelRange mine = labels_of(qd, min(tile_i0, a.nq), min(a.nq, (tile_i0 + (kTile >> t.pg_shift))));
-      if (!mine.bad && mine.lo == mine.hi) only = mine.lo;
+    // for the tile of this warpgroup: keys before `x` are visible to every row that exists; `y` is the one label of its queries
+    const uint32_t rule = place + 32 + 8 * w;
+    {
+      const int tile_i0 = (row0 + (PAIR ? w * kTile : 0)) >> t.pg_shift;
+      int only = -1;
+      if (kd) {
+        const LabelRange mine = labels_of(qd, min(tile_i0, a.nq), min(a.nq, (tile_i0 + (kTile >> t.pg_shift))));
+        if (!mine.bad && mine.lo == mine.hi) only = mine.lo;
+      }
+      // all four warps write the same
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(rule), "r"(lim.row_end(min(tile_i0, a.nq - 1), a.causal)), "r"(only) : "memory");
+      __syncwarp();
     }
-    const float f2 = a.scale;  // raw score -> base 2, where nothing else is done to it
+    const float f2 = CAP ? a.cap2 : a.scale;  // raw score, or its tanh -> base 2; done last where there is no bias
     float m = -INFINITY;       // of the weights, base 2
     float l = 0.f;
     bool ok = true;
-    int turn = 0;
-    for (int step = PAIR ? 0 : w; step < steps && ok; step += PAIR ? 1 : 2) {
-      ok = wait_bar(sfull(w), (uint32_t)turn & 1);
-      ++turn;
+    for (int step = PAIR ? 0 : w; step < steps; step += PAIR ? 1 : 2) {
+      ok = wait_bar(sfull(w), (uint32_t)(PAIR ? step : step >> 1) & 1);
       if (!ok) break;
       if (!live) {  // the weights of rows that do not exist reach nothing
         if (elect_one()) mbar_arrive(pfull(w));
@@ -272,6 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const Tile e = get_tile(slots, step);
       const int k0 = e.at * kTile;
+      int all_before, only;
+      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(all_before), "=r"(only) : "r"(rule) : "memory");
       const bool whole = k0 + kTile <= all_before && (a.kdocs == nullptr || (e.label >= 0 && e.label == only));
       uint32_t s[4][32];
       const uint32_t at = ts(w) + lane_at;
@@ -279,12 +266,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int p = 0; p < 4; ++p) tmem_ld32(at + 32 * p, s[p]);
 #pragma unroll
       for (int p = 0; p < 4; ++p) tmem_ld_wait_on(s[p]);
-      transform<CAP, BIAS>(s, a, slope2, (float)(pos - k0));
+      if constexpr (CAP) to_tanh(s, a.scale);
+      if constexpr (BIAS) {
+        const float d0 = (float)(pos - k0);
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            s[p][c] = __float_as_uint(fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), __uint_as_float(s[p][c]) * f2));
+      }
       if (!whole) {
         const int4 x = get_place(place + 16);
         const int r = row0 + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
         const int end = r < t.rows ? Limits{x.x, x.y, x.z}.row_end(r >> t.pg_shift, a.causal) : 0;
-        const int* labels = a.kdocs == nullptr ? nullptr : a.kdocs + (int64_t)get_place(place).y * a.nk_pad + k0;
+        const int b = get_place(place).y;
+        const int* labels = a.kdocs == nullptr ? nullptr : a.kdocs + (int64_t)b * a.nk_pad + k0;
+        const int my = labels != nullptr && r < t.rows ? __ldg(a.qdocs + (int64_t)b * a.nq_pad + (r >> t.pg_shift)) : -2;
 #pragma unroll
         for (int p = 0; p < 4; ++p) hide_columns(s[p], seen_columns(end - k0 - 32 * p, labels == nullptr ? nullptr : labels + 32 * p, my));
       }
@@ -297,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         top[p] = fmaxf(top[p], __uint_as_float(s[p][31]));
       }
       float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if constexpr (!CAP && !BIAS) mt *= f2;
+      if constexpr (!BIAS) mt *= f2;
       const bool grow = mt > m + 8.f || (m == -INFINITY && mt != -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
         const float mn = grow ? mt : m;
@@ -327,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 32; c += 2) {
           const uint32_t s0 = s[p][c], s1 = s[p][c + 1];
           const uint64_t v = tc::pack2(__uint_as_float(s0), __uint_as_float(s1));
-          const uint64_t x = CAP || BIAS ? tc::add2(v, mv) : tc::fma2(v, f2v, mv);
+          const uint64_t x = BIAS ? tc::add2(v, mv) : tc::fma2(v, f2v, mv);
           float x0, x1, p0, p1;
           tc::unpack2(x, x0, x1);
           p0 = ex2_approx(x0);
@@ -347,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       l += u0 + u1;
     }
     // ---- results
-    const bool worked = turn > 0;
+    const bool worked = steps > (PAIR ? 0 : w);
     if (worked && ok) ok = wait_bar(odone(w), 0);
     tc_fence_after();
     const bool none = m == -INFINITY;
@@ -434,17 +431,20 @@ __global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
   const int c = lane * 4;
   if (c >= a.d) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (top != -INFINITY)
+  if (top != -INFINITY) {
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
       const float e = t.part_lse[p * n + row];
-      if (e == -INFINITY) continue;
       const float w = exp2f(e - top) * inv;
-      const float4 v = *reinterpret_cast<const float4*>(t.part_o + (p * n + row) * a.d + c);
+      // a part that saw nothing has written nothing
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (e != -INFINITY) v = *reinterpret_cast<const float4*>(t.part_o + (p * n + row) * a.d + c);
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
       acc.z = fmaf(w, v.z, acc.z);
       acc.w = fmaf(w, v.w, acc.w);
     }
+  }
   const int64_t at = b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh + c;
   const uint2 v = make_uint2(pack16<T>(acc.x, acc.y), pack16<T>(acc.z, acc.w));
   *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o.p) + at) = v;
@@ -455,28 +455,48 @@ __global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
   }
 }
 
-// Parts of the key axis.  With PAIR, one part where the blocks fill the SMs; else the number with the lowest
-// max(waves) x (tiles of a part + 3 tiles' time for a block's start and end).
 struct Plan {
   bool pair;
   int pg, pg_shift, hp, rows, blocks, splits, parts;
 };
-inline Plan make_plan(int b, int nq, int nk, int hq, int hk) {
-  Plan p{};
+// Heads packed into a tile's rows: all that share a key head, where that is a power of two.
+inline int packed_heads(int hq, int hk) {
   const int grp = hq / hk;
-  p.pg = (grp & (grp - 1)) == 0 && grp <= 64 ? grp : 1;
+  return (grp & (grp - 1)) == 0 && grp <= 64 ? grp : 1;
+}
+// Time of `blocks` x `s` blocks on all SMs, in us: blocks take `longest / s` steps at most and `mean / s` on average, a step
+// takes `step` us, a block's start and end 4 us.  Blocks of one length run in waves; blocks of different lengths (uneven) fill
+// gaps, all but half of the last one.
+inline double time_of(int64_t blocks, int64_t s, double longest, double mean, double step, bool uneven) {
+  const double one = longest / s * step + 4;
+  if (!uneven) return (double)ceil_div(blocks * s, kNumSMs) * one;
+  const double shared = (double)blocks * (mean * step + 4.0 * s) / kNumSMs + one / 2;
+  return shared > one ? shared : one;
+}
+// Parts of the key axis: the number with the lowest estimate, joining included (3 us and its traffic at 5 TB/s).
+// Steps of 128 keys take about 1.5 us with heads of 128 and 0.9 us with heads of 64.
+inline Plan make_plan(int b, int nq, int nk, int hq, int hk, int d, bool causal, bool documents, bool lens) {
+  Plan p{};
+  p.pg = packed_heads(hq, hk);
   while ((1 << p.pg_shift) < p.pg) ++p.pg_shift;
   p.hp = hq / p.pg;
   p.rows = nq * p.pg;
   p.pair = p.rows > 128;
   p.blocks = (int)ceil_div(p.rows, p.pair ? 256 : 128);
   const int64_t blocks = (int64_t)p.blocks * p.hp * b, tiles = ceil_div(nk, kTile);
+  const double step = d <= 64 ? 0.9 : 1.5, joined = (double)b * p.hp * p.rows * d * 8.0 / 5e6;
+  double mean = (double)tiles;
+  if (causal && nk > 0) mean *= 1.0 - 0.5 * (nq < nk ? (double)nq / nk : 1.0);
+  if (documents) mean *= 0.5;
+  if (lens) mean *= 0.75;
+  const bool uneven = mean < 0.95 * (double)tiles;
   p.splits = 1;
   double best = 1e300;
   const int64_t least = p.pair ? 4 : 2;  // key tiles of a part
   for (int64_t s = 1; s <= 64 && (s == 1 || s * least <= tiles); ++s) {
-    const double cost = (double)ceil_div(blocks * s, kNumSMs) * ((double)ceil_div(tiles, s) + 3) + (s > 1 || !p.pair ? 0.05 * s : 0.0);
-    if (cost < best * 0.97) best = cost, p.splits = (int)s;
+    const int64_t parts = p.pair ? s : 2 * s;
+    const double cost = time_of(blocks, s, (double)tiles, mean, step, uneven) + (parts > 1 ? 3 + parts * joined : 0);
+    if (cost < best * 0.98) best = cost, p.splits = (int)s;
   }
   p.parts = p.pair ? p.splits : 2 * p.splits;
   return p;

@@ -207,45 +207,68 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
                     a.o_lo == nullptr ? nullptr : (T*)a.o_lo + b * a.o.sb + h * a.o.sh);
 }
 
-// delta_i = dO_i . O_i, a group of 16 lanes per row of one head, and the largest |dO| of the rows that see something (`amax`, as
-// bits, unless null; a maximum does not depend on the order it is taken in)
-template <typename T>
+// delta_i = dO_i . O_i, a group of LANES lanes per row of one head (16 bytes of each array per lane), two rows per group at a time,
+// and the largest |dO| of the rows that see something (`amax`, as bits, unless null; a maximum does not depend on the order it
+// is taken in).  Bound by the bytes of dO, O and what rounding took from O.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_kernel(const Args a, uint32_t* amax) {
-  const int lane = threadIdx.x & 15;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i, h), h fastest
-  const int64_t n = (int64_t)a.b * a.nq * a.hq;
-  if (row >= n) return;
-  const int h = (int)(row % a.hq);
-  const int64_t bi = row / a.hq;
-  const int i = (int)(bi % a.nq), b = (int)(bi / a.nq);
-  const T* x = (const T*)a.dout.p + b * a.dout.sb + i * a.dout.sn + h * a.dout.sh;
-  const T* y = (const T*)a.o.p + b * a.o.sb + i * a.o.sn + h * a.o.sh;
-  float s = 0.f, top = 0.f;
-  constexpr int kVec = 16 / sizeof(T);
-  for (int c = lane * kVec; c < a.d; c += 16 * kVec) {
-    T u[kVec], w[kVec];
-    *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(x + c);
-    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(y + c);
+  constexpr int kVec = 16 / sizeof(T), kGroups = 256 / LANES;
+  const uint32_t n = (uint32_t)a.nq * (uint32_t)a.hq;
+  const int b = blockIdx.y, c = (threadIdx.x % LANES) * kVec;
+  const T *dout = (const T*)a.dout.p + b * a.dout.sb, *o = (const T*)a.o.p + b * a.o.sb;
+  const T* lo = a.o_lo == nullptr ? nullptr : (const T*)a.o_lo + b * a.o.sb;
+  float s[2] = {0.f, 0.f}, top[2] = {0.f, 0.f};
+  int64_t at[2];
+  bool on[2];
+  uint4 u[2], w[2], x[2];
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
-      top = fmaxf(top, fabsf(to_f<T>(u[e])));
-    }
-    if (a.o_lo != nullptr) {
-      *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>((const T*)a.o_lo + (y - (const T*)a.o.p) + c);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) s = fmaf(to_f<T>(u[e]), to_f<T>(w[e]), s);
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t row = (blockIdx.x * 2 + e) * kGroups + threadIdx.x / LANES;  // (i, h), h fastest
+    on[e] = row < n;
+    const uint32_t i = on[e] ? row / (uint32_t)a.hq : 0, h = on[e] ? row - i * (uint32_t)a.hq : 0;
+    at[e] = ((int64_t)b * a.hq + h) * a.nq + i;
+    u[e] = w[e] = x[e] = make_uint4(0, 0, 0, 0);
+    if (on[e] && c < a.d) {
+      const int64_t off = i * a.o.sn + h * a.o.sh + c;
+      u[e] = *reinterpret_cast<const uint4*>(dout + i * a.dout.sn + h * a.dout.sh + c);
+      w[e] = *reinterpret_cast<const uint4*>(o + off);
+      if (lo != nullptr) x[e] = *reinterpret_cast<const uint4*>(lo + off);
     }
   }
-  // all 16 lanes of the group are here; the mask names them alone, so that groups behind the last row may be gone
-  const unsigned mask = 0xffffu << (threadIdx.x & 16);
-  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
-  const int64_t at = ((int64_t)b * a.hq + h) * a.nq + i;
-  if (lane == 0) a.delta[at] = s;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const T *p = reinterpret_cast<const T*>(&u[e]), *q = reinterpret_cast<const T*>(&w[e]), *r = reinterpret_cast<const T*>(&x[e]);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      const float g = to_f<T>(p[k]);
+      s[e] = fmaf(g, to_f<T>(q[k]), s[e]);
+      if (sizeof(T) == 2) s[e] = fmaf(g, to_f<T>(r[k]), s[e]);
+      top[e] = fmaxf(top[e], fabsf(g));
+    }
+    for (int k = LANES / 2; k > 0; k >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], k);
+    if (c == 0 && on[e]) a.delta[at[e]] = s[e];
+  }
   if (amax != nullptr) {
-    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-    if (lane == 0 && a.lse[at] != -INFINITY && __float_as_uint(top) > *reinterpret_cast<volatile uint32_t*>(amax)) atomicMax(amax, __float_as_uint(top));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (!on[e] || a.lse[at[e]] == -INFINITY) top[e] = 0.f;
+      for (int k = 16; k > 0; k >>= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], k));
+    }
+    const uint32_t bits = __float_as_uint(fmaxf(top[0], top[1]));
+    if ((threadIdx.x & 31) == 0 && bits > *reinterpret_cast<volatile uint32_t*>(amax)) atomicMax(amax, bits);
   }
+}
+template <typename T>
+inline int launch_delta(const Args& a, uint32_t* amax, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int64_t n = (int64_t)a.nq * a.hq;
+  const int lanes = a.d <= 8 * kVec ? 8 : a.d <= 16 * kVec ? 16 : 32;
+  const dim3 grid((unsigned)ceil_div(n, 2 * 256 / lanes), a.b);
+  if (lanes == 8) delta_kernel<T, 8><<<grid, 256, 0, st>>>(a, amax);
+  else if (lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a, amax);
+  else delta_kernel<T, 32><<<grid, 256, 0, st>>>(a, amax);
+  count_launch();
+  return FLK_OK;
 }
 
 // Largest |v| of the rows that may be seen, as bits.

@@ -63,16 +63,15 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Shared-memory matrix descriptors of a 128-byte-swizzled tile (8-row groups of 1024 bytes).
-__device__ __forceinline__ uint64_t desc_base(uint32_t lead_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)(lead_bytes >> 4) << 16;  // MN-major: from one block of 64 columns to the next; K-major: unused
-  d |= (uint64_t)(1024 >> 4) << 32;        // from one group of 8 rows to the next
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;  // SWIZZLE_128B
-  return d;
+// Shared-memory matrix descriptors of a 128-byte-swizzled tile (8-row groups of 1024 bytes).  Only the low word changes from one
+// product to the next: it is kept in one register and stepped by immediates.
+constexpr uint32_t kDescHigh = (1024 >> 4)       // from one group of 8 rows to the next
+                               | (1u << 14)      // version
+                               | (2u << 29);     // SWIZZLE_128B
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead_bytes) {
+  // MN-major: `lead_bytes` from one block of 64 columns to the next; K-major: unused
+  return ((addr >> 4) & 0x3FFF) | (lead_bytes >> 4) << 16;
 }
-__device__ __forceinline__ uint64_t desc_at(uint64_t base, uint32_t addr) { return base | (uint64_t)((addr >> 4) & 0x3FFF); }
 
 template <typename T>
 __host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
@@ -80,34 +79,46 @@ __host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
   return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
-// A from tensor memory (16-bit values, two per column), B from shared memory
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// A and B from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A from tensor memory (16-bit values, two per column), B from shared memory
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
 // scores: D[128 x 128] = A B^T along DP columns
 template <typename T, int DP>
 __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a, uint32_t b) {
-  const uint64_t base = desc_base(16);
+  const uint32_t al = desc_low(a, 16), bl = desc_low(b, 16);
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
-    const uint32_t off = (ks / 4) * kBlockBytes + (ks % 4) * 32;
-    tc::mma_f16(d_tmem, desc_at(base, a + off), desc_at(base, b + off), instr_desc<T>(kTile, false), ks > 0);
+    const uint32_t off = ((ks / 4) * kBlockBytes + (ks % 4) * 32) >> 4;
+    mma_ss(d_tmem, al + off, bl + off, instr_desc<T>(kTile, false), ks > 0);
   }
 }
-// accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B
-// (HALVES: the weights of rows 64 and up lie 64 columns behind those of rows 0 to 63, in place of 32)
-template <typename T, int DP, bool HALVES>
+// accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B; weights of the rows
+// [16 K0, 16 K1).  HALVES: the weights of rows 64 and up lie 64 columns behind those of rows 0 to 63, in place of 32
+template <typename T, int DP, bool HALVES, int K0 = 0, int K1 = kTile / 16>
 __device__ __forceinline__ void issue_weighted(uint32_t d_tmem, uint32_t w_tmem, uint32_t b, bool accumulate) {
-  const uint64_t base = desc_base(kBlockBytes);
+  const uint32_t bl = desc_low(b, kBlockBytes);
 #pragma unroll
-  for (int ks = 0; ks < kTile / 16; ++ks)
-    mma_ts(d_tmem, w_tmem + ks * 8 + (HALVES && ks >= 4 ? 32 : 0), desc_at(base, b + ks * 2048), instr_desc<T>(DP, true), accumulate || ks > 0);
+  for (int ks = K0; ks < K1; ++ks)
+    mma_ts(d_tmem, w_tmem + ks * 8 + (HALVES && ks >= 4 ? 32 : 0), bl + ks * (2048 >> 4), instr_desc<T>(DP, true), accumulate || ks > 0);
 }
 
 #define FLK_R32_IN(r)                                                                                                    \
@@ -146,6 +157,48 @@ __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// s -> tanh(s * scale), in place, for N x 32 raw scores of a row.  Where all of a warp's arguments lie in [-1, 1], and scores
+// below the cap do, an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: x p(x^2) with p of
+// degree 6 fitted to tanh(x) / x at Chebyshev nodes (relative error 1.1e-7 in fp32).  With both on the MUFU unit, the
+// exponential of the weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle
+// are 3072 cycles against 1024 of the two products.
+__device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
+template <int N>
+__device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], float scale) {
+  float big = 0.f;
+#pragma unroll
+  for (int p = 0; p < N; ++p)
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(s[p][c]))), fabsf(__uint_as_float(s[p][c + 1])));
+  if (__all_sync(0xffffffffu, big * fabsf(scale) <= 1.f)) {
+#pragma unroll
+    for (int p = 0; p < N; ++p)
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const uint64_t x = tc::mul2(tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1])), both(scale));
+        const uint64_t z = tc::mul2(x, x);
+        uint64_t y = tc::fma2(z, both(0.0010380251333117485f), both(-0.0061943246982991695f));
+        y = tc::fma2(y, z, both(0.02027970738708973f));
+        y = tc::fma2(y, z, both(-0.053451646119356155f));
+        y = tc::fma2(y, z, both(0.13325075805187225f));
+        y = tc::fma2(y, z, both(-0.3333282768726349f));
+        y = tc::fma2(y, z, both(0.9999999403953552f));
+        y = tc::mul2(y, x);
+        float y0, y1;
+        tc::unpack2(y, y0, y1);
+        s[p][c] = __float_as_uint(y0);
+        s[p][c + 1] = __float_as_uint(y1);
+      }
+  } else {
+    const float f = scale * (2.f * kLog2e);
+#pragma unroll
+    for (int p = 0; p < N; ++p)
+#pragma unroll
+      for (int c = 0; c < 32; ++c)  // tanh(x) = 1 - 2 / (1 + e^2x)
+        s[p][c] = __float_as_uint(fmaf(-2.f, rcp_approx(1.f + ex2_approx(__uint_as_float(s[p][c]) * f)), 1.f));
+  }
 }
 
 // What the tensor-core kernels need on top of Args.

@@ -71,11 +71,14 @@ class AttentionFn(torch.autograd.Function):
         ctx.opts = tuple(None if isinstance(t, torch.Tensor) else t for t in opts)
         ctx.held = tuple(isinstance(t, torch.Tensor) for t in opts)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return None, None, None, None
         q, k, v, out, out_lo, lse, *kept = ctx.saved_tensors
         kept = iter(kept)
         opts = tuple(next(kept) if held else t for t, held in zip(ctx.opts, ctx.held))
