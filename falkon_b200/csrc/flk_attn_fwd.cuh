@@ -1,11 +1,12 @@
 // Forward attention on tcgen05: out, and the log-sum-exp of every row.
 //
-// A block has 12 warps: two softmax warpgroups (a thread owns one packed query row), a warp that issues the matrix products
-// and one that issues the copies.  Tensor memory holds two score tiles of 128 x 128 and two accumulators of 128 x DP, all
-// 512 columns.  The two warpgroups take turns on the tensor cores: while one turns its scores into weights, the products
-// of the other run.
+// A block has 18 warps: two groups of eight turn scores into weights, one issues the matrix products, one the copies.  A group
+// serves one score tile; two threads share a row, each with half of the columns, and tell each other the largest score.  Tensor
+// memory holds two score tiles of 128 x 128 and two accumulators of 128 x DP, all 512 columns.  The two groups take turns on the
+// tensor cores: while one turns its scores into weights, the products of the other run.  With a group of four warps (a row
+// per thread) a step of two tiles took 3470 cycles, of which 1570 were spent waiting for the next scores; the products take 2048.
 //   PAIR   two row tiles (256 rows) against the same key tiles, for prompts and training
-//   !PAIR  one row tile; the warpgroups take the even and the odd key tiles, and end with a partial result each: few
+//   !PAIR  one row tile; the groups take the even and the odd key tiles, and end with a partial result each: few
 //          rows over a long key axis (single tokens)
 // Weights are exp2(s - m) with a maximum m that follows the running one only when that has grown by more than 8: weights
 // stay below 2^8, and the accumulator is rescaled a few times in a row's life instead of once per tile.  The sum of the
@@ -20,11 +21,11 @@ namespace flk {
 namespace attn {
 namespace fwd {
 
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
-// registers: 384 threads are launched with 168 each (64512); two warpgroups of 216 and one of 72 make the same sum
-constexpr int kRegsSoftmax = 216, kRegsOther = 72;
-static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * 168, "registers");
+constexpr int kThreads = 640;
+// registers: 640 threads are launched with 96 each (61440); four warpgroups of 104 and one of 64 make the same sum
+constexpr int kRegsSoftmax = 104, kRegsOther = 64;
+static_assert(4 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * 96, "registers");
+constexpr int kMmaWarp = 16, kLoadWarp = 17;
 
 template <int DP, bool PAIR>
 struct Layout {
@@ -33,7 +34,7 @@ struct Layout {
   static constexpr uint32_t kRing = (PAIR ? 2 : 1) * kTileBytes;
   static constexpr int kStages = (int)((224 * 1024 - kRing) / kTileBytes) < 8 ? (int)((224 * 1024 - kRing) / kTileBytes) : 8;
   static constexpr uint32_t kBars = kRing + kStages * kTileBytes;
-  static constexpr uint32_t kBytes = kBars + 512 + 1024;  // barriers and slots, and room to align the tiles to 1024 bytes
+  static constexpr uint32_t kBytes = kBars + 512 + 2048 + 512;  // barriers and slots, the halves' maxima, and some room
 };
 static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
 
@@ -44,21 +45,40 @@ __device__ __forceinline__ int4 get_place(uint32_t at) {
   return v;
 }
 
+// Scores in base 2 from raw scores (or their tanh) and the distance bias; column 0 lies d0 before the row's position.  Where all
+// columns lie on one side of all rows of the warp, the bias is linear.
+__device__ __forceinline__ void add_bias(uint32_t (&s)[2][32], float f2, float slope2, float d0) {
+  const bool before = __all_sync(0xffffffffu, d0 >= 63.f);
+  if (before) {
+    const float at = -slope2 * d0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int c = 0; c < 32; ++c) s[p][c] = __float_as_uint(fmaf(__uint_as_float(s[p][c]), f2, fmaf(slope2, (float)(32 * p + c), at)));
+  } else {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        s[p][c] = __float_as_uint(fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), __uint_as_float(s[p][c]) * f2));
+  }
+}
+
 template <typename T, int DP, bool CAP, bool BIAS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const TcArgs t) {
   using L = Layout<DP, PAIR>;
   constexpr int kStages = L::kStages;
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   const Args& a = t.a;
-  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const uint32_t bars = base + L::kBars;
+  const uint32_t base = smem_u32(raw), bars = base + L::kBars;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + 64 + s * 8; };
   auto sfull = [&](int w) { return bars + 128 + w * 8; };
   auto pfull = [&](int w) { return bars + 144 + w * 8; };
   auto odone = [&](int w) { return bars + 160 + w * 8; };
-  const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320;
+  const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320, halves = bars + 512;
+  auto xbar = [&](int w) { return bars + 384 + w * 8; };
   const int warp = threadIdx.x >> 5;
 
   // block -> (row block, part of the key axis, sequence, packed head); late row blocks have the most keys under a causal
@@ -86,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-      for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 4), mbar_init(odone(w), 1);
+      for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 8), mbar_init(odone(w), 1), mbar_init(xbar(w), 8);
       mbar_init(qfull, 1);
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place + 16), "r"(lim.len), "r"(lim.start), "r"(lim.prefix), "r"(0) : "memory");
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(hp), "r"(b), "r"(split), "r"(row0) : "memory");
@@ -104,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto ts = [&](int w) { return tmem + (uint32_t)w * kTile; };                  // scores, then weights
   auto to = [&](int w) { return tmem + 2 * kTile + (uint32_t)w * DP; };  // accumulators
 
-  if (warp >= 8) {
+  if (warp >= kMmaWarp) {
     tc::reg_release<kRegsOther>();
     if (warp == kLoadWarp) {
       TileWalk walk(ktab, first, last, lab.lo, lab.hi);
@@ -173,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && w == 0 && more) ok = ready(2 * i + 2);
             tc_fence_after();
             if (ok && elect_one()) {
-              issue_weighted<T, DP, false>(to(w), ts(w), stage(2 * i + 1), i > 0);
+              issue_weighted<T, DP, true>(to(w), ts(w), stage(2 * i + 1), i > 0);
               if (w == 1) mma_commit(empty((2 * i + 1) % kStages));
               if (more) {
                 issue_scores<T, DP>(ts(w), base + w * L::kTileBytes, stage(2 * i + 2));
@@ -202,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && wait_bar(pfull(w), (uint32_t)(i >> 1) & 1);
           tc_fence_after();
           if (ok && elect_one()) {
-            issue_weighted<T, DP, false>(to(w), ts(w), stage(2 * i + 1), i > 1);
+            issue_weighted<T, DP, true>(to(w), ts(w), stage(2 * i + 1), i > 1);
             mma_commit(empty((2 * i + 1) % kStages));
           }
           __syncwarp();
@@ -221,10 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     tc::reg_claim<kRegsSoftmax>();
-    const int w = warp >> 2, lane_row = threadIdx.x & 127;
+    const int w = warp >> 3, side = (warp >> 2) & 1;       // score tile; half of its columns
     const uint32_t lane_at = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in bits 16 and up
-    const int r = row0 + (PAIR ? w * kTile : 0) + lane_row;  // packed row
-    const bool live = (r & ~31) < t.rows;                     // some row of this warp exists
+    const int r = row0 + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);  // packed row
+    const bool live = (r & ~31) < t.rows;                                   // some row of this warp exists
+    const uint32_t mine = halves + (w * 256 + side * 128 + (threadIdx.x & 127)) * 4, other = side == 0 ? mine + 512 : mine - 512;
     const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
     const bool exists = r < t.rows;
     const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
@@ -238,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const LabelRange mine = labels_of(qd, min(tile_i0, a.nq), min(a.nq, (tile_i0 + (kTile >> t.pg_shift))));
         if (!mine.bad && mine.lo == mine.hi) only = mine.lo;
       }
-      // all four warps write the same
+      // all eight warps write the same
       asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(rule), "r"(lim.row_end(min(tile_i0, a.nq - 1), a.causal)), "r"(only) : "memory");
       __syncwarp();
     }
@@ -246,35 +267,43 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY;       // of the weights, base 2
     float l = 0.f;
     bool ok = true;
+    // what the two threads of a row tell each other: one value per phase of `xbar`, which all warps of the tile pass
+    uint32_t phase = 0;
+    auto exchange = [&](float v, float& theirs) {
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine), "f"(v) : "memory");
+      __syncwarp();
+      if (elect_one()) mbar_arrive(xbar(w));
+      __syncwarp();
+      const bool ok = wait_bar(xbar(w), phase & 1);
+      ++phase;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(theirs) : "r"(other) : "memory");
+      return ok;
+    };
     for (int step = PAIR ? 0 : w; step < steps; step += PAIR ? 1 : 2) {
       ok = wait_bar(sfull(w), (uint32_t)(PAIR ? step : step >> 1) & 1);
       if (!ok) break;
       if (!live) {  // the weights of rows that do not exist reach nothing
-        if (elect_one()) mbar_arrive(pfull(w));
+        if (elect_one()) {
+          mbar_arrive(xbar(w));
+          mbar_arrive(pfull(w));
+        }
         __syncwarp();
         continue;
       }
       tc_fence_after();
       const Tile e = get_tile(slots, step);
-      const int k0 = e.at * kTile;
+      const int k0 = e.at * kTile + 64 * side;
       int all_before, only;
       asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(all_before), "=r"(only) : "r"(rule) : "memory");
-      const bool whole = k0 + kTile <= all_before && (a.kdocs == nullptr || (e.label >= 0 && e.label == only));
-      uint32_t s[4][32];
-      const uint32_t at = ts(w) + lane_at;
+      const bool whole = k0 + 64 <= all_before && (a.kdocs == nullptr || (e.label >= 0 && e.label == only));
+      uint32_t s[2][32];
+      const uint32_t at = ts(w) + lane_at + 64 * side;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) tmem_ld32(at + 32 * p, s[p]);
+      for (int p = 0; p < 2; ++p) tmem_ld32(at + 32 * p, s[p]);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) tmem_ld_wait_on(s[p]);
+      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
       if constexpr (CAP) to_tanh(s, a.scale);
-      if constexpr (BIAS) {
-        const float d0 = (float)(pos - k0);
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            s[p][c] = __float_as_uint(fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), __uint_as_float(s[p][c]) * f2));
-      }
+      if constexpr (BIAS) add_bias(s, f2, slope2, (float)(pos - k0));
       if (!whole) {
         const int4 x = get_place(place + 16);
         const int r = row0 + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
@@ -283,26 +312,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int* labels = a.kdocs == nullptr ? nullptr : a.kdocs + (int64_t)b * a.nk_pad + k0;
         const int my = labels != nullptr && r < t.rows ? __ldg(a.qdocs + (int64_t)b * a.nq_pad + (r >> t.pg_shift)) : -2;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) hide_columns(s[p], seen_columns(end - k0 - 32 * p, labels == nullptr ? nullptr : labels + 32 * p, my));
+        for (int p = 0; p < 2; ++p) hide_columns(s[p], seen_columns(end - k0 - 32 * p, labels == nullptr ? nullptr : labels + 32 * p, my));
       }
       float top[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        top[p] = __uint_as_float(s[p][0]);
+        const int c0 = 16 * (p & 1);
+        top[p] = fmaxf(__uint_as_float(s[p / 2][c0]), __uint_as_float(s[p / 2][c0 + 1]));
 #pragma unroll
-        for (int c = 1; c < 31; c += 2) top[p] = fmaxf(fmaxf(top[p], __uint_as_float(s[p][c])), __uint_as_float(s[p][c + 1]));
-        top[p] = fmaxf(top[p], __uint_as_float(s[p][31]));
+        for (int c = 2; c < 16; c += 2) top[p] = fmaxf(fmaxf(top[p], __uint_as_float(s[p / 2][c0 + c])), __uint_as_float(s[p / 2][c0 + c + 1]));
       }
-      float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), theirs;
+      ok = exchange(mt, theirs);
+      if (!ok) break;
+      mt = fmaxf(mt, theirs);
       if constexpr (!BIAS) mt *= f2;
-      const bool grow = mt > m + 8.f || (m == -INFINITY && mt != -INFINITY);
+      const bool grow = mt > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float mn = grow ? mt : m;
         const float f = m == mn ? 1.f : ex2_approx(m - mn);
         if (step > (PAIR ? 0 : 1)) {
           // s_full of this step says that the weighted sums before it are done
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 16) {
+          for (int c = side * (DP / 2); c < (side + 1) * (DP / 2); c += 16) {
             uint32_t o[16];
             tc::tmem_ld16(to(w) + lane_at + c, o);
             tmem_ld_wait_on(o);
@@ -316,23 +348,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float mb = m == -INFINITY ? 0.f : m;
       const uint64_t f2v = tc::pack2(f2, f2), mv = tc::pack2(-mb, -mb);
-      uint64_t sum[2] = {0, 0};
+      uint64_t sum = 0;
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        uint32_t o[16];
+        uint32_t o[8];
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const uint32_t s0 = s[p][c], s1 = s[p][c + 1];
-          const uint64_t v = tc::pack2(__uint_as_float(s0), __uint_as_float(s1));
+        for (int c = 0; c < 16; c += 2) {
+          const int at = 16 * (p & 1) + c;
+          const uint64_t v = tc::pack2(__uint_as_float(s[p / 2][at]), __uint_as_float(s[p / 2][at + 1]));
           const uint64_t x = BIAS ? tc::add2(v, mv) : tc::fma2(v, f2v, mv);
           float x0, x1, p0, p1;
           tc::unpack2(x, x0, x1);
           p0 = ex2_approx(x0);
           p1 = ex2_approx(x1);
-          sum[(c / 2) & 1] = tc::add2(sum[(c / 2) & 1], tc::pack2(p0, p1));
+          sum = tc::add2(sum, tc::pack2(p0, p1));
           o[c / 2] = pack16<T>(p0, p1);
         }
-        tmem_st16(at + 16 * p, o);
+        tmem_st8(at + 8 * p, o);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -340,12 +372,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) mbar_arrive(pfull(w));
       __syncwarp();
       float u0, u1;
-      tc::unpack2(tc::add2(sum[0], sum[1]), u0, u1);
+      tc::unpack2(sum, u0, u1);
       l += u0 + u1;
     }
     // ---- results
     const bool worked = steps > (PAIR ? 0 : w);
-    if (worked && ok) ok = wait_bar(odone(w), 0);
+    if (worked && ok) {
+      // the products being done, all warps of the tile have passed the last step's exchange
+      ok = wait_bar(odone(w), 0);
+      float theirs = 0.f;
+      if (ok && live)
+        ok = exchange(l, theirs);
+      else if (elect_one())
+        mbar_arrive(xbar(w));
+      __syncwarp();
+      l = side == 0 ? l + theirs : theirs + l;  // the same sum on both sides
+    }
     tc_fence_after();
     const bool none = m == -INFINITY;
     const float inv = none ? 0.f : 1.0f / l, lse2 = none ? -INFINITY : m + log2f(l);
@@ -358,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool parts = !PAIR || t.splits > 1;
       const int part = PAIR ? split : 2 * split + w;
       const int64_t prow = (((int64_t)part * a.b + b) * t.hp + hp) * t.rows + r;
-      if (exists) {
+      if (exists && side == 0) {
         if (parts)
           t.part_lse[prow] = lse2;
         else if (a.lse != nullptr)
@@ -367,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       T* out = reinterpret_cast<T*>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
       T* lo = a.o_lo == nullptr ? nullptr : reinterpret_cast<T*>(a.o_lo) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = side * (DP / 2); c < (side + 1) * (DP / 2); c += 32) {
         uint32_t o[32];
         if (worked) {
           tmem_ld32(to(w) + lane_at + c, o);
