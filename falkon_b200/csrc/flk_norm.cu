@@ -4,12 +4,15 @@
 //   forward    y = xh * w + b                        (mu and r are kept for the backward pass, in fp32)
 //   backward   g = dy * w,   dx = r (g - mean(g) - xh mean(g xh)),   dw = sum_rows dy xh,   db = sum_rows dy
 //
-// Both passes are bound by HBM: forward moves 2 row lengths per row, backward 3.  A row is therefore read once, kept in
-// registers by the group of threads that owns it, and every statistic is taken from those registers (the variance from
-// the centred values, so a large mean costs no digits).  The grid is persistent: a group walks over rows, holds its
-// slice of w (and, backward, its partial sums of dw and db) in registers all along, and issues the loads of its next row
-// before it reduces the present one.  dw and db: every block adds up its groups in a fixed order and writes one partial
-// row; a second kernel adds the partial rows, also in a fixed order, so results do not depend on timing.
+// Both passes are bound by HBM: forward moves 2 row lengths per row, backward 3.  A row is therefore read once, and every
+// statistic is taken from registers (the variance from the centred values, so a large mean costs no digits).  Rows whose
+// address and length are multiples of 16 bytes, up to 16384 values, go through the ring kernels: the threads that share a row (16
+// values each) copy the rows that come next into a ring in shared memory (cp.async, every thread its own pieces, so nothing
+// but the copies' own completion is waited for), and 4 rows are under way while one is worked on.  That keeps over 64 KB per SM
+// in flight without spending registers on it.  Other rows use plain loads, or, above 16384 values, are read more than once.
+// The grid is persistent.  dw and db: every thread adds up its columns in registers over all its rows, every block adds up its
+// groups in a fixed order and writes one partial row; a second kernel adds the partial rows, also in a fixed order, so results
+// do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -349,6 +352,236 @@ __global__ void __launch_bounds__(1024) backward_long_kernel(const Args a) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// ring kernels
+// ---------------------------------------------------------------------------------------------------------------------
+// Shared memory: w (and, forward, b) as fp32, in the order the threads read it (16 bytes per thread and step), then the ring.
+// Piece p of a row belongs to thread p % tpr of its group.
+template <int VEC>
+__device__ __forceinline__ void fill_columns(float* dst, const void* src, int dtype, float missing, int d, int tpr) {
+  const int packs = d / VEC;
+  for (int e = threadIdx.x; e < packs * (VEC / 4); e += blockDim.x) {
+    const int p = e / (VEC / 4), q = e % (VEC / 4), lane = p % tpr, i = p / tpr;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = p * VEC + 4 * q + k;
+      dst[(((i * (VEC / 4)) + q) * tpr + lane) * 4 + k] = src != nullptr ? load_any(src, dtype, c) : missing;
+    }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void read_columns(float (&v)[VEC], const float* src, int i, int lane, int tpr) {
+#pragma unroll
+  for (int q = 0; q < VEC / 4; ++q) {
+    const float4 x = *reinterpret_cast<const float4*>(src + (((i * (VEC / 4)) + q) * tpr + lane) * 4);
+    v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+  }
+}
+template <typename T, int VEC, int V>
+__device__ __forceinline__ void copy_row(char* slot, const T* row, int lane, int tpr, int packs) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (lane + i * tpr < packs) cp_async16(slot + (i * blockDim.x + threadIdx.x) * 16, row + (int64_t)(lane + i * tpr) * VEC);
+}
+
+template <typename T, int V, int STAGES>
+__global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) float cols[];
+  __shared__ float red[2 * 32];
+  const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
+  float *w = cols, *b = cols + a.tpr * V * VEC;
+  char* ring = reinterpret_cast<char*>(cols + 2 * a.tpr * V * VEC);
+  const int stage_bytes = blockDim.x * V * 16;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  T* y = reinterpret_cast<T*>(a.y);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) {
+    if (row + s * step < a.n) copy_row<T, VEC, V>(ring + s * stage_bytes, x + a.xr.at(row + s * step), lane, a.tpr, packs);
+    cp_async_commit();
+  }
+  fill_columns<VEC>(w, a.w, a.wdtype, 1.f, a.d, a.tpr);
+  fill_columns<VEC>(b, a.b, a.wdtype, 0.f, a.d, a.tpr);
+  __syncthreads();
+  int flip = 0, at = 0;
+  // every group makes the same number of turns, so that the barriers inside the sums match
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.n; r0 += step, row += step) {
+    const bool on = row < a.n;
+    char* slot = ring + at * stage_bytes;
+    at = at + 1 == STAGES ? 0 : at + 1;
+    cp_async_wait<STAGES - 1>();
+    float v[V][VEC];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const bool have = on && lane + i * a.tpr < packs;
+      Pack<T, VEC> raw;
+      if (have) raw = *reinterpret_cast<const Pack<T, VEC>*>(slot + (i * blockDim.x + threadIdx.x) * 16);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = have ? to_f<T>(raw.v[j]) : 0.f;
+        s[0] += v[i][j];
+      }
+    }
+    if (row + STAGES * step < a.n) copy_row<T, VEC, V>(slot, x + a.xr.at(row + STAGES * step), lane, a.tpr, packs);
+    cp_async_commit();
+    group_sum<1>(s, a.tpr, red, flip);
+    const float mu = s[0] * a.inv_d;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = lane + i * a.tpr < packs ? v[i][j] - mu : 0.f;
+        s[0] = fmaf(v[i][j], v[i][j], s[0]);
+      }
+    group_sum<1>(s, a.tpr, red, flip);
+    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    if (on) {
+      if (lane == 0 && a.mean != nullptr) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int p = lane + i * a.tpr;
+        if (p >= packs) continue;
+        float ww[VEC], bb[VEC];
+        read_columns<VEC>(ww, w, i, lane, a.tpr);
+        read_columns<VEC>(bb, b, i, lane, a.tpr);
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out.v[j] = from_f<T>(fmaf(v[i][j] * r, ww[j], bb[j]));
+        *reinterpret_cast<Pack<T, VEC>*>(y + row * a.d + (int64_t)p * VEC) = out;
+      }
+    }
+  }
+}
+
+template <typename T, int V, int STAGES, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) float cols[];
+  __shared__ float red[2 * 32 * 2];
+  const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
+  const int stage_bytes = blockDim.x * V * 32 + blockDim.x * 8;
+  float* w = cols;
+  char* ring = reinterpret_cast<char*>(cols + a.tpr * V * VEC);
+  const T *x = reinterpret_cast<const T*>(a.x), *dy = reinterpret_cast<const T*>(a.dy);
+  T* dx = reinterpret_cast<T*>(a.dx);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  // the first lane of a group in each warp fetches mean and rstd for it
+  const int lead = threadIdx.x & ~((a.tpr < 32 ? a.tpr : 32) - 1);
+  auto fetch = [&](char* slot, int64_t r) {
+    copy_row<T, VEC, V>(slot, x + a.xr.at(r), lane, a.tpr, packs);
+    copy_row<T, VEC, V>(slot + blockDim.x * V * 16, dy + a.dyr.at(r), lane, a.tpr, packs);
+    if ((int)threadIdx.x == lead) {
+      cp_async_small<4>(slot + blockDim.x * V * 32 + threadIdx.x * 8, a.mean + r);
+      cp_async_small<4>(slot + blockDim.x * V * 32 + threadIdx.x * 8 + 4, a.rstd + r);
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) {
+    if (row + s * step < a.n) fetch(ring + s * stage_bytes, row + s * step);
+    cp_async_commit();
+  }
+  fill_columns<VEC>(w, a.w, a.wdtype, 1.f, a.d, a.tpr);
+  __syncthreads();
+  float dw[V][VEC], db[V][VEC];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
+  int flip = 0, at = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.n; r0 += step, row += step) {
+    const bool on = row < a.n;
+    char* slot = ring + at * stage_bytes;
+    at = at + 1 == STAGES ? 0 : at + 1;
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const float2 st = *reinterpret_cast<const float2*>(slot + blockDim.x * V * 32 + lead * 8);
+    const float mu = on ? st.x : 0.f, r = on ? st.y : 0.f;
+    // what the second half of the work needs again: with 1024 threads, which have 64 registers, the raw pieces
+    constexpr bool kRaw = THREADS == 1024;
+    float g[kRaw ? 1 : V][VEC], xh[kRaw ? 1 : V][VEC], s[2] = {0.f, 0.f};
+    Pack<T, VEC> kx[kRaw ? V : 1], kg[kRaw ? V : 1];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const bool have = on && lane + i * a.tpr < packs;
+      Pack<T, VEC> px, pg;
+      float ww[VEC];
+      if (have) {
+        px = *reinterpret_cast<const Pack<T, VEC>*>(slot + (i * blockDim.x + threadIdx.x) * 16);
+        pg = *reinterpret_cast<const Pack<T, VEC>*>(slot + ((V + i) * blockDim.x + threadIdx.x) * 16);
+        read_columns<VEC>(ww, w, i, lane, a.tpr);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float g0 = have ? to_f<T>(pg.v[j]) : 0.f;
+        const float h = have ? (to_f<T>(px.v[j]) - mu) * r : 0.f, gw = have ? g0 * ww[j] : 0.f;
+        if constexpr (!kRaw) xh[i][j] = h, g[i][j] = gw;
+        s[0] += gw;
+        s[1] = fmaf(gw, h, s[1]);
+        dw[i][j] = fmaf(g0, h, dw[i][j]);
+        db[i][j] += g0;
+      }
+      if constexpr (kRaw) kx[i] = px, kg[i] = pg;
+    }
+    __syncwarp();  // the slot's mean and rstd have been read
+    if (row + STAGES * step < a.n) fetch(slot, row + STAGES * step);
+    cp_async_commit();
+    group_sum<2>(s, a.tpr, red, flip);
+    const float m1 = s[0] * a.inv_d, m2 = s[1] * a.inv_d;
+    if (on && dx != nullptr) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int p = lane + i * a.tpr;
+        if (p >= packs) continue;
+        Pack<T, VEC> out;
+        float ww[VEC];
+        if constexpr (kRaw) read_columns<VEC>(ww, w, i, lane, a.tpr);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float h, gw;
+          if constexpr (kRaw)
+            h = (to_f<T>(kx[i].v[j]) - mu) * r, gw = to_f<T>(kg[i].v[j]) * ww[j];
+          else
+            h = xh[i][j], gw = g[i][j];
+          out.v[j] = from_f<T>((gw - m1 - h * m2) * r);
+        }
+        *reinterpret_cast<Pack<T, VEC>*>(dx + row * a.d + (int64_t)p * VEC) = out;
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  cp_async_wait<0>();
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.d;
+  float* sums = reinterpret_cast<float*>(ring);  // [groups][d]: no more than threads * V * VEC values, the ring is larger
+  for (int which = 0; which < 2; ++which) {
+    if (groups > 1) __syncthreads();
+    float* to = groups > 1 ? sums + group * a.d : part + which * a.d;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (lane + i * a.tpr >= packs) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        const float(&v)[VEC] = which == 0 ? dw[i] : db[i];
+        *reinterpret_cast<float4*>(to + (lane + i * a.tpr) * VEC + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    }
+    if (groups == 1) continue;
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      float t = 0.f;
+      for (int q = 0; q < groups; ++q) t += sums[q * a.d + c];
+      part[which * a.d + c] = t;
+    }
+  }
+}
+
 // dw, db = sums of the blocks' partial rows: 32 columns per block, 8 slices of partial rows added side by side and then
 // in order.
 __global__ void __launch_bounds__(256) reduce_kernel(const float* part, int64_t blocks, int d, void* dw, void* db, int wdtype) {
@@ -370,39 +603,54 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* part, int64_t 
 
 // How a call is laid out: values per load, loads per thread, threads per row and per block, blocks.
 struct Plan {
-  int vec, v, tpr, threads;
+  int vec, v, tpr, threads, stages;
   bool is_long;
   int64_t blocks;
+  size_t smem;
 };
 
-// Threads per row: the fewest (a power of two) whose registers hold the row; short rows share a block of 256 threads.
-// `most` is the number of values a thread may hold (its registers hold them once forward, up to four times backward).
 static Plan make_plan(int esize, int64_t n, int64_t d, bool aligned, bool backward) {
   Plan p{};
   const int full = 16 / esize;
-  p.vec = aligned && d % full == 0 ? full : 1;
-  const int64_t packs = d / p.vec;
-  const int choices_vec[3] = {1, 2, 4}, choices_one[3] = {2, 8, 16};
-  p.is_long = true;
-  for (int i = 0; i < 3 && p.is_long; ++i) {
-    p.v = p.vec == 1 ? choices_one[i] : choices_vec[i];
-    const int values = p.v * p.vec;
-    const int limit = backward ? (values > 16 ? 256 : values > 8 ? 512 : 1024) : (values > 16 ? 512 : 1024);
-    int tpr = 4;
-    while ((int64_t)tpr * p.v < packs) tpr <<= 1;
-    // two 16-byte loads per thread and array keep enough bytes in flight; one would not
-    if (tpr <= limit && (i > 0 || tpr <= 32)) {
-      p.tpr = tpr;
-      p.is_long = false;
+  int64_t resident;
+  if (aligned && d % full == 0 && d <= 16384) {
+    // ring kernels: 16 values per thread, fewer where a row has no more than 4 pieces
+    p.vec = full;
+    const int64_t packs = d / full;
+    p.v = 16 / full;
+    while (p.v > 1 && packs <= p.v * 2) p.v >>= 1;
+    p.tpr = 1;
+    while ((int64_t)p.tpr * p.v < packs) p.tpr <<= 1;
+    p.threads = p.tpr < 256 ? 256 : p.tpr;
+    const size_t columns = (size_t)p.tpr * p.v * full * 4 * (backward ? 1 : 2);
+    const size_t stage = backward ? (size_t)p.threads * (p.v * 32 + 8) : (size_t)p.threads * p.v * 16;
+    p.stages = columns + 4 * stage <= 224 * 1024 ? 4 : columns + 2 * stage <= 224 * 1024 ? 2 : 1;
+    p.smem = columns + p.stages * stage;
+    // blocks per SM: by shared memory, and by registers (about 64 a thread forward, 96 backward)
+    resident = (int64_t)(224 * 1024 / (p.smem + 1024));
+    const int64_t by_regs = (backward ? 640 : 1024) / p.threads;
+    if (resident > by_regs) resident = by_regs;
+  } else {
+    p.vec = 1;
+    p.is_long = true;
+    const int choices[3] = {2, 8, 16};
+    for (int i = 0; i < 3 && p.is_long; ++i) {
+      p.v = choices[i];
+      const int limit = backward ? (p.v > 8 ? 512 : 1024) : 1024;
+      int tpr = 4;
+      while ((int64_t)tpr * p.v < d) tpr <<= 1;
+      if (tpr <= limit && (i > 0 || tpr <= 32)) {
+        p.tpr = tpr;
+        p.is_long = false;
+      }
     }
+    if (p.is_long) p.tpr = 1024, p.v = 1;
+    p.threads = p.tpr < 256 ? 256 : p.tpr;
+    p.smem = backward && !p.is_long && p.tpr < p.threads ? (size_t)(p.threads / p.tpr) * d * 4 : 0;
+    resident = backward ? (p.v > 8 ? 512 : 1024) / p.threads : 2048 / p.threads;
   }
-  if (p.is_long) p.tpr = 1024, p.v = 1, p.vec = 1;
-  p.threads = p.tpr < 256 ? 256 : p.tpr;
-  const int64_t groups = p.threads / p.tpr;
-  int64_t resident = 2048 / p.threads;
-  if (backward) resident = p.threads >= 1024 ? 1 : (p.v * p.vec > 8 ? 512 : 1024) / p.threads;
   if (resident < 1) resident = 1;
-  const int64_t need = ceil_div(n, groups);
+  const int64_t need = ceil_div(n, p.threads / p.tpr);
   p.blocks = need < kNumSMs * resident ? need : kNumSMs * resident;
   if (p.blocks < 1) p.blocks = 1;
   return p;
@@ -412,29 +660,48 @@ static bool is_aligned(const void* p, int64_t s0, int64_t s1, int esize) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 * esize % 16 == 0 && s1 * esize % 16 == 0;
 }
 
-#define FLK_NORM_LAUNCH(KERNEL, VECFULL, SMEM)                                                                          \
-  if (p.is_long) KERNEL##_long_kernel<T><<<(unsigned)p.blocks, p.threads, 0, st>>>(a);                                  \
-  else if (p.vec > 1 && p.v == 1) KERNEL##_kernel<T, VECFULL, 1><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);       \
-  else if (p.vec > 1 && p.v == 2) KERNEL##_kernel<T, VECFULL, 2><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);       \
-  else if (p.vec > 1) KERNEL##_kernel<T, VECFULL, 4><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                   \
-  else if (p.v == 2) KERNEL##_kernel<T, 1, 2><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                          \
-  else if (p.v == 8) KERNEL##_kernel<T, 1, 8><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);                          \
-  else KERNEL##_kernel<T, 1, 16><<<(unsigned)p.blocks, p.threads, SMEM, st>>>(a);
-
-template <typename T>
-static void launch_forward(const Args& a, const Plan& p, cudaStream_t st) {
-  FLK_NORM_LAUNCH(forward, (16 / (int)sizeof(T)), 0)
+static int run(void (*fn)(const Args), const Args& a, const Plan& p, cudaStream_t st) {
+  if (p.smem > 40 * 1024) FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+  fn<<<(unsigned)p.blocks, p.threads, p.smem, st>>>(a);
   count_launch();
+  return FLK_OK;
 }
 
-// Several groups share a block only up to 128 threads per row, at most 64 * 32 * 64 ... values: the sums of a block's
-// groups take threads * V * VEC floats, 32 KB at most.
+template <typename T, int V>
+static int forward_ring(const Args& a, const Plan& p, cudaStream_t st) {
+  return p.stages == 4   ? run(forward_ring_kernel<T, V, 4>, a, p, st)
+         : p.stages == 2 ? run(forward_ring_kernel<T, V, 2>, a, p, st)
+                         : run(forward_ring_kernel<T, V, 1>, a, p, st);
+}
 template <typename T>
-static void launch_backward(const Args& a, const Plan& p, cudaStream_t st) {
-  const int groups = p.threads / p.tpr;
-  const size_t smem = groups > 1 ? (size_t)groups * a.d * 4 : 0;
-  FLK_NORM_LAUNCH(backward, (16 / (int)sizeof(T)), smem)
-  count_launch();
+static int launch_forward(const Args& a, const Plan& p, cudaStream_t st) {
+  if (p.is_long) return run(forward_long_kernel<T>, a, p, st);
+  if (p.vec == 1) return p.v == 2 ? run(forward_kernel<T, 1, 2>, a, p, st) : p.v == 8 ? run(forward_kernel<T, 1, 8>, a, p, st) : run(forward_kernel<T, 1, 16>, a, p, st);
+  if (p.v == 1) return forward_ring<T, 1>(a, p, st);
+  if (p.v == 2) return forward_ring<T, 2>(a, p, st);
+  if constexpr (sizeof(T) == 4) return forward_ring<T, 4>(a, p, st);
+  return fail(FLK_ERR_UNSUPPORTED, "no kernel for %d loads per thread", p.v);
+}
+
+template <typename T, int V>
+static int backward_ring(const Args& a, const Plan& p, cudaStream_t st) {
+  if (p.threads == 1024) {
+    if (p.stages == 4) return run(backward_ring_kernel<T, V, 4, 1024>, a, p, st);
+    if (p.stages == 2) return run(backward_ring_kernel<T, V, 2, 1024>, a, p, st);
+    return run(backward_ring_kernel<T, V, 1, 1024>, a, p, st);
+  }
+  if (p.stages == 4) return run(backward_ring_kernel<T, V, 4, 512>, a, p, st);
+  if (p.stages == 2) return run(backward_ring_kernel<T, V, 2, 512>, a, p, st);
+  return run(backward_ring_kernel<T, V, 1, 512>, a, p, st);
+}
+template <typename T>
+static int launch_backward(const Args& a, const Plan& p, cudaStream_t st) {
+  if (p.is_long) return run(backward_long_kernel<T>, a, p, st);
+  if (p.vec == 1) return p.v == 2 ? run(backward_kernel<T, 1, 2>, a, p, st) : p.v == 8 ? run(backward_kernel<T, 1, 8>, a, p, st) : run(backward_kernel<T, 1, 16>, a, p, st);
+  if (p.v == 1) return backward_ring<T, 1>(a, p, st);
+  if (p.v == 2) return backward_ring<T, 2>(a, p, st);
+  if constexpr (sizeof(T) == 4) return backward_ring<T, 4>(a, p, st);
+  return fail(FLK_ERR_UNSUPPORTED, "no kernel for %d loads per thread", p.v);
 }
 
 static int esize_of(int dtype) { return dtype == FLK_F32 ? 4 : 2; }
@@ -481,9 +748,9 @@ int flk_layer_norm_forward(const flk_layer_norm_args* p, void* stream) {
   const norm::Plan plan = norm::plan_of(p, false);
   a.tpr = plan.tpr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == FLK_F32) norm::launch_forward<float>(a, plan, st);
-  else if (p->dtype == FLK_BF16) norm::launch_forward<__nv_bfloat16>(a, plan, st);
-  else norm::launch_forward<__half>(a, plan, st);
+  if (p->dtype == FLK_F32) FLK_TRY(norm::launch_forward<float>(a, plan, st));
+  else if (p->dtype == FLK_BF16) FLK_TRY(norm::launch_forward<__nv_bfloat16>(a, plan, st));
+  else FLK_TRY(norm::launch_forward<__half>(a, plan, st));
   FLK_CUDA_TRY(cudaGetLastError());
   return FLK_OK;
 }
@@ -517,9 +784,9 @@ int flk_layer_norm_backward(const flk_layer_norm_args* p, void* stream) {
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p->n > 0) {
-    if (p->dtype == FLK_F32) norm::launch_backward<float>(a, plan, st);
-    else if (p->dtype == FLK_BF16) norm::launch_backward<__nv_bfloat16>(a, plan, st);
-    else norm::launch_backward<__half>(a, plan, st);
+    if (p->dtype == FLK_F32) FLK_TRY(norm::launch_backward<float>(a, plan, st));
+    else if (p->dtype == FLK_BF16) FLK_TRY(norm::launch_backward<__nv_bfloat16>(a, plan, st));
+    else FLK_TRY(norm::launch_backward<__half>(a, plan, st));
   }
   if (sums) {
     norm::reduce_kernel<<<dim3((unsigned)ceil_div(p->d, 32), 2), 256, 0, st>>>(a.part, p->n > 0 ? plan.blocks : 0, a.d,
