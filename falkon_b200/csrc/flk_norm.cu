@@ -100,12 +100,12 @@ __device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float* red, in
     for (int k = 0; k < K; ++k) buf[warp * K + k] = v[k];
   }
   __syncthreads();
-  const int warps = tpr >> 5, first = warp / warps * warps;
+  const int warps = tpr >> 5, first = warp / warps * warps, at = threadIdx.x & 31;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float s = 0.f;
-    for (int i = 0; i < warps; ++i) s += buf[(first + i) * K + k];
-    v[k] = s;
+  for (int k = 0; k < K; ++k) v[k] = at < warps ? buf[(first + at) * K + k] : 0.f;
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   }
 }
 
@@ -625,6 +625,8 @@ static Plan make_plan(int esize, int64_t n, int64_t d, bool aligned, bool backwa
     const size_t columns = (size_t)p.tpr * p.v * full * 4 * (backward ? 1 : 2);
     const size_t stage = backward ? (size_t)p.threads * (p.v * 32 + 8) : (size_t)p.threads * p.v * 16;
     p.stages = columns + 4 * stage <= 224 * 1024 ? 4 : columns + 2 * stage <= 224 * 1024 ? 2 : 1;
+    // forward, two blocks with two stages each hide each other's barriers
+    if (!backward && p.stages == 4 && columns + 4 * stage > 110 * 1024 && columns + 2 * stage <= 110 * 1024) p.stages = 2;
     p.smem = columns + p.stages * stage;
     // blocks per SM: by shared memory, and by registers (about 64 a thread forward, 96 backward)
     resident = (int64_t)(224 * 1024 / (p.smem + 1024));
