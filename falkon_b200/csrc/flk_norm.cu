@@ -16,7 +16,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "flk_common.cuh"
+#include "flk_ptx.cuh"
 
 namespace flk {
 namespace norm {
@@ -369,12 +372,60 @@ __device__ __forceinline__ void fill_columns(float* dst, const void* src, int dt
     }
   }
 }
-template <int VEC>
-__device__ __forceinline__ void read_columns(float (&v)[VEC], const float* src, int i, int lane, int tpr) {
+// Values are worked on in pairs (packed fp32): these kernels are short of issue slots before they are short of anything else but
+// HBM.  16 bytes of T <-> pairs:
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& raw, uint64_t (&f)[8 / sizeof(T)]) {
+  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (sizeof(T) == 4) {
+    f[0] = tc::pack2(__uint_as_float(u[0]), __uint_as_float(u[1]));
+    f[1] = tc::pack2(__uint_as_float(u[2]), __uint_as_float(u[3]));
+  } else {
 #pragma unroll
-  for (int q = 0; q < VEC / 4; ++q) {
-    const float4 x = *reinterpret_cast<const float4*>(src + (((i * (VEC / 4)) + q) * tpr + lane) * 4);
-    v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
+        f[k] = tc::pack2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xffff0000u));
+      } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+        f[k] = tc::pack2(v.x, v.y);
+      }
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 from_pairs(const uint64_t (&f)[8 / sizeof(T)]) {
+  uint32_t u[4];
+  float x, y;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      tc::unpack2(f[k], x, y);
+      u[2 * k] = __float_as_uint(x), u[2 * k + 1] = __float_as_uint(y);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      tc::unpack2(f[k], x, y);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[k]) : "f"(y), "f"(x));
+      else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[k]) : "f"(y), "f"(x));
+    }
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ uint64_t both(float v) { return tc::pack2(v, v); }
+__device__ __forceinline__ float sum2(uint64_t v) {
+  float x, y;
+  tc::unpack2(v, x, y);
+  return x + y;
+}
+template <int NP>
+__device__ __forceinline__ void read_columns(uint64_t (&v)[NP], const float* src, int i, int lane, int tpr) {
+#pragma unroll
+  for (int q = 0; q < NP / 2; ++q) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(src + (((i * (NP / 2)) + q) * tpr + lane) * 4);
+    v[2 * q] = x.x, v[2 * q + 1] = x.y;
   }
 }
 template <typename T, int VEC, int V>
@@ -386,7 +437,7 @@ __device__ __forceinline__ void copy_row(char* slot, const T* row, int lane, int
 
 template <typename T, int V, int STAGES>
 __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
-  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), NP = VEC / 2;
   extern __shared__ __align__(16) float cols[];
   __shared__ float red[2 * 32];
   const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
@@ -412,31 +463,31 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
     char* slot = ring + at * stage_bytes;
     at = at + 1 == STAGES ? 0 : at + 1;
     cp_async_wait<STAGES - 1>();
-    float v[V][VEC];
-    float s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const bool have = on && lane + i * a.tpr < packs;
-      Pack<T, VEC> raw;
-      if (have) raw = *reinterpret_cast<const Pack<T, VEC>*>(slot + (i * blockDim.x + threadIdx.x) * 16);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] = have ? to_f<T>(raw.v[j]) : 0.f;
-        s[0] += v[i][j];
-      }
-    }
-    if (row + STAGES * step < a.n) copy_row<T, VEC, V>(slot, x + a.xr.at(row + STAGES * step), lane, a.tpr, packs);
-    cp_async_commit();
-    group_sum<1>(s, a.tpr, red, flip);
-    const float mu = s[0] * a.inv_d;
-    s[0] = 0.f;
+    uint64_t v[V][NP], acc = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i)
+      if (on && lane + i * a.tpr < packs) {
+        to_pairs<T>(*reinterpret_cast<const uint4*>(slot + (i * blockDim.x + threadIdx.x) * 16), v[i]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] = lane + i * a.tpr < packs ? v[i][j] - mu : 0.f;
-        s[0] = fmaf(v[i][j], v[i][j], s[0]);
+        for (int j = 0; j < NP; ++j) acc = tc::add2(acc, v[i][j]);
       }
+    if (row + STAGES * step < a.n) copy_row<T, VEC, V>(slot, x + a.xr.at(row + STAGES * step), lane, a.tpr, packs);
+    cp_async_commit();
+    float s[1] = {sum2(acc)};
+    group_sum<1>(s, a.tpr, red, flip);
+    const float mu = s[0] * a.inv_d;
+    const uint64_t mu2 = both(mu);
+    acc = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (on && lane + i * a.tpr < packs) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          v[i][j] = tc::sub2(v[i][j], mu2);
+          acc = tc::fma2(v[i][j], v[i][j], acc);
+        }
+      }
+    s[0] = sum2(acc);
     group_sum<1>(s, a.tpr, red, flip);
     const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
     if (on) {
@@ -444,17 +495,18 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
         a.mean[row] = mu;
         a.rstd[row] = r;
       }
+      const uint64_t r2 = both(r);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int p = lane + i * a.tpr;
-        if (p >= packs) continue;
-        float ww[VEC], bb[VEC];
-        read_columns<VEC>(ww, w, i, lane, a.tpr);
-        read_columns<VEC>(bb, b, i, lane, a.tpr);
-        Pack<T, VEC> out;
+        if (p < packs) {
+          uint64_t ww[NP], bb[NP];
+          read_columns<NP>(ww, w, i, lane, a.tpr);
+          read_columns<NP>(bb, b, i, lane, a.tpr);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) out.v[j] = from_f<T>(fmaf(v[i][j] * r, ww[j], bb[j]));
-        *reinterpret_cast<Pack<T, VEC>*>(y + row * a.d + (int64_t)p * VEC) = out;
+          for (int j = 0; j < NP; ++j) ww[j] = tc::fma2(tc::mul2(v[i][j], r2), ww[j], bb[j]);
+          *reinterpret_cast<uint4*>(y + row * a.d + (int64_t)p * VEC) = from_pairs<T>(ww);
+        }
       }
     }
   }
@@ -462,7 +514,7 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
 
 template <typename T, int V, int STAGES, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a) {
-  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), NP = VEC / 2;
   extern __shared__ __align__(16) float cols[];
   __shared__ float red[2 * 32 * 2];
   const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
@@ -490,11 +542,11 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
   }
   fill_columns<VEC>(w, a.w, a.wdtype, 1.f, a.d, a.tpr);
   __syncthreads();
-  float dw[V][VEC], db[V][VEC];
+  uint64_t dw[V][NP], db[V][NP];
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
+    for (int j = 0; j < NP; ++j) dw[i][j] = db[i][j] = 0;
   int flip = 0, at = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.n; r0 += step, row += step) {
     const bool on = row < a.n;
@@ -503,56 +555,59 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
     cp_async_wait<STAGES - 1>();
     __syncwarp();
     const float2 st = *reinterpret_cast<const float2*>(slot + blockDim.x * V * 32 + lead * 8);
-    const float mu = on ? st.x : 0.f, r = on ? st.y : 0.f;
+    const float r = st.y;
+    const uint64_t mu2 = both(st.x), r2 = both(r);
     // what the second half of the work needs again: with 1024 threads, which have 64 registers, the raw pieces
     constexpr bool kRaw = THREADS == 1024;
-    float g[kRaw ? 1 : V][VEC], xh[kRaw ? 1 : V][VEC], s[2] = {0.f, 0.f};
-    Pack<T, VEC> kx[kRaw ? V : 1], kg[kRaw ? V : 1];
+    uint64_t g[kRaw ? 1 : V][NP], xh[kRaw ? 1 : V][NP], acc[2] = {0, 0};
+    uint4 kx[kRaw ? V : 1], kg[kRaw ? V : 1];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const bool have = on && lane + i * a.tpr < packs;
-      Pack<T, VEC> px, pg;
-      float ww[VEC];
-      if (have) {
-        px = *reinterpret_cast<const Pack<T, VEC>*>(slot + (i * blockDim.x + threadIdx.x) * 16);
-        pg = *reinterpret_cast<const Pack<T, VEC>*>(slot + ((V + i) * blockDim.x + threadIdx.x) * 16);
-        read_columns<VEC>(ww, w, i, lane, a.tpr);
-      }
+    for (int i = 0; i < V; ++i)
+      if (on && lane + i * a.tpr < packs) {
+        const uint4 px = *reinterpret_cast<const uint4*>(slot + (i * blockDim.x + threadIdx.x) * 16);
+        const uint4 pg = *reinterpret_cast<const uint4*>(slot + ((V + i) * blockDim.x + threadIdx.x) * 16);
+        uint64_t ww[NP], fx[NP], fg[NP];
+        read_columns<NP>(ww, w, i, lane, a.tpr);
+        to_pairs<T>(px, fx);
+        to_pairs<T>(pg, fg);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float g0 = have ? to_f<T>(pg.v[j]) : 0.f;
-        const float h = have ? (to_f<T>(px.v[j]) - mu) * r : 0.f, gw = have ? g0 * ww[j] : 0.f;
-        if constexpr (!kRaw) xh[i][j] = h, g[i][j] = gw;
-        s[0] += gw;
-        s[1] = fmaf(gw, h, s[1]);
-        dw[i][j] = fmaf(g0, h, dw[i][j]);
-        db[i][j] += g0;
+        for (int j = 0; j < NP; ++j) {
+          fx[j] = tc::mul2(tc::sub2(fx[j], mu2), r2);
+          dw[i][j] = tc::fma2(fg[j], fx[j], dw[i][j]);
+          db[i][j] = tc::add2(db[i][j], fg[j]);
+          fg[j] = tc::mul2(fg[j], ww[j]);
+          acc[0] = tc::add2(acc[0], fg[j]);
+          acc[1] = tc::fma2(fg[j], fx[j], acc[1]);
+          if constexpr (!kRaw) xh[i][j] = fx[j], g[i][j] = fg[j];
+        }
+        if constexpr (kRaw) kx[i] = px, kg[i] = pg;
       }
-      if constexpr (kRaw) kx[i] = px, kg[i] = pg;
-    }
     __syncwarp();  // the slot's mean and rstd have been read
     if (row + STAGES * step < a.n) fetch(slot, row + STAGES * step);
     cp_async_commit();
+    float s[2] = {sum2(acc[0]), sum2(acc[1])};
     group_sum<2>(s, a.tpr, red, flip);
-    const float m1 = s[0] * a.inv_d, m2 = s[1] * a.inv_d;
     if (on && dx != nullptr) {
+      const uint64_t m1 = both(-s[0] * a.inv_d), m2 = both(-s[1] * a.inv_d);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int p = lane + i * a.tpr;
-        if (p >= packs) continue;
-        Pack<T, VEC> out;
-        float ww[VEC];
-        if constexpr (kRaw) read_columns<VEC>(ww, w, i, lane, a.tpr);
+        if (p < packs) {
+          uint64_t out[NP];
+          if constexpr (kRaw) {
+            uint64_t ww[NP], fx[NP], fg[NP];
+            read_columns<NP>(ww, w, i, lane, a.tpr);
+            to_pairs<T>(kx[i], fx);
+            to_pairs<T>(kg[i], fg);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float h, gw;
-          if constexpr (kRaw)
-            h = (to_f<T>(kx[i].v[j]) - mu) * r, gw = to_f<T>(kg[i].v[j]) * ww[j];
-          else
-            h = xh[i][j], gw = g[i][j];
-          out.v[j] = from_f<T>((gw - m1 - h * m2) * r);
+            for (int j = 0; j < NP; ++j)
+              out[j] = tc::mul2(tc::fma2(tc::mul2(tc::sub2(fx[j], mu2), r2), m2, tc::add2(tc::mul2(fg[j], ww[j]), m1)), r2);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) out[j] = tc::mul2(tc::fma2(xh[i][j], m2, tc::add2(g[i][j], m1)), r2);
+          }
+          *reinterpret_cast<uint4*>(dx + row * a.d + (int64_t)p * VEC) = from_pairs<T>(out);
         }
-        *reinterpret_cast<Pack<T, VEC>*>(dx + row * a.d + (int64_t)p * VEC) = out;
       }
     }
   }
@@ -567,9 +622,9 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
     for (int i = 0; i < V; ++i) {
       if (lane + i * a.tpr >= packs) continue;
 #pragma unroll
-      for (int j = 0; j < VEC; j += 4) {
-        const float(&v)[VEC] = which == 0 ? dw[i] : db[i];
-        *reinterpret_cast<float4*>(to + (lane + i * a.tpr) * VEC + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      for (int j = 0; j < NP; j += 2) {
+        const uint64_t v0 = which == 0 ? dw[i][j] : db[i][j], v1 = which == 0 ? dw[i][j + 1] : db[i][j + 1];
+        *reinterpret_cast<ulonglong2*>(to + (lane + i * a.tpr) * VEC + 2 * j) = make_ulonglong2(v0, v1);
       }
     }
     if (groups == 1) continue;
