@@ -89,27 +89,43 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
 // is a 2 x 32 x K shared array: calls alternate between its halves (`flip`), so one barrier per call is enough.
 template <int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float* red, int& flip) {
-  const int lanes = tpr < 32 ? tpr : 32;
-  for (int o = lanes >> 1; o > 0; o >>= 1) {
+  if (tpr < 32) {
+    for (int o = tpr >> 1; o > 0; o >>= 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    }
+    return;
   }
-  if (tpr <= 32) return;
-  float* buf = red + flip * (32 * K);
-  flip ^= 1;
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) buf[warp * K + k] = v[k];
-  }
-  __syncthreads();
-  const int warps = tpr >> 5, first = warp / warps * warps, at = threadIdx.x & 31;
-#pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = at < warps ? buf[(first + at) * K + k] : 0.f;
   for (int o = 16; o > 0; o >>= 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   }
+  if (tpr == 32) return;
+  float* buf = red + flip * (32 * K);
+  flip ^= 1;
+  const int warp = threadIdx.x >> 5, at = threadIdx.x & 31, warps = tpr >> 5;
+  if (at == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) buf[warp * K + k] = v[k];
+  }
+  __syncthreads();
+  // every warp adds the sums of its group's warps; their number is a power of two, so lanes take them round and round
+  const int from = (warp & ~(warps - 1)) + (at & (warps - 1));
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = buf[from * K + k];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o < warps) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    }
+  }
+}
+// 1 / sqrt(x): the hardware's approximation and one step of Newton's method
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = rsqrtf(x);
+  return r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
 template <typename T, int VEC, int V>
@@ -167,7 +183,7 @@ __global__ void __launch_bounds__(1024 / (V * VEC > 16 ? 2 : 1)) forward_kernel(
         s[0] = fmaf(v[i][j], v[i][j], s[0]);
       }
     group_sum<1>(s, a.tpr, red, flip);
-    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    const float r = inverse_root(fmaf(s[0], a.inv_d, a.eps));
     if (on) {
       if (lane == 0 && a.mean != nullptr) {
         a.mean[row] = mu;
@@ -204,7 +220,7 @@ __global__ void __launch_bounds__(1024) forward_long_kernel(const Args a) {
       s[0] = fmaf(v, v, s[0]);
     }
     group_sum<1>(s, blockDim.x, red, flip);
-    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    const float r = inverse_root(fmaf(s[0], a.inv_d, a.eps));
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mu;
       a.rstd[row] = r;
@@ -420,11 +436,12 @@ __device__ __forceinline__ float sum2(uint64_t v) {
   tc::unpack2(v, x, y);
   return x + y;
 }
+// `src`: the thread's first 16 bytes; the following ones lie `step` bytes apart
 template <int NP>
-__device__ __forceinline__ void read_columns(uint64_t (&v)[NP], const float* src, int i, int lane, int tpr) {
+__device__ __forceinline__ void read_columns(uint64_t (&v)[NP], const char* src, int step, int i) {
 #pragma unroll
   for (int q = 0; q < NP / 2; ++q) {
-    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(src + (((i * (NP / 2)) + q) * tpr + lane) * 4);
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(src + (i * (NP / 2) + q) * step);
     v[2 * q] = x.x, v[2 * q + 1] = x.y;
   }
 }
@@ -442,6 +459,7 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
   __shared__ float red[2 * 32];
   const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
   float *w = cols, *b = cols + a.tpr * V * VEC;
+  const char *my_w = reinterpret_cast<const char*>(w) + lane * 16, *my_b = reinterpret_cast<const char*>(b) + lane * 16;
   char* ring = reinterpret_cast<char*>(cols + 2 * a.tpr * V * VEC);
   const int stage_bytes = blockDim.x * V * 16;
   const T* x = reinterpret_cast<const T*>(a.x);
@@ -489,7 +507,7 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
       }
     s[0] = sum2(acc);
     group_sum<1>(s, a.tpr, red, flip);
-    const float r = 1.0f / sqrtf(fmaf(s[0], a.inv_d, a.eps));
+    const float r = inverse_root(fmaf(s[0], a.inv_d, a.eps));
     if (on) {
       if (lane == 0 && a.mean != nullptr) {
         a.mean[row] = mu;
@@ -501,8 +519,8 @@ __global__ void __launch_bounds__(1024) forward_ring_kernel(const Args a) {
         const int p = lane + i * a.tpr;
         if (p < packs) {
           uint64_t ww[NP], bb[NP];
-          read_columns<NP>(ww, w, i, lane, a.tpr);
-          read_columns<NP>(bb, b, i, lane, a.tpr);
+          read_columns<NP>(ww, my_w, a.tpr * 16, i);
+          read_columns<NP>(bb, my_b, a.tpr * 16, i);
 #pragma unroll
           for (int j = 0; j < NP; ++j) ww[j] = tc::fma2(tc::mul2(v[i][j], r2), ww[j], bb[j]);
           *reinterpret_cast<uint4*>(y + row * a.d + (int64_t)p * VEC) = from_pairs<T>(ww);
@@ -520,6 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
   const int lane = threadIdx.x % a.tpr, group = threadIdx.x / a.tpr, groups = blockDim.x / a.tpr, packs = a.d / VEC;
   const int stage_bytes = blockDim.x * V * 32 + blockDim.x * 8;
   float* w = cols;
+  const char* my_w = reinterpret_cast<const char*>(w) + lane * 16;
   char* ring = reinterpret_cast<char*>(cols + a.tpr * V * VEC);
   const T *x = reinterpret_cast<const T*>(a.x), *dy = reinterpret_cast<const T*>(a.dy);
   T* dx = reinterpret_cast<T*>(a.dx);
@@ -567,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
         const uint4 px = *reinterpret_cast<const uint4*>(slot + (i * blockDim.x + threadIdx.x) * 16);
         const uint4 pg = *reinterpret_cast<const uint4*>(slot + ((V + i) * blockDim.x + threadIdx.x) * 16);
         uint64_t ww[NP], fx[NP], fg[NP];
-        read_columns<NP>(ww, w, i, lane, a.tpr);
+        read_columns<NP>(ww, my_w, a.tpr * 16, i);
         to_pairs<T>(px, fx);
         to_pairs<T>(pg, fg);
 #pragma unroll
@@ -596,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const Args a)
           uint64_t out[NP];
           if constexpr (kRaw) {
             uint64_t ww[NP], fx[NP], fg[NP];
-            read_columns<NP>(ww, w, i, lane, a.tpr);
+            read_columns<NP>(ww, my_w, a.tpr * 16, i);
             to_pairs<T>(kx[i], fx);
             to_pairs<T>(kg[i], fg);
 #pragma unroll
