@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 import re
 import threading
@@ -250,13 +251,13 @@ _SIGNATURES = {
     "flk_kgrad": (_int, [_int, _int] + _MAT + _MAT + [_i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _dp, _i64, _vp, _i64, _int, _vp]),
     "flk_fmm": (_int, [_int, _int] + _MAT + _MAT + [_i64, _vp, _i64, _i64, _dp, _i64, _vp, _i64, _int, _vp]),
     # struct, backward / stream
-    "flk_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionArgs), _int]),
-    "flk_attention_forward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
-    "flk_attention_backward": (_int, [ctypes.POINTER(AttentionArgs), _vp]),
+    "flk_attention_workspace_bytes": (_i64, [_vp, _int]),
+    "flk_attention_forward": (_int, [_vp, _vp]),
+    "flk_attention_backward": (_int, [_vp, _vp]),
     "flk_attention_status": (_int, [_vp, ctypes.POINTER(_int)]),
-    "flk_layer_norm_workspace_bytes": (_i64, [ctypes.POINTER(LayerNormArgs)]),
-    "flk_layer_norm_forward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
-    "flk_layer_norm_backward": (_int, [ctypes.POINTER(LayerNormArgs), _vp]),
+    "flk_layer_norm_workspace_bytes": (_i64, [_vp]),
+    "flk_layer_norm_forward": (_int, [_vp, _vp]),
+    "flk_layer_norm_backward": (_int, [_vp, _vp]),
     "flk_tc_status": (_int, [_vp, _vp, ctypes.POINTER(_int)]),
     "flk_range_flag": (_int, [_vp, _vp, ctypes.POINTER(_int)]),
     "flk_probe_mufu": (_int, [_int, _vp, ctypes.POINTER(_i64), _vp]),
@@ -270,6 +271,8 @@ EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 def load() -> ctypes.CDLL:
     """Loads the shared library (once per process); raises if it does not exist."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -709,25 +712,32 @@ def row_dtype_code(dtype: torch.dtype) -> int:
     return code
 
 
-def call_struct(name: str, args: ctypes.Structure, device: torch.device, *query):
-    """Calls the entry point ``flk_<name>`` on ``args`` with the device's current stream.  Its workspace comes from torch's
-    caching allocator and belongs to this call alone, so that calls on several streams, and captured graphs, share none
-    (``query``: name of the workspace query, and its further arguments)."""
-    lib = load()
-    ref = ctypes.byref(args)
+# The structs of the row operators as bytes: every field has 8 bytes, and packing them costs a third of filling a
+# ctypes.Structure.  The workspace's two fields come last.
+_ATTENTION_HEAD = struct.Struct("@9q2d16q6q4q16q")
+_LAYER_NORM_HEAD = struct.Struct("@4qdq3q6q3q3q")
+_WORKSPACE = struct.Struct("@2q")
+_NO_WORKSPACE = _WORKSPACE.pack(0, 0)
+assert _ATTENTION_HEAD.size + 16 == ctypes.sizeof(AttentionArgs) and _LAYER_NORM_HEAD.size + 16 == ctypes.sizeof(LayerNormArgs)
+
+
+def call_rows(fn, head: bytes, device: torch.device, query=None, *query_args):
+    """Calls a row operator's entry point on the struct that begins with ``head``, with the device's current stream.  Its
+    workspace (``query``: the entry point that tells its size) comes from torch's caching allocator and belongs to this call
+    alone, so that calls on several streams, and captured graphs, share none."""
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return call_struct(name, args, device, *query)
+            return call_rows(fn, head, device, query, *query_args)
     ws = None
-    if query:
-        need = getattr(lib, query[0])(ref, *query[1:])
+    args = head + _NO_WORKSPACE
+    if query is not None:
+        need = query(args, *query_args)
         if need < 0:
             raise_for_status(int(need))
         if need > 0:
             ws = torch.empty(need, dtype=torch.uint8, device=device)
-            args.workspace = ws.data_ptr()
-            args.workspace_bytes = need
-    status = getattr(lib, "flk_" + name)(ref, torch.cuda.current_stream(device).cuda_stream)
+            args = head + _WORKSPACE.pack(ws.data_ptr(), need)
+    status = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
     if status != 0:
         raise_for_status(status)
 

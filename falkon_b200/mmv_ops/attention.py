@@ -14,7 +14,7 @@ from .fmmv import _require_cuda
 
 __all__ = ("attention", "AttentionFn")
 
-_NONE4 = _lib.Tensor4(None, 0, 0, 0)
+_NO_TENSOR = (0, 0, 0, 0)
 
 
 def _strided(t: torch.Tensor) -> torch.Tensor:
@@ -30,33 +30,55 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
 
 
 def _t4(t: Optional[torch.Tensor]):
-    if t is None:
-        return _NONE4
-    sb, sn, sh, _ = t.stride()
-    return _lib.Tensor4(t.data_ptr(), sb, sn, sh)
+    return _NO_TENSOR if t is None else (t.data_ptr(), *t.stride()[:3])
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _fill(q, k, v, out, out_lo, lse, opts, grads=(None, None, None, None)):
+def _pack(q, k, v, out, out_lo, lse, opts, dout=None, dq=None, dk=None, dv=None) -> bytes:
     scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs, flags = opts
     b, nq, hq, d = q.shape
-    return _lib.AttentionArgs(
-        _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, 1 if causal else 0, flags, scale, softcap,
-        _t4(q), _t4(k), _t4(v), _t4(out), _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens), _ptr(q_starts),
-        _ptr(q_docs), 0 if q_docs is None else q_docs.stride(0), _ptr(k_docs), 0 if k_docs is None else k_docs.stride(0),
-        *(_t4(g) for g in grads), None, 0)
+    return _lib._ATTENTION_HEAD.pack(
+        _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, causal, flags, scale, softcap,
+        *_t4(q), *_t4(k), *_t4(v), *_t4(out), _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens),
+        _ptr(q_starts), _ptr(q_docs), 0 if q_docs is None else q_docs.stride(0), _ptr(k_docs),
+        0 if k_docs is None else k_docs.stride(0), *_t4(dout), *_t4(dq), *_t4(dk), *_t4(dv))
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _forward(q, k, v, opts, with_lse, with_lo=False):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out_lo = torch.empty_like(out) if with_lo and q.dtype != torch.float32 else None
+    lib = _lib.load()
+    out = _dense_like(q)
+    out_lo = _dense_like(q) if with_lo and q.dtype != torch.float32 else None
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if with_lse else None
-    args = _fill(q, k, v, out, out_lo, lse, opts)
-    _lib.call_struct("attention_forward", args, q.device, "flk_attention_workspace_bytes", 0)
+    _lib.call_rows(lib.flk_attention_forward, _pack(q, k, v, out, out_lo, lse, opts), q.device, lib.flk_attention_workspace_bytes, 0)
     return out, out_lo, lse
+
+
+def _backward(ctx, dout, _):
+    if dout is None:
+        return None, None, None, None
+    q, k, v, out, out_lo, lse, *kept = ctx.saved_tensors
+    kept = iter(kept)
+    opts = tuple(next(kept) if held else t for t, held in zip(ctx.opts, ctx.held))
+    need_q, need_k, need_v, _ = ctx.needs_input_grad
+    dq = _dense_like(q) if need_q else None
+    dk = dv = None
+    if need_k or need_v:
+        dk, dv = _dense_like(k), _dense_like(v)
+    lib = _lib.load()
+    head = _pack(q, k, v, out, out_lo, lse, opts, _strided(dout), dq, dk, dv)
+    _lib.call_rows(lib.flk_attention_backward, head, q.device, lib.flk_attention_workspace_bytes, 1)
+    return dq, dk if need_k else None, dv if need_v else None, None
+
+
+# what backward returns under create_graph=True cannot be differentiated again; the wrapper says so where that is tried
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class AttentionFn(torch.autograd.Function):
@@ -75,23 +97,8 @@ class AttentionFn(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
-        if dout is None:
-            return None, None, None, None
-        q, k, v, out, out_lo, lse, *kept = ctx.saved_tensors
-        kept = iter(kept)
-        opts = tuple(next(kept) if held else t for t, held in zip(ctx.opts, ctx.held))
-        need_q, need_k, need_v, _ = ctx.needs_input_grad
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
-        dk = dv = None
-        if need_k or need_v:
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        dout = _strided(dout)
-        args = _fill(q, k, v, out, out_lo, lse, opts, (dout, dq, dk, dv))
-        _lib.call_struct("attention_backward", args, q.device, "flk_attention_workspace_bytes", 1)
-        return dq, dk if need_k else None, dv if need_v else None, None
+    def backward(ctx, *grads):
+        return _backward_once(ctx, *grads) if torch.is_grad_enabled() else _backward(ctx, *grads)
 
 
 def _table(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[torch.Tensor]:
@@ -193,7 +200,7 @@ def attention(
         if nq != nk:
             raise ValueError("q_documents must be given where queries and keys differ in number")
         q_documents = documents
-    opts = (scale, softcap, bool(causal), slopes, _table("prefix_lens", prefix_lens, (b,), dev),
+    opts = (scale, softcap, 1 if causal else 0, slopes, _table("prefix_lens", prefix_lens, (b,), dev),
             _table("kv_lens", kv_lens, (b,), dev), _table("q_starts", q_starts, (b,), dev),
             _table("q_documents", q_documents, (b, nq), dev), _table("documents", documents, (b, nk), dev), int(flk_flags))
     pad = -d % 8

@@ -38,21 +38,48 @@ def _rows(t: torch.Tensor):
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _forward(x, weight, bias, eps, with_stats):
     x, n, inner, so, si = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if with_stats else None
     if n > 0:
-        mean = None if stats is None else stats.data_ptr()
+        mean = 0 if stats is None else stats.data_ptr()
+        code = _lib.row_dtype_code(x.dtype)
         w = weight if weight is not None else bias
-        args = _lib.LayerNormArgs(
-            _lib.row_dtype_code(x.dtype), _lib.row_dtype_code(x.dtype if w is None else w.dtype), n, x.shape[-1], eps,
-            x.data_ptr(), inner, so, si, _ptr(weight), _ptr(bias), y.data_ptr(), mean, None if mean is None else mean + 4 * n)
-        _lib.call_struct("layer_norm_forward", args, x.device)
+        head = _lib._LAYER_NORM_HEAD.pack(
+            code, code if w is None else _lib.row_dtype_code(w.dtype), n, x.shape[-1], eps, x.data_ptr(), inner, so, si,
+            _ptr(weight), _ptr(bias), y.data_ptr(), mean, mean and mean + 4 * n, 0, 1, 0, 0, 0, 0, 0)
+        _lib.call_rows(_lib.load().flk_layer_norm_forward, head, x.device)
     return y, stats
+
+
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    d, dev = x.shape[-1], x.device
+    dx = _dense_like(x) if need_x else None
+    dw = torch.empty(d, dtype=ctx.wdtype, device=dev) if need_w else None
+    db = torch.empty(d, dtype=ctx.wdtype, device=dev) if need_b else None
+    x, n, inner, so, si = _rows(x)
+    dy, _, dinner, dso, dsi = _rows(dy)
+    mean = stats.data_ptr()
+    head = _lib._LAYER_NORM_HEAD.pack(
+        _lib.row_dtype_code(x.dtype), _lib.row_dtype_code(ctx.wdtype), n, d, ctx.eps, x.data_ptr(), inner, so, si, _ptr(weight), 0, 0,
+        mean, mean + 4 * n, dy.data_ptr(), dinner, dso, dsi, _ptr(dx), _ptr(dw), _ptr(db))
+    lib = _lib.load()
+    _lib.call_rows(lib.flk_layer_norm_backward, head, dev, lib.flk_layer_norm_workspace_bytes)
+    return dx, dw, db, None
+
+
+# what backward returns under create_graph=True cannot be differentiated again; the wrapper says so where that is tried
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class LayerNormFn(torch.autograd.Function):
@@ -67,22 +94,8 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        d, dev = x.shape[-1], x.device
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(d, dtype=ctx.wdtype, device=dev) if need_w else None
-        db = torch.empty(d, dtype=ctx.wdtype, device=dev) if need_b else None
-        x, n, inner, so, si = _rows(x)
-        dy, _, dinner, dso, dsi = _rows(dy)
-        mean = stats.data_ptr()
-        args = _lib.LayerNormArgs(
-            _lib.row_dtype_code(x.dtype), _lib.row_dtype_code(ctx.wdtype), n, d, ctx.eps, x.data_ptr(), inner, so, si,
-            _ptr(weight), None, None, mean, mean + 4 * n, dy.data_ptr(), dinner, dso, dsi, _ptr(dx), _ptr(dw), _ptr(db))
-        _lib.call_struct("layer_norm_backward", args, dev, "flk_layer_norm_workspace_bytes")
-        return dx, dw, db, None
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def layer_norm(

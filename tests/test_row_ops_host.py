@@ -60,7 +60,7 @@ def test_attention_options(opts, error, gpu_claimed, monkeypatch):
     def on_gpu(t):
         return t.as_subclass(Cuda) if isinstance(t, torch.Tensor) else t
 
-    monkeypatch.setattr(_lib, "call_struct", lambda *a: pytest.fail("a refused call reached the library"))
+    monkeypatch.setattr(_lib, "call_rows", lambda *a: pytest.fail("a refused call reached the library"))
     with pytest.raises(error):
         attention(*map(on_gpu, qkv()), **{n: on_gpu(t) for n, t in opts.items()})
 
