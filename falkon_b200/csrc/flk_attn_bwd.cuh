@@ -9,7 +9,7 @@
 //                   The tensor cores run dV(i), S(i+1) while dS(i) is being made and dK(i), dP(i+1) while P(i+1) is.
 //   queries kernel  a block owns 128 packed query rows and walks over the key tiles:  S = Q K^T (two buffers), dP = dO V^T,
 //                   dQ += dS K.
-// Both have 12 warps: two warpgroups that turn scores into weights (a thread owns one row and half of the columns), a warp that
+// Both have 20 warps: four warpgroups that turn scores into weights (a thread owns one row and a quarter of the columns), a warp that
 // issues products, one that issues copies, and in the keys kernel one that gathers what the columns need (lse, delta, ...).
 //
 // P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass.  In fp16 they would
@@ -23,14 +23,11 @@ namespace flk {
 namespace attn {
 namespace bwd {
 
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kStatWarp = 10;
-// registers of the two working warpgroups, and of the third; the block is launched with 384 x 168
-template <bool KEYS>
-struct Regs {
-  static constexpr int kWork = KEYS ? 216 : 208, kOther = KEYS ? 72 : 88;
-  static_assert(2 * 128 * kWork + 128 * kOther <= kThreads * 168, "registers");
-};
+constexpr int kThreads = 640;
+constexpr int kMmaWarp = 16, kLoadWarp = 17, kStatWarp = 18;
+// registers: 640 threads are launched with 96 each (61440); four warpgroups of 104 and one of 64 make the same sum
+constexpr int kRegsWork = 104, kRegsOther = 64;
+static_assert(4 * 128 * kRegsWork + 128 * kRegsOther <= kThreads * 96, "registers");
 
 // what the columns (queries) of a tile bring into the keys kernel
 enum { kLse = 0, kDelta = 128, kSlope = 256, kPos = 384, kEnd = 512, kLabel = 640, kStatWords = 768 };
@@ -46,7 +43,7 @@ struct Layout {
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kStatAt = kRing + kStages * kTileBytes;
   static constexpr uint32_t kBars = kStatAt + kStats;
-  static constexpr uint32_t kBytes = kBars + 512 + 1024;
+  static constexpr uint32_t kBytes = kBars + 512;
 };
 static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
 static_assert(Layout<128, true>::kStages >= 4 && Layout<128, false>::kStages >= 5, "stages");
@@ -67,19 +64,19 @@ struct Scales {
   }
 };
 
-// accumulator half (DP / 2 columns from c0) times f -> a row of 16-bit values, or of fp32 partial results
+// accumulator quarter (DP / 4 columns from c0) times f -> a row of 16-bit values, or of fp32 partial results
 template <typename T, int DP>
-__device__ __forceinline__ void store_half(uint32_t acc, int c0, float f, bool exists, bool zero, int d, T* row, float* part) {
+__device__ __forceinline__ void store_quarter(uint32_t acc, int c0, float f, bool exists, bool zero, int d, T* row, float* part) {
 #pragma unroll
-  for (int c = 0; c < DP / 2; c += 32) {
-    uint32_t o[32];
-    tmem_ld32(acc + c0 + c, o);
+  for (int c = 0; c < DP / 4; c += 16) {
+    uint32_t o[16];
+    tc::tmem_ld16(acc + c0 + c, o);
     tmem_ld_wait_on(o);
     if (exists) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+      for (int e = 0; e < 16; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
+      for (int e = 0; e < 16; e += 8) {
         const int col = c0 + c + e;
         if (col < d) {
           if (part != nullptr) {
@@ -100,7 +97,7 @@ __device__ __forceinline__ void store_half(uint32_t acc, int c0, float f, bool e
 template <typename T, int DP>
 __device__ __forceinline__ void store_zeros(int c0, bool exists, int d, T* row, float* part) {
   if (!exists) return;
-  for (int c = c0; c < c0 + DP / 2 && c < d; c += 8) {
+  for (int c = c0; c < c0 + DP / 4 && c < d; c += 8) {
     if (part != nullptr)
       *reinterpret_cast<uint4*>(part + c) = *reinterpret_cast<uint4*>(part + c + 4) = make_uint4(0, 0, 0, 0);
     else
@@ -143,9 +140,9 @@ template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant__ Maps maps, const TcArgs t) {
   using L = Layout<DP, true>;
   constexpr int kStages = L::kStages;
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   const Args& a = t.a;
-  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, bars = base + L::kBars;
+  const uint32_t base = smem_u32(raw), bars = base + L::kBars;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + 64 + s * 8; };
   const uint32_t own = bars + 128, sfull = bars + 136, pfull = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176;
@@ -181,8 +178,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   if (warp == kMmaWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-      mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 8), mbar_init(dpfull, 1), mbar_init(dsfull, 8), mbar_init(done, 1);
-      for (int s = 0; s < kStatSlots; ++s) mbar_init(statfull(s), 1), mbar_init(statempty(s), 8);
+      mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 16), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
+      for (int s = 0; s < kStatSlots; ++s) mbar_init(statfull(s), 1), mbar_init(statempty(s), 16);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -196,8 +193,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
   const uint32_t ts = tmem, tp = tmem + 128, tdv = tmem + 256, tdk = tmem + 256 + DP;
 
-  if (warp >= 8) {
-    tc::reg_release<Regs<true>::kOther>();
+  if (warp >= kMmaWarp) {
+    tc::reg_release<kRegsOther>();
     if (warp == kLoadWarp) {
       bool ok = true;
       if (steps > 0 && elect_one()) {
@@ -319,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         ok = wait_bar(pfull, (uint32_t)i & 1);
         tc_fence_after();
         if (ok && elect_one()) {
-          issue_weighted<T, DP, true>(tdv, ts, stage(2 * i + 1), i > 0);
+          issue_weighted<T, DP, 32>(tdv, ts, stage(2 * i + 1), i > 0);
           mma_commit(empty((2 * i + 1) % kStages));
         }
         __syncwarp();
@@ -335,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         ok = ok && wait_bar(dsfull, (uint32_t)i & 1);
         tc_fence_after();
         if (ok && elect_one()) {
-          issue_weighted<T, DP, true>(tdk, tp, stage(2 * i), i > 0);
+          issue_weighted<T, DP, 32>(tdk, tp, stage(2 * i), i > 0);
           mma_commit(empty((2 * i) % kStages));
         }
         __syncwarp();
@@ -356,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
     }
   } else {
-    tc::reg_claim<Regs<true>::kWork>();
+    tc::reg_claim<kRegsWork>();
     const int w = warp >> 2;
-    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, half = 64 * w;
+    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, mine0 = 32 * w;
     const int key = k0 + (int)(threadIdx.x & 127);
     const float mine = (float)(threadIdx.x & 127);  // key - k0
     const int my = kd ? kd[key] : 0;
@@ -369,25 +366,23 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     bool ok = true;
     for (int i = 0; i < steps && ok; ++i) {
       const int slot = i % kStatSlots;
-      const uint32_t st = base + L::kStatAt + slot * kStatWords * 4 + half * 4;
+      const uint32_t st = base + L::kStatAt + slot * kStatWords * 4 + mine0 * 4;
       ok = wait_bar(statfull(slot), (uint32_t)(i / kStatSlots) & 1);
       ok = ok && wait_bar(sfull, (uint32_t)i & 1);
       if (!ok) break;
       tc_fence_after();
       const Tile e = get_tile(slots, i);
       const bool whole = k0 + kTile <= lim.row_end((e.at * kTile) >> t.pg_shift, a.causal) && (kd == nullptr || (e.label >= 0 && e.label == only));
-      uint32_t s[2][32];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld32(ts + lane_at + half + 32 * p, s[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
+      uint32_t s[1][32];
+      tmem_ld32(ts + lane_at + mine0, s[0]);
+      tmem_ld_wait_on(s[0]);
       if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t o[16];
+      for (int p = 0; p < 4; ++p) {
+        uint32_t o[4];
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const uint32_t at = st + (32 * p + c) * 4;
+        for (int c = 8 * p; c < 8 * p + 8; c += 4) {
+          const uint32_t at = st + c * 4;
           float x[4], add[4];
           tc::ld_shared_f4(at + kLse * 4, add[0], add[1], add[2], add[3]);
           if constexpr (BIAS) {
@@ -398,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
             for (int q = 0; q < 4; ++q) add[q] = fmaf(sl[q], fabsf(ps[q] - mine), add[q]);
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[p][c + q]), f, add[q]);
+          for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[0][c + q]), f, add[q]);
           if (!whole) {
             int en[4], lb[4];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(at + kEnd * 4) : "memory");
@@ -412,12 +407,12 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           for (int q = 0; q < 4; ++q) {
             pr[q] = ex2_approx(x[q]);
             // with a cap, the weight times 1 - tanh^2
-            s[p][c + q] = __float_as_uint(CAP ? pr[q] * fmaf(-__uint_as_float(s[p][c + q]), __uint_as_float(s[p][c + q]), 1.f) : pr[q]);
+            s[0][c + q] = __float_as_uint(CAP ? pr[q] * fmaf(-__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q]), 1.f) : pr[q]);
           }
-          o[c / 2] = pack16<T>(pr[0], pr[1]);
-          o[c / 2 + 1] = pack16<T>(pr[2], pr[3]);
+          o[c % 8 / 2] = pack16<T>(pr[0], pr[1]);
+          o[c % 8 / 2 + 1] = pack16<T>(pr[2], pr[3]);
         }
-        tmem_st16(ts + lane_at + half + 16 * p, o);
+        tmem_st4(ts + lane_at + mine0 + 4 * p, o);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -427,27 +422,22 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       ok = wait_bar(dpfull, (uint32_t)i & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t d[2][32];
+      uint32_t d[32];
+      tmem_ld32(tp + lane_at + mine0, d);
+      tmem_ld_wait_on(d);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld32(tp + lane_at + half + 32 * p, d[p]);
+      for (int p = 0; p < 4; ++p) {
+        uint32_t o[4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(d[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t o[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
+        for (int c = 8 * p; c < 8 * p + 8; c += 4) {
           float dl[4], y[4];
-          tc::ld_shared_f4(st + (kDelta + 32 * p + c) * 4, dl[0], dl[1], dl[2], dl[3]);
+          tc::ld_shared_f4(st + (kDelta + c) * 4, dl[0], dl[1], dl[2], dl[3]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float pr = __uint_as_float(s[p][c + q]);
-            y[q] = pr * fmaf(__uint_as_float(d[p][c + q]), g, dl[q]);
-          }
-          o[c / 2] = pack16<T>(y[0], y[1]);
-          o[c / 2 + 1] = pack16<T>(y[2], y[3]);
+          for (int q = 0; q < 4; ++q) y[q] = __uint_as_float(s[0][c + q]) * fmaf(__uint_as_float(d[c + q]), g, dl[q]);
+          o[c % 8 / 2] = pack16<T>(y[0], y[1]);
+          o[c % 8 / 2 + 1] = pack16<T>(y[2], y[3]);
         }
-        tmem_st16(tp + lane_at + half + 16 * p, o);
+        tmem_st4(tp + lane_at + mine0 + 4 * p, o);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -463,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     if (ok) {
       const bool exists = key < a.nk;
       const bool zero = key >= lim.len || (kd != nullptr && my < 0);  // keys that nobody sees
-      const int c0 = w * (DP / 2);
+      const int c0 = w * (DP / 4);
       T* rk = reinterpret_cast<T*>(a.dk.p) + b * a.dk.sb + (int64_t)key * a.dk.sn + hk * a.dk.sh;
       T* rv = reinterpret_cast<T*>(a.dv.p) + b * a.dv.sb + (int64_t)key * a.dv.sn + hk * a.dv.sh;
       float *pk = nullptr, *pv = nullptr;
@@ -473,8 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         pv = pk + n;
       }
       if (steps > 0) {
-        store_half<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, exists, zero, a.d, rk, pk);
-        store_half<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, exists, zero, a.d, rv, pv);
+        store_quarter<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, exists, zero, a.d, rk, pk);
+        store_quarter<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, exists, zero, a.d, rv, pv);
       } else {
         store_zeros<T, DP>(c0, exists, a.d, rk, pk);
         store_zeros<T, DP>(c0, exists, a.d, rv, pv);
@@ -518,9 +508,9 @@ template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_constant__ Maps maps, const TcArgs t) {
   using L = Layout<DP, false>;
   constexpr int kStages = L::kStages;
-  extern __shared__ uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   const Args& a = t.a;
-  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, bars = base + L::kBars;
+  const uint32_t base = smem_u32(raw), bars = base + L::kBars;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + 64 + s * 8; };
   auto sfull = [&](int s) { return bars + 128 + s * 8; };
@@ -545,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   if (warp == kMmaWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-      mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 8), mbar_init(done, 1);
+      mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -560,8 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   auto ts = [&](int i) { return tmem + (uint32_t)(i & 1) * 128; };
   const uint32_t tp = tmem + 256, tdq = tmem + 384;
 
-  if (warp >= 8) {
-    tc::reg_release<Regs<false>::kOther>();
+  if (warp >= kMmaWarp) {
+    tc::reg_release<kRegsOther>();
     if (warp == kLoadWarp) {
       bool ok = true;
       if (steps > 0 && elect_one()) {
@@ -629,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         tc_fence_after();
         if (i + 1 < steps) ok = ok && products(i + 1);
         if (ok && elect_one()) {
-          issue_weighted<T, DP, true>(tdq, ts(i), stage(2 * i), i > 0);
+          issue_weighted<T, DP, 32>(tdq, ts(i), stage(2 * i), i > 0);
           mma_commit(empty((2 * i) % kStages));
         }
         __syncwarp();
@@ -642,9 +632,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       }
     }
   } else {
-    tc::reg_claim<Regs<false>::kWork>();
+    tc::reg_claim<kRegsWork>();
     const int w = warp >> 2;
-    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, half = 64 * w;
+    const uint32_t lane_at = (uint32_t)(warp & 3) << 21, mine0 = 32 * w;
     const int r = row0 + (int)(threadIdx.x & 127), i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
     const bool exists = r < t.rows;
     const int end = exists ? lim.row_end(i, a.causal) : 0;
@@ -672,54 +662,44 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       const Tile e = get_tile(slots, step);
       const int k0 = e.at * kTile;
       const bool whole = k0 + kTile <= all_before && (kd == nullptr || (e.label >= 0 && e.label == only));
-      uint32_t s[2][32];
-      const uint32_t at = ts(step) + lane_at + half;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld32(at + 32 * p, s[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
-      const float d0 = (float)(pos - k0 - (int)half);
-      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-      if (!whole) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          seen[p] = seen_columns(end - k0 - (int)half - 32 * p, kd == nullptr ? nullptr : kd + k0 + half + 32 * p, my);
-      }
+      uint32_t s[1][32];
+      const uint32_t at = ts(step) + lane_at + mine0;
+      tmem_ld32(at, s[0]);
+      tmem_ld_wait_on(s[0]);
+      const float d0 = (float)(pos - k0 - (int)mine0);
+      uint32_t seen = 0xffffffffu;
+      if (!whole) seen = seen_columns(end - k0 - (int)mine0, kd == nullptr ? nullptr : kd + k0 + mine0, my);
       if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float raw = __uint_as_float(s[p][c]);
-          float x = fmaf(raw, f, add);
-          if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)(32 * p + c)), x);
-          if (!whole && (seen[p] >> c & 1) == 0) x = -INFINITY;
-          x = ex2_approx(x);
-          s[p][c] = __float_as_uint(CAP ? x * fmaf(-raw, raw, 1.f) : x);
-        }
+      for (int c = 0; c < 32; ++c) {
+        const float raw = __uint_as_float(s[0][c]);
+        float x = fmaf(raw, f, add);
+        if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)c), x);
+        if (!whole && (seen >> c & 1) == 0) x = -INFINITY;
+        x = ex2_approx(x);
+        s[0][c] = __float_as_uint(CAP ? x * fmaf(-raw, raw, 1.f) : x);
+      }
       ok = wait_bar(dpfull, (uint32_t)step & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t d[2][32];
+      uint32_t d[32];
+      tmem_ld32(tp + lane_at + mine0, d);
+      tmem_ld_wait_on(d);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld32(tp + lane_at + half + 32 * p, d[p]);
+      for (int p = 0; p < 4; ++p) {
+        uint32_t o[4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(d[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t o[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
+        for (int c = 8 * p; c < 8 * p + 8; c += 2) {
           float y[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            y[q] = __uint_as_float(s[p][c + q]) * fmaf(__uint_as_float(d[p][c + q]), gs, nd);
+            y[q] = __uint_as_float(s[0][c + q]) * fmaf(__uint_as_float(d[c + q]), gs, nd);
             // V rows that nobody may see are not cleaned here: their products may be anything
-            if (!whole && (seen[p] >> (c + q) & 1) == 0) y[q] = 0.f;
+            if (!whole && (seen >> (c + q) & 1) == 0) y[q] = 0.f;
           }
-          o[c / 2] = pack16<T>(y[0], y[1]);
+          o[c % 8 / 2] = pack16<T>(y[0], y[1]);
         }
-        tmem_st16(at + 16 * p, o);
+        tmem_st4(at + 4 * p, o);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -731,9 +711,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     tc_fence_after();
     if (ok) {
       T* row = reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.sn + h * a.dq.sh;
-      const int c0 = w * (DP / 2);
+      const int c0 = w * (DP / 4);
       if (steps > 0)
-        store_half<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, exists, add == -INFINITY, a.d, row, nullptr);
+        store_quarter<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, exists, add == -INFINITY, a.d, row, nullptr);
       else
         store_zeros<T, DP>(c0, exists, a.d, row, nullptr);
     }

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && w == 0 && more) ok = ready(2 * i + 2);
             tc_fence_after();
             if (ok && elect_one()) {
-              issue_weighted<T, DP, true>(to(w), ts(w), stage(2 * i + 1), i > 0);
+              issue_weighted<T, DP, 64>(to(w), ts(w), stage(2 * i + 1), i > 0);
               if (w == 1) mma_commit(empty((2 * i + 1) % kStages));
               if (more) {
                 issue_scores<T, DP>(ts(w), base + w * L::kTileBytes, stage(2 * i + 2));
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && wait_bar(pfull(w), (uint32_t)(i >> 1) & 1);
           tc_fence_after();
           if (ok && elect_one()) {
-            issue_weighted<T, DP, true>(to(w), ts(w), stage(2 * i + 1), i > 1);
+            issue_weighted<T, DP, 64>(to(w), ts(w), stage(2 * i + 1), i > 1);
             mma_commit(empty((2 * i + 1) % kStages));
           }
           __syncwarp();

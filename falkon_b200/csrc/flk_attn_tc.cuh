@@ -111,14 +111,16 @@ __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a, uint32
     mma_ss(d_tmem, al + off, bl + off, instr_desc<T>(kTile, false), ks > 0);
   }
 }
-// accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B; weights of the rows
-// [16 K0, 16 K1).  HALVES: the weights of rows 64 and up lie 64 columns behind those of rows 0 to 63, in place of 32
-template <typename T, int DP, bool HALVES, int K0 = 0, int K1 = kTile / 16>
+// accumulation: D[128 x DP] (+)= W[128 x 128] B, with the weights W in tensor memory and the 128 rows of B.  The 128 columns of
+// scores that the weights came from are shared by 128 / OWN threads of a row; each has put its weights, two per column, at the
+// start of its own OWN columns.
+template <typename T, int DP, int OWN>
 __device__ __forceinline__ void issue_weighted(uint32_t d_tmem, uint32_t w_tmem, uint32_t b, bool accumulate) {
   const uint32_t bl = desc_low(b, kBlockBytes);
+  constexpr int kPer = OWN / 16;  // products per thread's share
 #pragma unroll
-  for (int ks = K0; ks < K1; ++ks)
-    mma_ts(d_tmem, w_tmem + ks * 8 + (HALVES && ks >= 4 ? 32 : 0), bl + ks * (2048 >> 4), instr_desc<T>(DP, true), accumulate || ks > 0);
+  for (int ks = 0; ks < kTile / 16; ++ks)
+    mma_ts(d_tmem, w_tmem + ks / kPer * OWN + ks % kPer * 8, bl + ks * (2048 >> 4), instr_desc<T>(DP, true), accumulate || ks > 0);
 }
 
 #define FLK_R32_IN(r)                                                                                                    \
@@ -141,6 +143,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
