@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   auto statempty = [&](int s) { return bars + 224 + s * 8; };
   const uint32_t slots = bars + 256;
   const int warp = threadIdx.x >> 5;
+  if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
   int64_t id = blockIdx.x;
   const int hk = (int)(id % a.hk);
@@ -229,40 +230,45 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       if (steps > 0) wait_bar(own, 0);
       for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
-    } else if (warp == kStatWarp) {
+    } else if (warp >= kStatWarp) {
+      // two warps take turns; all loads of a step are under way at once
       bool ok = true;
       StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
       const float g = Scales<T>::ds(t) * Scales<T>::kUnshift;
       for (int step = 0; step < steps && ok; ++step) {
         const Tile e = walk.next();
+        if ((step & 1) != warp - kStatWarp) continue;
         const int slot = step % kStatSlots;
+        float lse[4], delta[4], slope[4];
+        int label[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int c = (threadIdx.x & 31) + 32 * x, r = e.at * kTile + c, i = r >> t.pg_shift;
+          const int h = hk * a.grp + walk.head * t.pg + (r & (t.pg - 1));
+          const bool exists = r < t.rows;
+          const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
+          lse[x] = exists ? __ldg(a.lse + row) : -INFINITY;
+          delta[x] = exists ? __ldg(a.delta + row) : 0.f;
+          label[x] = qd != nullptr && exists ? __ldg(qd + i) : -2;
+          if constexpr (BIAS) slope[x] = a.slopes != nullptr ? __ldg(a.slopes + h) : 0.f;
+        }
         if (step >= kStatSlots) ok = wait_bar(statempty(slot), (uint32_t)(step / kStatSlots - 1) & 1);
         if (!ok) break;
         const uint32_t at = base + L::kStatAt + slot * kStatWords * 4;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int c = (threadIdx.x & 31) + 32 * x, r = e.at * kTile + c, i = r >> t.pg_shift;
-          const int h = hk * a.grp + walk.head * t.pg + (r & (t.pg - 1));
-          float lse = -INFINITY, delta = 0.f;
-          int end = 0, label = -2;
-          if (r < t.rows) {
-            const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
-            lse = a.lse[row];
-            delta = a.delta[row];
-            end = lim.row_end(i, a.causal);
-            if (qd) label = qd[i];
-          }
           // rows that see nothing: weights exp2(s - inf) = 0, and no delta, which may be NaN there
-          const bool none = lse == -INFINITY;
+          const bool none = lse[x] == -INFINITY;
           auto put = [&](int word, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + (word + c) * 4), "r"(v) : "memory"); };
-          put(kLse, __float_as_uint(none ? -INFINITY : fmaf(-lse, kLog2e, Scales<T>::kShift)));  // added to the score
-          put(kDelta, __float_as_uint(none ? 0.f : -delta * g));
+          put(kLse, __float_as_uint(none ? -INFINITY : fmaf(-lse[x], kLog2e, Scales<T>::kShift)));  // added to the score
+          put(kDelta, __float_as_uint(none ? 0.f : -delta[x] * g));
           if constexpr (BIAS) {
-            put(kSlope, __float_as_uint(a.slopes == nullptr ? 0.f : -a.slopes[h] * kLog2e));
+            put(kSlope, __float_as_uint(-slope[x] * kLog2e));
             put(kPos, __float_as_uint((float)(lim.start + i - k0)));
           }
-          put(kEnd, (uint32_t)(end - k0));
-          put(kLabel, (uint32_t)label);
+          put(kEnd, (uint32_t)((r < t.rows ? lim.row_end(i, a.causal) : 0) - k0));
+          put(kLabel, (uint32_t)label[x]);
         }
         __syncwarp();
         if (elect_one()) mbar_arrive(statfull(slot));
@@ -516,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   auto sfull = [&](int s) { return bars + 128 + s * 8; };
   const uint32_t own = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, slots = bars + 256;
   const int warp = threadIdx.x >> 5;
+  if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
   int64_t id = blockIdx.x;
   const int hp = (int)(id % t.hp);

@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320, halves = bars + 512;
   auto xbar = [&](int w) { return bars + 384 + w * 8; };
   const int warp = threadIdx.x >> 5;
+  if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
 
   // block -> (row block, part of the key axis, sequence, packed head); late row blocks have the most keys under a causal
   // mask and start first

@@ -63,6 +63,10 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // Shared-memory matrix descriptors of a 128-byte-swizzled tile (8-row groups of 1024 bytes).  Only the low word changes from one
 // product to the next: it is kept in one register and stepped by immediates.
 constexpr uint32_t kDescHigh = (1024 >> 4)       // from one group of 8 rows to the next
@@ -234,36 +238,49 @@ struct Tile {
 struct TileWalk {
   const int4* tab;
   int at, last, lo, hi;
-  uint32_t mask;
-  int4 mine;
+  uint32_t mask[4];  // what is left of 128 tiles from `base` on
   int base;
   __device__ __forceinline__ TileWalk(const int4* table, int first, int end, int l, int h)
-      : tab(table), at(first), last(end), lo(l), hi(h), mask(0), mine(make_int4(0, 0, 0, 0)), base(first - 32) {}
+      : tab(table), at(first), last(end), lo(l), hi(h), mask{0, 0, 0, 0}, base(first - 128) {}
   __device__ __forceinline__ Tile next() {
     if (tab == nullptr) return Tile{at < last ? at++ : -1, -1, false};
-    while (mask == 0) {
-      base += 32;
+    while ((mask[0] | mask[1] | mask[2] | mask[3]) == 0) {
+      base += 128;
       if (base >= last) return Tile{-1, -1, false};
-      const int t = base + (int)(threadIdx.x & 31);
-      mine = t < last ? __ldg(tab + t) : make_int4(1, 0, 0, 0);
-      mask = __ballot_sync(0xffffffffu, mine.x <= hi && lo <= mine.y && mine.x <= mine.y);
+      int4 r[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int t = base + 32 * w + (int)(threadIdx.x & 31);
+        r[w] = t < last ? __ldg(tab + t) : make_int4(1, 0, 0, 0);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mask[w] = __ballot_sync(0xffffffffu, r[w].x <= hi && lo <= r[w].y && r[w].x <= r[w].y);
     }
-    const int b = __ffs(mask) - 1;
-    mask &= mask - 1;
-    const bool dirty = __shfl_sync(0xffffffffu, mine.z, b) != 0;
-    const int x = __shfl_sync(0xffffffffu, mine.x, b), y = __shfl_sync(0xffffffffu, mine.y, b);
-    return Tile{base + b, !dirty && x == y ? x : -1, dirty};
+    int w = 0, found = 0;
+#pragma unroll
+    for (int e = 3; e >= 0; --e)
+      if (mask[e] != 0) w = e, found = __ffs(mask[e]) - 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e == w) mask[e] &= mask[e] - 1;
+    const int t = base + 32 * w + found;
+    const int4 r = __ldg(tab + t);
+    return Tile{t, r.z == 0 && r.x == r.y ? r.x : -1, r.z != 0};
   }
 };
 // how many tiles such a walk visits
 __device__ __forceinline__ int count_tiles(const int4* tab, int first, int last, int lo, int hi) {
   if (tab == nullptr) return max(last - first, 0);
   int n = 0;
-  for (int t0 = first; t0 < last; t0 += 32) {
-    const int t = t0 + (int)(threadIdx.x & 31);
-    const int4 r = t < last ? __ldg(tab + t) : make_int4(1, 0, 0, 0);
-    n += __popc(__ballot_sync(0xffffffffu, r.x <= hi && lo <= r.y && r.x <= r.y));
+  for (int t0 = first + (int)(threadIdx.x & 31); t0 < last; t0 += 256) {
+    int4 r[8];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) r[w] = t0 + 32 * w < last ? __ldg(tab + t0 + 32 * w) : make_int4(1, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) n += r[w].x <= hi && lo <= r[w].y && r[w].x <= r[w].y;
   }
+  __syncwarp();
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n;
 }
 // The loading warp tells the others which tile a step works on through a ring of 16 slots; it is never that many steps ahead
@@ -322,6 +339,7 @@ struct LabelRange {
 };
 __device__ __forceinline__ LabelRange labels_of(const int* docs, int i0, int i1) {
   LabelRange r{INT32_MAX, INT32_MIN, false};
+#pragma unroll 4
   for (int i = i0 + (int)(threadIdx.x & 31); i < i1; i += 32) {
     const int id = __ldg(docs + i);
     if (id >= 0) {
