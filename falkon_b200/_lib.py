@@ -43,7 +43,7 @@ TC_LAUNCH_REGISTERS = 80
 ATTENTION_LAUNCH_REGISTERS = 96
 # Some of them spill scalars of the loading warp, or a few that are stored once and read in several places; a row's scores
 # are read with asynchronous loads too, but there the wait follows at once, so none is in flight where a register is spilled.
-ATTENTION_SPILL_ALLOWANCE = (64, 128)
+ATTENTION_SPILL_ALLOWANCE = (64, 144)
 # A few instantiations of the K-loop kernel still spill one or two 32-bit values that are stored once before the
 # warp roles split (none inside a tile loop); the build tolerates up to this many bytes of spill stores / loads
 # there and fails beyond (a regression guard, not an endorsement).

@@ -64,35 +64,59 @@ struct Scales {
   }
 };
 
-// accumulator quarter (DP / 4 columns from c0) times f -> a row of 16-bit values, or of fp32 partial results
-template <typename T, int DP>
-__device__ __forceinline__ void store_quarter(uint32_t acc, int c0, float f, bool exists, bool zero, int d, T* row, float* part) {
-#pragma unroll
-  for (int c = 0; c < DP / 4; c += 16) {
-    uint32_t o[16];
-    tc::tmem_ld16(acc + c0 + c, o);
-    tmem_ld_wait_on(o);
-    if (exists) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
-#pragma unroll
-      for (int e = 0; e < 16; e += 8) {
-        const int col = c0 + c + e;
-        if (col < d) {
-          if (part != nullptr) {
-            *reinterpret_cast<uint4*>(part + col) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            *reinterpret_cast<uint4*>(part + col + 4) = make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
-          } else {
-            uint32_t v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = pack16<T>(__uint_as_float(o[e + 2 * q]), __uint_as_float(o[e + 2 * q + 1]));
-            *reinterpret_cast<uint4*>(row + col) = make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
-      }
-    }
-    __syncwarp();
+// What dS is made from later, in the place of the scores s0, s1: the weights, times 1 - tanh^2 where s is the tanh of a capped score
+template <bool CAP>
+__device__ __forceinline__ void weight_slope(uint32_t& s0, uint32_t& s1, float p0, float p1) {
+  if constexpr (CAP) {
+    const uint64_t v = tc::pack2(__uint_as_float(s0), __uint_as_float(s1));
+    tc::unpack2(tc::mul2(tc::pack2(p0, p1), tc::fma2(tc::mul2(v, both(-1.f)), v, both(1.f))), p0, p1);
   }
+  s0 = __float_as_uint(p0);
+  s1 = __float_as_uint(p1);
+}
+
+// A quarter of the accumulator (DP / 4 columns from c0 on) times f: 16-bit values of 32 rows, rows side by side
+// (`at(row)`: where row `row` of the warp begins, or null where it is not to be written).
+template <typename T, int DP, typename At>
+__device__ __forceinline__ void store_quarter(uint32_t acc, int c0, float f, bool zero, int d, uint32_t room, At at) {
+  constexpr int kWords = DP / 4;
+  uint32_t o[kWords];
+#pragma unroll
+  for (int c = 0; c < kWords; c += 16) tc::tmem_ld16(acc + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
+#pragma unroll
+  for (int c = 0; c < kWords; c += 16) tmem_ld_wait_on(*reinterpret_cast<uint32_t(*)[16]>(o + c));
+#pragma unroll
+  for (int e = 0; e < kWords; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+  store_rows32<kWords / 8>(
+      room,
+      [&](uint32_t p) {
+        uint32_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = pack16<T>(__uint_as_float(o[8 * p + 2 * q]), __uint_as_float(o[8 * p + 2 * q + 1]));
+        return make_uint4(v[0], v[1], v[2], v[3]);
+      },
+      [&](int row, int p, const uint4& v) {
+        T* to = at(row);
+        if (to != nullptr && c0 + 8 * p < d) *reinterpret_cast<uint4*>(to + c0 + 8 * p) = v;
+      });
+}
+// The same as fp32 partial results.
+template <int DP, typename At>
+__device__ __forceinline__ void store_partial(uint32_t acc, int c0, float f, bool zero, int d, uint32_t room, At at) {
+  constexpr int kWords = DP / 4;
+  uint32_t o[kWords];
+#pragma unroll
+  for (int c = 0; c < kWords; c += 16) tc::tmem_ld16(acc + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
+#pragma unroll
+  for (int c = 0; c < kWords; c += 16) tmem_ld_wait_on(*reinterpret_cast<uint32_t(*)[16]>(o + c));
+#pragma unroll
+  for (int e = 0; e < kWords; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+  store_rows32<kWords / 4>(
+      room, [&](uint32_t p) { return make_uint4(o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]); },
+      [&](int row, int p, const uint4& v) {
+        float* to = at(row);
+        if (to != nullptr && c0 + 4 * p < d) *reinterpret_cast<uint4*>(to + c0 + 4 * p) = v;
+      });
 }
 template <typename T, int DP>
 __device__ __forceinline__ void store_zeros(int c0, bool exists, int d, T* row, float* part) {
@@ -152,12 +176,12 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
-  int64_t id = blockIdx.x;
-  const int hk = (int)(id % a.hk);
-  id /= a.hk;
-  const int b = (int)(id % a.b);
-  id /= a.b;
-  const int split = (int)(id % t.splits), k0 = (int)(id / t.splits) * kTile;
+  uint32_t id = blockIdx.x;
+  const int hk = (int)(id % (uint32_t)a.hk);
+  id /= (uint32_t)a.hk;
+  const int b = (int)(id % (uint32_t)a.b);
+  id /= (uint32_t)a.b;
+  const int split = (int)(id % (uint32_t)t.splits), k0 = (int)(id / (uint32_t)t.splits) * kTile;
   const Limits lim = limits_of(a, b);
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
@@ -173,10 +197,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   if (kd) lab = labels_of(kd, k0, k0 + kTile);
   const int heads = a.grp >> t.pg_shift;
   const int per_head = count_tiles(qtab, first, last, lab.lo, lab.hi);
-  const int64_t total = (int64_t)per_head * heads;
-  const int skip = (int)(total * split / t.splits), steps = (int)(total * (split + 1) / t.splits) - skip;
+  // parts of at most one step more than others
+  const uint32_t total = (uint32_t)(per_head * heads), even = total / (uint32_t)t.splits, more = total % (uint32_t)t.splits;
+  const int skip = (int)(split * even + min((uint32_t)split, more)), steps = (int)(even + ((uint32_t)split < more ? 1 : 0));
 
-  if (warp == kMmaWarp) {
+  if (warp == kLoadWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 16), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
@@ -184,12 +209,16 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       tc::fence_barrier_init();
     }
     __syncwarp();
-    tmem_alloc(tmem_at, 512);
-    tmem_relinquish();
+    start_arrive<kThreads>();
+  } else {
+    if (warp == kMmaWarp) {
+      tmem_alloc(tmem_at, 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    start_wait<kThreads>();
+    tc_fence_after();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
   const uint32_t ts = tmem, tp = tmem + 128, tdv = tmem + 256, tdk = tmem + 256 + DP;
@@ -399,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
             for (int q = 0; q < 4; ++q) add[q] = fmaf(sl[q], fabsf(ps[q] - mine), add[q]);
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = fmaf(__uint_as_float(s[0][c + q]), f, add[q]);
+          for (int q = 0; q < 4; q += 2)
+            tc::unpack2(tc::fma2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])), both(f), tc::pack2(add[q], add[q + 1])), x[q], x[q + 1]);
           if (!whole) {
             int en[4], lb[4];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(at + kEnd * 4) : "memory");
@@ -410,11 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           }
           float pr[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            pr[q] = ex2_approx(x[q]);
-            // with a cap, the weight times 1 - tanh^2
-            s[0][c + q] = __float_as_uint(CAP ? pr[q] * fmaf(-__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q]), 1.f) : pr[q]);
-          }
+          for (int q = 0; q < 4; ++q) pr[q] = ex2_approx(x[q]);
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) weight_slope<CAP>(s[0][c + q], s[0][c + q + 1], pr[q], pr[q + 1]);
           o[c % 8 / 2] = pack16<T>(pr[0], pr[1]);
           o[c % 8 / 2 + 1] = pack16<T>(pr[2], pr[3]);
         }
@@ -439,7 +467,10 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           float dl[4], y[4];
           tc::ld_shared_f4(st + (kDelta + c) * 4, dl[0], dl[1], dl[2], dl[3]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) y[q] = __uint_as_float(s[0][c + q]) * fmaf(__uint_as_float(d[c + q]), g, dl[q]);
+          for (int q = 0; q < 4; q += 2)
+            tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])),
+                                 tc::fma2(tc::pack2(__uint_as_float(d[c + q]), __uint_as_float(d[c + q + 1])), both(g), tc::pack2(dl[q], dl[q + 1]))),
+                        y[q], y[q + 1]);
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
           o[c % 8 / 2 + 1] = pack16<T>(y[2], y[3]);
         }
@@ -469,8 +500,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         pv = pk + n;
       }
       if (steps > 0) {
-        store_quarter<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, exists, zero, a.d, rk, pk);
-        store_quarter<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, exists, zero, a.d, rv, pv);
+        // the ring is free: all products are done, and with them all copies
+        const uint32_t room = base + L::kRing + warp * 4096;
+        const int lane = threadIdx.x & 31, first = key - lane, rows = a.nk - first;
+        if (pk != nullptr) {
+          const int64_t step = (int64_t)a.hk * a.d;
+          store_partial<DP>(tdk + lane_at, c0, a.scale_raw / gs, zero, a.d, room, [&](int r) { return r < rows ? pk + (r - lane) * step : nullptr; });
+          store_partial<DP>(tdv + lane_at, c0, Scales<T>::kUnshift, zero, a.d, room, [&](int r) { return r < rows ? pv + (r - lane) * step : nullptr; });
+        } else {
+          store_quarter<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, zero, a.d, room, [&](int r) { return r < rows ? rk + (r - lane) * a.dk.sn : nullptr; });
+          store_quarter<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, zero, a.d, room, [&](int r) { return r < rows ? rv + (r - lane) * a.dv.sn : nullptr; });
+        }
       } else {
         store_zeros<T, DP>(c0, exists, a.d, rk, pk);
         store_zeros<T, DP>(c0, exists, a.d, rv, pv);
@@ -524,11 +564,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
-  int64_t id = blockIdx.x;
-  const int hp = (int)(id % t.hp);
-  id /= t.hp;
-  const int b = (int)(id % a.b);
-  const int row0 = (t.blocks - 1 - (int)(id / a.b)) * kTile, hk = hp * t.pg / a.grp;
+  uint32_t id = blockIdx.x;
+  const int hp = (int)(id % (uint32_t)t.hp);
+  id /= (uint32_t)t.hp;
+  const int b = (int)(id % (uint32_t)a.b);
+  const int row0 = (t.blocks - 1 - (int)(id / (uint32_t)a.b)) * kTile, hk = (int)((uint32_t)(hp * t.pg) / (uint32_t)a.grp);
   const int i0 = row0 >> t.pg_shift, i1 = min(a.nq, (row0 + kTile) >> t.pg_shift);
   const Limits lim = limits_of(a, b);
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
@@ -539,19 +579,23 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   if (kd) lab = labels_of(qd, i0, i1);
   const int steps = count_tiles(ktab, 0, last, lab.lo, lab.hi);
 
-  if (warp == kMmaWarp) {
+  if (warp == kLoadWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
       tc::fence_barrier_init();
     }
     __syncwarp();
-    tmem_alloc(tmem_at, 512);
-    tmem_relinquish();
+    start_arrive<kThreads>();
+  } else {
+    if (warp == kMmaWarp) {
+      tmem_alloc(tmem_at, 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    start_wait<kThreads>();
+    tc_fence_after();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
   auto ts = [&](int i) { return tmem + (uint32_t)(i & 1) * 128; };
@@ -678,13 +722,16 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       if (!whole) seen = seen_columns(end - k0 - (int)mine0, kd == nullptr ? nullptr : kd + k0 + mine0, my);
       if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float raw = __uint_as_float(s[0][c]);
-        float x = fmaf(raw, f, add);
-        if constexpr (BIAS) x = fmaf(-slope2, fabsf(d0 - (float)c), x);
-        if (!whole && (seen >> c & 1) == 0) x = -INFINITY;
-        x = ex2_approx(x);
-        s[0][c] = __float_as_uint(CAP ? x * fmaf(-raw, raw, 1.f) : x);
+      for (int c = 0; c < 32; c += 2) {
+        float x[2];
+        tc::unpack2(tc::fma2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])), both(f), both(add)), x[0], x[1]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if constexpr (BIAS) x[q] = fmaf(-slope2, fabsf(d0 - (float)(c + q)), x[q]);
+          if (!whole && (seen >> (c + q) & 1) == 0) x[q] = -INFINITY;
+          x[q] = ex2_approx(x[q]);
+        }
+        weight_slope<CAP>(s[0][c], s[0][c + 1], x[0], x[1]);
       }
       ok = wait_bar(dpfull, (uint32_t)step & 1);
       if (!ok) break;
@@ -698,9 +745,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
 #pragma unroll
         for (int c = 8 * p; c < 8 * p + 8; c += 2) {
           float y[2];
+          tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])),
+                               tc::fma2(tc::pack2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), both(gs), both(nd))),
+                      y[0], y[1]);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            y[q] = __uint_as_float(s[0][c + q]) * fmaf(__uint_as_float(d[c + q]), gs, nd);
             // V rows that nobody may see are not cleaned here: their products may be anything
             if (!whole && (seen >> (c + q) & 1) == 0) y[q] = 0.f;
           }
@@ -720,7 +769,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       T* row = reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.sn + h * a.dq.sh;
       const int c0 = w * (DP / 4);
       if (steps > 0)
-        store_quarter<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, exists, add == -INFINITY, a.d, row, nullptr);
+        store_quarter<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, add == -INFINITY, a.d, base + L::kRing + warp * 4096, [&](int e) {
+          const int rr = r - (int)(threadIdx.x & 31) + e;
+          return rr < t.rows ? reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)(rr >> t.pg_shift) * a.dq.sn + (hp * t.pg + (rr & (t.pg - 1))) * a.dq.sh
+                             : nullptr;
+        });
       else
         store_zeros<T, DP>(c0, exists, a.d, row, nullptr);
     }

@@ -84,27 +84,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // block -> (row block, part of the key axis, sequence, packed head); late row blocks have the most keys under a causal
   // mask and start first
-  int64_t id = blockIdx.x;
-  const int hp = (int)(id % t.hp);
-  id /= t.hp;
-  const int b = (int)(id % a.b);
-  id /= a.b;
-  const int split = (int)(id % t.splits);
-  const int rb = t.blocks - 1 - (int)(id / t.splits);
+  uint32_t id = blockIdx.x;
+  const int hp = (int)(id % (uint32_t)t.hp);
+  id /= (uint32_t)t.hp;
+  const int b = (int)(id % (uint32_t)a.b);
+  id /= (uint32_t)a.b;
+  const int split = (int)(id % (uint32_t)t.splits);
+  const int rb = t.blocks - 1 - (int)(id / (uint32_t)t.splits);
   constexpr int kRows = PAIR ? 256 : 128;
-  const int row0 = rb * kRows, hk = hp * t.pg / a.grp;
+  const int row0 = rb * kRows, hk = (int)((uint32_t)(hp * t.pg) / (uint32_t)a.grp);
   const int i0 = row0 >> t.pg_shift, i1 = min(a.nq, (row0 + kRows) >> t.pg_shift);  // queries of this block
   const Limits lim = limits_of(a, b);
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int4* ktab = kd ? a.ktab + (int64_t)b * (a.nk_pad / kTile) : nullptr;
   const int tiles = (lim.row_end(i1 - 1, a.causal) + kTile - 1) / kTile;
-  const int first = (int)((int64_t)tiles * split / t.splits), last = (int)((int64_t)tiles * (split + 1) / t.splits);
+  // parts of at most one tile more than others
+  const int even = (int)((uint32_t)tiles / (uint32_t)t.splits), odd = tiles - even * t.splits;
+  const int first = split * even + min(split, odd), last = first + even + (split < odd ? 1 : 0);
   LabelRange lab{0, 0, false};
   if (kd) lab = labels_of(qd, i0, i1);
   const int steps = count_tiles(ktab, first, last, lab.lo, lab.hi);
 
-  if (warp == kMmaWarp) {
+  if (warp == kLoadWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 8), mbar_init(odone(w), 1), mbar_init(xbar(w), 8);
@@ -114,12 +116,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_barrier_init();
     }
     __syncwarp();
-    tmem_alloc(tmem_at, 512);
-    tmem_relinquish();
+    start_arrive<kThreads>();
+  } else {
+    if (warp == kMmaWarp) {
+      tmem_alloc(tmem_at, 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    start_wait<kThreads>();
+    tc_fence_after();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
   auto ts = [&](int w) { return tmem + (uint32_t)w * kTile; };                  // scores, then weights
@@ -407,10 +413,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (a.lse != nullptr)
           a.lse[((int64_t)b * a.hq + h) * a.nq + i] = lse2 * kLn2;
       }
-      T* out = reinterpret_cast<T*>(a.o.p) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
-      T* lo = a.o_lo == nullptr ? nullptr : reinterpret_cast<T*>(a.o_lo) + b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
+      // rows of the warp side by side.  The ring is free: this group has waited for all products, and with them for all copies; a
+      // group that had no tile has waited for nothing, but then either nobody had one, or there is nothing to write
+      const uint32_t room = base + L::kRing + warp * 4096;
+      const int r0 = r - (int)(threadIdx.x & 31);
 #pragma unroll
-      for (int c = side * (DP / 2); c < (side + 1) * (DP / 2); c += 32) {
+      for (int c = side * (DP / 2); c < (side + 1) * (DP / 2) && (worked || !parts); c += 32) {
         uint32_t o[32];
         if (worked) {
           tmem_ld32(to(w) + lane_at + c, o);
@@ -419,28 +427,42 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
         if (parts) {
-          if (exists && !none) {  // the joining kernel does not read empty rows
+          // the joining kernel does not read rows that saw nothing
+          const int64_t base_row = (((int64_t)part * a.b + b) * t.hp + hp) * t.rows;
+          store_rows32<8>(
+              room, [&](uint32_t p) { return make_uint4(o[4 * p], o[4 * p + 1], o[4 * p + 2], o[4 * p + 3]); },
+              [&](int e, int p, const uint4& v) {
+                if (r0 + e < t.rows && c + 4 * p < a.d) *reinterpret_cast<uint4*>(t.part_o + (base_row + r0 + e) * a.d + c + 4 * p) = v;
+              });
+        } else {
+          auto at_row = [&](int e, int p) -> int64_t {  // -1: not to be written
+            const int rr = r0 + e;
+            if (rr >= t.rows || c + 8 * p >= a.d) return -1;
+            return b * a.o.sb + (int64_t)(rr >> t.pg_shift) * a.o.sn + (hp * t.pg + (rr & (t.pg - 1))) * a.o.sh + c + 8 * p;
+          };
+          auto piece = [&](uint32_t p, bool low) {
+            uint32_t v[4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c + e < a.d) *reinterpret_cast<uint4*>(t.part_o + prow * a.d + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        } else if (exists) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (c + e < a.d) {
-              uint32_t v[4], x[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float y0 = __uint_as_float(o[e + 2 * q]), y1 = __uint_as_float(o[e + 2 * q + 1]);
-                v[q] = pack16<T>(y0, y1);
-                x[q] = pack16<T>(y0 - to_f<T>(from_f<T>(y0)), y1 - to_f<T>(from_f<T>(y1)));
-              }
-              *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
-              if (lo != nullptr) *reinterpret_cast<uint4*>(lo + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+            for (int q = 0; q < 4; ++q) {
+              const float y0 = __uint_as_float(o[8 * p + 2 * q]), y1 = __uint_as_float(o[8 * p + 2 * q + 1]);
+              v[q] = low ? pack16<T>(y0 - to_f<T>(from_f<T>(y0)), y1 - to_f<T>(from_f<T>(y1))) : pack16<T>(y0, y1);
             }
-          }
+            return make_uint4(v[0], v[1], v[2], v[3]);
+          };
+          store_rows32<4>(
+              room, [&](uint32_t p) { return piece(p, false); },
+              [&](int e, int p, const uint4& v) {
+                const int64_t to = at_row(e, p);
+                if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.o.p) + to) = v;
+              });
+          if (a.o_lo != nullptr)
+            store_rows32<4>(
+                room, [&](uint32_t p) { return piece(p, true); },
+                [&](int e, int p, const uint4& v) {
+                  const int64_t to = at_row(e, p);
+                  if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.o_lo) + to) = v;
+                });
         }
-        __syncwarp();
       }
     }
     tc_fence_before();

@@ -173,9 +173,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// s -> tanh(s * scale), in place, for N x 32 raw scores of a row.  Where all of a warp's arguments lie in [-1, 1], and scores
-// below the cap do, an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: x p(x^2) with p of
-// degree 6 fitted to tanh(x) / x at Chebyshev nodes (relative error 1.1e-7 in fp32).  With both on the MUFU unit, the
+// s -> tanh(s * scale), in place, for N x 32 raw scores of a row.  Where all of a warp's arguments lie in [-1/2, 1/2], and scores
+// of up to half the cap do, an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: x p(x^2) with
+// p of degree 4 fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32).  With both on the MUFU unit, the
 // exponential of the weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle
 // are 3072 cycles against 1024 of the two products.
 __device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
@@ -186,19 +186,17 @@ __device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], float scale) {
   for (int p = 0; p < N; ++p)
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(s[p][c]))), fabsf(__uint_as_float(s[p][c + 1])));
-  if (__all_sync(0xffffffffu, big * fabsf(scale) <= 1.f)) {
+  if (__all_sync(0xffffffffu, big * fabsf(scale) <= 0.5f)) {
 #pragma unroll
     for (int p = 0; p < N; ++p)
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         const uint64_t x = tc::mul2(tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1])), both(scale));
         const uint64_t z = tc::mul2(x, x);
-        uint64_t y = tc::fma2(z, both(0.0010380251333117485f), both(-0.0061943246982991695f));
-        y = tc::fma2(y, z, both(0.02027970738708973f));
-        y = tc::fma2(y, z, both(-0.053451646119356155f));
-        y = tc::fma2(y, z, both(0.13325075805187225f));
-        y = tc::fma2(y, z, both(-0.3333282768726349f));
-        y = tc::fma2(y, z, both(0.9999999403953552f));
+        uint64_t y = tc::fma2(z, both(0.017131345346570015f), both(-0.05298423767089844f));
+        y = tc::fma2(y, z, both(0.133247509598732f));
+        y = tc::fma2(y, z, both(-0.3333306908607483f));
+        y = tc::fma2(y, z, both(1.0f));
         y = tc::mul2(y, x);
         float y0, y1;
         tc::unpack2(y, y0, y1);
@@ -213,6 +211,38 @@ __device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], float scale) {
       for (int c = 0; c < 32; ++c)  // tanh(x) = 1 - 2 / (1 + e^2x)
         s[p][c] = __float_as_uint(fmaf(-2.f, rcp_approx(1.f + ex2_approx(__uint_as_float(s[p][c]) * f)), 1.f));
   }
+}
+
+// The block's first barrier (id 1): the loading warp, which has set up the mbarriers, goes on to its copies without waiting for
+// the others.
+template <int THREADS>
+__device__ __forceinline__ void start_arrive() { asm volatile("barrier.cta.arrive 1, %0;" ::"n"(THREADS) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void start_wait() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
+// A warp's 32 rows of N 16-byte pieces each, from a row per lane to lanes side by side in a row: `piece(p)` gives the lane's own
+// pieces, `put(row, p, v)` takes them.  A store of a row per lane would touch 32 cache lines at a time; this touches 32 / N rows.
+// `room`: 32 * N * 16 bytes of shared memory of the warp's own, 16-byte aligned.
+template <int N, typename Piece, typename Put>
+__device__ __forceinline__ void store_rows32(uint32_t room, Piece piece, Put put) {
+  const uint32_t lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (uint32_t p = 0; p < N; ++p) {
+    const uint4 v = piece(p);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(room + (lane * N + (p ^ (lane & (N - 1)))) * 16), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
+  }
+  __syncwarp();
+#pragma unroll
+  for (uint32_t e = 0; e < N; ++e) {
+    const uint32_t at = e * 32 + lane, row = at / N, p = at % N;
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(room + (row * N + (p ^ (row & (N - 1)))) * 16) : "memory");
+    put((int)row, (int)p, v);
+  }
+  __syncwarp();
 }
 
 // What the tensor-core kernels need on top of Args.
