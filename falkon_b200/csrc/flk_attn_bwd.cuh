@@ -408,43 +408,47 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       tc_fence_after();
       const Tile e = get_tile(slots, i);
       const bool whole = k0 + kTile <= lim.row_end((e.at * kTile) >> t.pg_shift, a.causal) && (kd == nullptr || (e.label >= 0 && e.label == only));
-      uint32_t s[1][32];
+      uint32_t s[1][32], pr[32];
       tmem_ld32(ts + lane_at + mine0, s[0]);
       tmem_ld_wait_on(s[0]);
       if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const uint32_t at = st + c * 4;
+        float x[4], add[4];
+        tc::ld_shared_f4(at + kLse * 4, add[0], add[1], add[2], add[3]);
+        if constexpr (BIAS) {
+          float sl[4], ps[4];
+          tc::ld_shared_f4(at + kSlope * 4, sl[0], sl[1], sl[2], sl[3]);
+          tc::ld_shared_f4(at + kPos * 4, ps[0], ps[1], ps[2], ps[3]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) add[q] = fmaf(sl[q], fabsf(ps[q] - mine), add[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q += 2)
+          tc::unpack2(tc::fma2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])), both(f), tc::pack2(add[q], add[q + 1])), x[q], x[q + 1]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pr[c + q] = __float_as_uint(ex2_approx(x[q]));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          int en[4], lb[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(st + (kEnd + c) * 4) : "memory");
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(lb[0]), "=r"(lb[1]), "=r"(lb[2]), "=r"(lb[3]) : "r"(st + (kLabel + c) * 4) : "memory");
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (key - k0 >= en[q] || (kd != nullptr && lb[q] != my)) pr[c + q] = 0;
+        }
+      }
+#pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[4];
 #pragma unroll
-        for (int c = 8 * p; c < 8 * p + 8; c += 4) {
-          const uint32_t at = st + c * 4;
-          float x[4], add[4];
-          tc::ld_shared_f4(at + kLse * 4, add[0], add[1], add[2], add[3]);
-          if constexpr (BIAS) {
-            float sl[4], ps[4];
-            tc::ld_shared_f4(at + kSlope * 4, sl[0], sl[1], sl[2], sl[3]);
-            tc::ld_shared_f4(at + kPos * 4, ps[0], ps[1], ps[2], ps[3]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) add[q] = fmaf(sl[q], fabsf(ps[q] - mine), add[q]);
-          }
-#pragma unroll
-          for (int q = 0; q < 4; q += 2)
-            tc::unpack2(tc::fma2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])), both(f), tc::pack2(add[q], add[q + 1])), x[q], x[q + 1]);
-          if (!whole) {
-            int en[4], lb[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(at + kEnd * 4) : "memory");
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(lb[0]), "=r"(lb[1]), "=r"(lb[2]), "=r"(lb[3]) : "r"(at + kLabel * 4) : "memory");
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (key - k0 >= en[q] || (kd != nullptr && lb[q] != my)) x[q] = -INFINITY;
-          }
-          float pr[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) pr[q] = ex2_approx(x[q]);
-#pragma unroll
-          for (int q = 0; q < 4; q += 2) weight_slope<CAP>(s[0][c + q], s[0][c + q + 1], pr[q], pr[q + 1]);
-          o[c % 8 / 2] = pack16<T>(pr[0], pr[1]);
-          o[c % 8 / 2 + 1] = pack16<T>(pr[2], pr[3]);
+        for (int c = 8 * p; c < 8 * p + 8; c += 2) {
+          const float p0 = __uint_as_float(pr[c]), p1 = __uint_as_float(pr[c + 1]);
+          weight_slope<CAP>(s[0][c], s[0][c + 1], p0, p1);
+          o[c % 8 / 2] = pack16<T>(p0, p1);
         }
         tmem_st4(ts + lane_at + mine0 + 4 * p, o);
       }
@@ -640,11 +644,15 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       bool ok = steps == 0 || wait_bar(own, 0);
       auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
       auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
-      // keys that nobody may see: dQ takes dS K, and their dS is zero, so K has to be finite there
+      // keys that nobody may see: their weights are zero, and what these meet, dP and K, has to be finite
+      auto arrived = [&](int n) {
+        if (!ready(n)) return false;
+        const Tile e = get_tile(slots, n / 2);
+        if (e.dirty || (e.at + 1) * kTile > lim.len) clean_tile<DP>(stage(n), e.at * kTile, lim.len, kd);
+        return true;
+      };
       auto scores = [&](int i) {
-        if (!ready(2 * i)) return false;
-        const Tile e = get_tile(slots, i);
-        if (e.dirty || (e.at + 1) * kTile > lim.len) clean_tile<DP>(stage(2 * i), e.at * kTile, lim.len, kd);
+        if (!arrived(2 * i)) return false;
         tc_fence_after();
         if (elect_one()) {
           issue_scores<T, DP>(ts(i), base, stage(2 * i));
@@ -654,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         return true;
       };
       auto products = [&](int i) {
-        if (!ready(2 * i + 1)) return false;
+        if (!arrived(2 * i + 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           issue_scores<T, DP>(tp, base + L::kTileBytes, stage(2 * i + 1));
@@ -718,8 +726,6 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       tmem_ld32(at, s[0]);
       tmem_ld_wait_on(s[0]);
       const float d0 = (float)(pos - k0 - (int)mine0);
-      uint32_t seen = 0xffffffffu;
-      if (!whole) seen = seen_columns(end - k0 - (int)mine0, kd == nullptr ? nullptr : kd + k0 + mine0, my);
       if constexpr (CAP) to_tanh(s, a.scale);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
@@ -728,10 +734,15 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           if constexpr (BIAS) x[q] = fmaf(-slope2, fabsf(d0 - (float)(c + q)), x[q]);
-          if (!whole && (seen >> (c + q) & 1) == 0) x[q] = -INFINITY;
           x[q] = ex2_approx(x[q]);
         }
         weight_slope<CAP>(s[0][c], s[0][c + 1], x[0], x[1]);
+      }
+      if (!whole) {
+        const uint32_t seen = seen_columns(end - k0 - (int)mine0, kd == nullptr ? nullptr : kd + k0 + mine0, my);
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if ((seen >> c & 1) == 0) s[0][c] = 0;
       }
       ok = wait_bar(dpfull, (uint32_t)step & 1);
       if (!ok) break;
@@ -748,11 +759,6 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
           tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])),
                                tc::fma2(tc::pack2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), both(gs), both(nd))),
                       y[0], y[1]);
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            // V rows that nobody may see are not cleaned here: their products may be anything
-            if (!whole && (seen >> (c + q) & 1) == 0) y[q] = 0.f;
-          }
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
         }
         tmem_st4(at + 4 * p, o);
