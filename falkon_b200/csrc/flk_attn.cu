@@ -3,6 +3,7 @@
 #include "flk_attn_bwd.cuh"
 #include "flk_attn_fwd.cuh"
 #include "flk_attn_simt.cuh"
+#include "flk_attn_token.cuh"
 
 namespace flk {
 namespace attn {
@@ -11,6 +12,8 @@ int forward_bf16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
 int forward_f16(const TcArgs& t, const fwd::Plan& p, cudaStream_t st);
 int forward_status_bf16(cudaStream_t st, int* out);
 int forward_status_f16(cudaStream_t st, int* out);
+int token_bf16(const TcArgs& t, int splits, cudaStream_t st);
+int token_f16(const TcArgs& t, int splits, cudaStream_t st);
 int backward_bf16(const TcArgs& t, const bwd::Plan& p, cudaStream_t st);
 int backward_f16(const TcArgs& t, const bwd::Plan& p, cudaStream_t st);
 int backward_status_bf16(cudaStream_t st, int* out);
@@ -110,6 +113,9 @@ static fwd::Plan forward_plan(const flk_attention_args* p) {
                         p->kv_lens != nullptr);
 }
 
+// A few rows over many keys (their bytes are the bound) go to the kernel for single tokens.
+static bool by_token(const flk_attention_args* p) { return on_tensor_cores(p) && token::takes((int)p->nq, (int)(p->hq / p->hk)); }
+static int token_splits(const flk_attention_args* p) { return token::splits_of((int)p->batch, (int)p->nk, (int)p->hk); }
 static bwd::Plan backward_plan(const flk_attention_args* p) {
   return bwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d, p->causal != 0, p->q_documents != nullptr);
 }
@@ -140,7 +146,7 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
     if (on_tensor_cores(p)) w.part_o = take(bwd::partial_floats(backward_plan(p), p->batch, p->nk, p->hk, p->d) * 4);
   }
   if (!backward && on_tensor_cores(p) && p->batch > 0 && p->nq > 0) {
-    const int64_t rows = fwd::partial_rows(forward_plan(p), (int)p->batch);
+    const int64_t rows = by_token(p) ? (int64_t)token_splits(p) * p->batch * p->hq * p->nq : fwd::partial_rows(forward_plan(p), (int)p->batch);
     w.part_o = take(rows * p->d * 4);
     w.part_lse = take(rows * 4);
   }
@@ -242,7 +248,10 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
     char* ws = reinterpret_cast<char*>(p->workspace);
     t.part_o = reinterpret_cast<float*>(ws + w.part_o), t.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
     const attn::fwd::Plan plan = attn::forward_plan(p);
-    FLK_TRY(p->dtype == FLK_BF16 ? attn::forward_bf16(t, plan, st) : attn::forward_f16(t, plan, st));
+    if (attn::by_token(p))
+      FLK_TRY(p->dtype == FLK_BF16 ? attn::token_bf16(t, attn::token_splits(p), st) : attn::token_f16(t, attn::token_splits(p), st));
+    else
+      FLK_TRY(p->dtype == FLK_BF16 ? attn::forward_bf16(t, plan, st) : attn::forward_f16(t, plan, st));
   } else if (p->dtype == FLK_F32) FLK_TRY(attn::simt_forward<float>(a, st));
   else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_forward<__nv_bfloat16>(a, st));
   else FLK_TRY(attn::simt_forward<__half>(a, st));

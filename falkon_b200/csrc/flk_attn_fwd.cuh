@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
   const int lane = threadIdx.x & 31;
   if (row >= n) return;
   const int r = (int)(row % t.rows), hp = (int)(row / t.rows % t.hp), b = (int)(row / t.rows / t.hp);
-  const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+  const int i = (int)((uint32_t)r / (uint32_t)t.pg), h = hp * t.pg + (r - i * t.pg);
   float top = -INFINITY;
   for (int p = lane; p < parts; p += 32) top = fmaxf(top, t.part_lse[p * n + row]);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -589,6 +589,13 @@ inline int launch_some(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
 }
 
 template <typename T>
+inline int launch_join(const TcArgs& t, int parts, cudaStream_t st) {
+  join_kernel<T><<<(unsigned)ceil_div((int64_t)t.a.b * t.hp * t.rows, 8), 256, 0, st>>>(t, parts);
+  count_launch();
+  return FLK_OK;
+}
+
+template <typename T>
 inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
@@ -601,11 +608,7 @@ inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
     FLK_TRY((p.pair ? launch_some<T, 64, true>(tq, tk, tv, t, st) : launch_some<T, 64, false>(tq, tk, tv, t, st)));
   else
     FLK_TRY((p.pair ? launch_some<T, 128, true>(tq, tk, tv, t, st) : launch_some<T, 128, false>(tq, tk, tv, t, st)));
-  if (p.parts > 1) {
-    join_kernel<T><<<(unsigned)ceil_div((int64_t)a.b * t.hp * t.rows, 8), 256, 0, st>>>(t, p.parts);
-    count_launch();
-  }
-  return FLK_OK;
+  return p.parts > 1 ? launch_join<T>(t, p.parts, st) : FLK_OK;
 }
 
 }  // namespace fwd
