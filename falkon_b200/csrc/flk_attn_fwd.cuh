@@ -9,9 +9,10 @@
 //   !PAIR  one row tile; the groups take the even and the odd key tiles, and end with a partial result each: few
 //          rows over a long key axis (single tokens)
 // Weights are exp2(s - m) with a maximum m that follows the running one only when that has grown by more than 8: weights
-// stay below 2^8, and the accumulator is rescaled a few times in a row's life instead of once per tile.  The sum of the
-// weights is taken before they are rounded to the data's 16 bits (a relative error of half a step per weight, which is what the
-// result itself is rounded by); it, the maximum and the accumulators are fp32.
+// stay below 2^8, and the accumulator is rescaled a few times in a row's life instead of once per tile.  Weights are rounded to
+// the data's 16 bits before they meet V (a relative error of half a step each, which is what the result itself is rounded by).
+// The result is divided by the sum of the rounded weights, so that their common error cancels; the log-sum-exp, which the
+// backward pass makes exact weights from, has the sum of the weights as they were.  Sums, maximum and accumulators are fp32.
 // Where blocks are fewer than SMs, the key axis is cut into parts, whose normalised fp32 results a second kernel joins.
 #pragma once
 
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const float f2 = CAP ? a.cap2 : a.scale;  // raw score, or its tanh -> base 2; done last where there is no bias
     float m = -INFINITY;       // of the weights, base 2
-    float l = 0.f;
+    float l = 0.f, lr = 0.f;  // sums of the weights, and of the rounded weights
     bool ok = true;
     // what the two threads of a row tell each other: one value per phase of `xbar`, which all warps of the tile pass
     uint32_t phase = 0;
@@ -294,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(xbar(w));
           mbar_arrive(pfull(w));
         }
+        ++phase;
         __syncwarp();
         continue;
       }
@@ -351,11 +353,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         l *= f;
+        lr *= f;
         m = mn;
       }
       const float mb = m == -INFINITY ? 0.f : m;
       const uint64_t f2v = tc::pack2(f2, f2), mv = tc::pack2(-mb, -mb);
-      uint64_t sum = 0;
+      uint64_t sum = 0, rounded = 0;
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[8];
@@ -370,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           p1 = ex2_approx(x1);
           sum = tc::add2(sum, tc::pack2(p0, p1));
           o[c / 2] = pack16<T>(p0, p1);
+          rounded = tc::add2(rounded, unpack16<T>(o[c / 2]));
         }
         tmem_st8(at + 8 * p, o);
       }
@@ -381,23 +385,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       float u0, u1;
       tc::unpack2(sum, u0, u1);
       l += u0 + u1;
+      tc::unpack2(rounded, u0, u1);
+      lr += u0 + u1;
     }
     // ---- results
     const bool worked = steps > (PAIR ? 0 : w);
     if (worked && ok) {
       // the products being done, all warps of the tile have passed the last step's exchange
       ok = wait_bar(odone(w), 0);
-      float theirs = 0.f;
-      if (ok && live)
-        ok = exchange(l, theirs);
-      else if (elect_one())
-        mbar_arrive(xbar(w));
+      // both sums, through what was the ring (behind what the stores below use)
+      const uint32_t sums = base + L::kRing + 65536;
+      static_assert(L::kStages * L::kTileBytes >= 65536 + 512 * 8, "ring");
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sums + threadIdx.x * 8), "f"(l), "f"(lr) : "memory");
       __syncwarp();
-      l = side == 0 ? l + theirs : theirs + l;  // the same sum on both sides
+      if (elect_one()) mbar_arrive(xbar(w));
+      __syncwarp();
+      ok = ok && wait_bar(xbar(w), phase & 1);
+      float x, y;
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(sums + (threadIdx.x ^ 128) * 8) : "memory");
+      l = side == 0 ? l + x : x + l;  // the same sums on both sides
+      lr = side == 0 ? lr + y : y + lr;
     }
     tc_fence_after();
     const bool none = m == -INFINITY;
-    const float inv = none ? 0.f : 1.0f / l, lse2 = none ? -INFINITY : m + log2f(l);
+    const float inv = none ? 0.f : 1.0f / lr, lse2 = none ? -INFINITY : m + log2f(l);
     if (live && ok) {
       // read again instead of held in registers through the loop above
       const int4 at = get_place(place);

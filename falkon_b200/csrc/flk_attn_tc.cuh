@@ -167,6 +167,16 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// the pair of fp32 values that a packed pair holds
+template <typename T>
+__device__ __forceinline__ uint64_t unpack16(uint32_t v) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return tc::pack2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return tc::pack2(f.x, f.y);
+  }
+}
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

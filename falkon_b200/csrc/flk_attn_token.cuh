@@ -3,10 +3,10 @@
 // Bound by the bytes of the cache.  The rows that share a key head, up to 16, are the 16 rows of mma.sync tiles; a warp walks
 // over 16 keys at a time, which it copies itself (cp.async) into a ring of its own in shared memory, so warps never wait for one
 // another before the end.  Scores stay in registers and become the A operand of the second product as they are.  Blocks of four
-// warps, two to an SM, keep about 100 KB per SM under way, whatever the lengths.  The tensor-core work is far from any bound
+// warps, two or three to an SM, keep about 128 KB per SM under way, whatever the lengths.  The tensor-core work is far from any bound
 // here (16 rows of 16 keys are read once and used once), so the tcgen05 pipeline, its tensor memory and its barriers would only
-// add latency: one token over 5001 ragged keys of 24 x 16 heads of 64 took 96 us with the prompts' kernel, 38 us being the
-// bytes' time.
+// add latency: one token over ragged caches of up to 5001 keys, 24 x 16 heads of 64, took 96 us with the prompts' kernel and
+// takes 54 us with this one, 38 us being the bytes' time.
 // Every block writes partial results (fp32, normalised) that the joining kernel of the prompts adds up in a fixed order.
 #pragma once
 
@@ -22,7 +22,7 @@ template <int DP>
 struct Layout {
   static constexpr int kRowBytes = DP * 2;
   static constexpr int kHalf = kKeys * kRowBytes;  // K or V of a stage
-  static constexpr int kStages = DP == 64 ? 5 : 3;
+  static constexpr int kStages = DP == 64 ? 4 : 3;
   static constexpr int kWarpBytes = kStages * 2 * kHalf;
   static constexpr int kBytes = kWarps * kWarpBytes;
 };
@@ -53,7 +53,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kWarps * 32, 2) kernel(const TcArgs t) {
+__global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const TcArgs t) {
   using L = Layout<DP>;
   extern __shared__ __align__(1024) uint8_t raw[];
   __shared__ float shared_m[kWarps][kRows], shared_l[kWarps][kRows];
@@ -272,11 +272,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kernel(const TcArgs t) {
   }
 }
 
-// Whether this kernel takes a call, and the parts of the key axis: about four blocks for each of the two places on an SM, so that
-// ragged lengths even out, but no less than 128 keys to a block.
+// Whether this kernel takes a call, and the parts of the key axis: about 12 blocks per SM, so that ragged lengths even out (32 caches of 16384 to 32768 keys:
+// 515 us with 2 blocks per SM, 479 with 8, 470 with 12), but no less than 128 keys to a block.
 inline bool takes(int nq, int grp) { return (int64_t)nq * grp <= kRows; }
 inline int splits_of(int b, int nk, int hk) {
-  const int64_t blocks = (int64_t)b * hk, want = ceil_div((int64_t)8 * kNumSMs, blocks), most = ceil_div(nk, 128);
+  const int64_t blocks = (int64_t)b * hk, want = ceil_div((int64_t)12 * kNumSMs, blocks), most = ceil_div(nk, 128);
   return (int)(want < most ? want : most);
 }
 
