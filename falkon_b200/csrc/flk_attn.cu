@@ -2,6 +2,7 @@
 #include "flk_attn.cuh"
 #include "flk_attn_bwd.cuh"
 #include "flk_attn_fwd.cuh"
+#include "flk_attn_rows.cuh"
 #include "flk_attn_simt.cuh"
 #include "flk_attn_token.cuh"
 
@@ -77,6 +78,7 @@ static int check_sizes(const flk_attention_args* p) {
   if (p == nullptr) return fail(FLK_ERR_BAD_ARG, "args: null pointer");
   if (p->dtype != FLK_F32 && p->dtype != FLK_BF16 && p->dtype != FLK_F16)
     return fail(FLK_ERR_BAD_ARG, "attention takes fp32, bf16 or fp16 data, not dtype %lld", (long long)p->dtype);
+  if (p->flags != 0) return fail(FLK_ERR_BAD_ARG, "flags: none are defined, 0 is expected");
   if (p->batch < 0 || p->nq < 0 || p->nk < 0 || p->hq < 1 || p->hk < 1 || p->d < 1)
     return fail(FLK_ERR_BAD_ARG, "negative or empty sizes");
   if (p->batch > 65535 || p->hq > 65535 || p->nq > (1 << 29) || p->nk > (1 << 29))
@@ -106,7 +108,7 @@ static int check_tensor(const char* name, const flk_tensor4& t, int64_t b, int64
 
 // The tensor-core kernels take 16-bit data; without keys there is nothing for them to do.
 static bool on_tensor_cores(const flk_attention_args* p) {
-  return p->dtype != FLK_F32 && p->nk > 0 && (p->flags & FLK_FLAG_FORCE_SIMT) == 0;
+  return p->dtype != FLK_F32 && p->nk > 0;
 }
 static fwd::Plan forward_plan(const flk_attention_args* p) {
   return fwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d, p->causal != 0, p->q_documents != nullptr,
@@ -192,28 +194,22 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
   return FLK_OK;
 }
 
-template <typename T>
-static int simt_forward(const Args& a, cudaStream_t st) {
-  return a.d <= 64 ? simt::launch_forward<T, 64>(a, st) : simt::launch_forward<T, 128>(a, st);
-}
-template <typename T>
-static int simt_backward(const Args& a, cudaStream_t st) {
-  if (a.nq > 0) {
-    FLK_TRY(simt::launch_delta<T>(a, nullptr, st));
-  }
-  return a.d <= 64 ? simt::launch_backward<T, 64>(a, st) : simt::launch_backward<T, 128>(a, st);
-}
-
 // delta, and for fp16 the largest magnitudes that the scale of dS is taken from
 template <typename T>
 static int prepare_backward(const Args& a, uint32_t* amax, cudaStream_t st) {
   if (amax != nullptr) {
     FLK_CUDA_TRY(cudaMemsetAsync(amax, 0, 8, st));
     const int64_t packs = (int64_t)a.b * a.nk * a.hk * a.d / 8, blocks = ceil_div(packs, 256 * 8);
-    simt::largest_value_kernel<T><<<(unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 256, 0, st>>>(a, amax + 1);
+    largest_value_kernel<T><<<(unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 256, 0, st>>>(a, amax + 1);
     count_launch();
   }
-  return simt::launch_delta<T>(a, amax, st);
+  return launch_delta<T>(a, amax, st);
+}
+
+// Zeros for a tensor (and -inf for `lse`, unless null): calls without keys, gradients without queries.
+static int write_nothing(int64_t dtype, const Tensor4& o, int b, int n, int h, int d, float* lse, cudaStream_t st) {
+  if (dtype == FLK_F32) return launch_nothing<float>(o, b, n, h, d, lse, st);
+  return launch_nothing<__half>(o, b, n, h, d, lse, st);  // zeros are the same in both 16-bit types
 }
 
 }  // namespace attn
@@ -241,7 +237,10 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   attn::Args a;
   FLK_TRY(attn::make_args(p, false, a, st));
-  if (attn::on_tensor_cores(p)) {
+  if (a.nk == 0) {
+    FLK_TRY(attn::write_nothing(p->dtype, a.o, a.b, a.nq, a.hq, a.d, a.lse, st));
+    if (a.o_lo != nullptr) FLK_TRY(attn::write_nothing(p->dtype, attn::Tensor4{a.o_lo, a.o.sb, a.o.sn, a.o.sh}, a.b, a.nq, a.hq, a.d, nullptr, st));
+  } else if (attn::on_tensor_cores(p)) {
     attn::TcArgs t{};
     t.a = a;
     const attn::Workspace w = attn::plan_workspace(p, false);
@@ -252,9 +251,9 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
       FLK_TRY(p->dtype == FLK_BF16 ? attn::token_bf16(t, attn::token_splits(p), st) : attn::token_f16(t, attn::token_splits(p), st));
     else
       FLK_TRY(p->dtype == FLK_BF16 ? attn::forward_bf16(t, plan, st) : attn::forward_f16(t, plan, st));
-  } else if (p->dtype == FLK_F32) FLK_TRY(attn::simt_forward<float>(a, st));
-  else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_forward<__nv_bfloat16>(a, st));
-  else FLK_TRY(attn::simt_forward<__half>(a, st));
+  } else {
+    FLK_TRY(a.d <= 64 ? attn::simt::launch_forward<64>(a, st) : attn::simt::launch_forward<128>(a, st));
+  }
   FLK_CUDA_TRY(cudaGetLastError());
   return FLK_OK;
 }
@@ -292,9 +291,13 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   attn::Args a;
   FLK_TRY(attn::make_args(p, true, a, st));
-  if (a.nq == 0) a.dq.p = nullptr;
-  if (a.nk == 0) a.dk.p = a.dv.p = nullptr;
-  if (attn::on_tensor_cores(p) && a.nq > 0) {
+  if (a.nq == 0 || a.nk == 0) {
+    if (a.nq > 0 && a.dq.p != nullptr) FLK_TRY(attn::write_nothing(p->dtype, a.dq, a.b, a.nq, a.hq, a.d, nullptr, st));
+    if (a.nk > 0 && a.dk.p != nullptr) {
+      FLK_TRY(attn::write_nothing(p->dtype, a.dk, a.b, a.nk, a.hk, a.d, nullptr, st));
+      FLK_TRY(attn::write_nothing(p->dtype, a.dv, a.b, a.nk, a.hk, a.d, nullptr, st));
+    }
+  } else if (attn::on_tensor_cores(p)) {
     attn::TcArgs t{};
     t.a = a;
     const attn::Workspace w = attn::plan_workspace(p, true);
@@ -310,9 +313,10 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
       FLK_TRY(attn::prepare_backward<__half>(a, amax, st));
       FLK_TRY(attn::backward_f16(t, plan, st));
     }
-  } else if (p->dtype == FLK_F32) FLK_TRY(attn::simt_backward<float>(a, st));
-  else if (p->dtype == FLK_BF16) FLK_TRY(attn::simt_backward<__nv_bfloat16>(a, st));
-  else FLK_TRY(attn::simt_backward<__half>(a, st));
+  } else {
+    FLK_TRY(attn::launch_delta<float>(a, nullptr, st));
+    FLK_TRY(a.d <= 64 ? attn::simt::launch_backward<64>(a, st) : attn::simt::launch_backward<128>(a, st));
+  }
   FLK_CUDA_TRY(cudaGetLastError());
   return FLK_OK;
 }

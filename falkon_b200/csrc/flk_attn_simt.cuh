@@ -1,13 +1,15 @@
-// Attention on the FP32 pipe, forward and backward: fp32 data, and the check of the tensor-core kernels.
+// Attention of fp32 data on the FP32 pipe, forward and backward.
 //
 // Tiles of 64 queries x 64 keys, 256 threads; a thread owns a 4 x 4 patch of the scores (rows 4 ty .. 4 ty + 3, columns
-// tx + 16 c) and 4 rows x DM / 16 columns of the accumulators.  Operands are converted to fp32 in shared memory; rows
-// that no query may see are written as zeros there, so what such rows hold (NaN, infinities) reaches nothing.  All sums
-// run in fp32 in a fixed order.  Bound by the FP32 pipe and by the shared-memory reads that feed it: per 4 values of d a
-// thread reads 8 vectors for 64 multiply-adds.
+// tx + 16 c) and 4 rows x DM / 16 columns of the accumulators.  Operands come by cp.async, one tile ahead of the one that is worked
+// on; rows that no query may see arrive as zeros, so what such rows hold (NaN, infinities) reaches nothing.  All sums run in
+// fp32, in pairs (packed multiply-adds), in a fixed order.  Bound by the FP32 pipe and by the shared-memory reads that feed it:
+// per 4 values of d a thread reads 8 vectors for 64 multiply-adds.  (2 x 1000 rows, 4 heads of 64, not causal, capped scores:
+// forward 127 us, dK and dV 212 us, dQ 160 us while every tile was fetched between two barriers.)
 #pragma once
 
 #include "flk_attn.cuh"
+#include "flk_ptx.cuh"
 
 namespace flk {
 namespace attn {
@@ -22,92 +24,94 @@ struct Smem {
   static constexpr int kLd = DM + 4;
   static constexpr int kRows = kT * kLd;  // floats of one operand tile
   static constexpr int kPair = kT * kPs;  // floats of one score tile
+  // buffers of a streamed operand: two where both fit beside the rest
+  static constexpr int kBuf = DM == 64 ? 2 : 1;
 };
 
-// rows [r0, r0 + 64) of one head into shared memory as fp32; rows at or behind `end`, and rows that the labels rule
-// out, as zeros
-template <typename T, int DM>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t sn, int r0, int end, int d, const int* docs) {
-  constexpr int kLd = Smem<DM>::kLd;
+// rows [r0, r0 + 64) of one head on their way into shared memory; rows at or behind `end`, and rows without a label, as zeros
+template <int DM>
+__device__ __forceinline__ void fetch_tile(float* dst, const Tensor4& t, int b, int h, int r0, int end, int d, const int* docs) {
+  const float* src = (const float*)t.p + b * t.sb + h * t.sh;
+  const uint32_t to = tc::smem_u32(dst);
+#pragma unroll
   for (int e = threadIdx.x; e < kT * (DM / 4); e += kThreads) {
     const int r = e / (DM / 4), c = (e - r * (DM / 4)) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r0 + r < end && c < d && (docs == nullptr || docs[r0 + r] >= 0)) {
-      const T* s = src + (int64_t)(r0 + r) * sn + c;
-      if constexpr (sizeof(T) == 4) {
-        v = *reinterpret_cast<const float4*>(s);
-      } else {
-        T t[4];
-        *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(s);
-        v = make_float4(to_f<T>(t[0]), to_f<T>(t[1]), to_f<T>(t[2]), to_f<T>(t[3]));
-      }
-    }
-    *reinterpret_cast<float4*>(dst + r * kLd + c) = v;
+    const bool valid = r0 + r < end && c < d && (docs == nullptr || __ldg(docs + r0 + r) >= 0);
+    // an address inside the tensor even where nothing is read
+    const float* s = src + (valid ? (int64_t)(r0 + r) * t.sn + c : 0);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (r * Smem<DM>::kLd + c) * 4), "l"(s), "r"(valid ? 16 : 0) : "memory");
   }
 }
 
-// acc[i][j] += sum over d of A[4 ty + i][:] . B[tx + 16 j][:]
+// acc[i][j] = sum over d of A[4 ty + i][:] . B[tx + 16 j][:]
 template <int DM>
 __device__ __forceinline__ void dots(float (&acc)[4][4], const float* A, const float* B, int ty, int tx) {
   constexpr int kLd = Smem<DM>::kLd;
+  uint64_t s[4][4] = {};
 #pragma unroll 4
   for (int c = 0; c < DM; c += 4) {
-    float4 x[4], y[4];
+    ulonglong2 x[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(A + (4 * ty + i) * kLd + c);
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const ulonglong2*>(A + (4 * ty + i) * kLd + c);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(B + (tx + 16 * j) * kLd + c);
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * j) * kLd + c);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+        s[i][j] = tc::fma2(x[i].x, y[j].x, s[i][j]);
+        s[i][j] = tc::fma2(x[i].y, y[j].y, s[i][j]);
       }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float u, v;
+      tc::unpack2(s[i][j], u, v);
+      acc[i][j] = u + v;
+    }
 }
 
 // acc[i][:] += sum over t of W[t][4 ty + i] * B[t][4 tx + 64 c ..]   (W is stored [t][row])
 template <int DM>
-__device__ __forceinline__ void outer(float (&acc)[4][DM / 16], const float* W, const float* B, int ty, int tx) {
+__device__ __forceinline__ void outer(uint64_t (&acc)[4][DM / 32], const float* W, const float* B, int ty, int tx) {
   constexpr int kLd = Smem<DM>::kLd;
 #pragma unroll 4
   for (int t = 0; t < kT; ++t) {
     const float4 w = *reinterpret_cast<const float4*>(W + t * kPs + 4 * ty);
-    const float ww[4] = {w.x, w.y, w.z, w.w};
+    const uint64_t ww[4] = {tc::pack2(w.x, w.x), tc::pack2(w.y, w.y), tc::pack2(w.z, w.z), tc::pack2(w.w, w.w)};
 #pragma unroll
     for (int c = 0; c < DM / 64; ++c) {
-      const float4 y = *reinterpret_cast<const float4*>(B + t * kLd + 4 * tx + 64 * c);
+      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(B + t * kLd + 4 * tx + 64 * c);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        acc[i][4 * c + 0] = fmaf(ww[i], y.x, acc[i][4 * c + 0]);
-        acc[i][4 * c + 1] = fmaf(ww[i], y.y, acc[i][4 * c + 1]);
-        acc[i][4 * c + 2] = fmaf(ww[i], y.z, acc[i][4 * c + 2]);
-        acc[i][4 * c + 3] = fmaf(ww[i], y.w, acc[i][4 * c + 3]);
+        acc[i][2 * c] = tc::fma2(ww[i], y.x, acc[i][2 * c]);
+        acc[i][2 * c + 1] = tc::fma2(ww[i], y.y, acc[i][2 * c + 1]);
       }
     }
   }
 }
 
-template <typename T, int DM>
-__device__ __forceinline__ void store_rows(T* dst, int64_t sn, int r0, int n, int d, const float (&acc)[4][DM / 16], const float (&f)[4],
-                                           int ty, int tx, T* lo = nullptr) {
+template <int DM>
+__device__ __forceinline__ void store_rows(const Tensor4& t, int b, int h, int r0, int n, int d, const uint64_t (&acc)[4][DM / 32], const float (&f)[4],
+                                           int ty, int tx) {
+  float* dst = (float*)t.p + b * t.sb + h * t.sh;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + 4 * ty + i;
     if (r >= n) continue;
 #pragma unroll
-    for (int c = 0; c < DM / 64; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = 4 * tx + 64 * c + e;
-        if (col >= d) continue;
-        const float y = acc[i][4 * c + e] * f[i];
-        dst[(int64_t)r * sn + col] = from_f<T>(y);
-        if (lo != nullptr) lo[(int64_t)r * sn + col] = from_f<T>(y - to_f<T>(from_f<T>(y)));
-      }
+    for (int c = 0; c < DM / 64; ++c) {
+      const int col = 4 * tx + 64 * c;
+      float x, y, z, w;
+      tc::unpack2(acc[i][2 * c], x, y);
+      tc::unpack2(acc[i][2 * c + 1], z, w);
+      // a row that saw nothing is zero, whatever met its weights of zero
+      if (col < d)
+        *reinterpret_cast<float4*>(dst + (int64_t)r * t.sn + col) =
+            f[i] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x * f[i], y * f[i], z * f[i], w * f[i]);
+    }
   }
 }
 
@@ -122,18 +126,26 @@ __device__ __forceinline__ float score(const Args& a, float raw, float slope2, i
   return fmaf(-slope2, fabsf((float)dist), s);
 }
 
-template <typename T, int DM>
+// whether the labels of a query tile and a key tile have a common range
+__device__ __forceinline__ bool labels_meet(const Args& a, int b, int q0, int k0) {
+  if (a.kdocs == nullptr) return true;
+  const int4 x = __ldg(a.qtab + (int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows), y = __ldg(a.ktab + (int64_t)b * (a.nk_pad / kTile) + k0 / kTile);
+  return x.y >= y.x && y.y >= x.x;
+}
+
+template <int DM>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   extern __shared__ float sm[];
-  float *Q = sm, *KV = Q + Smem<DM>::kRows, *P = KV + Smem<DM>::kRows;
+  constexpr int kRows = Smem<DM>::kRows;
+  float *Q = sm, *K = Q + kRows, *V = K + 2 * kRows, *P = V + 2 * kRows;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int q0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
   const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-  load_tile<T, DM>(Q, (const T*)a.q.p + b * a.q.sb + h * a.q.sh, a.q.sn, q0, a.nq, a.d, qd);
-  float m[4], l[4], acc[4][DM / 16];
+  float m[4], l[4];
+  uint64_t acc[4][DM / 32] = {};
   int end[4], id[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -142,20 +154,28 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
     id[i] = qd && r < a.nq ? qd[r] : -2;
     m[i] = -INFINITY;
     l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < DM / 16; ++c) acc[i][c] = 0.f;
   }
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
-  for (int k0 = 0; k0 < last; k0 += kT) {
-    if (kd != nullptr) {  // no label in common: nothing to see
-      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
-      if (x.y < y.x || y.y < x.x) continue;
-    }
-    __syncthreads();
-    load_tile<T, DM>(KV, (const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.sn, k0, lim.len, a.d, kd);
-    __syncthreads();
-    float s[4][4] = {};
-    dots<DM>(s, Q, KV, ty, tx);
+  auto next = [&](int k0) {
+    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT;
+    return k0;
+  };
+  int k0 = next(0), buf = 0;
+  fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd);
+  if (k0 < last) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd);
+  cp_async_commit();
+  if (k0 < last) fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd);
+  cp_async_commit();
+  while (k0 < last) {
+    const int k1 = next(k0 + kT);
+    if (k1 < last) fetch_tile<DM>(K + (buf ^ 1) * kRows, a.k, b, hk, k1, lim.len, a.d, kd);
+    cp_async_commit();
+    cp_async_wait<2>();
+    __syncthreads();  // K is here; all have done with the weights and values of the tile before
+    if (k1 < last) fetch_tile<DM>(V + (buf ^ 1) * kRows, a.v, b, hk, k1, lim.len, a.d, kd);
+    cp_async_commit();
+    float s[4][4];
+    dots<DM>(s, Q, K + buf * kRows, ty, tx);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int pos = lim.start + q0 + 4 * ty + i;
@@ -165,8 +185,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
         const int col = k0 + tx + 16 * j;
         float t;
         const float v = score(a, s[i][j], slope2, pos - col, t);
-        const bool see = col < end[i] && (kd == nullptr || kd[col] == id[i]);
-        s[i][j] = see ? v : -INFINITY;
+        s[i][j] = col < end[i] && (kd == nullptr || kd[col] == id[i]) ? v : -INFINITY;
         top = fmaxf(top, s[i][j]);
       }
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -181,205 +200,137 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
       }
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       l[i] = fmaf(l[i], f, sum);
+      const uint64_t ff = tc::pack2(f, f);
 #pragma unroll
-      for (int c = 0; c < DM / 16; ++c) acc[i][c] *= f;
+      for (int c = 0; c < DM / 32; ++c) acc[i][c] = tc::mul2(acc[i][c], ff);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) P[(tx + 16 * j) * kPs + 4 * ty + i] = s[i][j];
-    __syncthreads();
-    load_tile<T, DM>(KV, (const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.sn, k0, lim.len, a.d, kd);
-    __syncthreads();
-    outer<DM>(acc, P, KV, ty, tx);
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(P + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    cp_async_wait<2>();
+    __syncthreads();  // V is here, and the weights
+    outer<DM>(acc, P, V + buf * kRows, ty, tx);
+    k0 = k1;
+    buf ^= 1;
   }
+  cp_async_wait<0>();
   float f[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = q0 + 4 * ty + i;
     f[i] = l[i] == 0.f ? 0.f : 1.0f / l[i];
-    if (l[i] == 0.f)
-      for (int c = 0; c < DM / 16; ++c) acc[i][c] = 0.f;
     if (tx == 0 && r < a.nq && a.lse != nullptr)
       a.lse[((int64_t)b * a.hq + h) * a.nq + r] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
-  store_rows<T, DM>((T*)a.o.p + b * a.o.sb + h * a.o.sh, a.o.sn, q0, a.nq, a.d, acc, f, ty, tx,
-                    a.o_lo == nullptr ? nullptr : (T*)a.o_lo + b * a.o.sb + h * a.o.sh);
-}
-
-// delta_i = dO_i . O_i, a group of LANES lanes per row of one head (16 bytes of each array per lane), two rows per group at a time,
-// and the largest |dO| of the rows that see something (`amax`, as bits, unless null; a maximum does not depend on the order it
-// is taken in).  Bound by the bytes of dO, O and what rounding took from O.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(256) delta_kernel(const Args a, uint32_t* amax) {
-  constexpr int kVec = 16 / sizeof(T), kGroups = 256 / LANES;
-  const uint32_t n = (uint32_t)a.nq * (uint32_t)a.hq;
-  const int b = blockIdx.y, c = (threadIdx.x % LANES) * kVec;
-  const T *dout = (const T*)a.dout.p + b * a.dout.sb, *o = (const T*)a.o.p + b * a.o.sb;
-  const T* lo = a.o_lo == nullptr ? nullptr : (const T*)a.o_lo + b * a.o.sb;
-  float s[2] = {0.f, 0.f}, top[2] = {0.f, 0.f};
-  int64_t at[2];
-  bool on[2];
-  uint4 u[2], w[2], x[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint32_t row = (blockIdx.x * 2 + e) * kGroups + threadIdx.x / LANES;  // (i, h), h fastest
-    on[e] = row < n;
-    const uint32_t i = on[e] ? row / (uint32_t)a.hq : 0, h = on[e] ? row - i * (uint32_t)a.hq : 0;
-    at[e] = ((int64_t)b * a.hq + h) * a.nq + i;
-    u[e] = w[e] = x[e] = make_uint4(0, 0, 0, 0);
-    if (on[e] && c < a.d) {
-      const int64_t off = i * a.o.sn + h * a.o.sh + c;
-      u[e] = *reinterpret_cast<const uint4*>(dout + i * a.dout.sn + h * a.dout.sh + c);
-      w[e] = *reinterpret_cast<const uint4*>(o + off);
-      if (lo != nullptr) x[e] = *reinterpret_cast<const uint4*>(lo + off);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const T *p = reinterpret_cast<const T*>(&u[e]), *q = reinterpret_cast<const T*>(&w[e]), *r = reinterpret_cast<const T*>(&x[e]);
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const float g = to_f<T>(p[k]);
-      s[e] = fmaf(g, to_f<T>(q[k]), s[e]);
-      if (sizeof(T) == 2) s[e] = fmaf(g, to_f<T>(r[k]), s[e]);
-      top[e] = fmaxf(top[e], fabsf(g));
-    }
-    for (int k = LANES / 2; k > 0; k >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], k);
-    if (c == 0 && on[e]) a.delta[at[e]] = s[e];
-  }
-  if (amax != nullptr) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (!on[e] || a.lse[at[e]] == -INFINITY) top[e] = 0.f;
-      for (int k = 16; k > 0; k >>= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], k));
-    }
-    const uint32_t bits = __float_as_uint(fmaxf(top[0], top[1]));
-    if ((threadIdx.x & 31) == 0 && bits > *reinterpret_cast<volatile uint32_t*>(amax)) atomicMax(amax, bits);
-  }
-}
-template <typename T>
-inline int launch_delta(const Args& a, uint32_t* amax, cudaStream_t st) {
-  constexpr int kVec = 16 / sizeof(T);
-  const int64_t n = (int64_t)a.nq * a.hq;
-  const int lanes = a.d <= 8 * kVec ? 8 : a.d <= 16 * kVec ? 16 : 32;
-  const dim3 grid((unsigned)ceil_div(n, 2 * 256 / lanes), a.b);
-  if (lanes == 8) delta_kernel<T, 8><<<grid, 256, 0, st>>>(a, amax);
-  else if (lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a, amax);
-  else delta_kernel<T, 32><<<grid, 256, 0, st>>>(a, amax);
-  count_launch();
-  return FLK_OK;
-}
-
-// Largest |v| of the rows that may be seen, as bits.
-template <typename T>
-__global__ void __launch_bounds__(256) largest_value_kernel(const Args a, uint32_t* amax) {
-  constexpr int kVec = 16 / sizeof(T);
-  const int packs = a.d / kVec;
-  const int64_t n = (int64_t)a.b * a.nk * a.hk * packs;
-  float top = 0.f;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    const int c = (int)(e % packs) * kVec;
-    const int64_t row = e / packs;
-    const int h = (int)(row % a.hk), j = (int)(row / a.hk % a.nk), b = (int)(row / a.hk / a.nk);
-    if (j >= (a.kv_lens != nullptr ? a.kv_lens[b] : a.nk) || (a.kdocs != nullptr && a.kdocs[(int64_t)b * a.nk_pad + j] < 0)) continue;
-    T u[kVec];
-    *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>((const T*)a.v.p + b * a.v.sb + j * a.v.sn + h * a.v.sh + c);
-#pragma unroll
-    for (int x = 0; x < kVec; ++x) top = fmaxf(top, fabsf(to_f<T>(u[x])));
-  }
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) atomicMax(amax, __float_as_uint(top));
+  store_rows<DM>(a.o, b, h, q0, a.nq, a.d, acc, f, ty, tx);
 }
 
 // Gradients of 64 keys and values: loops over the query heads that share them and over their query tiles.
-template <typename T, int DM>
+template <int DM>
 __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
   extern __shared__ float sm[];
-  constexpr int kRows = Smem<DM>::kRows;
-  float *K = sm, *V = K + kRows, *QD = V + kRows, *W = QD + kRows;
-  float *sl = W + Smem<DM>::kPair, *sd = sl + kT;
+  constexpr int kRows = Smem<DM>::kRows, kBuf = Smem<DM>::kBuf;
+  float *K = sm, *V = K + kRows, *Q = V + kRows, *G = Q + kBuf * kRows, *P = G + kBuf * kRows, *W = P + Smem<DM>::kPair;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int k0 = blockIdx.x * kT, hk = blockIdx.y, b = blockIdx.z;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
-  load_tile<T, DM>(K, (const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.sn, k0, lim.len, a.d, kd);
-  load_tile<T, DM>(V, (const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.sn, k0, lim.len, a.d, kd);
-  float dk[4][DM / 16] = {}, dv[4][DM / 16] = {};
+  uint64_t dk[4][DM / 32] = {}, dv[4][DM / 32] = {};
   int id[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) id[i] = kd ? kd[min(k0 + 4 * ty + i, a.nk_pad - 1)] : 0;
-  for (int g = 0; g < a.grp && k0 < lim.len; ++g) {
-    const int h = hk * a.grp + g;
+  // steps: query tiles of one head after the other
+  const int tiles = (a.nq + kT - 1) / kT;
+  const int64_t steps = k0 < lim.len ? (int64_t)a.grp * tiles : 0;
+  auto next = [&](int64_t s) {
+    for (; s < steps; ++s) {
+      const int q0 = (int)(s % tiles) * kT;
+      if (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) > k0 && labels_meet(a, b, q0, k0)) break;
+    }
+    return s;
+  };
+  auto fetch = [&](int64_t s, int buf) {
+    const int h = hk * a.grp + (int)(s / tiles), q0 = (int)(s % tiles) * kT;
+    fetch_tile<DM>(Q + buf * kRows, a.q, b, h, q0, a.nq, a.d, qd);
+    fetch_tile<DM>(G + buf * kRows, a.dout, b, h, q0, a.nq, a.d, qd);
+  };
+  int64_t step = next(0);
+  int buf = 0;
+  fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd);
+  fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd);
+  if (step < steps) fetch(step, 0);
+  cp_async_commit();
+  while (step < steps) {
+    const int64_t after = next(step + 1);
+    const int h = hk * a.grp + (int)(step / tiles), q0 = (int)(step % tiles) * kT;
     const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     const float *lse = a.lse + ((int64_t)b * a.hq + h) * a.nq, *delta = a.delta + ((int64_t)b * a.hq + h) * a.nq;
-    for (int q0 = 0; q0 < a.nq; q0 += kT) {
-      if (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) <= k0) continue;
-      if (kd != nullptr) {
-        const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
-        if (x.y < y.x || y.y < x.x) continue;
-      }
-      __syncthreads();
-      load_tile<T, DM>(QD, (const T*)a.q.p + b * a.q.sb + h * a.q.sh, a.q.sn, q0, a.nq, a.d, qd);
-      if (threadIdx.x < kT) {
-        const int r = q0 + threadIdx.x;
-        sl[threadIdx.x] = r < a.nq ? lse[r] * kLog2e : 0.f;
-        sd[threadIdx.x] = r < a.nq ? delta[r] : 0.f;
-      }
-      __syncthreads();
-      float s[4][4] = {}, p[4][4];  // rows: keys, columns: queries
-      dots<DM>(s, K, QD, ty, tx);
+    float lse2[4], dl[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = k0 + 4 * ty + i, r = q0 + tx + 16 * j;
-          float t;
-          const float v = score(a, s[i][j], slope2, lim.start + r - key, t);
-          const bool see = r < a.nq && key < lim.row_end(r, a.causal) && (kd == nullptr || qd[r] == id[i]);
-          p[i][j] = see ? exp2f(v - sl[tx + 16 * j]) : 0.f;
-          s[i][j] = 1.f - t * t;
-          W[(tx + 16 * j) * kPs + 4 * ty + i] = p[i][j];
-        }
-      // dK needs Q after dO has been here: Q is loaded again (from L2); one operand tile less keeps the block small
-      __syncthreads();
-      load_tile<T, DM>(QD, (const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh, a.dout.sn, q0, a.nq, a.d, qd);
-      __syncthreads();
-      outer<DM>(dv, W, QD, ty, tx);
-      float dp[4][4] = {};
-      dots<DM>(dp, V, QD, ty, tx);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          W[(tx + 16 * j) * kPs + 4 * ty + i] = p[i][j] == 0.f ? 0.f : p[i][j] * (dp[i][j] - sd[tx + 16 * j]) * s[i][j];
-      load_tile<T, DM>(QD, (const T*)a.q.p + b * a.q.sb + h * a.q.sh, a.q.sn, q0, a.nq, a.d, qd);
-      __syncthreads();
-      outer<DM>(dk, W, QD, ty, tx);
+    for (int j = 0; j < 4; ++j) {
+      const int r = q0 + tx + 16 * j;
+      lse2[j] = r < a.nq ? __ldg(lse + r) * kLog2e : 0.f;
+      dl[j] = r < a.nq ? __ldg(delta + r) : 0.f;
     }
+    if constexpr (kBuf == 2) {
+      __syncthreads();  // all have done with the other buffer
+      if (after < steps) fetch(after, buf ^ 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    float s[4][4], dp[4][4];  // rows: keys, columns: queries
+    dots<DM>(s, K, Q + buf * kRows, ty, tx);
+    dots<DM>(dp, V, G + buf * kRows, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + 4 * ty + i, r = q0 + tx + 16 * j;
+        float t;
+        const float v = score(a, s[i][j], slope2, lim.start + r - key, t);
+        const bool see = r < a.nq && key < lim.row_end(r, a.causal) && (kd == nullptr || qd[r] == id[i]);
+        s[i][j] = see ? exp2f(v - lse2[j]) : 0.f;
+        dp[i][j] = see ? s[i][j] * (dp[i][j] - dl[j]) * (1.f - t * t) : 0.f;
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      *reinterpret_cast<float4*>(P + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+      *reinterpret_cast<float4*>(W + (tx + 16 * j) * kPs + 4 * ty) = make_float4(dp[0][j], dp[1][j], dp[2][j], dp[3][j]);
+    }
+    __syncthreads();
+    outer<DM>(dv, P, G + buf * kRows, ty, tx);
+    outer<DM>(dk, W, Q + buf * kRows, ty, tx);
+    if constexpr (kBuf == 1) {
+      __syncthreads();
+      if (after < steps) fetch(after, 0);
+      cp_async_commit();
+    }
+    step = after;
+    if (kBuf == 2) buf ^= 1;
   }
+  cp_async_wait<0>();
   const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {a.scale_raw, a.scale_raw, a.scale_raw, a.scale_raw};
-  store_rows<T, DM>((T*)a.dk.p + b * a.dk.sb + hk * a.dk.sh, a.dk.sn, k0, a.nk, a.d, dk, sc, ty, tx);
-  store_rows<T, DM>((T*)a.dv.p + b * a.dv.sb + hk * a.dv.sh, a.dv.sn, k0, a.nk, a.d, dv, one, ty, tx);
+  store_rows<DM>(a.dk, b, hk, k0, a.nk, a.d, dk, sc, ty, tx);
+  store_rows<DM>(a.dv, b, hk, k0, a.nk, a.d, dv, one, ty, tx);
 }
 
 // Gradient of 64 queries.
-template <typename T, int DM>
+template <int DM>
 __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
   extern __shared__ float sm[];
-  constexpr int kRows = Smem<DM>::kRows;
-  float *Q = sm, *G = Q + kRows, *KV = G + kRows, *W = KV + kRows;
+  constexpr int kRows = Smem<DM>::kRows, kBuf = Smem<DM>::kBuf;
+  float *Q = sm, *G = Q + kRows, *K = G + kRows, *V = K + kBuf * kRows, *W = V + kBuf * kRows;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int q0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
   const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-  load_tile<T, DM>(Q, (const T*)a.q.p + b * a.q.sb + h * a.q.sh, a.q.sn, q0, a.nq, a.d, qd);
-  load_tile<T, DM>(G, (const T*)a.dout.p + b * a.dout.sb + h * a.dout.sh, a.dout.sn, q0, a.nq, a.d, qd);
-  float dq[4][DM / 16] = {}, lse2[4], delta[4];
+  uint64_t dq[4][DM / 32] = {};
+  float lse2[4], delta[4];
   int end[4], id[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -390,20 +341,33 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
     delta[i] = r < a.nq ? a.delta[((int64_t)b * a.hq + h) * a.nq + r] : 0.f;
   }
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
-  for (int k0 = 0; k0 < last; k0 += kT) {
-    if (kd != nullptr) {
-      const int4 x = a.qtab[(int64_t)b * (a.nq_pad / a.q_rows) + q0 / a.q_rows], y = a.ktab[(int64_t)b * (a.nk_pad / kTile) + k0 / kTile];
-      if (x.y < y.x || y.y < x.x) continue;
+  auto next = [&](int k0) {
+    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT;
+    return k0;
+  };
+  auto fetch = [&](int k0, int buf) {
+    fetch_tile<DM>(K + buf * kRows, a.k, b, hk, k0, lim.len, a.d, kd);
+    fetch_tile<DM>(V + buf * kRows, a.v, b, hk, k0, lim.len, a.d, kd);
+  };
+  int k0 = next(0), buf = 0;
+  fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd);
+  fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, qd);
+  if (k0 < last) fetch(k0, 0);
+  cp_async_commit();
+  while (k0 < last) {
+    const int k1 = next(k0 + kT);
+    if constexpr (kBuf == 2) {
+      __syncthreads();  // all have done with the other buffer, and with the weights
+      if (k1 < last) fetch(k1, buf ^ 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
     }
-    float s[4][4] = {}, dp[4][4] = {};
     __syncthreads();
-    load_tile<T, DM>(KV, (const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.sn, k0, lim.len, a.d, kd);
-    __syncthreads();
-    dots<DM>(dp, G, KV, ty, tx);
-    __syncthreads();
-    load_tile<T, DM>(KV, (const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.sn, k0, lim.len, a.d, kd);
-    __syncthreads();
-    dots<DM>(s, Q, KV, ty, tx);
+    float s[4][4], dp[4][4];
+    dots<DM>(s, Q, K + buf * kRows, ty, tx);
+    dots<DM>(dp, G, V + buf * kRows, ty, tx);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -412,38 +376,48 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
         float t;
         const float v = score(a, s[i][j], slope2, lim.start + q0 + 4 * ty + i - col, t);
         const bool see = col < end[i] && (kd == nullptr || kd[col] == id[i]);
-        const float p = see ? exp2f(v - lse2[i]) : 0.f;
-        W[(tx + 16 * j) * kPs + 4 * ty + i] = see ? p * (dp[i][j] - delta[i]) * (1.f - t * t) : 0.f;
+        s[i][j] = see ? exp2f(v - lse2[i]) * (dp[i][j] - delta[i]) * (1.f - t * t) : 0.f;
       }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(W + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
     __syncthreads();
-    outer<DM>(dq, W, KV, ty, tx);
+    outer<DM>(dq, W, K + buf * kRows, ty, tx);
+    if constexpr (kBuf == 1) {
+      __syncthreads();
+      if (k1 < last) fetch(k1, 0);
+      cp_async_commit();
+    }
+    k0 = k1;
+    if (kBuf == 2) buf ^= 1;
   }
+  cp_async_wait<0>();
   const float sc[4] = {a.scale_raw, a.scale_raw, a.scale_raw, a.scale_raw};
-  store_rows<T, DM>((T*)a.dq.p + b * a.dq.sb + h * a.dq.sh, a.dq.sn, q0, a.nq, a.d, dq, sc, ty, tx);
+  store_rows<DM>(a.dq, b, h, q0, a.nq, a.d, dq, sc, ty, tx);
 }
 
 template <int DM>
-constexpr size_t forward_smem() { return (2 * Smem<DM>::kRows + Smem<DM>::kPair) * 4; }
+constexpr size_t forward_smem() { return (5 * Smem<DM>::kRows + Smem<DM>::kPair) * 4; }
 template <int DM>
-constexpr size_t backward_smem() { return (3 * Smem<DM>::kRows + Smem<DM>::kPair + 2 * kT) * 4; }
+constexpr size_t backward_smem() { return ((2 + 2 * Smem<DM>::kBuf) * Smem<DM>::kRows + 2 * Smem<DM>::kPair) * 4; }
+static_assert(forward_smem<128>() <= 227 * 1024 && backward_smem<64>() <= 227 * 1024 && backward_smem<128>() <= 227 * 1024, "shared memory");
 
-template <typename T, int DM>
+template <int DM>
 inline int launch_forward(const Args& a, cudaStream_t st) {
-  FLK_CUDA_TRY(cudaFuncSetAttribute(forward_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)forward_smem<DM>()));
-  forward_kernel<T, DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, forward_smem<DM>(), st>>>(a);
+  FLK_CUDA_TRY(cudaFuncSetAttribute(forward_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)forward_smem<DM>()));
+  forward_kernel<DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, forward_smem<DM>(), st>>>(a);
   count_launch();
   return FLK_OK;
 }
-template <typename T, int DM>
+template <int DM>
 inline int launch_backward(const Args& a, cudaStream_t st) {
-  FLK_CUDA_TRY(cudaFuncSetAttribute(backward_kv_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
-  FLK_CUDA_TRY(cudaFuncSetAttribute(backward_q_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
   if (a.dk.p != nullptr) {
-    backward_kv_kernel<T, DM><<<dim3((unsigned)ceil_div(a.nk, kT), a.hk, a.b), kThreads, backward_smem<DM>(), st>>>(a);
+    FLK_CUDA_TRY(cudaFuncSetAttribute(backward_kv_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
+    backward_kv_kernel<DM><<<dim3((unsigned)ceil_div(a.nk, kT), a.hk, a.b), kThreads, backward_smem<DM>(), st>>>(a);
     count_launch();
   }
   if (a.dq.p != nullptr) {
-    backward_q_kernel<T, DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, backward_smem<DM>(), st>>>(a);
+    FLK_CUDA_TRY(cudaFuncSetAttribute(backward_q_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
+    backward_q_kernel<DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, backward_smem<DM>(), st>>>(a);
     count_launch();
   }
   return FLK_OK;

@@ -38,10 +38,10 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _pack(q, k, v, out, out_lo, lse, opts, dout=None, dq=None, dk=None, dv=None) -> bytes:
-    scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs, flags = opts
+    scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs = opts
     b, nq, hq, d = q.shape
     return _lib._ATTENTION_HEAD.pack(
-        _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, causal, flags, scale, softcap,
+        _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, causal, 0, scale, softcap,
         *_t4(q), *_t4(k), *_t4(v), *_t4(out), _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens),
         _ptr(q_starts), _ptr(q_docs), 0 if q_docs is None else q_docs.stride(0), _ptr(k_docs),
         0 if k_docs is None else k_docs.stride(0), *_t4(dout), *_t4(dq), *_t4(dk), *_t4(dv))
@@ -133,7 +133,6 @@ def attention(
     kv_lens: Optional[torch.Tensor] = None,
     q_starts: Optional[torch.Tensor] = None,
     return_lse: bool = False,
-    flk_flags: int = 0,
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``out[b, i, h] = sum_j softmax_j(s_ij) v[b, j, h']`` over the keys j that query i may see.
 
@@ -202,7 +201,7 @@ def attention(
         q_documents = documents
     opts = (scale, softcap, 1 if causal else 0, slopes, _table("prefix_lens", prefix_lens, (b,), dev),
             _table("kv_lens", kv_lens, (b,), dev), _table("q_starts", q_starts, (b,), dev),
-            _table("q_documents", q_documents, (b, nq), dev), _table("documents", documents, (b, nk), dev), int(flk_flags))
+            _table("q_documents", q_documents, (b, nq), dev), _table("documents", documents, (b, nk), dev))
     pad = -d % 8
     if pad:  # the kernels read whole vectors of 16 bytes; zeros change no dot product
         q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))

@@ -271,7 +271,7 @@ int flk_kgrad(int dtype, int kernel,
  * arrays of one entry per sequence (values outside [0, nk], and positions beyond 2^29, are clamped); documents: int32, one row per
  * sequence with the given stride; slopes: fp32, one per query head.  All of them may be NULL.
  *
- * flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
+ * flags is 0: none are defined.  flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
  * v, out, lse and dout and writes dq, dk, dv (dk and dv are given together; dq.data or both may be NULL).  Sums run in
  * an order fixed by the sizes: results are the same from run to run.  The workspace query takes the same struct
  * (pointers other than the documents' are not looked at).
