@@ -115,16 +115,47 @@ __device__ __forceinline__ void store_rows(const Tensor4& t, int b, int h, int r
   }
 }
 
-// raw dot -> score in base 2; t = tanh of the capped score (0 without a cap)
-__device__ __forceinline__ float score(const Args& a, float raw, float slope2, int dist, float& t) {
-  float s = raw * a.scale;
-  t = 0.f;
-  if (a.cap2 != 0.f) {
-    t = tanhf(s);
-    s = a.cap2 * t;
+// The thread's 16 raw dots -> scores in base 2 without the distance bias, and, with a cap, the tanh of each in t (else 0).
+// tanh is x p(x^2), p of degree 4 (relative error 6e-8, see to_tanh), where the whole warp's arguments lie in [-1/2, 1/2].
+__device__ __forceinline__ void scores(const Args& a, float (&s)[4][4], float (&t)[4][4]) {
+  if (a.cap2 == 0.f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] *= a.scale;
+        t[i][j] = 0.f;
+      }
+    return;
   }
-  return fmaf(-slope2, fabsf((float)dist), s);
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      t[i][j] = s[i][j] * a.scale;
+      big = fmaxf(big, fabsf(t[i][j]));
+    }
+  if (__all_sync(0xffffffffu, big <= 0.5f)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = t[i][j], z = x * x;
+        t[i][j] = x * fmaf(fmaf(fmaf(fmaf(0.017131345346570015f, z, -0.05298423767089844f), z, 0.133247509598732f), z, -0.3333306908607483f), z, 1.0f);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[i][j] = tanhf(t[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = a.cap2 * t[i][j];
 }
+__device__ __forceinline__ float biased(float s, float slope2, int dist) { return fmaf(-slope2, fabsf((float)dist), s); }
 
 // whether the labels of a query tile and a key tile have a common range
 __device__ __forceinline__ bool labels_meet(const Args& a, int b, int q0, int k0) {
@@ -176,6 +207,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
     cp_async_commit();
     float s[4][4];
     dots<DM>(s, Q, K + buf * kRows, ty, tx);
+    float t[4][4];
+    scores(a, s, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int pos = lim.start + q0 + 4 * ty + i;
@@ -183,19 +216,18 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = k0 + tx + 16 * j;
-        float t;
-        const float v = score(a, s[i][j], slope2, pos - col, t);
+        const float v = biased(s[i][j], slope2, pos - col);
         s[i][j] = col < end[i] && (kd == nullptr || kd[col] == id[i]) ? v : -INFINITY;
         top = fmaxf(top, s[i][j]);
       }
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float mn = fmaxf(m[i], top), base = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2f(m[i] - base);
+      const float f = ex2_approx(m[i] - base);
       m[i] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = exp2f(s[i][j] - base);
+        s[i][j] = ex2_approx(s[i][j] - base);
         sum += s[i][j];
       }
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -284,16 +316,17 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
     float s[4][4], dp[4][4];  // rows: keys, columns: queries
     dots<DM>(s, K, Q + buf * kRows, ty, tx);
     dots<DM>(dp, V, G + buf * kRows, ty, tx);
+    float t[4][4];
+    scores(a, s, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = k0 + 4 * ty + i, r = q0 + tx + 16 * j;
-        float t;
-        const float v = score(a, s[i][j], slope2, lim.start + r - key, t);
+        const float v = biased(s[i][j], slope2, lim.start + r - key);
         const bool see = r < a.nq && key < lim.row_end(r, a.causal) && (kd == nullptr || qd[r] == id[i]);
-        s[i][j] = see ? exp2f(v - lse2[j]) : 0.f;
-        dp[i][j] = see ? s[i][j] * (dp[i][j] - dl[j]) * (1.f - t * t) : 0.f;
+        s[i][j] = see ? ex2_approx(v - lse2[j]) : 0.f;
+        dp[i][j] = see ? s[i][j] * (dp[i][j] - dl[j]) * (1.f - t[i][j] * t[i][j]) : 0.f;
       }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -368,15 +401,16 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
     float s[4][4], dp[4][4];
     dots<DM>(s, Q, K + buf * kRows, ty, tx);
     dots<DM>(dp, G, V + buf * kRows, ty, tx);
+    float t[4][4];
+    scores(a, s, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = k0 + tx + 16 * j;
-        float t;
-        const float v = score(a, s[i][j], slope2, lim.start + q0 + 4 * ty + i - col, t);
+        const float v = biased(s[i][j], slope2, lim.start + q0 + 4 * ty + i - col);
         const bool see = col < end[i] && (kd == nullptr || kd[col] == id[i]);
-        s[i][j] = see ? exp2f(v - lse2[i]) * (dp[i][j] - delta[i]) * (1.f - t * t) : 0.f;
+        s[i][j] = see ? ex2_approx(v - lse2[i]) * (dp[i][j] - delta[i]) * (1.f - t[i][j] * t[i][j]) : 0.f;
       }
 #pragma unroll
     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(W + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
