@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       lr = side == 0 ? lr + y : y + lr;
     }
     tc_fence_after();
-    const bool none = m == -INFINITY;
+    // nothing seen: all weights were zero (a score that is not a number makes the sums, and so the row, NaN)
+    const bool none = l == 0.f;
     const float inv = none ? 0.f : 1.0f / lr, lse2 = none ? -INFINITY : m + log2f(l);
     if (live && ok) {
       // read again instead of held in registers through the loop above
@@ -497,17 +498,17 @@ __global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
   float top = -INFINITY;
   for (int p = lane; p < parts; p += 32) top = fmaxf(top, t.part_lse[p * n + row]);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f;
-  if (top != -INFINITY)
-    for (int p = lane; p < parts; p += 32) sum += exp2f(t.part_lse[p * n + row] - top);
+  if (top == -INFINITY) top = 0.f;
+  float sum = 0.f;  // 0 where no part saw a key, NaN where a part's is
+  for (int p = lane; p < parts; p += 32) sum += exp2f(t.part_lse[p * n + row] - top);
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = top == -INFINITY ? 0.f : 1.0f / sum;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   if (lane == 0 && a.lse != nullptr)
-    a.lse[((int64_t)b * a.hq + h) * a.nq + i] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+    a.lse[((int64_t)b * a.hq + h) * a.nq + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
   const int c = lane * 4;
   if (c >= a.d) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (top != -INFINITY) {
+  if (sum != 0.f) {
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) {
       const float e = t.part_lse[p * n + row];

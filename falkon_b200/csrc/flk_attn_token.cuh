@@ -249,13 +249,14 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
 #pragma unroll
     for (int x = 0; x < kWarps; ++x) top = fmaxf(top, shared_m[x][r]);
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x) sum += top == -INFINITY ? 0.f : shared_l[x][r] * ex2_approx(shared_m[x][r] - top);
-    const float f = m[e] == -INFINITY ? 0.f : ex2_approx(m[e] - top) / sum;
+    // a warp whose maximum is -inf has a sum of zero, or NaN where a score is
+    for (int x = 0; x < kWarps; ++x) sum += shared_l[x][r] * (shared_m[x][r] == -INFINITY ? 1.f : ex2_approx(shared_m[x][r] - top));
+    const float f = sum == 0.f ? 0.f : (m[e] == -INFINITY ? 1.f : ex2_approx(m[e] - top)) / sum;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
       *reinterpret_cast<float2*>(buf + (warp * kRows + r) * kLd + n * 8 + 2 * (lane % 4)) = make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
     if (warp == 0 && lane % 4 == 0 && r < t.rows)
-      t.part_lse[(((int64_t)split * a.b + b) * a.hk + hk) * t.rows + r] = top == -INFINITY ? -INFINITY : top + log2f(sum);
+      t.part_lse[(((int64_t)split * a.b + b) * a.hk + hk) * t.rows + r] = sum == 0.f ? -INFINITY : top + log2f(sum);
   }
   __syncthreads();
   const int64_t row0 = (((int64_t)split * a.b + b) * a.hk + hk) * t.rows;

@@ -124,8 +124,8 @@ __device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float* red, in
 }
 // 1 / sqrt(x): the hardware's approximation and one step of Newton's method
 __device__ __forceinline__ float inverse_root(float x) {
-  const float r = rsqrtf(x);
-  return r * fmaf(-0.5f * x * r, r, 1.5f);
+  const float r = rsqrtf(x), s = r * fmaf(-0.5f * x * r, r, 1.5f);
+  return x > 1e-30f && x < 1e30f ? s : r;  // beyond, the step itself would leave fp32
 }
 
 template <typename T, int VEC, int V>

@@ -11,6 +11,7 @@ import torch
 
 from .. import _lib
 from .fmmv import _require_cuda
+from .utils import differentiable_once
 
 __all__ = ("attention", "AttentionFn")
 
@@ -77,10 +78,6 @@ def _backward(ctx, dout, _):
     return dq, dk if need_k else None, dv if need_v else None, None
 
 
-# what backward returns under create_graph=True cannot be differentiated again; the wrapper says so where that is tried
-_backward_once = torch.autograd.function.once_differentiable(_backward)
-
-
 class AttentionFn(torch.autograd.Function):
     """``attention`` with a backward pass for q, k and v (the log-sum-exp that it also returns passes no gradient).  With
     16-bit data it also keeps what rounding took from ``out``, as large as ``out``: the backward pass subtracts
@@ -98,7 +95,11 @@ class AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        return _backward_once(ctx, *grads) if torch.is_grad_enabled() else _backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return _backward(ctx, *grads)
+        with torch.no_grad():  # create_graph=True
+            out = _backward(ctx, *grads)
+        return differentiable_once("attention", out, [*ctx.saved_tensors[:3], *(g for g in grads if g is not None)])
 
 
 def _table(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[torch.Tensor]:
@@ -148,7 +149,7 @@ def attention(
     slopes : (Hq,) float32, the distance bias of each query head (a constant: it gets no gradient)
     prefix_lens : (B,) integers; with ``causal``, the first keys of a sequence that every query may see
     documents : (B, Nk) integers; a query sees the keys of its own document only.  A negative label marks padding, which
-        sees and shows nothing
+        sees and shows nothing; labels lie below 2^31
     q_documents : (B, Nq) integers, the queries' documents; default ``documents`` where Nq == Nk
     kv_lens : (B,) integers; keys at or behind this length do not exist (a cache's length), default Nk
     q_starts : (B,) integers, position of the first query of a sequence; by default the last query stands at the last
@@ -157,7 +158,7 @@ def attention(
 
     A query that sees no key gets zeros, and -inf in the log-sum-exp.  What padding rows and rows behind ``kv_lens``
     hold does not matter, NaN included.  Integer tables are read on the device: lengths beyond [0, Nk] count as the nearer
-    end.  Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates
+    end.  At most 65535 sequences, 65535 heads, 2^29 rows.  Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates
     its output and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has
     it for every operator, only while no graph of the same leaves that was built outside of the capture is alive).
     """

@@ -10,6 +10,7 @@ import torch
 
 from .. import _lib
 from .fmmv import _require_cuda
+from .utils import differentiable_once
 
 __all__ = ("layer_norm", "LayerNormFn")
 
@@ -78,10 +79,6 @@ def _backward(ctx, dy):
     return dx, dw, db, None
 
 
-# what backward returns under create_graph=True cannot be differentiated again; the wrapper says so where that is tried
-_backward_once = torch.autograd.function.once_differentiable(_backward)
-
-
 class LayerNormFn(torch.autograd.Function):
     """``layer_norm`` with a backward pass for x, weight and bias."""
 
@@ -95,7 +92,11 @@ class LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+        if not torch.is_grad_enabled():
+            return _backward(ctx, dy)
+        with torch.no_grad():  # create_graph=True
+            out = _backward(ctx, dy)
+        return differentiable_once("layer_norm", out, [t for t in (*ctx.saved_tensors[:2], dy) if t is not None])
 
 
 def layer_norm(

@@ -9,7 +9,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-__all__ = ("is_contig", "is_f_contig", "check_contiguity", "create_output_mat", "create_same_stride")
+__all__ = ("differentiable_once", "is_contig", "is_f_contig", "check_contiguity", "create_output_mat", "create_same_stride")
 
 
 def is_contig(tensor: torch.Tensor) -> bool:
@@ -69,3 +69,23 @@ def create_output_mat(
     return create_same_stride(
         shape, other_mat, dtype, device=out_dev, pin_memory=out_dev.type != "cuda" and comp_dev_type == "cuda"
     )
+
+
+class _OnceFn(torch.autograd.Function):
+    """Gradients that depend on ``anchors`` in a way that has no derivative here: differentiating them again raises."""
+
+    @staticmethod
+    def forward(ctx, what, n, *tensors):
+        ctx.what = what
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError(f"{ctx.what} is differentiable once: its gradients cannot be differentiated again.")
+
+
+def differentiable_once(what: str, grads, anchors):
+    """``grads`` (None among them) as they are to leave a backward pass that runs under ``create_graph=True``."""
+    there = [g for g in grads if g is not None]
+    out = iter(_OnceFn.apply(what, len(there), *there, *anchors))
+    return tuple(None if g is None else next(out) for g in grads)

@@ -307,6 +307,87 @@ def test_normalised_heads_through_attention():
         assert float((a.double() - r).abs().max()) <= 1e-4 * float(r.abs().max())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,nq,nk,hq,hk,d", [(1, 150, 3001, 2, 1, 128), (1, 40, 5000, 2, 2, 64), (1, 2000, 2000, 2, 1, 64), (2, 1500, 1500, 6, 2, 96)])
+def test_long_axes_in_parts(b, nq, nk, hq, hk, d, dtype):
+    """Few rows over many keys, few keys under many rows: parts that are worked on apart and joined."""
+    q, k, v, do = make(b, nq, nk, hq, hk, d, dtype, seed=18)
+    run_and_check(q, k, v, do, causal=True, softcap=20.0)
+    if nq == nk:
+        lens = [n * nq // 15 for n in (1, 2, 3, 4)]
+        docs = docs_of(b, nq, lens + [nq - sum(lens) - 37], 37)
+        run_and_check(q, k, v, do, causal=True, documents=docs, slopes=slopes_of(hq))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq", [1, 20, 300])
+def test_not_a_number_is_passed_on(nq, dtype):
+    """A query that is not a number makes its own row so, and no other; a key that some see, the rows of those that see it."""
+    q, k, v, _ = make(1, nq, 300, 2, 1, 64, dtype, seed=19)
+    want = attention(q, k, v)
+    bad = q.clone()
+    bad[0, nq // 2, 1] = float("nan")
+    out, lse = attention(bad, k, v, return_lse=True)
+    assert bool(out[0, nq // 2, 1].isnan().all()) and bool(lse[0, 1, nq // 2].isnan())
+    out[0, nq // 2, 1] = want[0, nq // 2, 1]
+    assert torch.equal(out, want)
+    worse = k.clone()
+    worse[0, 77] = float("nan")
+    assert bool(attention(q, worse, v).isnan().all())
+
+
+def test_offsets_beyond_32_bits():
+    """The second sequence lies more than 2^31 elements behind the first."""
+    n, hk, d, far = 257, 2, 64, 2**31 + 4096
+    room = torch.empty(far + 2 * n * hk * d, device=DEV, dtype=torch.bfloat16)
+    k = room.as_strided((2, n, hk, d), (far, hk * d, d, 1))
+    v = room.as_strided((2, n, hk, d), (far, hk * d, d, 1), n * hk * d)
+    q, k0, v0, do = make(2, n, n, 4, hk, d, torch.bfloat16, seed=20)
+    k.copy_(k0)
+    v.copy_(v0)
+    run_and_check(q, k, v, do, causal=True)
+    run_and_check(q[:, :1], k, v, kv_lens=torch.tensor([n, 100], device=DEV))
+
+
+def test_differentiable_once():
+    q, k, v, do = (t.float() for t in make(1, 20, 20, 1, 1, 64, torch.bfloat16, seed=21))
+    q.requires_grad_()
+    g, = torch.autograd.grad(attention(q, k, v), q, do, create_graph=True)
+    with pytest.raises(NotImplementedError, match="once"):
+        g.square().sum().backward()
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(NotImplementedError, match="once"):
+        g.square().sum().backward()
+
+
+def test_calls_side_by_side():
+    """Two streams at once, many times: calls share nothing but the GPU."""
+    a = make(2, 300, 300, 4, 2, 64, torch.bfloat16, seed=22)
+    b = make(1, 700, 700, 2, 1, 128, torch.bfloat16, seed=23)
+
+    def work(x):
+        q, k, v, do = (t.detach().requires_grad_() for t in x)
+        out = attention(q, k, v, causal=True)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), do.detach()))
+
+    want = [work(a), work(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        got = []
+        for s, x in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(work(x))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+def test_no_wait_gave_up():
+    assert _lib.attention_status(torch.device("cuda", torch.cuda.current_device())) == 0
+
+
 def test_launches_are_counted():
     q, k, v, _ = make(1, 64, 64, 1, 1, 64, torch.bfloat16)
     before = _lib.launch_count()

@@ -120,7 +120,7 @@ def attention_args(**change):
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=_lib.FLK_F64), _lib.FLK_ERR_BAD_ARG), (dict(dtype=9), _lib.FLK_ERR_BAD_ARG), (dict(nq=-1), _lib.FLK_ERR_BAD_ARG),
-    (dict(hk=0), _lib.FLK_ERR_BAD_ARG), (dict(hq=3, hk=2), _lib.FLK_ERR_BAD_ARG), (dict(d=0), _lib.FLK_ERR_BAD_ARG),
+    (dict(flags=1), _lib.FLK_ERR_BAD_ARG), (dict(nq=2**28, hq=8, hk=8), _lib.FLK_ERR_UNSUPPORTED), (dict(hk=0), _lib.FLK_ERR_BAD_ARG), (dict(hq=3, hk=2), _lib.FLK_ERR_BAD_ARG), (dict(d=0), _lib.FLK_ERR_BAD_ARG),
     (dict(d=136), _lib.FLK_ERR_UNSUPPORTED), (dict(d=12), _lib.FLK_ERR_UNSUPPORTED), (dict(nk=2**30), _lib.FLK_ERR_UNSUPPORTED),
     (dict(batch=70000), _lib.FLK_ERR_UNSUPPORTED), (dict(scale=float("nan")), _lib.FLK_ERR_BAD_ARG), (dict(softcap=-1.0), _lib.FLK_ERR_BAD_ARG),
     (dict(q_documents=4096), _lib.FLK_ERR_BAD_ARG), (dict(prefix_lens=4096), _lib.FLK_ERR_BAD_ARG),
