@@ -715,11 +715,13 @@ def row_dtype_code(dtype: torch.dtype) -> int:
 
 # The structs of the row operators as bytes: every field has 8 bytes, and packing them costs a third of filling a
 # ctypes.Structure.  The workspace's two fields come last.
-_ATTENTION_HEAD = struct.Struct("@9q2d16q6q4q16q")
+_ATTENTION_FORWARD = struct.Struct("@9q2d16q6q4q")  # what forward reads
+_ATTENTION_GRADS = struct.Struct("@16q")            # dout, dq, dk, dv, which follow
+_ATTENTION_NO_GRADS = bytes(128)
 _LAYER_NORM_HEAD = struct.Struct("@4qdq3q6q3q3q")
 _WORKSPACE = struct.Struct("@2q")
 _NO_WORKSPACE = _WORKSPACE.pack(0, 0)
-assert _ATTENTION_HEAD.size + 16 == ctypes.sizeof(AttentionArgs) and _LAYER_NORM_HEAD.size + 16 == ctypes.sizeof(LayerNormArgs)
+assert _ATTENTION_FORWARD.size + 128 + 16 == ctypes.sizeof(AttentionArgs) and _LAYER_NORM_HEAD.size + 16 == ctypes.sizeof(LayerNormArgs)
 
 
 def call_rows(fn, head: bytes, device: torch.device, query=None, *query_args):

@@ -826,7 +826,8 @@ inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
   if (a.dk.p != nullptr) {
     auto* fn = kernel_keys<T, DP, CAP, BIAS>;
     constexpr int kBytes = (int)Layout<DP, true>::kBytes;
-    FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    static std::atomic<uint64_t> done{0};
+    FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
     const int64_t grid = ceil_div(a.nk, kTile) * t.splits * a.b * a.hk;
     if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many key blocks");
     fn<<<(unsigned)grid, kThreads, kBytes, st>>>(m, t);
@@ -839,7 +840,8 @@ inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
   if (a.dq.p != nullptr) {
     auto* fn = kernel_queries<T, DP, CAP, BIAS>;
     constexpr int kBytes = (int)Layout<DP, false>::kBytes;
-    FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    static std::atomic<uint64_t> done{0};
+    FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
     const int64_t grid = (int64_t)t.blocks * a.b * t.hp;
     if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many row blocks");
     fn<<<(unsigned)grid, kThreads, kBytes, st>>>(m, t);

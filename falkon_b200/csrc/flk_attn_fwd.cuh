@@ -584,7 +584,8 @@ template <typename T, int DP, bool CAP, bool BIAS, bool PAIR>
 inline int launch_one(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcArgs& t, cudaStream_t st) {
   auto* fn = kernel<T, DP, CAP, BIAS, PAIR>;
   constexpr int kBytes = (int)Layout<DP, PAIR>::kBytes;
-  FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  static std::atomic<uint64_t> done{0};
+  FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
   const int64_t grid = (int64_t)t.blocks * t.splits * t.a.b * t.hp;
   if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many row blocks");
   fn<<<(unsigned)grid, kThreads, kBytes, st>>>(tq, tk, tv, t);

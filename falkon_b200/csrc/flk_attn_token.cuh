@@ -285,7 +285,8 @@ template <typename T, int DP, bool CAP, bool BIAS>
 inline int launch_one(const TcArgs& t, cudaStream_t st) {
   auto* fn = kernel<T, DP, CAP, BIAS>;
   constexpr int kBytes = Layout<DP>::kBytes;
-  FLK_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  static std::atomic<uint64_t> done{0};
+  FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
   const int64_t grid = (int64_t)t.splits * t.a.b * t.a.hk;
   if (grid > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "too many blocks");
   fn<<<(unsigned)grid, kWarps * 32, kBytes, st>>>(t);

@@ -49,6 +49,18 @@ inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_
 
 constexpr int kNumSMs = 148;  // B200
 
+// Lets a kernel have `bytes` of dynamic shared memory; asked of the driver once per kernel (`done`, a bit per device) and device.
+inline int allow_shared(const void* fn, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && (bit == 0 || (done.load(std::memory_order_relaxed) & bit) == 0)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return e == cudaSuccess ? FLK_OK : fail(FLK_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+}
+
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t ceil_div(int64_t x, int64_t m) { return (x + m - 1) / m; }
 

@@ -15,9 +15,6 @@ from .utils import differentiable_once
 
 __all__ = ("attention", "AttentionFn")
 
-_NO_TENSOR = (0, 0, 0, 0)
-
-
 def _strided(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a dense copy of it where its layout is none that the kernels read (unit stride over the head dimension,
     16-byte aligned address and strides, no dimension that is broadcast)."""
@@ -30,22 +27,27 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _t4(t: Optional[torch.Tensor]):
-    return _NO_TENSOR if t is None else (t.data_ptr(), *t.stride()[:3])
+def _t4(t: torch.Tensor):
+    b, n, h, _ = t.stride()
+    return t.data_ptr(), b, n, h
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return 0 if t is None else t.data_ptr()
 
 
-def _pack(q, k, v, out, out_lo, lse, opts, dout=None, dq=None, dk=None, dv=None) -> bytes:
+def _pack(q, k, v, out, out_lo, lse, opts) -> bytes:
+    """flk_attention_args up to the gradients' tensors."""
     scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs = opts
     b, nq, hq, d = q.shape
-    return _lib._ATTENTION_HEAD.pack(
-        _lib.row_dtype_code(q.dtype), b, nq, k.shape[1], hq, k.shape[2], d, causal, 0, scale, softcap,
-        *_t4(q), *_t4(k), *_t4(v), *_t4(out), _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens),
-        _ptr(q_starts), _ptr(q_docs), 0 if q_docs is None else q_docs.stride(0), _ptr(k_docs),
-        0 if k_docs is None else k_docs.stride(0), *_t4(dout), *_t4(dq), *_t4(dk), *_t4(dv))
+    _, nk, hk, _ = k.shape
+    qd, qs, kd, ks = (0, 0, 0, 0) if k_docs is None else (q_docs.data_ptr(), q_docs.stride(0), k_docs.data_ptr(), k_docs.stride(0))
+    return _lib._ATTENTION_FORWARD.pack(
+        _lib._ROW_TYPES[q.dtype], b, nq, nk, hq, hk, d, causal, 0, scale, softcap, *_t4(q), *_t4(k), *_t4(v), *_t4(out),
+        _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens), _ptr(q_starts), qd, qs, kd, ks)
+
+
+_NO_TENSOR = (0, 0, 0, 0)
 
 
 def _dense_like(t: torch.Tensor) -> torch.Tensor:
@@ -57,7 +59,8 @@ def _forward(q, k, v, opts, with_lse, with_lo=False):
     out = _dense_like(q)
     out_lo = _dense_like(q) if with_lo and q.dtype != torch.float32 else None
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if with_lse else None
-    _lib.call_rows(lib.flk_attention_forward, _pack(q, k, v, out, out_lo, lse, opts), q.device, lib.flk_attention_workspace_bytes, 0)
+    _lib.call_rows(lib.flk_attention_forward, _pack(q, k, v, out, out_lo, lse, opts) + _lib._ATTENTION_NO_GRADS, q.device,
+                   lib.flk_attention_workspace_bytes, 0)
     return out, out_lo, lse
 
 
@@ -73,7 +76,10 @@ def _backward(ctx, dout, _):
     if need_k or need_v:
         dk, dv = _dense_like(k), _dense_like(v)
     lib = _lib.load()
-    head = _pack(q, k, v, out, out_lo, lse, opts, _strided(dout), dq, dk, dv)
+    dout = _strided(dout)
+    grads = _lib._ATTENTION_GRADS.pack(*_t4(dout), *(_NO_TENSOR if dq is None else _t4(dq)), *(_NO_TENSOR if dk is None else _t4(dk)),
+                        *(_NO_TENSOR if dv is None else _t4(dv)))
+    head = _pack(q, k, v, out, out_lo, lse, opts) + grads
     _lib.call_rows(lib.flk_attention_backward, head, q.device, lib.flk_attention_workspace_bytes, 1)
     return dq, dk if need_k else None, dv if need_v else None, None
 
@@ -119,6 +125,28 @@ def _table(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[torc
     return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _refuse(q, k, v):
+    """Says what is wrong with operands that do not fit."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, not {type(t).__name__}")
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be 4-D (batch, rows, heads, head dimension), found {t.dim()}-D")
+    _lib.row_dtype_code(q.dtype)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"Data types of q, k and v must be equal (found {q.dtype}, {k.dtype}, {v.dtype})")
+    b, _, hq, d = q.shape
+    hk = k.shape[2]
+    if k.shape[0] != b or k.shape[3] != d or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if d < 1 or d > 128:
+        raise NotImplementedError(f"head dimension {d}: 1 to 128 are implemented")
+    if hk < 1 or hq < 1 or hq % hk != 0:
+        raise ValueError(f"{hq} query heads cannot share {hk} key heads")
+    _require_cuda(None)
+    raise ValueError(f"q, k and v must be on one CUDA device (found {q.device}, {k.device}, {v.device})")
+
+
 def attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -162,26 +190,17 @@ def attention(
     its output and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has
     it for every operator, only while no graph of the same leaves that was built outside of the capture is alive).
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor, not {type(t).__name__}")
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be 4-D (batch, rows, heads, head dimension), found {t.dim()}-D")
-    _lib.row_dtype_code(q.dtype)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"Data types of q, k and v must be equal (found {q.dtype}, {k.dtype}, {v.dtype})")
-    b, nq, hq, d = q.shape
-    _, nk, hk, _ = k.shape
-    if k.shape[0] != b or k.shape[3] != d or v.shape != k.shape:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    if d < 1 or d > 128:
-        raise NotImplementedError(f"head dimension {d}: 1 to 128 are implemented")
-    if hk < 1 or hq < 1 or hq % hk != 0:
-        raise ValueError(f"{hq} query heads cannot share {hk} key heads")
+    try:
+        fits = q.dtype is k.dtype is v.dtype and q.dtype in _lib._ROW_TYPES and k.shape == v.shape and q.device == k.device == v.device
+        b, nq, hq, d = q.shape
+        kb, nk, hk, kd = k.shape
+        fits = fits and kb == b and kd == d and 1 <= d <= 128 and hk >= 1 and hq >= 1 and hq % hk == 0 and q.device.type == "cuda"
+    except (AttributeError, ValueError, TypeError):
+        fits = False
+    if not fits:
+        _refuse(q, k, v)
     _require_cuda(None)
     dev = q.device
-    if dev.type != "cuda" or k.device != dev or v.device != dev:
-        raise ValueError(f"q, k and v must be on one CUDA device (found {q.device}, {k.device}, {v.device})")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
     if not math.isfinite(scale) or not (0.0 <= softcap < math.inf):
