@@ -1,11 +1,15 @@
 // Attention of fp32 data on the FP32 pipe, forward and backward.
 //
-// Tiles of 64 queries x 64 keys, 256 threads; a thread owns a 4 x 4 patch of the scores (rows 4 ty .. 4 ty + 3, columns
-// tx + 16 c) and 4 rows x DM / 16 columns of the accumulators.  Operands come by cp.async, one tile ahead of the one that is worked
-// on; rows that no query may see arrive as zeros, so what such rows hold (NaN, infinities) reaches nothing.  All sums run in
+// Tiles of 64 queries x 64 keys, worked on by groups of 256 threads; a thread owns a 4 x 4 patch of the scores (rows 4 ty ..
+// 4 ty + 3, columns tx + 16 c) and 4 rows x DM / 16 columns of the accumulators.  Operands come by cp.async: in the forward pass one tile
+// ahead of the one that is worked on, in the backward pass while the other group works; rows that no query may see arrive as zeros, so what such rows hold (NaN, infinities) reaches nothing.  All sums run in
 // fp32, in pairs (packed multiply-adds), in a fixed order.  Bound by the FP32 pipe and by the shared-memory reads that feed it:
-// per 4 values of d a thread reads 8 vectors for 64 multiply-adds.  (2 x 1000 rows, 4 heads of 64, not causal, capped scores:
-// forward 127 us, dK and dV 212 us, dQ 160 us while every tile was fetched between two barriers.)
+// per 4 values of d a thread reads 8 vectors for 64 multiply-adds.
+//
+// With heads of up to 64 a block has two groups: one takes the even tiles, one the odd, with accumulators of their own that are
+// joined at the end.  Eight warps on an SM would leave its pipes idle for most of the dependent steps (2 x 1000 rows, 4 heads of
+// 64, not causal, capped scores, 128 blocks: forward 93 -> 77 us, dK and dV 170 -> 147 us, dQ 133 -> 108 us).  Larger heads leave no
+// room for a second set of tiles.
 #pragma once
 
 #include "flk_attn.cuh"
@@ -16,25 +20,33 @@ namespace attn {
 namespace simt {
 
 constexpr int kT = 64;
-constexpr int kThreads = 256;
-constexpr int kPs = kT + 4;  // row length of the score tiles in shared memory
+constexpr int kThreads = 256;  // of a group
+constexpr int kPs = kT + 4;    // row length of the score tiles in shared memory
 
 template <int DM>
 struct Smem {
   static constexpr int kLd = DM + 4;
   static constexpr int kRows = kT * kLd;  // floats of one operand tile
   static constexpr int kPair = kT * kPs;  // floats of one score tile
-  // buffers of a streamed operand: two where both fit beside the rest
-  static constexpr int kBuf = DM == 64 ? 2 : 1;
+  static constexpr int kGroups = DM == 64 ? 2 : 1;
 };
+
+// A barrier of the threads of one group (number `g`), or of the block where it has one group.
+template <int GROUPS>
+__device__ __forceinline__ void sync_group(int g) {
+  if constexpr (GROUPS == 1)
+    __syncthreads();
+  else
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(g + 1), "n"(kThreads) : "memory");
+}
 
 // rows [r0, r0 + 64) of one head on their way into shared memory; rows at or behind `end`, and rows without a label, as zeros
 template <int DM>
-__device__ __forceinline__ void fetch_tile(float* dst, const Tensor4& t, int b, int h, int r0, int end, int d, const int* docs) {
+__device__ __forceinline__ void fetch_tile(float* dst, const Tensor4& t, int b, int h, int r0, int end, int d, const int* docs, int tid) {
   const float* src = (const float*)t.p + b * t.sb + h * t.sh;
   const uint32_t to = tc::smem_u32(dst);
 #pragma unroll
-  for (int e = threadIdx.x; e < kT * (DM / 4); e += kThreads) {
+  for (int e = tid; e < kT * (DM / 4); e += kThreads) {
     const int r = e / (DM / 4), c = (e - r * (DM / 4)) * 4;
     const bool valid = r0 + r < end && c < d && (docs == nullptr || __ldg(docs + r0 + r) >= 0);
     // an address inside the tensor even where nothing is read
@@ -164,12 +176,34 @@ __device__ __forceinline__ bool labels_meet(const Args& a, int b, int q0, int k0
   return x.y >= y.x && y.y >= x.x;
 }
 
+// Joins the two groups' accumulators: acc = acc * mine + the second group's * theirs, through shared memory (kRows floats).
 template <int DM>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
+__device__ __forceinline__ void put_rows(float* room, const uint64_t (&acc)[4][DM / 32], int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < DM / 64; ++c)
+      *reinterpret_cast<ulonglong2*>(room + (4 * ty + i) * Smem<DM>::kLd + 4 * tx + 64 * c) = make_ulonglong2(acc[i][2 * c], acc[i][2 * c + 1]);
+}
+template <int DM>
+__device__ __forceinline__ void add_rows(const float* room, uint64_t (&acc)[4][DM / 32], const float (&mine)[4], const float (&theirs)[4], int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < DM / 64; ++c) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(room + (4 * ty + i) * Smem<DM>::kLd + 4 * tx + 64 * c);
+      const uint64_t f = tc::pack2(mine[i], mine[i]), g = tc::pack2(theirs[i], theirs[i]);
+      acc[i][2 * c] = tc::fma2(acc[i][2 * c], f, tc::mul2(v.x, g));
+      acc[i][2 * c + 1] = tc::fma2(acc[i][2 * c + 1], f, tc::mul2(v.y, g));
+    }
+}
+
+template <int DM>
+__global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(const Args a) {
   extern __shared__ float sm[];
-  constexpr int kRows = Smem<DM>::kRows;
-  float *Q = sm, *K = Q + kRows, *V = K + 2 * kRows, *P = V + 2 * kRows;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  constexpr int kRows = Smem<DM>::kRows, kGroups = Smem<DM>::kGroups;
+  const int g = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, tx = tid & 15, ty = tid >> 4;
+  float *Q = sm, *K = Q + kRows + g * (4 * kRows + Smem<DM>::kPair), *V = K + 2 * kRows, *P = V + 2 * kRows;
   const int q0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
@@ -188,22 +222,24 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
   }
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   auto next = [&](int k0) {
-    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT;
+    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT * kGroups;
     return k0;
   };
-  int k0 = next(0), buf = 0;
-  fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd);
-  if (k0 < last) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd);
+  int k0 = next(g * kT), buf = 0;
+  if (g == 0) fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd, tid);
+  if (k0 < last) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd, tid);
   cp_async_commit();
-  if (k0 < last) fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd);
+  if (k0 < last) fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd, tid);
   cp_async_commit();
+  cp_async_wait<1>();
+  __syncthreads();  // both groups read Q
   while (k0 < last) {
-    const int k1 = next(k0 + kT);
-    if (k1 < last) fetch_tile<DM>(K + (buf ^ 1) * kRows, a.k, b, hk, k1, lim.len, a.d, kd);
+    const int k1 = next(k0 + kT * kGroups);
+    if (k1 < last) fetch_tile<DM>(K + (buf ^ 1) * kRows, a.k, b, hk, k1, lim.len, a.d, kd, tid);
     cp_async_commit();
     cp_async_wait<2>();
-    __syncthreads();  // K is here; all have done with the weights and values of the tile before
-    if (k1 < last) fetch_tile<DM>(V + (buf ^ 1) * kRows, a.v, b, hk, k1, lim.len, a.d, kd);
+    sync_group<kGroups>(g);  // K is here; all have done with the weights and values of the tile before
+    if (k1 < last) fetch_tile<DM>(V + (buf ^ 1) * kRows, a.v, b, hk, k1, lim.len, a.d, kd, tid);
     cp_async_commit();
     float s[4][4];
     dots<DM>(s, Q, K + buf * kRows, ty, tx);
@@ -239,12 +275,36 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(P + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
     cp_async_wait<2>();
-    __syncthreads();  // V is here, and the weights
+    sync_group<kGroups>(g);  // V is here, and the weights
     outer<DM>(acc, P, V + buf * kRows, ty, tx);
     k0 = k1;
     buf ^= 1;
   }
   cp_async_wait<0>();
+  if constexpr (kGroups == 2) {
+    __syncthreads();
+    float *room = sm + kRows, *stats = room + kRows;  // [row][2] behind the rows
+    if (g == 1) {
+      put_rows<DM>(room, acc, ty, tx);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tx == 0) stats[2 * (4 * ty + i)] = m[i], stats[2 * (4 * ty + i) + 1] = l[i];
+    }
+    __syncthreads();
+    if (g == 1) return;
+    float fm[4], ft[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float mt = stats[2 * (4 * ty + i)], lt = stats[2 * (4 * ty + i) + 1];
+      const float mn = fmaxf(m[i], mt), base = mn == -INFINITY ? 0.f : mn;
+      fm[i] = ex2_approx(m[i] - base);
+      ft[i] = ex2_approx(mt - base);
+      // scores that are not numbers leave the maximum at -inf and the sum NaN
+      l[i] = (m[i] == -INFINITY ? l[i] : l[i] * fm[i]) + (mt == -INFINITY ? lt : lt * ft[i]);
+      m[i] = mn;
+    }
+    add_rows<DM>(room, acc, fm, ft, ty, tx);
+  }
   float f[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -258,11 +318,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args a) {
 
 // Gradients of 64 keys and values: loops over the query heads that share them and over their query tiles.
 template <int DM>
-__global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) backward_kv_kernel(const Args a) {
   extern __shared__ float sm[];
-  constexpr int kRows = Smem<DM>::kRows, kBuf = Smem<DM>::kBuf;
-  float *K = sm, *V = K + kRows, *Q = V + kRows, *G = Q + kBuf * kRows, *P = G + kBuf * kRows, *W = P + Smem<DM>::kPair;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  constexpr int kRows = Smem<DM>::kRows, kGroups = Smem<DM>::kGroups;
+  const int g = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, tx = tid & 15, ty = tid >> 4;
+  float *K = sm, *V = K + kRows, *Q = V + kRows + g * (2 * kRows + 2 * Smem<DM>::kPair), *G = Q + kRows, *P = G + kRows, *W = P + Smem<DM>::kPair;
   const int k0 = blockIdx.x * kT, hk = blockIdx.y, b = blockIdx.z;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
@@ -275,25 +335,27 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
   const int tiles = (a.nq + kT - 1) / kT;
   const int64_t steps = k0 < lim.len ? (int64_t)a.grp * tiles : 0;
   auto next = [&](int64_t s) {
-    for (; s < steps; ++s) {
+    for (; s < steps; s += kGroups) {
       const int q0 = (int)(s % tiles) * kT;
       if (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) > k0 && labels_meet(a, b, q0, k0)) break;
     }
     return s;
   };
-  auto fetch = [&](int64_t s, int buf) {
+  auto fetch = [&](int64_t s) {
     const int h = hk * a.grp + (int)(s / tiles), q0 = (int)(s % tiles) * kT;
-    fetch_tile<DM>(Q + buf * kRows, a.q, b, h, q0, a.nq, a.d, qd);
-    fetch_tile<DM>(G + buf * kRows, a.dout, b, h, q0, a.nq, a.d, qd);
+    fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd, tid);
+    fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, qd, tid);
   };
-  int64_t step = next(0);
-  int buf = 0;
-  fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd);
-  fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd);
-  if (step < steps) fetch(step, 0);
+  int64_t step = next(g);
+  if (g == 0) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd, tid);
+  if (g == kGroups - 1) fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd, tid);
   cp_async_commit();
+  if (step < steps) fetch(step);
+  cp_async_commit();
+  cp_async_wait<1>();
+  __syncthreads();  // K and V are here
   while (step < steps) {
-    const int64_t after = next(step + 1);
+    const int64_t after = next(step + kGroups);
     const int h = hk * a.grp + (int)(step / tiles), q0 = (int)(step % tiles) * kT;
     const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     const float *lse = a.lse + ((int64_t)b * a.hq + h) * a.nq, *delta = a.delta + ((int64_t)b * a.hq + h) * a.nq;
@@ -304,18 +366,11 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
       lse2[j] = r < a.nq ? __ldg(lse + r) * kLog2e : 0.f;
       dl[j] = r < a.nq ? __ldg(delta + r) : 0.f;
     }
-    if constexpr (kBuf == 2) {
-      __syncthreads();  // all have done with the other buffer
-      if (after < steps) fetch(after, buf ^ 1);
-      cp_async_commit();
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();
+    cp_async_wait<0>();
+    sync_group<kGroups>(g);
     float s[4][4], dp[4][4];  // rows: keys, columns: queries
-    dots<DM>(s, K, Q + buf * kRows, ty, tx);
-    dots<DM>(dp, V, G + buf * kRows, ty, tx);
+    dots<DM>(s, K, Q, ty, tx);
+    dots<DM>(dp, V, G, ty, tx);
     float t[4][4];
     scores(a, s, t);
 #pragma unroll
@@ -333,18 +388,27 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
       *reinterpret_cast<float4*>(P + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
       *reinterpret_cast<float4*>(W + (tx + 16 * j) * kPs + 4 * ty) = make_float4(dp[0][j], dp[1][j], dp[2][j], dp[3][j]);
     }
-    __syncthreads();
-    outer<DM>(dv, P, G + buf * kRows, ty, tx);
-    outer<DM>(dk, W, Q + buf * kRows, ty, tx);
-    if constexpr (kBuf == 1) {
-      __syncthreads();
-      if (after < steps) fetch(after, 0);
-      cp_async_commit();
-    }
+    sync_group<kGroups>(g);
+    outer<DM>(dv, P, G, ty, tx);
+    outer<DM>(dk, W, Q, ty, tx);
+    sync_group<kGroups>(g);
+    if (after < steps) fetch(after);
+    cp_async_commit();
     step = after;
-    if (kBuf == 2) buf ^= 1;
   }
   cp_async_wait<0>();
+  if constexpr (kGroups == 2) {
+    __syncthreads();
+    if (g == 1) {
+      put_rows<DM>(sm, dk, ty, tx);
+      put_rows<DM>(sm + kRows, dv, ty, tx);
+    }
+    __syncthreads();
+    if (g == 1) return;
+    const float both[4] = {1.f, 1.f, 1.f, 1.f};
+    add_rows<DM>(sm, dk, both, both, ty, tx);
+    add_rows<DM>(sm + kRows, dv, both, both, ty, tx);
+  }
   const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {a.scale_raw, a.scale_raw, a.scale_raw, a.scale_raw};
   store_rows<DM>(a.dk, b, hk, k0, a.nk, a.d, dk, sc, ty, tx);
   store_rows<DM>(a.dv, b, hk, k0, a.nk, a.d, dv, one, ty, tx);
@@ -352,11 +416,11 @@ __global__ void __launch_bounds__(kThreads) backward_kv_kernel(const Args a) {
 
 // Gradient of 64 queries.
 template <int DM>
-__global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) backward_q_kernel(const Args a) {
   extern __shared__ float sm[];
-  constexpr int kRows = Smem<DM>::kRows, kBuf = Smem<DM>::kBuf;
-  float *Q = sm, *G = Q + kRows, *K = G + kRows, *V = K + kBuf * kRows, *W = V + kBuf * kRows;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  constexpr int kRows = Smem<DM>::kRows, kGroups = Smem<DM>::kGroups;
+  const int g = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, tx = tid & 15, ty = tid >> 4;
+  float *Q = sm, *G = Q + kRows, *K = G + kRows + g * (2 * kRows + Smem<DM>::kPair), *V = K + kRows, *W = V + kRows;
   const int q0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
@@ -375,32 +439,28 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
   }
   const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
   auto next = [&](int k0) {
-    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT;
+    while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT * kGroups;
     return k0;
   };
-  auto fetch = [&](int k0, int buf) {
-    fetch_tile<DM>(K + buf * kRows, a.k, b, hk, k0, lim.len, a.d, kd);
-    fetch_tile<DM>(V + buf * kRows, a.v, b, hk, k0, lim.len, a.d, kd);
+  auto fetch = [&](int k0) {
+    fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd, tid);
+    fetch_tile<DM>(V, a.v, b, hk, k0, lim.len, a.d, kd, tid);
   };
-  int k0 = next(0), buf = 0;
-  fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd);
-  fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, qd);
-  if (k0 < last) fetch(k0, 0);
+  int k0 = next(g * kT);
+  if (g == 0) fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd, tid);
+  if (g == kGroups - 1) fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, qd, tid);
   cp_async_commit();
+  if (k0 < last) fetch(k0);
+  cp_async_commit();
+  cp_async_wait<1>();
+  __syncthreads();  // Q and dO are here
   while (k0 < last) {
-    const int k1 = next(k0 + kT);
-    if constexpr (kBuf == 2) {
-      __syncthreads();  // all have done with the other buffer, and with the weights
-      if (k1 < last) fetch(k1, buf ^ 1);
-      cp_async_commit();
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();
+    const int k1 = next(k0 + kT * kGroups);
+    cp_async_wait<0>();
+    sync_group<kGroups>(g);
     float s[4][4], dp[4][4];
-    dots<DM>(s, Q, K + buf * kRows, ty, tx);
-    dots<DM>(dp, G, V + buf * kRows, ty, tx);
+    dots<DM>(s, Q, K, ty, tx);
+    dots<DM>(dp, G, V, ty, tx);
     float t[4][4];
     scores(a, s, t);
 #pragma unroll
@@ -414,46 +474,52 @@ __global__ void __launch_bounds__(kThreads) backward_q_kernel(const Args a) {
       }
 #pragma unroll
     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(W + (tx + 16 * j) * kPs + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
-    __syncthreads();
-    outer<DM>(dq, W, K + buf * kRows, ty, tx);
-    if constexpr (kBuf == 1) {
-      __syncthreads();
-      if (k1 < last) fetch(k1, 0);
-      cp_async_commit();
-    }
+    sync_group<kGroups>(g);
+    outer<DM>(dq, W, K, ty, tx);
+    sync_group<kGroups>(g);
+    if (k1 < last) fetch(k1);
+    cp_async_commit();
     k0 = k1;
-    if (kBuf == 2) buf ^= 1;
   }
   cp_async_wait<0>();
+  if constexpr (kGroups == 2) {
+    __syncthreads();
+    if (g == 1) put_rows<DM>(sm, dq, ty, tx);
+    __syncthreads();
+    if (g == 1) return;
+    const float both[4] = {1.f, 1.f, 1.f, 1.f};
+    add_rows<DM>(sm, dq, both, both, ty, tx);
+  }
   const float sc[4] = {a.scale_raw, a.scale_raw, a.scale_raw, a.scale_raw};
   store_rows<DM>(a.dq, b, h, q0, a.nq, a.d, dq, sc, ty, tx);
 }
 
 template <int DM>
-constexpr size_t forward_smem() { return (5 * Smem<DM>::kRows + Smem<DM>::kPair) * 4; }
+constexpr size_t forward_smem() { return (Smem<DM>::kRows + Smem<DM>::kGroups * (4 * Smem<DM>::kRows + Smem<DM>::kPair)) * 4; }
 template <int DM>
-constexpr size_t backward_smem() { return ((2 + 2 * Smem<DM>::kBuf) * Smem<DM>::kRows + 2 * Smem<DM>::kPair) * 4; }
-static_assert(forward_smem<128>() <= 227 * 1024 && backward_smem<64>() <= 227 * 1024 && backward_smem<128>() <= 227 * 1024, "shared memory");
+constexpr size_t kv_smem() { return (2 * Smem<DM>::kRows + Smem<DM>::kGroups * (2 * Smem<DM>::kRows + 2 * Smem<DM>::kPair)) * 4; }
+template <int DM>
+constexpr size_t q_smem() { return (2 * Smem<DM>::kRows + Smem<DM>::kGroups * (2 * Smem<DM>::kRows + Smem<DM>::kPair)) * 4; }
+static_assert(forward_smem<64>() <= 227 * 1024 && forward_smem<128>() <= 227 * 1024, "shared memory");
+static_assert(kv_smem<64>() <= 227 * 1024 && kv_smem<128>() <= 227 * 1024, "shared memory");
 
 template <int DM>
-inline int launch_forward(const Args& a, cudaStream_t st) {
-  FLK_CUDA_TRY(cudaFuncSetAttribute(forward_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)forward_smem<DM>()));
-  forward_kernel<DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, forward_smem<DM>(), st>>>(a);
+inline int run(void (*fn)(const Args), std::atomic<uint64_t>& done, const dim3& grid, size_t smem, const Args& a, cudaStream_t st) {
+  FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), (int)smem, done));
+  fn<<<grid, kThreads * Smem<DM>::kGroups, smem, st>>>(a);
   count_launch();
   return FLK_OK;
 }
 template <int DM>
+inline int launch_forward(const Args& a, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  return run<DM>(forward_kernel<DM>, done, dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), forward_smem<DM>(), a, st);
+}
+template <int DM>
 inline int launch_backward(const Args& a, cudaStream_t st) {
-  if (a.dk.p != nullptr) {
-    FLK_CUDA_TRY(cudaFuncSetAttribute(backward_kv_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
-    backward_kv_kernel<DM><<<dim3((unsigned)ceil_div(a.nk, kT), a.hk, a.b), kThreads, backward_smem<DM>(), st>>>(a);
-    count_launch();
-  }
-  if (a.dq.p != nullptr) {
-    FLK_CUDA_TRY(cudaFuncSetAttribute(backward_q_kernel<DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)backward_smem<DM>()));
-    backward_q_kernel<DM><<<dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), kThreads, backward_smem<DM>(), st>>>(a);
-    count_launch();
-  }
+  static std::atomic<uint64_t> done_kv{0}, done_q{0};
+  if (a.dk.p != nullptr) FLK_TRY(run<DM>(backward_kv_kernel<DM>, done_kv, dim3((unsigned)ceil_div(a.nk, kT), a.hk, a.b), kv_smem<DM>(), a, st));
+  if (a.dq.p != nullptr) FLK_TRY(run<DM>(backward_q_kernel<DM>, done_q, dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), q_smem<DM>(), a, st));
   return FLK_OK;
 }
 
