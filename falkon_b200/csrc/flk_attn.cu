@@ -83,7 +83,9 @@ static int check_sizes(const flk_attention_args* p) {
     return fail(FLK_ERR_BAD_ARG, "negative or empty sizes");
   if (p->batch > 65535 || p->hq > 65535 || p->nq > (1 << 29) || p->nk > (1 << 29))
     return fail(FLK_ERR_UNSUPPORTED, "at most 65535 sequences and heads, and 2^29 rows");
-  if (p->nq * p->hq > INT32_MAX || p->nk * p->hk > INT32_MAX) return fail(FLK_ERR_UNSUPPORTED, "at most 2^31 - 1 rows of all heads of a sequence");
+  // (a last tile's rows are counted up to its end)
+  if (p->nq * p->hq > INT32_MAX - 1023 || p->nk * p->hk > INT32_MAX - 1023)
+    return fail(FLK_ERR_UNSUPPORTED, "at most 2^31 - 1024 rows of all heads of a sequence");
   if (p->hq % p->hk != 0)
     return fail(FLK_ERR_BAD_ARG, "%lld query heads cannot share %lld key heads", (long long)p->hq, (long long)p->hk);
   const int unit = p->dtype == FLK_F32 ? 4 : 8;
@@ -91,6 +93,9 @@ static int check_sizes(const flk_attention_args* p) {
     return fail(FLK_ERR_UNSUPPORTED, "head dimension %lld: a multiple of %d up to %d", (long long)p->d, unit, kMaxHeadDim);
   if (!(p->softcap >= 0) || p->softcap > 1e30 || !(p->scale > -1e30 && p->scale < 1e30))
     return fail(FLK_ERR_BAD_ARG, "scale must be finite, softcap finite and not negative");
+  // the tanh's argument, scale / softcap, and the cap itself are held in fp32
+  if (p->softcap > 0 && (p->softcap < 1e-30 || (p->scale < 0 ? -p->scale : p->scale) > p->softcap * 1e30))
+    return fail(FLK_ERR_UNSUPPORTED, "softcap %g is too small for scale %g", p->softcap, p->scale);
   if ((p->q_documents == nullptr) != (p->k_documents == nullptr))
     return fail(FLK_ERR_BAD_ARG, "q_documents and k_documents are given together");
   if (p->prefix_lens != nullptr && p->causal == 0) return fail(FLK_ERR_BAD_ARG, "prefix_lens needs causal");

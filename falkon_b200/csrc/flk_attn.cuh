@@ -42,7 +42,7 @@ struct Args {
   float* delta;  // (b, hq, nq)
 };
 
-struct Limits {  // of one sequence
+struct Limits {  // of one sequence; no query sees keys at or behind `len`
   int len, start, prefix;
   __device__ __forceinline__ int row_end(int i, int causal) const {
     if (!causal) return len;
@@ -56,6 +56,8 @@ __device__ __forceinline__ Limits limits_of(const Args& a, int b) {
   // positions stay far from the ends of int, whatever the caller's table holds
   l.start = a.q_starts != nullptr ? min(max(a.q_starts[b], -(1 << 29)), 1 << 29) : l.len - a.nq;
   l.prefix = a.prefix != nullptr ? a.prefix[b] : 0;
+  // under a causal mask what lies behind the last query (the rest of a cache, say) may hold anything too
+  l.len = l.row_end(a.nq - 1, a.causal);
   return l;
 }
 

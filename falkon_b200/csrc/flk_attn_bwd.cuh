@@ -43,7 +43,7 @@ struct Layout {
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kStatAt = kRing + kStages * kTileBytes;
   static constexpr uint32_t kBars = kStatAt + kStats;
-  static constexpr uint32_t kBytes = kBars + 512;
+  static constexpr uint32_t kBytes = kBars + 512 + (KEYS ? kSlots * 16 : 0);
 };
 static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
 static_assert(Layout<128, true>::kStages >= 4 && Layout<128, false>::kStages >= 5, "stages");
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   const uint32_t own = bars + 128, sfull = bars + 136, pfull = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176;
   auto statfull = [&](int s) { return bars + 192 + s * 8; };
   auto statempty = [&](int s) { return bars + 224 + s * 8; };
-  const uint32_t slots = bars + 256;
+  const uint32_t slots = bars + 256, hollows = bars + 512;  // 128 bits per slot: rows of the tile that see nothing
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
@@ -237,17 +237,33 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       __syncwarp();
       StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
+      // queries that see nothing may hold anything; their weights are zero, and what those meet must be finite
+      const bool hollow = qd != nullptr || lim.row_end(0, a.causal) == 0;
       int n = 0;
       for (int step = 0; step < steps && ok; ++step) {
-        const Tile e = walk.next();
+        Tile e = walk.next();
         const int h = hk * a.grp + walk.head * t.pg;
+        uint32_t none[4] = {0, 0, 0, 0};
+        if (hollow) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = e.at * kTile + (int)(threadIdx.x & 31) + 32 * x;
+            const float lse = r < t.rows ? __ldg(a.lse + ((int64_t)b * a.hq + h + (r & (t.pg - 1))) * a.nq + (r >> t.pg_shift)) : 0.f;
+            none[x] = __ballot_sync(0xffffffffu, lse == -INFINITY);
+          }
+          e.dirty = (none[0] | none[1] | none[2] | none[3]) != 0;
+        }
 #pragma unroll
         for (int qo = 0; qo < 2; ++qo) {
           const int s = n % kStages;
           if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
           if (!ok) break;
           if (elect_one()) {
-            if (qo == 0) put_tile(slots, step, e);
+            if (qo == 0) {
+              put_tile(slots, step, e);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(hollows + (step % kSlots) * 16), "r"(none[0]), "r"(none[1]), "r"(none[2]), "r"(none[3])
+                           : "memory");
+            }
             mbar_expect_tx(full(s), L::kTileBytes);
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c)
@@ -307,27 +323,14 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       bool ok = steps == 0 || wait_bar(own, 0);
       auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
       auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
-      // queries without a label may hold anything; their weights are zero, and they must be
       auto arrived = [&](int n) {
         if (!ready(n)) return false;
-        if (qd != nullptr) {
-          const Tile e = get_tile(slots, n / 2);
-          if (e.dirty) {
-            // packed row r is query r >> pg_shift
-            const int lane = threadIdx.x & 31;
-            for (int r = lane; r < kTile; r += 32) {
-              const int i = (e.at * kTile + r) >> t.pg_shift;
-              if (i < a.nq && __ldg(qd + i) >= 0) continue;
-#pragma unroll
-              for (int blk = 0; blk < DP / 64; ++blk)
-#pragma unroll
-                for (int c = 0; c < 128; c += 16)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage(n) + blk * kBlockBytes + r * 128 + c), "r"(0) : "memory");
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-        }
+        if (get_tile(slots, n / 2).dirty)
+          clean_rows<DP>(stage(n), [&](int r) {
+            uint32_t none;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(none) : "r"(hollows + n / 2 % kSlots * 16 + r / 32 * 4) : "memory");
+            return (none >> (r & 31) & 1) == 0;
+          });
         return true;
       };
       if (steps > 0 && ok) {

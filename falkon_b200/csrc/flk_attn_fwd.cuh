@@ -255,7 +255,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool live = (r & ~31) < t.rows;                                   // some row of this warp exists
     const uint32_t mine = halves + (w * 256 + side * 128 + (threadIdx.x & 127)) * 4, other = side == 0 ? mine + 512 : mine - 512;
     const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
-    const bool exists = r < t.rows;
     const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
     const int pos = lim.start + i;
     // for the tile of this warpgroup: keys before `x` are visible to every row that exists; `y` is the one label of its queries

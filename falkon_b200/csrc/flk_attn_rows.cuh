@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) largest_value_kernel(const Args a, uint32
     const int c = (int)(e % packs) * kVec;
     const int64_t row = e / packs;
     const int h = (int)(row % a.hk), j = (int)(row / a.hk % a.nk), b = (int)(row / a.hk / a.nk);
-    if (j >= (a.kv_lens != nullptr ? a.kv_lens[b] : a.nk) || (a.kdocs != nullptr && a.kdocs[(int64_t)b * a.nk_pad + j] < 0)) continue;
+    if (j >= limits_of(a, b).len || (a.kdocs != nullptr && a.kdocs[(int64_t)b * a.nk_pad + j] < 0)) continue;
     T u[kVec];
     *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>((const T*)a.v.p + b * a.v.sb + j * a.v.sn + h * a.v.sh + c);
 #pragma unroll

@@ -40,15 +40,17 @@ __device__ __forceinline__ void sync_group(int g) {
     asm volatile("barrier.cta.sync %0, %1;" ::"r"(g + 1), "n"(kThreads) : "memory");
 }
 
-// rows [r0, r0 + 64) of one head on their way into shared memory; rows at or behind `end`, and rows without a label, as zeros
+// rows [r0, r0 + 64) of one head on their way into shared memory; rows at or behind `end`, rows without a label, and queries that
+// see nothing (a log-sum-exp of -inf) as zeros
 template <int DM>
-__device__ __forceinline__ void fetch_tile(float* dst, const Tensor4& t, int b, int h, int r0, int end, int d, const int* docs, int tid) {
+__device__ __forceinline__ void fetch_tile(float* dst, const Tensor4& t, int b, int h, int r0, int end, int d, const int* docs, int tid,
+                                           const float* lse = nullptr) {
   const float* src = (const float*)t.p + b * t.sb + h * t.sh;
   const uint32_t to = tc::smem_u32(dst);
 #pragma unroll
   for (int e = tid; e < kT * (DM / 4); e += kThreads) {
     const int r = e / (DM / 4), c = (e - r * (DM / 4)) * 4;
-    const bool valid = r0 + r < end && c < d && (docs == nullptr || __ldg(docs + r0 + r) >= 0);
+    const bool valid = r0 + r < end && c < d && (docs == nullptr || __ldg(docs + r0 + r) >= 0) && (lse == nullptr || __ldg(lse + r0 + r) != -INFINITY);
     // an address inside the tensor even where nothing is read
     const float* s = src + (valid ? (int64_t)(r0 + r) * t.sn + c : 0);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (r * Smem<DM>::kLd + c) * 4), "l"(s), "r"(valid ? 16 : 0) : "memory");
@@ -341,10 +343,12 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) backward_kv_kerne
     }
     return s;
   };
+  const bool hollow = qd != nullptr || lim.row_end(0, a.causal) == 0;  // some query may see nothing
   auto fetch = [&](int64_t s) {
     const int h = hk * a.grp + (int)(s / tiles), q0 = (int)(s % tiles) * kT;
-    fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd, tid);
-    fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, qd, tid);
+    const float* lse = hollow ? a.lse + ((int64_t)b * a.hq + h) * a.nq : nullptr;
+    fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, nullptr, tid, lse);
+    fetch_tile<DM>(G, a.dout, b, h, q0, a.nq, a.d, nullptr, tid, lse);
   };
   int64_t step = next(g);
   if (g == 0) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd, tid);

@@ -127,19 +127,6 @@ __device__ __forceinline__ void issue_weighted(uint32_t d_tmem, uint32_t w_tmem,
     mma_ts(d_tmem, w_tmem + ks / kPer * OWN + ks % kPer * 8, bl + ks * (2048 >> 4), instr_desc<T>(DP, true), accumulate || ks > 0);
 }
 
-#define FLK_R32_IN(r)                                                                                                    \
-  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),          \
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),        \
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),        \
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      FLK_R32_IN(r)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -264,7 +251,6 @@ struct TcArgs {
   int splits;        // parts of the key axis
   float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
   float* part_lse;   // [split][b][hp][rows], base 2
-  void* o_lo;        // what rounding took from `out` (same type, strides of out), or null
   const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
 };
 
@@ -335,12 +321,12 @@ __device__ __forceinline__ Tile get_tile(uint32_t slots, int step) {
   return Tile{x & ~(1 << 30), y, (x >> 30 & 1) != 0};
 }
 
-// Writes zeros over the rows of a 128-row operand tile that nobody may see (row index >= end, or label < 0), so that what
-// they hold meets no product.  One warp.
-template <int DP>
-__device__ __forceinline__ void clean_tile(uint32_t tile, int r0, int end, const int* docs) {
+// Writes zeros over the rows of a 128-row operand tile that are not `kept(row)`, so that what they hold meets no product.
+// One warp.
+template <int DP, typename Kept>
+__device__ __forceinline__ void clean_rows(uint32_t tile, Kept kept) {
   for (int r = threadIdx.x & 31; r < kTile; r += 32) {
-    if (r0 + r < end && (docs == nullptr || __ldg(docs + r0 + r) >= 0)) continue;
+    if (kept(r)) continue;
 #pragma unroll
     for (int b = 0; b < DP / 64; ++b)
 #pragma unroll
@@ -349,6 +335,11 @@ __device__ __forceinline__ void clean_tile(uint32_t tile, int r0, int end, const
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
+}
+// The same for keys that nobody may see: row index >= end, or label < 0.
+template <int DP>
+__device__ __forceinline__ void clean_tile(uint32_t tile, int r0, int end, const int* docs) {
+  clean_rows<DP>(tile, [&](int r) { return r0 + r < end && (docs == nullptr || __ldg(docs + r0 + r) >= 0); });
 }
 
 // Bit c: column c of 32 lies before `stop` and has the label `my` (`labels`: 32 of them, 16-byte aligned, or null)

@@ -15,13 +15,15 @@ from .utils import differentiable_once
 
 __all__ = ("attention", "AttentionFn")
 
+
 def _strided(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a dense copy of it where its layout is none that the kernels read (unit stride over the head dimension,
     16-byte aligned address and strides, no dimension that is broadcast)."""
     sb, sn, sh, sd = t.stride()
     b, n, h, _ = t.shape
     unit = 16 // t.element_size() - 1
-    if sd == 1 and t.data_ptr() & 15 == 0 and not (b > 1 and (sb & unit or sb < 1) or n > 1 and (sn & unit or sn < 1) or h > 1 and (sh & unit or sh < 1)):
+    odd = b > 1 and (sb & unit or sb < 1) or n > 1 and (sn & unit or sn < 1) or h > 1 and (sh & unit or sh < 1)
+    if sd == 1 and t.data_ptr() & 15 == 0 and not odd:
         return t
     # clone and not contiguous(): a dense tensor whose address is not aligned needs a copy too
     return t.clone(memory_format=torch.contiguous_format)
@@ -77,8 +79,8 @@ def _backward(ctx, dout, _):
         dk, dv = _dense_like(k), _dense_like(v)
     lib = _lib.load()
     dout = _strided(dout)
-    grads = _lib._ATTENTION_GRADS.pack(*_t4(dout), *(_NO_TENSOR if dq is None else _t4(dq)), *(_NO_TENSOR if dk is None else _t4(dk)),
-                        *(_NO_TENSOR if dv is None else _t4(dv)))
+    grads = _lib._ATTENTION_GRADS.pack(*_t4(dout), *(_NO_TENSOR if dq is None else _t4(dq)),
+                                       *(_NO_TENSOR if dk is None else _t4(dk)), *(_NO_TENSOR if dv is None else _t4(dv)))
     head = _pack(q, k, v, out, out_lo, lse, opts) + grads
     _lib.call_rows(lib.flk_attention_backward, head, q.device, lib.flk_attention_workspace_bytes, 1)
     return dq, dk if need_k else None, dv if need_v else None, None
@@ -184,11 +186,12 @@ def attention(
         key, that is at ``kv_lens - Nq``.  A right-padded batch of Nq == Nk rows takes zeros here
     return_lse : also return ``log sum_j exp(s_ij)``, (B, Hq, Nq) float32 (without gradient)
 
-    A query that sees no key gets zeros, and -inf in the log-sum-exp.  What padding rows and rows behind ``kv_lens``
-    hold does not matter, NaN included.  Integer tables are read on the device: lengths beyond [0, Nk] count as the nearer
-    end.  At most 65535 sequences, 65535 heads, 2^29 rows.  Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates
-    its output and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has
-    it for every operator, only while no graph of the same leaves that was built outside of the capture is alive).
+    A query that sees no key gets zeros, and -inf in the log-sum-exp.  What such queries, padding rows, keys behind
+    ``kv_lens`` and, with ``causal``, keys that no query reaches hold does not matter, NaN included.  Integer tables are
+    read on the device: lengths beyond [0, Nk] count as the nearer end.  At most 65535 sequences, 65535 heads, 2^29 rows.
+    Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates its output
+    and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has it for every
+    operator, only while no graph of the same leaves that was built outside of the capture is alive).
     """
     try:
         fits = q.dtype is k.dtype is v.dtype and q.dtype in _lib._ROW_TYPES and k.shape == v.shape and q.device == k.device == v.device

@@ -261,8 +261,9 @@ int flk_kgrad(int dtype, int kernel,
  * kv_len_b - nq + i) and sees key j when
  *      j < kv_lens[b] (default nk)  and  (causal == 0  or  j <= p_i  or  j < prefix_lens[b])
  *      and  (no documents  or  q_documents[b][i] == k_documents[b][j] >= 0).
- * A query that sees nothing gets out = 0 and lse = -inf, and passes no gradient.  Keys and values at or behind
- * kv_lens[b], and rows whose document is negative, may hold anything (NaN included).  A value or key that is not finite
+ * A query that sees nothing gets out = 0 and lse = -inf, and passes no gradient.  Such queries (q and dout), keys and values
+ * at or behind kv_lens[b] or, with causal, behind the last query's reach, and rows whose document is negative, may hold
+ * anything (NaN included).  A value or key that is not finite
  * and that some query may see reaches the outputs of the queries that share a tile with that one.
  *
  * Types FLK_F32, FLK_BF16, FLK_F16; 1 <= d <= 128, d a multiple of 8 (of 4 with FLK_F32); hq a multiple of hk (query
@@ -271,7 +272,8 @@ int flk_kgrad(int dtype, int kernel,
  * arrays of one entry per sequence (values outside [0, nk], and positions beyond 2^29, are clamped); documents: int32, one row per
  * sequence with the given stride; slopes: fp32, one per query head.  All of them may be NULL.
  *
- * flags is 0: none are defined.  flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
+ * flags is 0: none are defined.  A softcap below 1e-30, or below |scale| 1e-30, is refused unless it is 0.
+ * flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
  * v, out, lse and dout and writes dq, dk, dv (dk and dv are given together; dq.data or both may be NULL).  Sums run in
  * an order fixed by the sizes: results are the same from run to run.  The workspace query takes the same struct
  * (pointers other than the documents' are not looked at).

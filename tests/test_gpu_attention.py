@@ -393,3 +393,37 @@ def test_launches_are_counted():
     before = _lib.launch_count()
     attention(q, k, v)
     assert _lib.launch_count() > before
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (3, 3, 128), (6, 2, 32)])
+def test_garbage_in_queries_that_see_nothing(hq, hk, d, dtype):
+    """Queries before the first key, or of documents without keys, and their output gradients, reach no other row."""
+    q, k, v, do = make(2, 200, 230, hq, hk, d, dtype, seed=40)
+    starts = torch.tensor([-70, -1000], device=DEV)
+    for first, sequence in ((70, 0), (200, 1)):
+        q[sequence, :first] = float("nan")
+        do[sequence, :first] = float("inf")
+    out = run_and_check(q, k, v, do, causal=True, q_starts=starts, softcap=9.0)
+    assert not bool(out[0, :70].any()) and not bool(out[1].any())
+    q, k, v, do = make(1, 200, 230, hq, hk, d, dtype, seed=41)
+    docs, q_docs = (torch.arange(n, device=DEV)[None] // 20 for n in (230, 200))
+    q_docs = torch.where(q_docs % 3 == 1, q_docs + 1000, q_docs)
+    q[q_docs >= 1000] = float("inf")
+    do[q_docs >= 1000] = float("nan")
+    run_and_check(q, k, v, do, documents=docs, q_documents=q_docs)
+    run_and_check(q, k, v, do, causal=True, q_starts=torch.tensor([30], device=DEV), documents=docs, q_documents=q_docs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq", [1, 3, 20, 150])
+def test_garbage_in_keys_behind_the_last_query(nq, dtype):
+    """A causal call over a cache that is longer than what has been written, told by the queries' positions alone."""
+    q, k, v, do = make(3, nq, 400, 4, 2, 64, dtype, seed=42)
+    starts = torch.tensor([0, 129, 400 - nq], device=DEV)
+    prefix = torch.tensor([0, 200, 7], device=DEV)
+    for i in range(3):
+        reach = max(int(starts[i]) + nq, int(prefix[i]))
+        k[i, reach:] = float("nan")
+        v[i, reach:] = float("inf")
+    run_and_check(q, k, v, do, causal=True, q_starts=starts, prefix_lens=prefix)

@@ -181,3 +181,17 @@ def test_layer_norm_workspace(lib):
     assert lib.flk_layer_norm_forward(norm_args(n=0), None) == 0
     assert lib.flk_layer_norm_forward(norm_args(mean=None), None) == _lib.FLK_ERR_BAD_ARG
     assert lib.flk_layer_norm_forward(None, None) == _lib.FLK_ERR_BAD_ARG
+
+
+@pytest.mark.parametrize("scale,softcap", [(0.125, 1e-38), (0.125, 1e-40), (1e10, 1e-25), (-1e10, 1e-25)])
+def test_softcap_that_fp32_cannot_hold(lib, scale, softcap):
+    change = dict(scale=scale, softcap=softcap)
+    assert lib.flk_attention_forward(attention_args(**change), None) == _lib.FLK_ERR_UNSUPPORTED
+    assert lib.flk_attention_backward(attention_args(**change), None) == _lib.FLK_ERR_UNSUPPORTED
+    assert lib.flk_attention_workspace_bytes(attention_args(**change), 0) == _lib.FLK_ERR_UNSUPPORTED
+
+
+def test_rows_up_to_a_tile_behind_the_last(lib):
+    for change in (dict(nq=2**29 - 1, hq=4, hk=4), dict(nk=2**29 - 1, hq=4, hk=4)):
+        assert lib.flk_attention_workspace_bytes(attention_args(**change), 0) == _lib.FLK_ERR_UNSUPPORTED
+    assert lib.flk_attention_workspace_bytes(attention_args(nq=2**29 - 256, hq=4, hk=4), 0) >= 0
