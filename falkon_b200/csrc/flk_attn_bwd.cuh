@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       uint32_t s[1][32], pr[32];
       tmem_ld32(ts + lane_at + mine0, s[0]);
       tmem_ld_wait_on(s[0]);
-      if constexpr (CAP) to_tanh(s, a.scale);
+      if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const uint32_t at = st + c * 4;
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       tmem_ld32(at, s[0]);
       tmem_ld_wait_on(s[0]);
       const float d0 = (float)(pos - k0 - (int)mine0);
-      if constexpr (CAP) to_tanh(s, a.scale);
+      if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         float x[2];
@@ -858,6 +858,7 @@ inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
   t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.q_blocks, t.splits = p.splits;
+  t.tanh = make_tanh(a.scale, 1.f);
   Maps m;
   FLK_TRY(make_map(&m.q, a.q, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
   FLK_TRY(make_map(&m.dout, a.dout, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));

@@ -15,6 +15,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -170,33 +171,61 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// s -> tanh(s * scale), in place, for N x 32 raw scores of a row.  Where all of a warp's arguments lie in [-1/2, 1/2], and scores
-// of up to half the cap do, an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: x p(x^2) with
-// p of degree 4 fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32).  With both on the MUFU unit, the
-// exponential of the weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle
-// are 3072 cycles against 1024 of the two products.
+// The tanh of capped scores.  Where all of a warp's arguments x = scale s lie in [-1/2, 1/2], and scores of up to half the cap do,
+// an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: tanh(x) = x p(x^2) with p of degree 4
+// fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32).  With both on the MUFU unit, the exponential of the
+// weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle are 3072 cycles against
+// 1024 of the two products.  `scale`, and a factor of the result, are multiplied into the coefficients once per call (Tanh), which
+// saves a multiplication per score.
 __device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
+struct Tanh {
+  uint64_t c[5];  // coefficients, twice each
+  float limit;    // largest |s| of the polynomial; -1: none (powers of the scale that fp32 does not hold well)
+};
+inline Tanh make_tanh(float scale, float factor) {
+  const double p[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
+  Tanh t;
+  double f = (double)factor * scale;
+  for (int k = 0; k < 5; ++k, f *= (double)scale * scale) {
+    const float v = (float)(p[k] * f);
+    uint32_t u;
+    memcpy(&u, &v, 4);
+    t.c[k] = (uint64_t)u << 32 | u;
+  }
+  const float size = scale < 0 ? -scale : scale;
+  t.limit = size > 1e-3f && size < 1e3f ? 0.5f / size : -1.f;
+  return t;
+}
 template <int N>
-__device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], float scale) {
+__device__ __forceinline__ bool small_arguments(const uint32_t (&s)[N][32], float limit) {
   float big = 0.f;
 #pragma unroll
   for (int p = 0; p < N; ++p)
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(s[p][c]))), fabsf(__uint_as_float(s[p][c + 1])));
-  if (__all_sync(0xffffffffu, big * fabsf(scale) <= 0.5f)) {
+  return __all_sync(0xffffffffu, big <= limit);
+}
+__device__ __forceinline__ uint64_t tanh_slope(uint64_t s, const Tanh& t) {  // factor tanh(scale s) / s
+  const uint64_t z = tc::mul2(s, s);
+  uint64_t y = tc::fma2(z, t.c[4], t.c[3]);
+  y = tc::fma2(y, z, t.c[2]);
+  y = tc::fma2(y, z, t.c[1]);
+  return tc::fma2(y, z, t.c[0]);
+}
+__device__ __forceinline__ float tanh_mufu(float s, float scale2) {  // scale2 = 2 scale log2 e:  1 - 2 / (1 + e^2x)
+  return fmaf(-2.f, rcp_approx(1.f + ex2_approx(s * scale2)), 1.f);
+}
+// s -> tanh(scale s) in place, N x 32 raw scores of a row
+template <int N>
+__device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], const Tanh& t, float scale) {
+  if (small_arguments(s, t.limit)) {
 #pragma unroll
     for (int p = 0; p < N; ++p)
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        const uint64_t x = tc::mul2(tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1])), both(scale));
-        const uint64_t z = tc::mul2(x, x);
-        uint64_t y = tc::fma2(z, both(0.017131345346570015f), both(-0.05298423767089844f));
-        y = tc::fma2(y, z, both(0.133247509598732f));
-        y = tc::fma2(y, z, both(-0.3333306908607483f));
-        y = tc::fma2(y, z, both(1.0f));
-        y = tc::mul2(y, x);
+        const uint64_t x = tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1]));
         float y0, y1;
-        tc::unpack2(y, y0, y1);
+        tc::unpack2(tc::mul2(tanh_slope(x, t), x), y0, y1);
         s[p][c] = __float_as_uint(y0);
         s[p][c + 1] = __float_as_uint(y1);
       }
@@ -205,8 +234,7 @@ __device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], float scale) {
 #pragma unroll
     for (int p = 0; p < N; ++p)
 #pragma unroll
-      for (int c = 0; c < 32; ++c)  // tanh(x) = 1 - 2 / (1 + e^2x)
-        s[p][c] = __float_as_uint(fmaf(-2.f, rcp_approx(1.f + ex2_approx(__uint_as_float(s[p][c]) * f)), 1.f));
+      for (int c = 0; c < 32; ++c) s[p][c] = __float_as_uint(tanh_mufu(__uint_as_float(s[p][c]), f));
   }
 }
 
@@ -251,6 +279,7 @@ struct TcArgs {
   int splits;        // parts of the key axis
   float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
   float* part_lse;   // [split][b][hp][rows], base 2
+  Tanh tanh;         // of the cap; the backward pass's factor is 1, the forward pass's cap2 where a bias follows
   const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
 };
 

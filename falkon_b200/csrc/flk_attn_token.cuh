@@ -153,20 +153,19 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
       float big = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) big = fmaxf(big, fmaxf(fabsf(s[0][e]), fabsf(s[1][e])));
-      if (__all_sync(0xffffffffu, big * fabsf(a.scale) <= 0.5f)) {
+      const bool small = __all_sync(0xffffffffu, big <= t.tanh.limit);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // the polynomial of to_tanh
-            const float x = s[n][e] * a.scale, z = x * x;
-            s[n][e] = x * fmaf(fmaf(fmaf(fmaf(0.017131345346570015f, z, -0.05298423767089844f), z, 0.133247509598732f), z, -0.3333306908607483f), z, 1.0f);
+        for (int e = 0; e < 4; e += 2) {
+          const uint64_t x = tc::pack2(s[n][e], s[n][e + 1]);
+          if (small) {
+            tc::unpack2(tc::mul2(tanh_slope(x, t.tanh), x), s[n][e], s[n][e + 1]);
+          } else {
+            s[n][e] = tanh_mufu(s[n][e], a.scale * (2.f * kLog2e));
+            s[n][e + 1] = tanh_mufu(s[n][e + 1], a.scale * (2.f * kLog2e));
           }
-      } else {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = fmaf(-2.f, rcp_approx(1.f + ex2_approx(s[n][e] * (a.scale * (2.f * kLog2e)))), 1.f);
-      }
+        }
     }
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -297,6 +296,7 @@ template <typename T>
 inline int launch(TcArgs t, int splits, cudaStream_t st) {
   const Args& a = t.a;
   t.pg = a.grp, t.hp = a.hk, t.rows = a.nq * a.grp, t.splits = splits;
+  t.tanh = make_tanh(a.scale, 1.f);
   const bool cap = a.cap2 != 0.f, bias = a.slopes != nullptr;
   if (a.d <= 64) {
     if (cap) FLK_TRY((bias ? launch_one<T, 64, true, true>(t, st) : launch_one<T, 64, true, false>(t, st)));
