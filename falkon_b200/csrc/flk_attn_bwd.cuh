@@ -30,7 +30,7 @@ constexpr int kRegsWork = 104, kRegsOther = 64;
 static_assert(4 * 128 * kRegsWork + 128 * kRegsOther <= kThreads * 96, "registers");
 
 // what the columns (queries) of a tile bring into the keys kernel
-enum { kLse = 0, kDelta = 128, kSlope = 256, kPos = 384, kEnd = 512, kLabel = 640, kStatWords = 768 };
+enum { kLse = 0, kDelta = 128, kSlope = 256, kPos = 384, kLabel = 512, kStatWords = 640 };
 constexpr int kStatSlots = 4;
 
 template <int DP, bool KEYS>
@@ -312,7 +312,6 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
             put(kSlope, __float_as_uint(-slope[x] * kLog2e));
             put(kPos, __float_as_uint((float)(lim.start + i - k0)));
           }
-          put(kEnd, (uint32_t)((r < t.rows ? lim.row_end(i, a.causal) : 0) - k0));
           put(kLabel, (uint32_t)label[x]);
         }
         __syncwarp();
@@ -411,7 +410,20 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       tc_fence_after();
       const Tile e = get_tile(slots, i);
       const bool whole = k0 + kTile <= lim.row_end((e.at * kTile) >> t.pg_shift, a.causal) && (kd == nullptr || (e.label >= 0 && e.label == only));
-      uint32_t s[1][32], pr[32];
+      uint32_t seen = 0xffffffffu;  // columns (queries) that see this thread's key
+      if (!whole) {
+        // under a causal mask the queries from one on, and those that exist
+        const int row0 = e.at * kTile + (int)mine0;
+        const int from = a.causal && key >= lim.prefix ? min(max(key - lim.start, 0), a.nq) << t.pg_shift : 0;
+        seen = key < lim.len ? columns_before(t.rows - row0) & ~columns_before(from - row0) : 0;
+        if (kd != nullptr) {
+          int label;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(label) : "r"(st + (kLabel + (threadIdx.x & 31)) * 4) : "memory");
+          seen &= same_label(label, my);
+        }
+      }
+      uint32_t s[1][32];
+      uint32_t pr[32];
       tmem_ld32(ts + lane_at + mine0, s[0]);
       tmem_ld_wait_on(s[0]);
       if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
@@ -435,14 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          int en[4], lb[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(en[0]), "=r"(en[1]), "=r"(en[2]), "=r"(en[3]) : "r"(st + (kEnd + c) * 4) : "memory");
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(lb[0]), "=r"(lb[1]), "=r"(lb[2]), "=r"(lb[3]) : "r"(st + (kLabel + c) * 4) : "memory");
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (key - k0 >= en[q] || (kd != nullptr && lb[q] != my)) pr[c + q] = 0;
-        }
+        for (int c = 0; c < 32; ++c)
+          if ((seen & (1u << c)) == 0) pr[c] = 0;
       }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
@@ -582,6 +588,18 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int4* ktab = kd ? a.ktab + (int64_t)b * (a.nk_pad / kTile) : nullptr;
   const int last = (lim.row_end(i1 - 1, a.causal) + kTile - 1) / kTile;
+  // what a working thread has to know of its row; asked for first, so that its time is that of the tables below
+  const int r = row0 + (int)(threadIdx.x & 127), i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+  const bool exists = warp < kMmaWarp && r < t.rows;
+  float lse = -INFINITY, delta = 0.f, slope = 0.f;
+  int my = -2;
+  if (exists) {
+    const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
+    lse = __ldg(a.lse + row);
+    delta = __ldg(a.delta + row);
+    if (qd) my = __ldg(qd + i);
+    if (BIAS && a.slopes != nullptr) slope = __ldg(a.slopes + h);
+  }
   LabelRange lab{0, 0, false};
   if (kd) lab = labels_of(qd, i0, i1);
   const int steps = count_tiles(ktab, 0, last, lab.lo, lab.hi);
@@ -697,25 +715,15 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     tc::reg_claim<kRegsWork>();
     const int w = warp >> 2;
     const uint32_t lane_at = (uint32_t)(warp & 3) << 21, mine0 = 32 * w;
-    const int r = row0 + (int)(threadIdx.x & 127), i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
-    const bool exists = r < t.rows;
     const int end = exists ? lim.row_end(i, a.causal) : 0;
-    const int my = qd && exists ? qd[i] : -2;
-    const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+    const float slope2 = slope * kLog2e;
     const int pos = lim.start + i;
     const int all_before = lim.row_end(i0, a.causal);
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
     const float f = CAP ? a.cap2 : a.scale, gs = Scales<T>::ds(t);
-    float add = -INFINITY, nd = 0.f;  // of a row that sees nothing
-    if (exists) {
-      const int64_t row = ((int64_t)b * a.hq + h) * a.nq + i;
-      const float lse = a.lse[row];
-      if (lse != -INFINITY) {
-        add = -lse * kLog2e;
-        nd = -a.delta[row] * gs;
-      }
-    }
+    // a row that sees nothing has no weights, and no delta, which may be NaN there
+    const float add = lse == -INFINITY ? -INFINITY : -lse * kLog2e, nd = lse == -INFINITY ? 0.f : -delta * gs;
     bool ok = true;
     for (int step = 0; step < steps && ok; ++step) {
       ok = wait_bar(sfull(step & 1), (uint32_t)(step >> 1) & 1);
@@ -724,6 +732,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       const Tile e = get_tile(slots, step);
       const int k0 = e.at * kTile;
       const bool whole = k0 + kTile <= all_before && (kd == nullptr || (e.label >= 0 && e.label == only));
+      uint32_t seen = 0xffffffffu;
+      if (!whole) {
+        seen = columns_before(end - k0 - (int)mine0);
+        if (kd != nullptr) seen &= same_label(__ldg(kd + k0 + (int)mine0 + (int)(threadIdx.x & 31)), my);
+      }
       uint32_t s[1][32];
       const uint32_t at = ts(step) + lane_at + mine0;
       tmem_ld32(at, s[0]);
@@ -742,10 +755,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         weight_slope<CAP>(s[0][c], s[0][c + 1], x[0], x[1]);
       }
       if (!whole) {
-        const uint32_t seen = seen_columns(end - k0 - (int)mine0, kd == nullptr ? nullptr : kd + k0 + mine0, my);
 #pragma unroll
         for (int c = 0; c < 32; ++c)
-          if ((seen >> c & 1) == 0) s[0][c] = 0;
+          if ((seen & (1u << c)) == 0) s[0][c] = 0;
       }
       ok = wait_bar(dpfull, (uint32_t)step & 1);
       if (!ok) break;
@@ -858,7 +870,7 @@ inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
   t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.q_blocks, t.splits = p.splits;
-  t.tanh = make_tanh(a.scale, 1.f);
+  t.tanh = make_tanh(a.scale);
   Maps m;
   FLK_TRY(make_map(&m.q, a.q, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
   FLK_TRY(make_map(&m.dout, a.dout, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));

@@ -46,16 +46,15 @@ __device__ __forceinline__ int4 get_place(uint32_t at) {
   return v;
 }
 
-// Scores in base 2 with the distance bias; column 0 lies d0 before the row's position.  `f2` times the raw score (or its tanh),
-// or, with POLY, the tanh by its polynomial, which has the factor in it.  Where all columns lie on one side of all rows of the
-// warp, the bias is linear: one base per 8 columns and 4 pairs of offsets that all of them share.
-template <bool POLY>
-__device__ __forceinline__ void add_bias(uint32_t (&s)[2][32], const Tanh& t, float f2, float slope2, float d0) {
+// Scores in base 2 from raw scores (or their tanh) and the distance bias; column 0 lies d0 before the row's position.  Where all
+// columns lie on one side of all rows of the warp, the bias is linear: one base per 8 columns and 4 pairs of offsets that all of
+// them share.
+__device__ __forceinline__ void add_bias(uint32_t (&s)[2][32], float f2, float slope2, float d0) {
   const uint64_t f = both(f2);
   auto put = [&](int p, int c, uint64_t bias) {
     const uint64_t x = tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1]));
     float y0, y1;
-    tc::unpack2(tc::fma2(x, POLY ? tanh_slope(x, t) : f, bias), y0, y1);
+    tc::unpack2(tc::fma2(x, f, bias), y0, y1);
     s[p][c] = __float_as_uint(y0);
     s[p][c + 1] = __float_as_uint(y1);
   };
@@ -324,30 +323,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int p = 0; p < 2; ++p) tmem_ld32(at + 32 * p, s[p]);
 #pragma unroll
       for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
-      if constexpr (CAP && BIAS) {
-        if (small_arguments(s, t.tanh.limit)) {
-          add_bias<true>(s, t.tanh, f2, slope2, (float)(pos - k0));
-        } else {
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[p][c] = __float_as_uint(tanh_mufu(__uint_as_float(s[p][c]), a.scale * (2.f * kLog2e)));
-          add_bias<false>(s, t.tanh, f2, slope2, (float)(pos - k0));
-        }
-      } else if constexpr (CAP) {
-        to_tanh(s, t.tanh, a.scale);
-      } else if constexpr (BIAS) {
-        add_bias<false>(s, t.tanh, f2, slope2, (float)(pos - k0));
-      }
+      if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
+      if constexpr (BIAS) add_bias(s, f2, slope2, (float)(pos - k0));
       if (!whole) {
+        uint32_t seen[2];
         const int4 x = get_place(place + 16);
         const int r = row0 + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
         const int end = r < t.rows ? Limits{x.x, x.y, x.z}.row_end(r >> t.pg_shift, a.causal) : 0;
-        const int b = get_place(place).y;
-        const int* labels = a.kdocs == nullptr ? nullptr : a.kdocs + (int64_t)b * a.nk_pad + k0;
-        const int my = labels != nullptr && r < t.rows ? __ldg(a.qdocs + (int64_t)b * a.nq_pad + (r >> t.pg_shift)) : -2;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) hide_columns(s[p], seen_columns(end - k0 - 32 * p, labels == nullptr ? nullptr : labels + 32 * p, my));
+        for (int p = 0; p < 2; ++p) seen[p] = columns_before(end - k0 - 32 * p);
+        if (a.kdocs != nullptr) {
+          const int b = get_place(place).y, *labels = a.kdocs + (int64_t)b * a.nk_pad + k0 + (threadIdx.x & 31);
+          const int l0 = __ldg(labels), l1 = __ldg(labels + 32), my = r < t.rows ? __ldg(a.qdocs + (int64_t)b * a.nq_pad + (r >> t.pg_shift)) : -2;
+          seen[0] &= same_label(l0, my);
+          seen[1] &= same_label(l1, my);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) hide_columns(s[p], seen[p]);
       }
       float top[4];
 #pragma unroll
@@ -639,7 +631,7 @@ inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
   t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.blocks, t.splits = p.splits;
-  t.tanh = make_tanh(a.scale, a.slopes != nullptr ? a.cap2 : 1.f);
+  t.tanh = make_tanh(a.scale);
   CUtensorMap tq, tk, tv;
   FLK_TRY(make_map(&tq, a.q, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
   FLK_TRY(make_map(&tk, a.k, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));

@@ -173,40 +173,50 @@ __device__ __forceinline__ float rcp_approx(float x) {
 
 // The tanh of capped scores.  Where all of a warp's arguments x = scale s lie in [-1/2, 1/2], and scores of up to half the cap do,
 // an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: tanh(x) = x p(x^2) with p of degree 4
-// fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32).  With both on the MUFU unit, the exponential of the
+// fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32); up to 1/8 degree 2 does (6e-9).  With both on the MUFU unit, the exponential of the
 // weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle are 3072 cycles against
-// 1024 of the two products.  `scale`, and a factor of the result, are multiplied into the coefficients once per call (Tanh), which
-// saves a multiplication per score.
+// 1024 of the two products.  The scale is multiplied into the coefficients once per call (Tanh), which saves a
+// multiplication per score.
 __device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
 struct Tanh {
-  uint64_t c[5];  // coefficients, twice each
-  float limit;    // largest |s| of the polynomial; -1: none (powers of the scale that fp32 does not hold well)
+  uint64_t c[5], low[3];   // coefficients, twice each
+  float limit, low_limit;  // largest |s| of the polynomials; -1: none (powers of the scale that fp32 does not hold well)
 };
-inline Tanh make_tanh(float scale, float factor) {
-  const double p[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
-  Tanh t;
-  double f = (double)factor * scale;
-  for (int k = 0; k < 5; ++k, f *= (double)scale * scale) {
-    const float v = (float)(p[k] * f);
+inline Tanh make_tanh(float scale) {
+  const double c[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
+  const double low[3] = {0.999999993627153, -0.33332598923104395, 0.1320774045773301};
+  auto twice = [](double x) {
+    const float v = (float)x;
     uint32_t u;
     memcpy(&u, &v, 4);
-    t.c[k] = (uint64_t)u << 32 | u;
+    return (uint64_t)u << 32 | u;
+  };
+  Tanh t;
+  double f = scale;
+  for (int k = 0; k < 5; ++k, f *= (double)scale * scale) {
+    t.c[k] = twice(c[k] * f);
+    if (k < 3) t.low[k] = twice(low[k] * f);
   }
   const float size = scale < 0 ? -scale : scale;
-  t.limit = size > 1e-3f && size < 1e3f ? 0.5f / size : -1.f;
+  const bool held = size > 1e-3f && size < 1e3f;
+  t.limit = held ? 0.5f / size : -1.f;
+  t.low_limit = held ? 0.125f / size : -1.f;
   return t;
 }
+// which way a warp goes: 2, 1 (polynomial of degree 2, 4) or 0
 template <int N>
-__device__ __forceinline__ bool small_arguments(const uint32_t (&s)[N][32], float limit) {
+__device__ __forceinline__ int tanh_way(const uint32_t (&s)[N][32], const Tanh& t) {
   float big = 0.f;
 #pragma unroll
   for (int p = 0; p < N; ++p)
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(s[p][c]))), fabsf(__uint_as_float(s[p][c + 1])));
-  return __all_sync(0xffffffffu, big <= limit);
+  return __all_sync(0xffffffffu, big <= t.low_limit) ? 2 : __all_sync(0xffffffffu, big <= t.limit) ? 1 : 0;
 }
-__device__ __forceinline__ uint64_t tanh_slope(uint64_t s, const Tanh& t) {  // factor tanh(scale s) / s
+template <bool LOW>
+__device__ __forceinline__ uint64_t tanh_slope(uint64_t s, const Tanh& t) {  // tanh(scale s) / s
   const uint64_t z = tc::mul2(s, s);
+  if (LOW) return tc::fma2(tc::fma2(z, t.low[2], t.low[1]), z, t.low[0]);
   uint64_t y = tc::fma2(z, t.c[4], t.c[3]);
   y = tc::fma2(y, z, t.c[2]);
   y = tc::fma2(y, z, t.c[1]);
@@ -215,20 +225,27 @@ __device__ __forceinline__ uint64_t tanh_slope(uint64_t s, const Tanh& t) {  // 
 __device__ __forceinline__ float tanh_mufu(float s, float scale2) {  // scale2 = 2 scale log2 e:  1 - 2 / (1 + e^2x)
   return fmaf(-2.f, rcp_approx(1.f + ex2_approx(s * scale2)), 1.f);
 }
+template <bool LOW, int N>
+__device__ __forceinline__ void by_polynomial(uint32_t (&s)[N][32], const Tanh& t) {
+#pragma unroll
+  for (int p = 0; p < N; ++p)
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) {
+      const uint64_t x = tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1]));
+      float y0, y1;
+      tc::unpack2(tc::mul2(tanh_slope<LOW>(x, t), x), y0, y1);
+      s[p][c] = __float_as_uint(y0);
+      s[p][c + 1] = __float_as_uint(y1);
+    }
+}
 // s -> tanh(scale s) in place, N x 32 raw scores of a row
 template <int N>
 __device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], const Tanh& t, float scale) {
-  if (small_arguments(s, t.limit)) {
-#pragma unroll
-    for (int p = 0; p < N; ++p)
-#pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        const uint64_t x = tc::pack2(__uint_as_float(s[p][c]), __uint_as_float(s[p][c + 1]));
-        float y0, y1;
-        tc::unpack2(tc::mul2(tanh_slope(x, t), x), y0, y1);
-        s[p][c] = __float_as_uint(y0);
-        s[p][c + 1] = __float_as_uint(y1);
-      }
+  const int way = tanh_way(s, t);
+  if (way == 2) {
+    by_polynomial<true>(s, t);
+  } else if (way == 1) {
+    by_polynomial<false>(s, t);
   } else {
     const float f = scale * (2.f * kLog2e);
 #pragma unroll
@@ -279,7 +296,7 @@ struct TcArgs {
   int splits;        // parts of the key axis
   float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
   float* part_lse;   // [split][b][hp][rows], base 2
-  Tanh tanh;         // of the cap; the backward pass's factor is 1, the forward pass's cap2 where a bias follows
+  Tanh tanh;         // of the cap
   const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
 };
 
@@ -371,19 +388,19 @@ __device__ __forceinline__ void clean_tile(uint32_t tile, int r0, int end, const
   clean_rows<DP>(tile, [&](int r) { return r0 + r < end && (docs == nullptr || __ldg(docs + r0 + r) >= 0); });
 }
 
-// Bit c: column c of 32 lies before `stop` and has the label `my` (`labels`: 32 of them, 16-byte aligned, or null)
-__device__ __forceinline__ uint32_t seen_columns(int stop, const int* labels, int my) {
-  uint32_t seen = stop >= 32 ? 0xffffffffu : stop <= 0 ? 0u : (1u << stop) - 1u;
-  if (labels != nullptr) {
-    uint32_t bits = 0;
-#pragma unroll 1
-    for (int c = 0; c < 32; c += 4) {
-      const int4 v = __ldg(reinterpret_cast<const int4*>(labels + c));
-      bits |= ((uint32_t)(v.x == my) | (uint32_t)(v.y == my) << 1 | (uint32_t)(v.z == my) << 2 | (uint32_t)(v.w == my) << 3) << c;
-    }
-    seen &= bits;
+// Bit c: column c of 32 lies before `stop`
+__device__ __forceinline__ uint32_t columns_before(int stop) { return stop >= 32 ? 0xffffffffu : stop <= 0 ? 0u : (1u << stop) - 1u; }
+// Bit c: column c of 32 has the label of this lane's row.  The lanes of a whole warp bring a column's label (`theirs`) and a
+// row's (`my`) each; a round for every label that the rows have, one or two where documents follow one another.
+__device__ __forceinline__ uint32_t same_label(int theirs, int my) {
+  uint32_t bits = 0, todo = 0xffffffffu;
+  while (todo != 0) {
+    const int label = __shfl_sync(0xffffffffu, my, __ffs(todo) - 1);
+    const uint32_t columns = __ballot_sync(0xffffffffu, theirs == label);
+    if (my == label) bits = columns;
+    todo &= ~__ballot_sync(0xffffffffu, my == label);
   }
-  return seen;
+  return bits;
 }
 // -infinity in the columns whose bit is not set
 __device__ __forceinline__ void hide_columns(uint32_t (&s)[32], uint32_t seen) {

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
         for (int e = 0; e < 4; e += 2) {
           const uint64_t x = tc::pack2(s[n][e], s[n][e + 1]);
           if (small) {
-            tc::unpack2(tc::mul2(tanh_slope(x, t.tanh), x), s[n][e], s[n][e + 1]);
+            tc::unpack2(tc::mul2(tanh_slope<false>(x, t.tanh), x), s[n][e], s[n][e + 1]);
           } else {
             s[n][e] = tanh_mufu(s[n][e], a.scale * (2.f * kLog2e));
             s[n][e + 1] = tanh_mufu(s[n][e + 1], a.scale * (2.f * kLog2e));
@@ -296,7 +296,7 @@ template <typename T>
 inline int launch(TcArgs t, int splits, cudaStream_t st) {
   const Args& a = t.a;
   t.pg = a.grp, t.hp = a.hk, t.rows = a.nq * a.grp, t.splits = splits;
-  t.tanh = make_tanh(a.scale, 1.f);
+  t.tanh = make_tanh(a.scale);
   const bool cap = a.cap2 != 0.f, bias = a.slopes != nullptr;
   if (a.d <= 64) {
     if (cap) FLK_TRY((bias ? launch_one<T, 64, true, true>(t, st) : launch_one<T, 64, true, false>(t, st)));
