@@ -72,6 +72,70 @@ __global__ void __launch_bounds__(128) documents_kernel(const DocTables both) {
   if (4 * lane % a.per == 0) tab[(r0 + 4 * lane) / a.per] = make_int4(lo[0], hi[0], bad[0], 0);
 }
 
+// The order in which blocks start, those with the most tiles to visit first: with documents of several lengths a block that
+// starts late and works long would be what a kernel ends with (8192 rows of 7 documents: forward 128 -> 117 us, dK and dV 188 ->
+// 175 us; the blocks of dQ, many and short, gain nothing: 121, and 123 us in order).  One block: the other side's label ranges go to
+// shared memory, a few threads per entry count those that its range meets, and rank the counts.
+constexpr int kMostOrdered = 1024, kMostRanges = 2048;
+struct OrderList {
+  bool keys;        // of key tiles, else of row blocks of `per` tiles
+  int blocks, per;  // blocks of a sequence
+  int* out;
+};
+__global__ void __launch_bounds__(1024) order_kernel(const Args a, const OrderList o) {
+  __shared__ int2 range[kMostRanges];
+  __shared__ __align__(16) int work[kMostOrdered];
+  const int n = a.b * o.blocks, q_tiles = a.nq_pad / a.q_rows, k_tiles = a.nk_pad / kTile;
+  const int others = o.keys ? q_tiles : k_tiles;
+  const int4 *own_tab = o.keys ? a.ktab : a.qtab, *tab = o.keys ? a.qtab : a.ktab;
+  for (int e = threadIdx.x; e < a.b * others; e += 1024) {
+    const int4 r = __ldg(tab + e);
+    range[e] = make_int2(r.x, r.y);
+  }
+  int per = 32;  // threads per entry, a power of two
+  while (per > 1 && per * n > 1024) per >>= 1;
+  const int e = threadIdx.x / per, lane = threadIdx.x % per;
+  const bool on = e < n;
+  const int b = on ? e / o.blocks : 0, at = on ? e % o.blocks : 0;
+  int4 own = make_int4(0, 0, 0, 0);
+  int first = 0, last = 0;
+  if (on) {
+    const Limits lim = limits_of(a, b);
+    if (o.keys) {
+      own = __ldg(own_tab + (int64_t)b * k_tiles + at);
+      if (a.causal && lim.prefix <= at * kTile) first = min(max(at * kTile - lim.start, 0), a.nq) / a.q_rows;
+      last = at * kTile < lim.len ? q_tiles : 0;
+    } else {
+      own = __ldg(own_tab + (int64_t)b * q_tiles + at * o.per);
+      if (o.per == 2 && at * 2 + 1 < q_tiles) {
+        const int4 more = __ldg(own_tab + (int64_t)b * q_tiles + at * 2 + 1);
+        own.x = min(own.x, more.x);
+        own.y = max(own.y, more.y);
+      }
+      last = (lim.row_end(min(a.nq, (at + 1) * o.per * a.q_rows) - 1, a.causal) + kTile - 1) / kTile;
+    }
+  }
+  __syncthreads();
+  int count = 0;
+#pragma unroll 4
+  for (int x = first + lane; x < last; x += per) {
+    const int2 r = range[b * others + x];
+    count += r.x <= own.y && own.x <= r.y;
+  }
+  for (int x = per / 2; x > 0; x >>= 1) count += __shfl_xor_sync(0xffffffffu, count, x);
+  const int key = on ? count * kMostOrdered + (kMostOrdered - 1 - e) : -1;  // no two alike
+  if (lane == 0) work[e] = key;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 4
+  for (int x = 4 * lane; x < n; x += 4 * per) {
+    const int4 w = *reinterpret_cast<const int4*>(work + x);
+    rank += (w.x > key) + (w.y > key) + (w.z > key) + (w.w > key);
+  }
+  for (int x = per / 2; x > 0; x >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, x);
+  if (on && lane == 0) o.out[rank] = e;
+}
+
 static int esize_of(int64_t dtype) { return dtype == FLK_F32 ? 4 : 2; }
 
 static int check_sizes(const flk_attention_args* p) {
@@ -129,10 +193,21 @@ static bwd::Plan backward_plan(const flk_attention_args* p) {
 // Queries of a tile of the documents' table: those of a tile of 128 packed rows.
 static int query_rows(const flk_attention_args* p) { return on_tensor_cores(p) ? kTile / fwd::packed_heads((int)p->hq, (int)p->hk) : kTile; }
 
-struct Workspace {
-  int64_t qdocs, kdocs, qtab, ktab, delta, amax, part_o, part_lse, total;
-};
 static int64_t pad_rows(int64_t n) { return round_up(n, kTile); }
+// Entries of the list of blocks in order; 0: they start in the order of their numbers, because all start at once, or are too
+// many for the list.
+static int64_t ordered(const flk_attention_args* p, bool backward) {
+  if (p->q_documents == nullptr || !on_tensor_cores(p) || (!backward && by_token(p))) return 0;
+  const int64_t k_tiles = p->batch * ceil_div(p->nk, kTile), q_tiles = p->batch * pad_rows(p->nq) / query_rows(p);
+  const fwd::Plan f = forward_plan(p);
+  const int64_t entries = backward ? k_tiles : p->batch * f.blocks, ranges = backward ? q_tiles : k_tiles;
+  const int64_t blocks = entries * (backward ? p->hk * backward_plan(p).splits : (int64_t)f.hp * f.splits);
+  return entries <= kMostOrdered && ranges <= kMostRanges && blocks > kNumSMs ? entries : 0;
+}
+
+struct Workspace {
+  int64_t qdocs, kdocs, qtab, ktab, order, delta, amax, part_o, part_lse, total;
+};
 static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
   Workspace w{};
   int64_t at = 0;
@@ -146,6 +221,7 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
     w.kdocs = take(p->batch * pad_rows(p->nk) * 4);
     w.qtab = take(p->batch * pad_rows(p->nq) / query_rows(p) * 16);
     w.ktab = take(p->batch * pad_rows(p->nk) / kTile * 16);
+    w.order = take(ordered(p, backward) * 4);
   }
   if (backward) {
     w.delta = take(p->batch * p->hq * p->nq * 4);
@@ -196,6 +272,15 @@ static int make_args(const flk_attention_args* p, bool backward, Args& a, cudaSt
       count_launch();
     }
   }
+  return FLK_OK;
+}
+
+static int launch_order(const flk_attention_args* p, bool backward, int* list, TcArgs& t, cudaStream_t st) {
+  if (ordered(p, backward) == 0) return FLK_OK;
+  const fwd::Plan f = forward_plan(p);
+  t.order = list;
+  order_kernel<<<1, 1024, 0, st>>>(t.a, OrderList{backward, backward ? (int)ceil_div(p->nk, kTile) : f.blocks, f.pair ? 2 : 1, list});
+  count_launch();
   return FLK_OK;
 }
 
@@ -251,6 +336,7 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
     const attn::Workspace w = attn::plan_workspace(p, false);
     char* ws = reinterpret_cast<char*>(p->workspace);
     t.part_o = reinterpret_cast<float*>(ws + w.part_o), t.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
+    FLK_TRY(attn::launch_order(p, false, reinterpret_cast<int*>(ws + w.order), t, st));
     const attn::fwd::Plan plan = attn::forward_plan(p);
     if (attn::by_token(p))
       FLK_TRY(p->dtype == FLK_BF16 ? attn::token_bf16(t, attn::token_splits(p), st) : attn::token_f16(t, attn::token_splits(p), st));
@@ -308,6 +394,7 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
     const attn::Workspace w = attn::plan_workspace(p, true);
     char* ws = reinterpret_cast<char*>(p->workspace);
     t.part_o = reinterpret_cast<float*>(ws + w.part_o);
+    FLK_TRY(attn::launch_order(p, true, reinterpret_cast<int*>(ws + w.order), t, st));
     const attn::bwd::Plan plan = attn::backward_plan(p);
     if (p->dtype == FLK_BF16) {
       FLK_TRY(attn::prepare_backward<__nv_bfloat16>(a, nullptr, st));

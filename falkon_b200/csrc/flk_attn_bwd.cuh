@@ -179,9 +179,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   uint32_t id = blockIdx.x;
   const int hk = (int)(id % (uint32_t)a.hk);
   id /= (uint32_t)a.hk;
-  const int b = (int)(id % (uint32_t)a.b);
-  id /= (uint32_t)a.b;
-  const int split = (int)(id % (uint32_t)t.splits), k0 = (int)(id / (uint32_t)t.splits) * kTile;
+  const int split = (int)(id % (uint32_t)t.splits);
+  id /= (uint32_t)t.splits;
+  int b, k0;
+  if (t.order != nullptr) {
+    const uint32_t place = (uint32_t)__ldg(t.order + id), tiles = (uint32_t)a.nk_pad / kTile;
+    b = (int)(place / tiles);
+    k0 = (int)(place % tiles) * kTile;
+  } else {
+    b = (int)(id % (uint32_t)a.b);
+    k0 = (int)(id / (uint32_t)a.b) * kTile;
+  }
   const Limits lim = limits_of(a, b);
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;

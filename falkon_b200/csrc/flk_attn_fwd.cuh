@@ -96,15 +96,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
 
-  // block -> (row block, part of the key axis, sequence, packed head); late row blocks have the most keys under a causal
-  // mask and start first
+  // block -> (row block, part of the key axis, sequence, packed head); those with the most keys start first, which under a
+  // causal mask are the late ones
   uint32_t id = blockIdx.x;
   const int hp = (int)(id % (uint32_t)t.hp);
   id /= (uint32_t)t.hp;
-  const int b = (int)(id % (uint32_t)a.b);
-  id /= (uint32_t)a.b;
+  int b, rb;
   const int split = (int)(id % (uint32_t)t.splits);
-  const int rb = t.blocks - 1 - (int)(id / (uint32_t)t.splits);
+  id /= (uint32_t)t.splits;
+  if (t.order != nullptr) {
+    const uint32_t place = (uint32_t)__ldg(t.order + id);
+    b = (int)(place / (uint32_t)t.blocks);
+    rb = (int)(place % (uint32_t)t.blocks);
+  } else {
+    b = (int)(id % (uint32_t)a.b);
+    rb = t.blocks - 1 - (int)(id / (uint32_t)a.b);
+  }
   constexpr int kRows = PAIR ? 256 : 128;
   const int row0 = rb * kRows, hk = (int)((uint32_t)(hp * t.pg) / (uint32_t)a.grp);
   const int i0 = row0 >> t.pg_shift, i1 = min(a.nq, (row0 + kRows) >> t.pg_shift);  // queries of this block

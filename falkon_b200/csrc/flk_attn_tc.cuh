@@ -297,6 +297,8 @@ struct TcArgs {
   float* part_o;     // [split][b][hp][rows][d] partial results of the parts, fp32
   float* part_lse;   // [split][b][hp][rows], base 2
   Tanh tanh;         // of the cap
+  // the order in which the row blocks (backward: the key tiles) of all sequences start: sequence * blocks + block, or null
+  const int* order;
   const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
 };
 

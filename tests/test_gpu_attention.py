@@ -427,3 +427,22 @@ def test_garbage_in_keys_behind_the_last_query(nq, dtype):
         k[i, reach:] = float("nan")
         v[i, reach:] = float("inf")
     run_and_check(q, k, v, do, causal=True, q_starts=starts, prefix_lens=prefix)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,n,hq,hk", [(1, 1500, 16, 8), (5, 700, 12, 6), (3, 650, 21, 7), (40, 140, 4, 4)])
+def test_documents_of_many_lengths(b, n, hq, hk, causal, dtype):
+    """More blocks than SMs: they start in the order of their work, whatever the documents' order in the rows."""
+    q, k, v, do = make(b, n, n, hq, hk, 64, dtype, seed=43)
+    g = torch.Generator(device="cpu").manual_seed(n)
+    lens = [1, 400 % n, 3, 90, 37]
+    ids = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+    ids = torch.cat([ids, torch.full((n,), 7)])[:n]
+    docs = torch.stack([torch.roll(ids, int(torch.randint(0, n, (1,), generator=g))) for _ in range(b)])
+    docs[:, n - 11:n - 4] = -1
+    docs = docs.to(DEV)
+    run_and_check(q, k, v, do, causal=causal, documents=docs)
+    keys = torch.cat([docs, docs[:, :300 % n]], 1)
+    k, v = (torch.cat([t, t[:, :300 % n]], 1) for t in (k, v))
+    run_and_check(q, k, v, do, causal=causal, documents=keys, q_documents=docs, kv_lens=torch.full((b,), n + 17, device=DEV))
