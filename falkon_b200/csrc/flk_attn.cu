@@ -5,6 +5,7 @@
 #include "flk_attn_rows.cuh"
 #include "flk_attn_simt.cuh"
 #include "flk_attn_token.cuh"
+#include "flk_attn_token32.cuh"
 
 namespace flk {
 namespace attn {
@@ -187,6 +188,13 @@ static fwd::Plan forward_plan(const flk_attention_args* p) {
 // A few rows over many keys (their bytes are the bound) go to the kernel for single tokens.
 static bool by_token(const flk_attention_args* p) { return on_tensor_cores(p) && token::takes((int)p->nq, (int)(p->hq / p->hk)); }
 static int token_splits(const flk_attention_args* p) { return token::splits_of((int)p->batch, (int)p->nk, (int)p->hk); }
+// The same for fp32.
+static bool by_token32(const flk_attention_args* p) { return p->dtype == FLK_F32 && token32::takes((int)p->nq, (int)(p->hq / p->hk)); }
+static int simt_splits(const flk_attention_args* p) {
+  return by_token32(p) ? token32::splits_of((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d)
+                       : simt::splits_of((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->d, p->causal != 0, p->q_documents != nullptr,
+                                         p->kv_lens != nullptr);
+}
 static bwd::Plan backward_plan(const flk_attention_args* p) {
   return bwd::make_plan((int)p->batch, (int)p->nq, (int)p->nk, (int)p->hq, (int)p->hk, (int)p->d, p->causal != 0, p->q_documents != nullptr);
 }
@@ -228,8 +236,14 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
     w.amax = take(8);
     if (on_tensor_cores(p)) w.part_o = take(bwd::partial_floats(backward_plan(p), p->batch, p->nk, p->hk, p->d) * 4);
   }
-  if (!backward && on_tensor_cores(p) && p->batch > 0 && p->nq > 0) {
-    const int64_t rows = by_token(p) ? (int64_t)token_splits(p) * p->batch * p->hq * p->nq : fwd::partial_rows(forward_plan(p), (int)p->batch);
+  if (!backward && p->batch > 0 && p->nq > 0 && p->nk > 0) {
+    int64_t rows;
+    if (by_token(p) || p->dtype == FLK_F32) {
+      const int64_t parts = by_token(p) ? token_splits(p) : simt_splits(p);
+      rows = parts > 1 || by_token(p) || by_token32(p) ? parts * p->batch * p->hq * p->nq : 0;
+    } else {
+      rows = fwd::partial_rows(forward_plan(p), (int)p->batch);
+    }
     w.part_o = take(rows * p->d * 4);
     w.part_lse = take(rows * 4);
   }
@@ -330,20 +344,23 @@ int flk_attention_forward(const flk_attention_args* p, void* stream) {
   if (a.nk == 0) {
     FLK_TRY(attn::write_nothing(p->dtype, a.o, a.b, a.nq, a.hq, a.d, a.lse, st));
     if (a.o_lo != nullptr) FLK_TRY(attn::write_nothing(p->dtype, attn::Tensor4{a.o_lo, a.o.sb, a.o.sn, a.o.sh}, a.b, a.nq, a.hq, a.d, nullptr, st));
-  } else if (attn::on_tensor_cores(p)) {
+  } else {
     attn::TcArgs t{};
     t.a = a;
     const attn::Workspace w = attn::plan_workspace(p, false);
     char* ws = reinterpret_cast<char*>(p->workspace);
     t.part_o = reinterpret_cast<float*>(ws + w.part_o), t.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
     FLK_TRY(attn::launch_order(p, false, reinterpret_cast<int*>(ws + w.order), t, st));
-    const attn::fwd::Plan plan = attn::forward_plan(p);
-    if (attn::by_token(p))
+    if (attn::by_token32(p)) {
+      FLK_TRY(attn::token32::launch(t, attn::simt_splits(p), st));
+    } else if (p->dtype == FLK_F32) {
+      FLK_TRY(a.d <= 64 ? attn::simt::launch_forward<64>(t, attn::simt_splits(p), st) : attn::simt::launch_forward<128>(t, attn::simt_splits(p), st));
+    } else if (attn::by_token(p)) {
       FLK_TRY(p->dtype == FLK_BF16 ? attn::token_bf16(t, attn::token_splits(p), st) : attn::token_f16(t, attn::token_splits(p), st));
-    else
+    } else {
+      const attn::fwd::Plan plan = attn::forward_plan(p);
       FLK_TRY(p->dtype == FLK_BF16 ? attn::forward_bf16(t, plan, st) : attn::forward_f16(t, plan, st));
-  } else {
-    FLK_TRY(a.d <= 64 ? attn::simt::launch_forward<64>(a, st) : attn::simt::launch_forward<128>(a, st));
+    }
   }
   FLK_CUDA_TRY(cudaGetLastError());
   return FLK_OK;

@@ -548,12 +548,16 @@ __global__ void __launch_bounds__(256) join_kernel(const TcArgs t, int parts) {
     }
   }
   const int64_t at = b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh + c;
-  const uint2 v = make_uint2(pack16<T>(acc.x, acc.y), pack16<T>(acc.z, acc.w));
-  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o.p) + at) = v;
-  if (a.o_lo != nullptr) {
-    const uint2 x = make_uint2(pack16<T>(acc.x - to_f<T>(from_f<T>(acc.x)), acc.y - to_f<T>(from_f<T>(acc.y))),
-                               pack16<T>(acc.z - to_f<T>(from_f<T>(acc.z)), acc.w - to_f<T>(from_f<T>(acc.w))));
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o_lo) + at) = x;
+  if constexpr (std::is_same<T, float>::value) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.o.p) + at) = acc;
+  } else {
+    const uint2 v = make_uint2(pack16<T>(acc.x, acc.y), pack16<T>(acc.z, acc.w));
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o.p) + at) = v;
+    if (a.o_lo != nullptr) {
+      const uint2 x = make_uint2(pack16<T>(acc.x - to_f<T>(from_f<T>(acc.x)), acc.y - to_f<T>(from_f<T>(acc.y))),
+                                 pack16<T>(acc.z - to_f<T>(from_f<T>(acc.z)), acc.w - to_f<T>(from_f<T>(acc.w))));
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o_lo) + at) = x;
+    }
   }
 }
 

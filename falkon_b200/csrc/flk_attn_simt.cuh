@@ -12,8 +12,7 @@
 // room for a second set of tiles.
 #pragma once
 
-#include "flk_attn.cuh"
-#include "flk_ptx.cuh"
+#include "flk_attn_fwd.cuh"
 
 namespace flk {
 namespace attn {
@@ -201,12 +200,13 @@ __device__ __forceinline__ void add_rows(const float* room, uint64_t (&acc)[4][D
 }
 
 template <int DM>
-__global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(const TcArgs t) {
   extern __shared__ float sm[];
+  const Args& a = t.a;
   constexpr int kRows = Smem<DM>::kRows, kGroups = Smem<DM>::kGroups;
   const int g = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, tx = tid & 15, ty = tid >> 4;
   float *Q = sm, *K = Q + kRows + g * (4 * kRows + Smem<DM>::kPair), *V = K + 2 * kRows, *P = V + 2 * kRows;
-  const int q0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
+  const int q0 = (int)(blockIdx.x / (uint32_t)t.splits) * kT, split = (int)(blockIdx.x % (uint32_t)t.splits), h = blockIdx.y, b = blockIdx.z, hk = h / a.grp;
   const Limits lim = limits_of(a, b);
   const int* qd = a.qdocs ? a.qdocs + (int64_t)b * a.nq_pad : nullptr;
   const int* kd = a.kdocs ? a.kdocs + (int64_t)b * a.nk_pad : nullptr;
@@ -222,12 +222,15 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(co
     m[i] = -INFINITY;
     l[i] = 0.f;
   }
-  const int last = lim.row_end(min(q0 + kT, a.nq) - 1, a.causal);
+  // the block's keys: its part of those that its rows see, in whole tiles
+  const int tiles = (lim.row_end(min(q0 + kT, a.nq) - 1, a.causal) + kT - 1) / kT;
+  const int even = (int)((uint32_t)tiles / (uint32_t)t.splits), odd = tiles - even * t.splits;
+  const int first = (split * even + min(split, odd)) * kT, last = first + (even + (split < odd ? 1 : 0)) * kT;
   auto next = [&](int k0) {
     while (k0 < last && !labels_meet(a, b, q0, k0)) k0 += kT * kGroups;
     return k0;
   };
-  int k0 = next(g * kT), buf = 0;
+  int k0 = next(first + g * kT), buf = 0;
   if (g == 0) fetch_tile<DM>(Q, a.q, b, h, q0, a.nq, a.d, qd, tid);
   if (k0 < last) fetch_tile<DM>(K, a.k, b, hk, k0, lim.len, a.d, kd, tid);
   cp_async_commit();
@@ -245,8 +248,8 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(co
     cp_async_commit();
     float s[4][4];
     dots<DM>(s, Q, K + buf * kRows, ty, tx);
-    float t[4][4];
-    scores(a, s, t);
+    float tanh[4][4];
+    scores(a, s, tanh);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int pos = lim.start + q0 + 4 * ty + i;
@@ -312,10 +315,17 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(co
   for (int i = 0; i < 4; ++i) {
     const int r = q0 + 4 * ty + i;
     f[i] = l[i] == 0.f ? 0.f : 1.0f / l[i];
-    if (tx == 0 && r < a.nq && a.lse != nullptr)
-      a.lse[((int64_t)b * a.hq + h) * a.nq + r] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    if (tx != 0 || r >= a.nq) continue;
+    const float lse2 = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
+    if (t.splits > 1)
+      t.part_lse[(((int64_t)split * a.b + b) * a.hq + h) * a.nq + r] = lse2;
+    else if (a.lse != nullptr)
+      a.lse[((int64_t)b * a.hq + h) * a.nq + r] = lse2 * kLn2;
   }
-  store_rows<DM>(a.o, b, h, q0, a.nq, a.d, acc, f, ty, tx);
+  // a part's results are rows of [split][b][hq][nq][d]
+  const int64_t rows = (int64_t)a.hq * a.nq * a.d;
+  const Tensor4 to = t.splits > 1 ? Tensor4{t.part_o + (int64_t)split * a.b * rows, rows, a.d, (int64_t)a.nq * a.d} : a.o;
+  store_rows<DM>(to, b, h, q0, a.nq, a.d, acc, f, ty, tx);
 }
 
 // Gradients of 64 keys and values: loops over the query heads that share them and over their query tiles.
@@ -507,17 +517,38 @@ constexpr size_t q_smem() { return (2 * Smem<DM>::kRows + Smem<DM>::kGroups * (2
 static_assert(forward_smem<64>() <= 227 * 1024 && forward_smem<128>() <= 227 * 1024, "shared memory");
 static_assert(kv_smem<64>() <= 227 * 1024 && kv_smem<128>() <= 227 * 1024, "shared memory");
 
-template <int DM>
-inline int run(void (*fn)(const Args), std::atomic<uint64_t>& done, const dim3& grid, size_t smem, const Args& a, cudaStream_t st) {
+// Parts of the key axis (see fwd::make_plan): a block takes an SM, and about 5 us per tile of 64 keys with heads of 64, 9 with more
+// (100 rows over 3000 keys, 4 heads of 64: 206 us in one part, 31 in parts).
+inline int splits_of(int b, int nq, int nk, int hq, int d, bool causal, bool documents, bool lens) {
+  const int64_t blocks = ceil_div(nq, kT) * hq * b, tiles = ceil_div(nk, kT);
+  double mean = (double)tiles;
+  if (causal && nk > 0) mean *= 1.0 - 0.5 * (nq < nk ? (double)nq / nk : 1.0);
+  if (documents) mean *= 0.5;
+  if (lens) mean *= 0.75;
+  const double joined = (double)b * hq * nq * d * 8.0 / 5e6;
+  int best = 1;
+  double least = 1e300;
+  for (int64_t s = 1; s <= 64 && (s == 1 || s * 2 <= tiles); ++s) {
+    const double cost = fwd::time_of(blocks, s, (double)tiles, mean, d <= 64 ? 5 : 9, mean < 0.95 * (double)tiles) + (s > 1 ? 3 + s * joined : 0);
+    if (cost < least * 0.98) least = cost, best = (int)s;
+  }
+  return best;
+}
+
+template <int DM, typename A>
+inline int run(void (*fn)(const A), std::atomic<uint64_t>& done, const dim3& grid, size_t smem, const A& a, cudaStream_t st) {
   FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), (int)smem, done));
   fn<<<grid, kThreads * Smem<DM>::kGroups, smem, st>>>(a);
   count_launch();
   return FLK_OK;
 }
 template <int DM>
-inline int launch_forward(const Args& a, cudaStream_t st) {
+inline int launch_forward(TcArgs t, int splits, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  return run<DM>(forward_kernel<DM>, done, dim3((unsigned)ceil_div(a.nq, kT), a.hq, a.b), forward_smem<DM>(), a, st);
+  const Args& a = t.a;
+  t.pg = 1, t.hp = a.hq, t.rows = a.nq, t.splits = splits;
+  FLK_TRY(run<DM>(forward_kernel<DM>, done, dim3((unsigned)(ceil_div(a.nq, kT) * splits), a.hq, a.b), forward_smem<DM>(), t, st));
+  return splits > 1 ? fwd::launch_join<float>(t, splits, st) : FLK_OK;
 }
 template <int DM>
 inline int launch_backward(const Args& a, cudaStream_t st) {

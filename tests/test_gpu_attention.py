@@ -446,3 +446,14 @@ def test_documents_of_many_lengths(b, n, hq, hk, causal, dtype):
     keys = torch.cat([docs, docs[:, :300 % n]], 1)
     k, v = (torch.cat([t, t[:, :300 % n]], 1) for t in (k, v))
     run_and_check(q, k, v, do, causal=causal, documents=keys, q_documents=docs, kv_lens=torch.full((b,), n + 17, device=DEV))
+
+
+@pytest.mark.parametrize("nq,nk,hq,hk,d", [(100, 3000, 4, 4, 64), (70, 1500, 2, 1, 128), (1, 3000, 16, 1, 64), (2, 2500, 7, 1, 100), (3, 1000, 5, 5, 32),
+                                           (16, 700, 2, 2, 128), (17, 700, 2, 2, 64)])
+def test_fp32_parts_of_the_key_axis(nq, nk, hq, hk, d):
+    q, k, v, do = make(2, nq, nk, hq, hk, d, torch.float32, seed=44)
+    lens = torch.tensor([nk - 200, nk], device=DEV)
+    docs = (torch.arange(nk, device=DEV) // 300).expand(2, nk)
+    run_and_check(q, k, v, do, causal=True, kv_lens=lens, softcap=12.0, slopes=slopes_of(hq))
+    run_and_check(q, k, v, do, causal=True, prefix_lens=lens // 2, q_starts=torch.tensor([-1, nk // 3], device=DEV))
+    run_and_check(q * 4, k, v, documents=docs, q_documents=docs[:, nk - nq:] - (torch.arange(nq, device=DEV) == 1).long() * 100)
