@@ -15,6 +15,12 @@
 // P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass.  In fp16 they would
 // leave its range: weights are held times 2^12, and dS times a power of two that 2 d max|dO| max|V|, a bound of every
 // |dP - delta|, takes to at most 2^15.
+//
+// The dS of a row add up to zero, so where a row has few keys the terms of dQ and dK cancel, and the rounding of dS would be the
+// largest error (up to 1.8 times that of rounding the result, for rows of ten keys).  With up to 256 queries and keys, where a
+// call is bound by its launches, what rounding took from dS is kept beside it, in the other half of its columns, and multiplied
+// too.  Beyond, where the error stays at 1.5 times, the fourth and fifth product would cost 5 to 10% (8192 rows of documents 150
+// + 120 -> 157 + 135 us; 4 x 2048 rows, heads of 64, 104 + 74 -> 115 + 84).
 #pragma once
 
 #include "flk_attn_fwd.cuh"
@@ -73,6 +79,13 @@ __device__ __forceinline__ void weight_slope(uint32_t& s0, uint32_t& s1, float p
   }
   s0 = __float_as_uint(p0);
   s1 = __float_as_uint(p1);
+}
+
+// what rounding took from a pair of values, rounded itself
+template <typename T>
+__device__ __forceinline__ uint32_t left_over(float y0, float y1, uint32_t rounded) {
+  tc::unpack2(tc::sub2(tc::pack2(y0, y1), unpack16<T>(rounded)), y0, y1);
+  return pack16<T>(y0, y1);
 }
 
 // A quarter of the accumulator (DP / 4 columns from c0 on) times f: 16-bit values of 32 rows, rows side by side
@@ -160,7 +173,7 @@ struct Maps {
 // ---------------------------------------------------------------------------------------------------------------------
 // dK, dV
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant__ Maps maps, const TcArgs t) {
   using L = Layout<DP, true>;
   constexpr int kStages = L::kStages;
@@ -378,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         tc_fence_after();
         if (ok && elect_one()) {
           issue_weighted<T, DP, 32>(tdk, tp, stage(2 * i), i > 0);
+          if constexpr (FINE) issue_weighted<T, DP, 32>(tdk, tp + 16, stage(2 * i), true);
           mma_commit(empty((2 * i) % kStages));
         }
         __syncwarp();
@@ -482,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       tmem_ld_wait_on(d);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        uint32_t o[4];
+        uint32_t o[4], lo[4];
 #pragma unroll
         for (int c = 8 * p; c < 8 * p + 8; c += 4) {
           float dl[4], y[4];
@@ -494,8 +508,13 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
                         y[q], y[q + 1]);
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
           o[c % 8 / 2 + 1] = pack16<T>(y[2], y[3]);
+          if constexpr (FINE) {
+            lo[c % 8 / 2] = left_over<T>(y[0], y[1], o[c % 8 / 2]);
+            lo[c % 8 / 2 + 1] = left_over<T>(y[2], y[3], o[c % 8 / 2 + 1]);
+          }
         }
         tmem_st4(tp + lane_at + mine0 + 4 * p, o);
+        if constexpr (FINE) tmem_st4(tp + lane_at + mine0 + 16 + 4 * p, lo);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -571,7 +590,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const TcArgs t) {
 // ---------------------------------------------------------------------------------------------------------------------
 // dQ
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_constant__ Maps maps, const TcArgs t) {
   using L = Layout<DP, false>;
   constexpr int kStages = L::kStages;
@@ -708,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         if (i + 1 < steps) ok = ok && products(i + 1);
         if (ok && elect_one()) {
           issue_weighted<T, DP, 32>(tdq, ts(i), stage(2 * i), i > 0);
+          if constexpr (FINE) issue_weighted<T, DP, 32>(tdq, ts(i) + 16, stage(2 * i), true);
           mma_commit(empty((2 * i) % kStages));
         }
         __syncwarp();
@@ -775,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       tmem_ld_wait_on(d);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        uint32_t o[4];
+        uint32_t o[4], lo[4];
 #pragma unroll
         for (int c = 8 * p; c < 8 * p + 8; c += 2) {
           float y[2];
@@ -783,8 +803,10 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
                                tc::fma2(tc::pack2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), both(gs), both(nd))),
                       y[0], y[1]);
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
+          if constexpr (FINE) lo[c % 8 / 2] = left_over<T>(y[0], y[1], o[c % 8 / 2]);
         }
         tmem_st4(at + 4 * p, o);
+        if constexpr (FINE) tmem_st4(at + 16 + 4 * p, lo);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -842,11 +864,11 @@ inline Plan make_plan(int b, int nq, int nk, int hq, int hk, int d, bool causal,
 }
 inline int64_t partial_floats(const Plan& p, int64_t b, int64_t nk, int64_t hk, int64_t d) { return p.splits > 1 ? 2 * p.splits * b * nk * hk * d : 0; }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, int DP, bool CAP, bool BIAS, bool FINE>
 inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
   const Args& a = t.a;
   if (a.dk.p != nullptr) {
-    auto* fn = kernel_keys<T, DP, CAP, BIAS>;
+    auto* fn = kernel_keys<T, DP, CAP, BIAS, FINE>;
     constexpr int kBytes = (int)Layout<DP, true>::kBytes;
     static std::atomic<uint64_t> done{0};
     FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
@@ -860,7 +882,7 @@ inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
     }
   }
   if (a.dq.p != nullptr) {
-    auto* fn = kernel_queries<T, DP, CAP, BIAS>;
+    auto* fn = kernel_queries<T, DP, CAP, BIAS, FINE>;
     constexpr int kBytes = (int)Layout<DP, false>::kBytes;
     static std::atomic<uint64_t> done{0};
     FLK_TRY(allow_shared(reinterpret_cast<const void*>(fn), kBytes, done));
@@ -870,6 +892,13 @@ inline int launch_one(const Maps& m, const TcArgs& t, cudaStream_t st) {
     count_launch();
   }
   return FLK_OK;
+}
+
+template <typename T, int DP, bool FINE>
+inline int launch_some(const Maps& m, const TcArgs& t, cudaStream_t st) {
+  const bool bias = t.a.slopes != nullptr;
+  if (t.a.cap2 != 0.f) return bias ? launch_one<T, DP, true, true, FINE>(m, t, st) : launch_one<T, DP, true, false, FINE>(m, t, st);
+  return bias ? launch_one<T, DP, false, true, FINE>(m, t, st) : launch_one<T, DP, false, false, FINE>(m, t, st);
 }
 
 template <typename T>
@@ -883,13 +912,9 @@ inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   FLK_TRY(make_map(&m.dout, a.dout, dtype, a.d, a.hq, a.nq, a.b, p.pg, kTile / p.pg));
   FLK_TRY(make_map(&m.k, a.k, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
   FLK_TRY(make_map(&m.v, a.v, dtype, a.d, a.hk, a.nk, a.b, 1, kTile));
-  const bool cap = a.cap2 != 0.f, bias = a.slopes != nullptr;
-  if (a.d <= 64) {
-    if (cap) return bias ? launch_one<T, 64, true, true>(m, t, st) : launch_one<T, 64, true, false>(m, t, st);
-    return bias ? launch_one<T, 64, false, true>(m, t, st) : launch_one<T, 64, false, false>(m, t, st);
-  }
-  if (cap) return bias ? launch_one<T, 128, true, true>(m, t, st) : launch_one<T, 128, true, false>(m, t, st);
-  return bias ? launch_one<T, 128, false, true>(m, t, st) : launch_one<T, 128, false, false>(m, t, st);
+  const bool fine = a.nq <= 256 && a.nk <= 256;
+  if (a.d <= 64) return fine ? launch_some<T, 64, true>(m, t, st) : launch_some<T, 64, false>(m, t, st);
+  return fine ? launch_some<T, 128, true>(m, t, st) : launch_some<T, 128, false>(m, t, st);
 }
 
 }  // namespace bwd
