@@ -12,6 +12,10 @@
 // Both have 20 warps: four warpgroups that turn scores into weights (a thread owns one row and a quarter of the columns), a warp that
 // issues products, one that issues copies, and in the keys kernel one that gathers what the columns need (lse, delta, ...).
 //
+// Measured: 8192 rows of 7 documents, 16 heads of 128 on 2, capped: dK and dV 150 us (and 10 for adding parts), dQ 121; 4 x 2048
+// rows, 12 heads of 64, distance bias: 104 and 74.  A step takes 4.3 k and 3.0 k cycles with heads of 128 (capped), 3.3 k and
+// 2.5 k with 64: the chain product - exponentials - product, 16 warps on one tile; a block's start takes 2 to 5 k, its end 3 k.
+//
 // P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass.  In fp16 they would
 // leave its range: weights are held times 2^12, and dS times a power of two that 2 d max|dO| max|V|, a bound of every
 // |dP - delta|, takes to at most 2^15.

@@ -64,8 +64,8 @@ inline int launch_delta(const Args& a, uint32_t* amax, cudaStream_t st) {
   const int lanes = a.d <= 8 * kVec ? 8 : a.d <= 16 * kVec ? 16 : 32;
   const dim3 grid((unsigned)ceil_div(n, 2 * 256 / lanes), a.b);
   if (lanes == 8) delta_kernel<T, 8><<<grid, 256, 0, st>>>(a, amax);
-  else if (lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a, amax);
-  else delta_kernel<T, 32><<<grid, 256, 0, st>>>(a, amax);
+  else if (sizeof(T) == 2 || lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a, amax);
+  else if constexpr (sizeof(T) == 4) delta_kernel<T, 32><<<grid, 256, 0, st>>>(a, amax);
   count_launch();
   return FLK_OK;
 }

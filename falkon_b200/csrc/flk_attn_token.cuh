@@ -272,8 +272,8 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
   }
 }
 
-// Whether this kernel takes a call, and the parts of the key axis: about 12 blocks per SM, so that ragged lengths even out (32 caches of 16384 to 32768 keys:
-// 515 us with 2 blocks per SM, 479 with 8, 470 with 12), but no less than 128 keys to a block.
+// Whether this kernel takes a call, and the parts of the key axis: about 12 blocks per SM, so that ragged lengths even out (32
+// caches of 16384 to 32768 keys: 515 us with 2 blocks per SM, 479 with 8, 470 with 12), but no less than 128 keys to a block.
 inline bool takes(int nq, int grp) { return (int64_t)nq * grp <= kRows; }
 inline int splits_of(int b, int nk, int hk) {
   const int64_t blocks = (int64_t)b * hk, want = ceil_div((int64_t)12 * kNumSMs, blocks), most = ceil_div(nk, 128);
