@@ -202,7 +202,6 @@ def attention(
         fits = False
     if not fits:
         _refuse(q, k, v)
-    _require_cuda(None)
     dev = q.device
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)

@@ -128,8 +128,8 @@ def layer_norm(
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError("eps must be finite and not negative")
-    _require_cuda(None)
     if x.device.type != "cuda":
+        _require_cuda(None)
         raise ValueError(f"x must be on a CUDA device (found {x.device})")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
