@@ -276,7 +276,7 @@ int flk_kgrad(int dtype, int kernel,
  * flk_attention_forward writes out and, unless NULL, lse (batch, hq, nq; dense fp32).  flk_attention_backward reads q, k,
  * v, out, lse and dout and writes dq, dk, dv (dk and dv are given together; dq.data or both may be NULL).  Sums run in
  * an order fixed by the sizes: results are the same from run to run.  The workspace query takes the same struct
- * (pointers other than the documents' are not looked at).
+ * (of its pointers, whether documents and kv_lens are there).
  * out_lo (16-bit types; strides of out; may be NULL): forward stores there what rounding took from out, and backward,
  * which needs dout_i . out_i, adds it back; without it that sum carries the rounding of out into dq and dk.
  */
@@ -317,7 +317,8 @@ int flk_attention_status(void* stream, int* status_out);
  * a matrix (x_inner = 1), or the heads of a packed projection.  y and dx are dense.  Types FLK_F32, FLK_BF16, FLK_F16;
  * weight and bias (either may be NULL) and their gradients have type wdtype: the data's, or FLK_F32.
  * Forward writes y and, unless NULL, mean and rstd (n entries each, fp32), which backward reads; backward writes dx,
- * dweight and dbias where they are not NULL.  Only the sums over rows need a workspace.  Results are the same from run
+ * dweight and dbias where they are not NULL.  Only the sums over rows need a workspace (the
+ * query takes the same struct: the plan depends on alignment).  Results are the same from run
  * to run.
  */
 typedef struct flk_layer_norm_args {
