@@ -298,18 +298,6 @@ static int launch_order(const flk_attention_args* p, bool backward, int* list, T
   return FLK_OK;
 }
 
-// delta, and for fp16 the largest magnitudes that the scale of dS is taken from
-template <typename T>
-static int prepare_backward(const Args& a, uint32_t* amax, cudaStream_t st) {
-  if (amax != nullptr) {
-    FLK_CUDA_TRY(cudaMemsetAsync(amax, 0, 8, st));
-    const int64_t packs = (int64_t)a.b * a.nk * a.hk * a.d / 8, blocks = ceil_div(packs, 256 * 8);
-    largest_value_kernel<T><<<(unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 256, 0, st>>>(a, amax + 1);
-    count_launch();
-  }
-  return launch_delta<T>(a, amax, st);
-}
-
 // Zeros for a tensor (and -inf for `lse`, unless null): calls without keys, gradients without queries.
 static int write_nothing(int64_t dtype, const Tensor4& o, int b, int n, int h, int d, float* lse, cudaStream_t st) {
   if (dtype == FLK_F32) return launch_nothing<float>(o, b, n, h, d, lse, st);
@@ -414,12 +402,12 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
     FLK_TRY(attn::launch_order(p, true, reinterpret_cast<int*>(ws + w.order), t, st));
     const attn::bwd::Plan plan = attn::backward_plan(p);
     if (p->dtype == FLK_BF16) {
-      FLK_TRY(attn::prepare_backward<__nv_bfloat16>(a, nullptr, st));
+      FLK_TRY(attn::launch_delta<__nv_bfloat16>(a, nullptr, st));
       FLK_TRY(attn::backward_bf16(t, plan, st));
     } else {
       uint32_t* amax = reinterpret_cast<uint32_t*>(ws + w.amax);
       t.amax = amax;
-      FLK_TRY(attn::prepare_backward<__half>(a, amax, st));
+      FLK_TRY(attn::launch_delta<__half>(a, amax, st));  // and the magnitudes that the scale of dS is taken from
       FLK_TRY(attn::backward_f16(t, plan, st));
     }
   } else {
