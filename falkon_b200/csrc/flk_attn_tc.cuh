@@ -176,15 +176,21 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32); up to 1/8 degree 2 does (6e-9).  With both on the MUFU unit, the exponential of the
 // weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle are 3072 cycles against
 // 1024 of the two products.  The scale is multiplied into the coefficients once per call (Tanh), which saves a
-// multiplication per score.
+// multiplication per score.  Where one of the warp's arguments is larger, every score is scaled first and takes the polynomial or
+// the MUFU unit by its own size: 1 - 2 / (1 + e^2x) is off by 2e-7 whatever x is, and the cap, which may be as large as it likes,
+// multiplies that.
 __device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
+constexpr double kTanh4[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
+constexpr double kTanh2[3] = {0.999999993627153, -0.33332598923104395, 0.1320774045773301};
 struct Tanh {
   uint64_t c[5], low[3];   // coefficients, twice each
-  float limit, low_limit;  // largest |s| of the polynomials; -1: none (powers of the scale that fp32 does not hold well)
+  float limit, low_limit;  // largest |s| of the polynomials; -1: none
 };
+// The polynomials whose coefficients times powers of the scale fp32 holds as normal numbers: the last ones are 0.017 scale^9 and
+// 0.13 scale^5.  Smaller scales (caps of a million scores) leave what reads `c` with the short polynomial, or with none.
 inline Tanh make_tanh(float scale) {
-  const double c[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
-  const double low[3] = {0.999999993627153, -0.33332598923104395, 0.1320774045773301};
+  const float size = scale < 0 ? -scale : scale;
+  const bool four = size > 1e-4f && size < 1e3f, two = size > 1e-7f && size < 1e3f;
   auto twice = [](double x) {
     const float v = (float)x;
     uint32_t u;
@@ -194,13 +200,11 @@ inline Tanh make_tanh(float scale) {
   Tanh t;
   double f = scale;
   for (int k = 0; k < 5; ++k, f *= (double)scale * scale) {
-    t.c[k] = twice(c[k] * f);
-    if (k < 3) t.low[k] = twice(low[k] * f);
+    t.c[k] = twice(four ? kTanh4[k] * f : k < 3 ? kTanh2[k] * f : 0.0);
+    if (k < 3) t.low[k] = twice(kTanh2[k] * f);
   }
-  const float size = scale < 0 ? -scale : scale;
-  const bool held = size > 1e-3f && size < 1e3f;
-  t.limit = held ? 0.5f / size : -1.f;
-  t.low_limit = held ? 0.125f / size : -1.f;
+  t.low_limit = two ? 0.125f / size : -1.f;
+  t.limit = four ? 0.5f / size : t.low_limit;
   return t;
 }
 // which way a warp goes: 2, 1 (polynomial of degree 2, 4) or 0
@@ -222,8 +226,12 @@ __device__ __forceinline__ uint64_t tanh_slope(uint64_t s, const Tanh& t) {  // 
   y = tc::fma2(y, z, t.c[1]);
   return tc::fma2(y, z, t.c[0]);
 }
-__device__ __forceinline__ float tanh_mufu(float s, float scale2) {  // scale2 = 2 scale log2 e:  1 - 2 / (1 + e^2x)
-  return fmaf(-2.f, rcp_approx(1.f + ex2_approx(s * scale2)), 1.f);
+// tanh(scale s) whatever the two are
+__device__ __forceinline__ float tanh_any(float s, float scale) {
+  const float x = s * scale, z = x * x;
+  const float p = x * fmaf(fmaf(fmaf(fmaf((float)kTanh4[4], z, (float)kTanh4[3]), z, (float)kTanh4[2]), z, (float)kTanh4[1]), z, (float)kTanh4[0]);
+  const float m = fmaf(-2.f, rcp_approx(1.f + ex2_approx(x * (2.f * kLog2e))), 1.f);
+  return fabsf(x) <= 0.5f ? p : m;
 }
 template <bool LOW, int N>
 __device__ __forceinline__ void by_polynomial(uint32_t (&s)[N][32], const Tanh& t) {
@@ -247,11 +255,10 @@ __device__ __forceinline__ void to_tanh(uint32_t (&s)[N][32], const Tanh& t, flo
   } else if (way == 1) {
     by_polynomial<false>(s, t);
   } else {
-    const float f = scale * (2.f * kLog2e);
 #pragma unroll
     for (int p = 0; p < N; ++p)
 #pragma unroll
-      for (int c = 0; c < 32; ++c) s[p][c] = __float_as_uint(tanh_mufu(__uint_as_float(s[p][c]), f));
+      for (int c = 0; c < 32; ++c) s[p][c] = __float_as_uint(tanh_any(__uint_as_float(s[p][c]), scale));
   }
 }
 

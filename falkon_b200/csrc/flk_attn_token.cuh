@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
           if (small) {
             tc::unpack2(tc::mul2(tanh_slope<false>(x, t.tanh), x), s[n][e], s[n][e + 1]);
           } else {
-            s[n][e] = tanh_mufu(s[n][e], a.scale * (2.f * kLog2e));
-            s[n][e + 1] = tanh_mufu(s[n][e + 1], a.scale * (2.f * kLog2e));
+            s[n][e] = tanh_any(s[n][e], a.scale);
+            s[n][e + 1] = tanh_any(s[n][e + 1], a.scale);
           }
         }
     }
