@@ -255,6 +255,7 @@ _SIGNATURES = {
     "flk_attention_forward": (_int, [_vp, _vp]),
     "flk_attention_backward": (_int, [_vp, _vp]),
     "flk_attention_status": (_int, [_vp, ctypes.POINTER(_int)]),
+    "flk_attention_wait_limit": (_int, [_i64]),
     "flk_layer_norm_workspace_bytes": (_i64, [_vp]),
     "flk_layer_norm_forward": (_int, [_vp, _vp]),
     "flk_layer_norm_backward": (_int, [_vp, _vp]),
@@ -745,12 +746,18 @@ def call_rows(fn, head: bytes, device: torch.device, query=None, *query_args):
 
 
 def attention_status(device: torch.device) -> int:
-    """1 when a bounded wait of an attention kernel gave up on this device since the library was loaded, else 0."""
+    """1 when a bounded wait of an attention kernel gave up on this device since the last query, else 0.  The rows that it
+    could not finish are NaN."""
     out = ctypes.c_int(0)
     with torch.cuda.device(device):
         stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
         raise_for_status(load().flk_attention_status(stream, ctypes.byref(out)))
     return out.value
+
+
+def attention_wait_limit(ns: int) -> None:
+    """Limit of a wait inside attention's tensor-core kernels, for the calls that follow: 0 to 2e9 ns, at first 1e9."""
+    raise_for_status(load().flk_attention_wait_limit(ns))
 
 
 def tc_status(device: torch.device) -> int:

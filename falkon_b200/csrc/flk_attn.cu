@@ -366,6 +366,12 @@ int flk_attention_status(void* stream, int* out) {
   return FLK_OK;
 }
 
+int flk_attention_wait_limit(int64_t ns) {
+  if (ns < 0 || ns > 2000000000) return fail(FLK_ERR_BAD_ARG, "wait limit %lld: 0 to 2e9 ns", (long long)ns);
+  attn::g_wait_limit.store((uint32_t)ns, std::memory_order_relaxed);
+  return FLK_OK;
+}
+
 int flk_attention_backward(const flk_attention_args* p, void* stream) {
   FLK_TRY(attn::check_sizes(p));
   const int es = attn::esize_of(p->dtype);

@@ -135,14 +135,16 @@ __device__ __forceinline__ void store_partial(uint32_t acc, int c0, float f, boo
         if (to != nullptr && c0 + 4 * p < d) *reinterpret_cast<uint4*>(to + c0 + 4 * p) = v;
       });
 }
+// A quarter of a row of one value, zero or NaN (`row`: 16-bit values; `part`: fp32 partial results, unless null)
 template <typename T, int DP>
-__device__ __forceinline__ void store_zeros(int c0, bool exists, int d, T* row, float* part) {
+__device__ __forceinline__ void store_same(bool nan, int c0, bool exists, int d, T* row, float* part) {
   if (!exists) return;
+  const uint4 v = nan ? nan_piece() : make_uint4(0, 0, 0, 0);
   for (int c = c0; c < c0 + DP / 4 && c < d; c += 8) {
     if (part != nullptr)
-      *reinterpret_cast<uint4*>(part + c) = *reinterpret_cast<uint4*>(part + c + 4) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(part + c) = *reinterpret_cast<uint4*>(part + c + 4) = v;
     else
-      *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(row + c) = v;
   }
 }
 
@@ -186,10 +188,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   const uint32_t base = smem_u32(raw), bars = base + L::kBars;
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + 64 + s * 8; };
-  const uint32_t own = bars + 128, sfull = bars + 136, pfull = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176;
+  const uint32_t own = bars + 128, sfull = bars + 136, pfull = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, drained = bars + 184;
   auto statfull = [&](int s) { return bars + 192 + s * 8; };
   auto statempty = [&](int s) { return bars + 224 + s * 8; };
   const uint32_t slots = bars + 256, hollows = bars + 512;  // 128 bits per slot: rows of the tile that see nothing
+  auto wait = [&](uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, t.wait_ns); };
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
@@ -229,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   if (warp == kLoadWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-      mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 16), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
+      mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 16), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1), mbar_init(drained, 1);
       for (int s = 0; s < kStatSlots; ++s) mbar_init(statfull(s), 1), mbar_init(statempty(s), 16);
       tc::fence_barrier_init();
     }
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
 #pragma unroll
         for (int qo = 0; qo < 2; ++qo) {
           const int s = n % kStages;
-          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (n >= kStages) ok = ok && wait(empty(s), (uint32_t)(n / kStages - 1) & 1);
           if (!ok) break;
           if (elect_one()) {
             if (qo == 0) {
@@ -298,8 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           ++n;
         }
       }
-      if (steps > 0) wait_bar(own, 0);
-      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+      if (steps > 0) drain_bar(own, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) drain_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
     } else if (warp >= kStatWarp) {
       // two warps take turns; all loads of a step are under way at once
       bool ok = true;
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           label[x] = qd != nullptr && exists ? __ldg(qd + i) : -2;
           if constexpr (BIAS) slope[x] = a.slopes != nullptr ? __ldg(a.slopes + h) : 0.f;
         }
-        if (step >= kStatSlots) ok = wait_bar(statempty(slot), (uint32_t)(step / kStatSlots - 1) & 1);
+        if (step >= kStatSlots) ok = wait(statempty(slot), (uint32_t)(step / kStatSlots - 1) & 1);
         if (!ok) break;
         const uint32_t at = base + L::kStatAt + slot * kStatWords * 4;
 #pragma unroll
@@ -344,9 +347,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         __syncwarp();
       }
     } else if (warp == kMmaWarp) {
-      bool ok = steps == 0 || wait_bar(own, 0);
+      bool ok = steps == 0 || (t.wait_ns != 0 && wait(own, 0));
       auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
-      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      auto ready = [&](int n) { return wait(full(n % kStages), (uint32_t)(n / kStages) & 1); };
       auto arrived = [&](int n) {
         if (!ready(n)) return false;
         if (get_tile(slots, n / 2).dirty)
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       for (int i = 0; i < steps && ok; ++i) {
         const bool more = i + 1 < steps;
-        ok = wait_bar(pfull, (uint32_t)i & 1);
+        ok = wait(pfull, (uint32_t)i & 1);
         tc_fence_after();
         if (ok && elect_one()) {
           issue_weighted<T, DP, 32>(tdv, ts, stage(2 * i + 1), i > 0);
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           }
           __syncwarp();
         }
-        ok = ok && wait_bar(dsfull, (uint32_t)i & 1);
+        ok = ok && wait(dsfull, (uint32_t)i & 1);
         tc_fence_after();
         if (ok && elect_one()) {
           issue_weighted<T, DP, 32>(tdk, tp, stage(2 * i), i > 0);
@@ -409,11 +412,12 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           __syncwarp();
         }
       }
-      if (steps > 0 && ok) {
-        if (elect_one()) mma_commit(done);
-        __syncwarp();
-        wait_bar(done, 0);
-      }
+      if (steps > 0 && ok && elect_one()) mma_commit(done);
+      __syncwarp();
+      // no product may run, and no arrival come, after the block has gone
+      if (elect_one()) mma_commit(drained);
+      __syncwarp();
+      drain_bar(drained, 0);
     }
   } else {
     tc::reg_claim<kRegsWork>();
@@ -430,8 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     for (int i = 0; i < steps && ok; ++i) {
       const int slot = i % kStatSlots;
       const uint32_t st = base + L::kStatAt + slot * kStatWords * 4 + mine0 * 4;
-      ok = wait_bar(statfull(slot), (uint32_t)(i / kStatSlots) & 1);
-      ok = ok && wait_bar(sfull, (uint32_t)i & 1);
+      ok = wait(statfull(slot), (uint32_t)(i / kStatSlots) & 1);
+      ok = ok && wait(sfull, (uint32_t)i & 1);
       if (!ok) break;
       tc_fence_after();
       const Tile e = get_tile(slots, i);
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       __syncwarp();
       if (elect_one()) mbar_arrive(pfull);
       __syncwarp();
-      ok = wait_bar(dpfull, (uint32_t)i & 1);
+      ok = wait(dpfull, (uint32_t)i & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t d[32];
@@ -529,9 +533,9 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       __syncwarp();
     }
-    if (steps > 0 && ok) ok = wait_bar(done, 0);
+    if (steps > 0 && ok) ok = wait(done, 0);
     tc_fence_after();
-    if (ok) {
+    {
       const bool exists = key < a.nk;
       const bool zero = key >= lim.len || (kd != nullptr && my < 0);  // keys that nobody sees
       const int c0 = w * (DP / 4);
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
         pk = t.part_o + (int64_t)split * 2 * n + at;
         pv = pk + n;
       }
-      if (steps > 0) {
+      if (ok && steps > 0) {
         // the ring is free: all products are done, and with them all copies
         const uint32_t room = base + L::kRing + warp * 4096;
         const int lane = threadIdx.x & 31, first = key - lane, rows = a.nk - first;
@@ -556,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           store_quarter<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, zero, a.d, room, [&](int r) { return r < rows ? rv + (r - lane) * a.dv.sn : nullptr; });
         }
       } else {
-        store_zeros<T, DP>(c0, exists, a.d, rk, pk);
-        store_zeros<T, DP>(c0, exists, a.d, rv, pv);
+        store_same<T, DP>(!ok, c0, exists, a.d, rk, pk);
+        store_same<T, DP>(!ok, c0, exists, a.d, rv, pv);
       }
     }
     tc_fence_before();
@@ -604,7 +608,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   auto full = [&](int s) { return bars + s * 8; };
   auto empty = [&](int s) { return bars + 64 + s * 8; };
   auto sfull = [&](int s) { return bars + 128 + s * 8; };
-  const uint32_t own = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, slots = bars + 256;
+  const uint32_t own = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, drained = bars + 184, slots = bars + 256;
+  auto wait = [&](uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, t.wait_ns); };
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
 
@@ -638,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   if (warp == kLoadWarp) {
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-      mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1);
+      mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1), mbar_init(drained, 1);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -677,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int s = n % kStages;
-          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (n >= kStages) ok = ok && wait(empty(s), (uint32_t)(n / kStages - 1) & 1);
           if (!ok) break;
           if (elect_one()) {
             if (kv == 0) put_tile(slots, step, e);
@@ -690,12 +695,12 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
           ++n;
         }
       }
-      if (steps > 0) wait_bar(own, 0);
-      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+      if (steps > 0) drain_bar(own, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) drain_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
     } else if (warp == kMmaWarp) {
-      bool ok = steps == 0 || wait_bar(own, 0);
+      bool ok = steps == 0 || (t.wait_ns != 0 && wait(own, 0));
       auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
-      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      auto ready = [&](int n) { return wait(full(n % kStages), (uint32_t)(n / kStages) & 1); };
       // keys that nobody may see: their weights are zero, and what these meet, dP and K, has to be finite
       auto arrived = [&](int n) {
         if (!ready(n)) return false;
@@ -726,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       };
       if (steps > 0) ok = ok && scores(0) && products(0) && (steps == 1 || scores(1));
       for (int i = 0; i < steps && ok; ++i) {
-        ok = wait_bar(dsfull, (uint32_t)i & 1);
+        ok = wait(dsfull, (uint32_t)i & 1);
         tc_fence_after();
         if (i + 1 < steps) ok = ok && products(i + 1);
         if (ok && elect_one()) {
@@ -737,11 +742,12 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         __syncwarp();
         if (i + 2 < steps) ok = ok && scores(i + 2);
       }
-      if (steps > 0 && ok) {
-        if (elect_one()) mma_commit(done);
-        __syncwarp();
-        wait_bar(done, 0);
-      }
+      if (steps > 0 && ok && elect_one()) mma_commit(done);
+      __syncwarp();
+      // no product may run, and no arrival come, after the block has gone
+      if (elect_one()) mma_commit(drained);
+      __syncwarp();
+      drain_bar(drained, 0);
     }
   } else {
     tc::reg_claim<kRegsWork>();
@@ -758,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     const float add = lse == -INFINITY ? -INFINITY : -lse * kLog2e, nd = lse == -INFINITY ? 0.f : -delta * gs;
     bool ok = true;
     for (int step = 0; step < steps && ok; ++step) {
-      ok = wait_bar(sfull(step & 1), (uint32_t)(step >> 1) & 1);
+      ok = wait(sfull(step & 1), (uint32_t)(step >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
       const Tile e = get_tile(slots, step);
@@ -791,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         for (int c = 0; c < 32; ++c)
           if ((seen & (1u << c)) == 0) s[0][c] = 0;
       }
-      ok = wait_bar(dpfull, (uint32_t)step & 1);
+      ok = wait(dpfull, (uint32_t)step & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t d[32];
@@ -818,19 +824,19 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       if (elect_one()) mbar_arrive(dsfull);
       __syncwarp();
     }
-    if (steps > 0 && ok) ok = wait_bar(done, 0);
+    if (steps > 0 && ok) ok = wait(done, 0);
     tc_fence_after();
-    if (ok) {
+    {
       T* row = reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.sn + h * a.dq.sh;
       const int c0 = w * (DP / 4);
-      if (steps > 0)
+      if (ok && steps > 0)
         store_quarter<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, add == -INFINITY, a.d, base + L::kRing + warp * 4096, [&](int e) {
           const int rr = r - (int)(threadIdx.x & 31) + e;
           return rr < t.rows ? reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)(rr >> t.pg_shift) * a.dq.sn + (hp * t.pg + (rr & (t.pg - 1))) * a.dq.sh
                              : nullptr;
         });
       else
-        store_zeros<T, DP>(c0, exists, a.d, row, nullptr);
+        store_same<T, DP>(!ok, c0, exists, a.d, row, nullptr);
     }
     tc_fence_before();
   }
@@ -908,6 +914,7 @@ inline int launch_some(const Maps& m, const TcArgs& t, cudaStream_t st) {
 template <typename T>
 inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
+  t.wait_ns = wait_limit();
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
   t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.q_blocks, t.splits = p.splits;
   t.tanh = make_tanh(a.scale);

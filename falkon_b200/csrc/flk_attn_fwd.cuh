@@ -95,8 +95,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto sfull = [&](int w) { return bars + 128 + w * 8; };
   auto pfull = [&](int w) { return bars + 144 + w * 8; };
   auto odone = [&](int w) { return bars + 160 + w * 8; };
-  const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320, halves = bars + 512;
+  const uint32_t qfull = bars + 176, tmem_at = bars + 184, slots = bars + 192, place = bars + 320, drained = bars + 400, halves = bars + 512;
   auto xbar = [&](int w) { return bars + 384 + w * 8; };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, t.wait_ns); };
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
 
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 8), mbar_init(odone(w), 1), mbar_init(xbar(w), 8);
-      mbar_init(qfull, 1);
+      mbar_init(qfull, 1), mbar_init(drained, 1);
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place + 16), "r"(lim.len), "r"(lim.start), "r"(lim.prefix), "r"(0) : "memory");
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(hp), "r"(b), "r"(split), "r"(row0) : "memory");
       tc::fence_barrier_init();
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int s = n % kStages;
-          if (n >= kStages) ok = ok && wait_bar(empty(s), (uint32_t)(n / kStages - 1) & 1);
+          if (n >= kStages) ok = ok && wait(empty(s), (uint32_t)(n / kStages - 1) & 1);
           if (!ok) break;
           if (elect_one()) {
             if (kv == 0) put_tile(slots, step, e);
@@ -190,12 +191,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // no copy may land after the block has gone
-      if (steps > 0) wait_bar(qfull, 0);
-      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) wait_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
+      if (steps > 0) drain_bar(qfull, 0);
+      for (int i = n > kStages ? n - kStages : 0; i < n; ++i) drain_bar(full(i % kStages), (uint32_t)(i / kStages) & 1);
     } else if (warp == kMmaWarp) {
-      bool ok = steps == 0 || wait_bar(qfull, 0);
+      bool ok = steps == 0 || (t.wait_ns != 0 && wait(qfull, 0));
       auto stage = [&](int n) { return base + L::kRing + (uint32_t)(n % kStages) * L::kTileBytes; };
-      auto ready = [&](int n) { return wait_bar(full(n % kStages), (uint32_t)(n / kStages) & 1); };
+      auto ready = [&](int n) { return wait(full(n % kStages), (uint32_t)(n / kStages) & 1); };
       auto clean = [&](int step) {
         const Tile e = get_tile(slots, step);
         if (e.dirty || (e.at + 1) * kTile > lim.len) clean_tile<DP>(stage(2 * step + 1), e.at * kTile, lim.len, kd);
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ready(2 * i + 1);
           if (ok) clean(i);
           for (int w = 0; w < 2 && ok; ++w) {
-            ok = wait_bar(pfull(w), (uint32_t)i & 1);
+            ok = wait(pfull(w), (uint32_t)i & 1);
             if (ok && w == 0 && more) ok = ready(2 * i + 2);
             tc_fence_after();
             if (ok && elect_one()) {
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ok = ok && ready(2 * i + 1);
           if (ok) clean(i);
-          ok = ok && wait_bar(pfull(w), (uint32_t)(i >> 1) & 1);
+          ok = ok && wait(pfull(w), (uint32_t)(i >> 1) & 1);
           tc_fence_after();
           if (ok && elect_one()) {
             issue_weighted<T, DP, 64>(to(w), ts(w), stage(2 * i + 1), i > 1);
@@ -265,11 +266,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(odone(1));
       }
       __syncwarp();
-      // no arrival may come after the block has gone
-      if (steps > 0 && ok) {
-        wait_bar(odone(0), 0);
-        wait_bar(odone(1), 0);
-      }
+      // no product may run, and no arrival come, after the block has gone
+      if (elect_one()) mma_commit(drained);
+      __syncwarp();
+      drain_bar(drained, 0);
     }
   } else {
     tc::reg_claim<kRegsSoftmax>();
@@ -305,13 +305,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (elect_one()) mbar_arrive(xbar(w));
       __syncwarp();
-      const bool ok = wait_bar(xbar(w), phase & 1);
+      const bool ok = wait(xbar(w), phase & 1);
       ++phase;
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(theirs) : "r"(other) : "memory");
       return ok;
     };
     for (int step = PAIR ? 0 : w; step < steps; step += PAIR ? 1 : 2) {
-      ok = wait_bar(sfull(w), (uint32_t)(PAIR ? step : step >> 1) & 1);
+      ok = wait(sfull(w), (uint32_t)(PAIR ? step : step >> 1) & 1);
       if (!ok) break;
       if (!live) {  // the weights of rows that do not exist reach nothing
         if (elect_one()) {
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool worked = steps > (PAIR ? 0 : w);
     if (worked && ok) {
       // the products being done, all warps of the tile have passed the last step's exchange
-      ok = wait_bar(odone(w), 0);
+      ok = wait(odone(w), 0);
       // both sums, through what was the ring (behind what the stores below use)
       const uint32_t sums = base + L::kRing + 65536;
       static_assert(L::kStages * L::kTileBytes >= 65536 + 512 * 8, "ring");
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (elect_one()) mbar_arrive(xbar(w));
       __syncwarp();
-      ok = ok && wait_bar(xbar(w), phase & 1);
+      ok = ok && wait(xbar(w), phase & 1);
       float x, y;
       asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(sums + (threadIdx.x ^ 128) * 8) : "memory");
       l = side == 0 ? l + x : x + l;  // the same sums on both sides
@@ -438,6 +438,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     // nothing seen: all weights were zero (a score that is not a number makes the sums, and so the row, NaN)
     const bool none = l == 0.f;
+    if (live && !ok) {  // the joining kernel makes a row of parts NaN by the part's log-sum-exp alone
+      const int4 at = get_place(place);
+      const int hp = at.x, b = at.y, split = at.z, r = at.w + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
+      const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
+      if (r < t.rows && (!PAIR || t.splits > 1)) {
+        t.part_lse[(((int64_t)(PAIR ? split : 2 * split + w) * a.b + b) * t.hp + hp) * t.rows + r] = NAN;
+      } else if (r < t.rows) {
+        if (a.lse != nullptr) a.lse[((int64_t)b * a.hq + h) * a.nq + i] = NAN;
+        const int64_t row = b * a.o.sb + (int64_t)i * a.o.sn + h * a.o.sh;
+        for (int c = 0; c < a.d; c += 8) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.o.p) + row + c) = nan_piece();
+          if (a.o_lo != nullptr) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.o_lo) + row + c) = nan_piece();
+        }
+      }
+    }
     const float inv = none ? 0.f : 1.0f / lr, lse2 = none ? -INFINITY : m + log2f(l);
     if (live && ok) {
       // read again instead of held in registers through the loop above
@@ -644,6 +659,7 @@ inline int launch_join(const TcArgs& t, int parts, cudaStream_t st) {
 template <typename T>
 inline int launch(TcArgs t, const Plan& p, cudaStream_t st) {
   const Args& a = t.a;
+  t.wait_ns = wait_limit();
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? FLK_BF16 : FLK_F16;
   t.pg = p.pg, t.pg_shift = p.pg_shift, t.hp = p.hp, t.rows = p.rows, t.blocks = p.blocks, t.splits = p.splits;
   t.tanh = make_tanh(a.scale);

@@ -10,8 +10,8 @@
 // query r / pg of head r % pg.  A key tile then meets pg times as many rows, and the triangle of a causal mask is cut in
 // steps pg times as fine.
 //
-// Every wait on a barrier is bounded; when one gives up, the block records a code, stops issuing work, lets its copies
-// land, frees its tensor memory and returns.
+// Every wait on a barrier is bounded; when one gives up, the block records it, stops issuing work, lets its copies land and its
+// products end, makes the rows that it cannot finish NaN, frees its tensor memory and returns.
 #pragma once
 
 #include <cuda.h>
@@ -29,7 +29,6 @@ using tc::elect_one;
 using tc::mbar_arrive;
 using tc::mbar_expect_tx;
 using tc::mbar_init;
-using tc::mbar_try_wait;
 using tc::mma_commit;
 using tc::smem_u32;
 using tc::tc_fence_after;
@@ -42,20 +41,38 @@ using tc::tmem_relinquish;
 
 constexpr uint32_t kBlockBytes = kTile * 128;  // 128 rows x 64 columns of 16 bits
 
-// Set by a kernel whose bounded wait gave up (one word per translation unit).
-static __device__ int g_wait_status;
+// Set by a kernel whose bounded wait gave up (one word per translation unit), and what it was when it was last asked for.
+static __device__ int g_wait_status, g_wait_taken;
 
-// A waiting warp looks again without sleeping: the other roles of the block wait for what it does next.
-static __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+// Whether the barrier has passed the phase, the same answer for all lanes of a warp.  May suspend the warp for a while.
+__device__ __forceinline__ bool passed(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred q, p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A whole warp waits, and all of its lanes get the same answer: roles elect a lane for their work, which takes all of them.  A
+// waiting warp looks again without sleeping: the other roles of the block wait for what it does next.
+static __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t limit_ns) {
+  if (passed(bar, parity)) return true;
   const uint32_t t0 = tc::timer_lo_ns();
   for (uint32_t it = 0; it < (1u << 28); ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 15) == 15 && tc::timer_lo_ns() - t0 > 1000000000u) break;
+    if (passed(bar, parity)) return true;
+    if ((it & 15) == 15 && __any_sync(0xffffffffu, tc::timer_lo_ns() - t0 >= limit_ns)) break;
   }
   atomicExch(&g_wait_status, 1);
   return false;
 }
+// What a block waits for before it ends, whatever limit its other waits have: copies that are still to land in its shared memory,
+// products that are still to read that and to write its tensor memory.
+constexpr uint32_t kDrainNs = 1000000000u;
+static __device__ __forceinline__ bool drain_bar(uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, kDrainNs); }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
@@ -294,6 +311,9 @@ __device__ __forceinline__ void store_rows32(uint32_t room, Piece piece, Put put
   __syncwarp();
 }
 
+// 16 bytes of NaN in any of the types
+__device__ __forceinline__ uint4 nan_piece() { return make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu); }
+
 // What the tensor-core kernels need on top of Args.
 struct TcArgs {
   Args a;
@@ -307,6 +327,7 @@ struct TcArgs {
   // the order in which the row blocks (backward: the key tiles) of all sequences start: sequence * blocks + block, or null
   const int* order;
   const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
+  uint32_t wait_ns;      // limit of a wait; 0: the issuing warp gives up before its first product
 };
 
 // The tiles of [first, last) that a block has to look at: all of them or, with documents, those whose labels overlap [lo, hi].
@@ -446,6 +467,10 @@ __device__ __forceinline__ LabelRange labels_of(const int* docs, int i0, int i1)
 // ---------------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
+// Limit of a wait in the calls that follow, in ns (flk_attention_wait_limit).
+inline std::atomic<uint32_t> g_wait_limit{1000000000u};
+inline uint32_t wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -475,9 +500,13 @@ inline int make_map(CUtensorMap* m, const Tensor4& t, int dtype, int d, int h, i
   return FLK_OK;
 }
 
-// The status word of this translation unit's kernels; waits for the stream.
+// The status word of this translation unit's kernels, which goes back to 0; waits for the stream.
+static __global__ void take_status_kernel() { g_wait_taken = atomicExch(&g_wait_status, 0); }
 static int read_wait_status(cudaStream_t st, int* out) {
-  FLK_CUDA_TRY(cudaMemcpyFromSymbolAsync(out, g_wait_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  take_status_kernel<<<1, 1, 0, st>>>();
+  count_launch();
+  FLK_CUDA_TRY(cudaGetLastError());
+  FLK_CUDA_TRY(cudaMemcpyFromSymbolAsync(out, g_wait_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
   FLK_CUDA_TRY(cudaStreamSynchronize(st));
   return FLK_OK;
 }

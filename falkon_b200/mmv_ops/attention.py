@@ -191,7 +191,8 @@ def attention(
     read on the device: lengths beyond [0, Nk] count as the nearer end.  At most 65535 sequences, 65535 heads, 2^29 rows.
     Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates its output
     and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has it for every
-    operator, only while no graph of the same leaves that was built outside of the capture is alive).
+    operator, only while no graph of the same leaves that was built outside of the capture is alive).  With 16-bit data every wait
+    inside a kernel is bounded: rows that a stalled GPU does not finish within a second are NaN, and so are their gradients.
     """
     try:
         fits = q.dtype is k.dtype is v.dtype and q.dtype in _lib._ROW_TYPES and k.shape == v.shape and q.device == k.device == v.device

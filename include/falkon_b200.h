@@ -306,9 +306,13 @@ int64_t flk_attention_workspace_bytes(const flk_attention_args* args, int backwa
 int flk_attention_forward(const flk_attention_args* args, void* stream);
 int flk_attention_backward(const flk_attention_args* args, void* stream);
 
-/* 0, or 1 when a bounded wait of a tensor-core attention kernel has given up on the current device since the library was
- * loaded (the results of that call are not valid).  Synchronises the stream. */
+/* 0, or 1 when a bounded wait of a tensor-core attention kernel has given up on the current device since the last query (the
+ * rows that the block could not finish are NaN then, their log-sum-exp and gradients too).  Synchronises the stream. */
 int flk_attention_status(void* stream, int* status_out);
+
+/* Limit of such a wait in the calls that follow from this process, in ns: 0 to 2e9, at first 1e9.  A GPU that is shared in time
+ * slices longer than that needs more; with 0 every block that has work gives up (to test what handles it). */
+int flk_attention_wait_limit(int64_t ns);
 
 /*
  * Layer norm of rows (no counterpart in the reference):
