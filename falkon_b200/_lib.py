@@ -41,8 +41,8 @@ PTXAS_REPORT = LIB_PATH + ".ptxas.txt"
 TC_LAUNCH_REGISTERS = 80
 # Registers per thread that the attention kernels (20 warps) are launched with and re-partition:
 ATTENTION_LAUNCH_REGISTERS = 96
-# Most of them spill a few scalars that are stored once and read in several places; a row's scores are read with asynchronous
-# loads too, but there the wait follows at once, so none is in flight where a register is spilled.
+# Most of them spill a few scalars that are stored once and read in several places.  Their asynchronous loads have the wait in the
+# same statement, so no register is in flight where another is spilled.
 ATTENTION_SPILL_ALLOWANCE = (64, 144)
 # A few instantiations of the K-loop kernel still spill one or two 32-bit values that are stored once before the
 # warp roles split (none inside a tile loop); the build tolerates up to this many bytes of spill stores / loads

@@ -98,10 +98,10 @@ template <typename T, int DP, typename At>
 __device__ __forceinline__ void store_quarter(uint32_t acc, int c0, float f, bool zero, int d, uint32_t room, At at) {
   constexpr int kWords = DP / 4;
   uint32_t o[kWords];
-#pragma unroll
-  for (int c = 0; c < kWords; c += 16) tc::tmem_ld16(acc + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
-#pragma unroll
-  for (int c = 0; c < kWords; c += 16) tmem_ld_wait_on(*reinterpret_cast<uint32_t(*)[16]>(o + c));
+  if constexpr (kWords == 16)
+    tmem_read16(acc + c0, o);
+  else
+    tmem_read32(acc + c0, o);
 #pragma unroll
   for (int e = 0; e < kWords; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
   store_rows32<kWords / 8>(
@@ -122,10 +122,10 @@ template <int DP, typename At>
 __device__ __forceinline__ void store_partial(uint32_t acc, int c0, float f, bool zero, int d, uint32_t room, At at) {
   constexpr int kWords = DP / 4;
   uint32_t o[kWords];
-#pragma unroll
-  for (int c = 0; c < kWords; c += 16) tc::tmem_ld16(acc + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(o + c));
-#pragma unroll
-  for (int c = 0; c < kWords; c += 16) tmem_ld_wait_on(*reinterpret_cast<uint32_t(*)[16]>(o + c));
+  if constexpr (kWords == 16)
+    tmem_read16(acc + c0, o);
+  else
+    tmem_read32(acc + c0, o);
 #pragma unroll
   for (int e = 0; e < kWords; ++e) o[e] = zero ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
   store_rows32<kWords / 4>(
@@ -454,8 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       }
       uint32_t s[1][32];
       uint32_t pr[32];
-      tmem_ld32(ts + lane_at + mine0, s[0]);
-      tmem_ld_wait_on(s[0]);
+      tmem_read32(ts + lane_at + mine0, s[0]);
       if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
@@ -500,8 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       if (!ok) break;
       tc_fence_after();
       uint32_t d[32];
-      tmem_ld32(tp + lane_at + mine0, d);
-      tmem_ld_wait_on(d);
+      tmem_read32(tp + lane_at + mine0, d);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[4], lo[4];
@@ -777,8 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       }
       uint32_t s[1][32];
       const uint32_t at = ts(step) + lane_at + mine0;
-      tmem_ld32(at, s[0]);
-      tmem_ld_wait_on(s[0]);
+      tmem_read32(at, s[0]);
       const float d0 = (float)(pos - k0 - (int)mine0);
       if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
 #pragma unroll
@@ -801,8 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       if (!ok) break;
       tc_fence_after();
       uint32_t d[32];
-      tmem_ld32(tp + lane_at + mine0, d);
-      tmem_ld_wait_on(d);
+      tmem_read32(tp + lane_at + mine0, d);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[4], lo[4];

@@ -330,10 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = k0 + 64 <= all_before && (a.kdocs == nullptr || (e.label >= 0 && e.label == only));
       uint32_t s[2][32];
       const uint32_t at = ts(w) + lane_at + 64 * side;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld32(at + 32 * p, s[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tmem_ld_wait_on(s[p]);
+      tmem_read64(at, s[0], s[1]);
       if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
       if constexpr (BIAS) add_bias(s, f2, slope2, (float)(pos - k0));
       if (!whole) {
@@ -374,8 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = side * (DP / 2); c < (side + 1) * (DP / 2); c += 16) {
             uint32_t o[16];
-            tc::tmem_ld16(to(w) + lane_at + c, o);
-            tmem_ld_wait_on(o);
+            tmem_read16(to(w) + lane_at + c, o);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             tmem_st16(to(w) + lane_at + c, o);
@@ -476,10 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = side * (DP / 2); c < (side + 1) * (DP / 2) && (worked || !parts); c += 32) {
         uint32_t o[32];
-        if (worked) {
-          tmem_ld32(to(w) + lane_at + c, o);
-          tmem_ld_wait_on(o);
-        }
+        if (worked) tmem_read32(to(w) + lane_at + c, o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
         if (parts) {
