@@ -43,7 +43,7 @@ TC_LAUNCH_REGISTERS = 80
 ATTENTION_LAUNCH_REGISTERS = 96
 # Most of them spill a few scalars that are stored once and read in several places.  Their asynchronous loads have the wait in the
 # same statement, so no register is in flight where another is spilled.
-ATTENTION_SPILL_ALLOWANCE = (64, 144)
+ATTENTION_SPILL_ALLOWANCE = (64, 152)
 # A few instantiations of the K-loop kernel still spill one or two 32-bit values that are stored once before the
 # warp roles split (none inside a tile loop); the build tolerates up to this many bytes of spill stores / loads
 # there and fails beyond (a regression guard, not an endorsement).

@@ -214,7 +214,7 @@ static int64_t ordered(const flk_attention_args* p, bool backward) {
 }
 
 struct Workspace {
-  int64_t qdocs, kdocs, qtab, ktab, order, delta, amax, part_o, part_lse, total;
+  int64_t qdocs, kdocs, qtab, ktab, order, delta, part_o, part_lse, total;
 };
 static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
   Workspace w{};
@@ -233,7 +233,6 @@ static Workspace plan_workspace(const flk_attention_args* p, bool backward) {
   }
   if (backward) {
     w.delta = take(p->batch * p->hq * p->nq * 4);
-    w.amax = take(8);
     if (on_tensor_cores(p)) w.part_o = take(bwd::partial_floats(backward_plan(p), p->batch, p->nk, p->hk, p->d) * 4);
   }
   if (!backward && p->batch > 0 && p->nq > 0 && p->nk > 0) {
@@ -408,16 +407,14 @@ int flk_attention_backward(const flk_attention_args* p, void* stream) {
     FLK_TRY(attn::launch_order(p, true, reinterpret_cast<int*>(ws + w.order), t, st));
     const attn::bwd::Plan plan = attn::backward_plan(p);
     if (p->dtype == FLK_BF16) {
-      FLK_TRY(attn::launch_delta<__nv_bfloat16>(a, nullptr, st));
+      FLK_TRY(attn::launch_delta<__nv_bfloat16>(a, st));
       FLK_TRY(attn::backward_bf16(t, plan, st));
     } else {
-      uint32_t* amax = reinterpret_cast<uint32_t*>(ws + w.amax);
-      t.amax = amax;
-      FLK_TRY(attn::launch_delta<__half>(a, amax, st));  // and the magnitudes that the scale of dS is taken from
+      FLK_TRY(attn::launch_delta<__half>(a, st));
       FLK_TRY(attn::backward_f16(t, plan, st));
     }
   } else {
-    FLK_TRY(attn::launch_delta<float>(a, nullptr, st));
+    FLK_TRY(attn::launch_delta<float>(a, st));
     FLK_TRY(a.d <= 64 ? attn::simt::launch_backward<64>(a, st) : attn::simt::launch_backward<128>(a, st));
   }
   FLK_CUDA_TRY(cudaGetLastError());

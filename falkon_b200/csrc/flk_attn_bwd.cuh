@@ -17,8 +17,10 @@
 // 2.5 k with 64: the chain product - exponentials - product, 16 warps on one tile; a block's start takes 2 to 5 k, its end 3 k.
 //
 // P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass.  In fp16 they would
-// leave its range: weights are held times 2^12, and dS times a power of two that 2 d max|dO| max|V|, a bound of every
-// |dP - delta|, takes to at most 2^15.
+// leave its range: weights are held times 2^12, and the dS of a row (a key in the one kernel, a query in the other) times a power
+// of two of its own, which follows what the row has met so far as a running maximum does: the first terms take it to 2^4, and
+// terms beyond 2^15 take the row's accumulator down with it.  So no row, sequence or head costs another one bits, and
+// terms lost to fp16's lower end are 2^-29 of the row's largest.
 //
 // The dS of a row add up to zero, so where a row has few keys the terms of dQ and dK cancel, and the rounding of dS would be the
 // largest error (up to 1.8 times that of rounding the result, for rows of ten keys).  With up to 256 queries and keys, where a
@@ -53,7 +55,8 @@ struct Layout {
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kStatAt = kRing + kStages * kTileBytes;
   static constexpr uint32_t kBars = kStatAt + kStats;
-  static constexpr uint32_t kBytes = kBars + 512 + (KEYS ? kSlots * 16 : 0);
+  static constexpr uint32_t kTops = kBars + 512 + (KEYS ? kSlots * 16 : 0);  // fp16: 4 x 128 words
+  static constexpr uint32_t kBytes = kTops + 2048;
 };
 static_assert(Layout<128, true>::kBytes <= 227 * 1024 && Layout<128, false>::kBytes <= 227 * 1024, "shared memory");
 static_assert(Layout<128, true>::kStages >= 4 && Layout<128, false>::kStages >= 5, "stages");
@@ -64,15 +67,47 @@ struct Scales {
   static constexpr bool kHalf = !std::is_same<T, __nv_bfloat16>::value;
   static constexpr float kShift = kHalf ? 12.f : 0.f;
   static constexpr float kUnshift = kHalf ? 1.f / 4096.f : 1.f;
-  // the factor that dS is held with, a power of two
-  static __device__ __forceinline__ float ds(const TcArgs& t) {
-    if (!kHalf) return 1.f;
-    const float bound = 2.f * (float)t.a.d * __uint_as_float(t.amax[0]) * __uint_as_float(t.amax[1]);
-    if (!(bound > 0.f && bound < 1e30f)) return 1.f;
-    const int e = (int)(__float_as_uint(bound) >> 23) - 127;  // 2^e <= bound < 2^(e+1)
-    return __uint_as_float((uint32_t)(127 + min(max(14 - e, -100), 100)) << 23);
-  }
 };
+
+// fp16: the factor of a row's dS, the same in the four threads that share the row.  They tell each other their largest value
+// through shared memory: a word per thread, one phase of an mbarrier per step and warp of the row.
+struct RowScale {
+  float now = 0.f;  // 0: all terms so far were zero
+  // Whether terms of up to `top` need another factor; if so, it is set, and `change` is what to multiply the accumulator with.
+  __device__ __forceinline__ bool follow(float top, float& change) {
+    change = 1.f;
+    if (now == 0.f ? top == 0.f : top * now <= 32768.f) return false;
+    const int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
+    const float next = __uint_as_float((uint32_t)(127 + min(max(4 - e, -120), 120)) << 23);
+    const bool scaled = now != 0.f;
+    if (scaled) change = next / now;
+    now = next;
+    return scaled;
+  }
+  // of the finished accumulator
+  __device__ __forceinline__ float undo(float scale) const { return now == 0.f ? scale : scale / now; }
+};
+__device__ __forceinline__ void put_top(uint32_t tops, int w, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(tops + (w * kTile + (threadIdx.x & 127)) * 4), "f"(v) : "memory");
+}
+__device__ __forceinline__ float largest_top(uint32_t tops) {
+  float v[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[w]) : "r"(tops + (w * kTile + (threadIdx.x & 127)) * 4) : "memory");
+  return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+}
+// A quarter of the rows' accumulators (DP / 4 columns) times `f`.
+template <int DP>
+__device__ __forceinline__ void rescale_quarter(uint32_t acc, float f) {
+#pragma unroll 1
+  for (int c = 0; c < DP / 4; c += 16) {
+    uint32_t o[16];
+    tmem_read16(acc + c, o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    tmem_st16(acc + c, o);
+  }
+}
 
 // What dS is made from later, in the place of the scores s0, s1: the weights, times 1 - tanh^2 where s is the tanh of a capped score
 template <bool CAP>
@@ -192,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
   auto statfull = [&](int s) { return bars + 192 + s * 8; };
   auto statempty = [&](int s) { return bars + 224 + s * 8; };
   const uint32_t slots = bars + 256, hollows = bars + 512;  // 128 bits per slot: rows of the tile that see nothing
+  auto xbar = [&](int q) { return bars + 384 + q * 8; };
   auto wait = [&](uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, t.wait_ns); };
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
@@ -233,6 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       mbar_init(own, 1), mbar_init(sfull, 1), mbar_init(pfull, 16), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1), mbar_init(drained, 1);
+      if constexpr (Scales<T>::kHalf)
+        for (int q = 0; q < 4; ++q) mbar_init(xbar(q), 4);
       for (int s = 0; s < kStatSlots; ++s) mbar_init(statfull(s), 1), mbar_init(statempty(s), 16);
       tc::fence_barrier_init();
     }
@@ -307,7 +345,6 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       // two warps take turns; all loads of a step are under way at once
       bool ok = true;
       StepWalk walk(qtab, first, last, lab.lo, lab.hi, per_head, skip);
-      const float g = Scales<T>::ds(t) * Scales<T>::kUnshift;
       for (int step = 0; step < steps && ok; ++step) {
         const Tile e = walk.next();
         if ((step & 1) != warp - kStatWarp) continue;
@@ -335,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           const bool none = lse[x] == -INFINITY;
           auto put = [&](int word, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + (word + c) * 4), "r"(v) : "memory"); };
           put(kLse, __float_as_uint(none ? -INFINITY : fmaf(-lse[x], kLog2e, Scales<T>::kShift)));  // added to the score
-          put(kDelta, __float_as_uint(none ? 0.f : -delta[x] * g));
+          put(kDelta, __float_as_uint(none ? 0.f : -delta[x] * Scales<T>::kUnshift));
           if constexpr (BIAS) {
             put(kSlope, __float_as_uint(-slope[x] * kLog2e));
             put(kPos, __float_as_uint((float)(lim.start + i - k0)));
@@ -429,7 +466,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
     const float f = CAP ? a.cap2 : a.scale;  // raw score, or its tanh -> base 2
-    const float gs = Scales<T>::ds(t), g = gs * Scales<T>::kUnshift;
+    RowScale row_scale;
+    // four dS from column c on, in the place of the weights
+    auto slopes_at = [&](int c, const uint32_t (&d)[32], uint32_t (&s)[32], uint32_t st, float (&y)[4]) {
+      float dl[4];
+      tc::ld_shared_f4(st + (kDelta + c) * 4, dl[0], dl[1], dl[2], dl[3]);
+#pragma unroll
+      for (int q = 0; q < 4; q += 2)
+        tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[c + q]), __uint_as_float(s[c + q + 1])),
+                             tc::fma2(tc::pack2(__uint_as_float(d[c + q]), __uint_as_float(d[c + q + 1])), both(Scales<T>::kUnshift), tc::pack2(dl[q], dl[q + 1]))),
+                    y[q], y[q + 1]);
+    };
     bool ok = true;
     for (int i = 0; i < steps && ok; ++i) {
       const int slot = i % kStatSlots;
@@ -500,18 +547,40 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       tc_fence_after();
       uint32_t d[32];
       tmem_read32(tp + lane_at + mine0, d);
+      if constexpr (Scales<T>::kHalf) {
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          float y[4];
+          slopes_at(c, d, s[0], st, y);
+          top = fmaxf(fmaxf(top, fabsf(y[0])), fabsf(y[1]));
+          top = fmaxf(fmaxf(top, fabsf(y[2])), fabsf(y[3]));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) s[0][c + q] = __float_as_uint(y[q]);
+        }
+        put_top(base + L::kTops, w, top);
+        __syncwarp();
+        if (elect_one()) mbar_arrive(xbar(warp & 3));
+        __syncwarp();
+        ok = wait(xbar(warp & 3), (uint32_t)i & 1);
+        if (!ok) break;
+        float change;
+        const bool changes = row_scale.follow(largest_top(base + L::kTops), change);
+        // dP of this step is here, and was issued behind dK of the last one: nothing works on the accumulator
+        if (__any_sync(0xffffffffu, changes) && i > 0) rescale_quarter<DP>(tdk + lane_at + w * (DP / 4), change);
+      }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[4], lo[4];
 #pragma unroll
         for (int c = 8 * p; c < 8 * p + 8; c += 4) {
-          float dl[4], y[4];
-          tc::ld_shared_f4(st + (kDelta + c) * 4, dl[0], dl[1], dl[2], dl[3]);
+          float y[4];
+          if constexpr (Scales<T>::kHalf) {
 #pragma unroll
-          for (int q = 0; q < 4; q += 2)
-            tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])),
-                                 tc::fma2(tc::pack2(__uint_as_float(d[c + q]), __uint_as_float(d[c + q + 1])), both(g), tc::pack2(dl[q], dl[q + 1]))),
-                        y[q], y[q + 1]);
+            for (int q = 0; q < 4; ++q) y[q] = __uint_as_float(s[0][c + q]) * row_scale.now;
+          } else {
+            slopes_at(c, d, s[0], st, y);
+          }
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
           o[c % 8 / 2 + 1] = pack16<T>(y[2], y[3]);
           if constexpr (FINE) {
@@ -548,13 +617,14 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
       if (ok && steps > 0) {
         // the ring is free: all products are done, and with them all copies
         const uint32_t room = base + L::kRing + warp * 4096;
+        const float undo = Scales<T>::kHalf ? row_scale.undo(a.scale_raw) : a.scale_raw;
         const int lane = threadIdx.x & 31, first = key - lane, rows = a.nk - first;
         if (pk != nullptr) {
           const int64_t step = (int64_t)a.hk * a.d;
-          store_partial<DP>(tdk + lane_at, c0, a.scale_raw / gs, zero, a.d, room, [&](int r) { return r < rows ? pk + (r - lane) * step : nullptr; });
+          store_partial<DP>(tdk + lane_at, c0, undo, zero, a.d, room, [&](int r) { return r < rows ? pk + (r - lane) * step : nullptr; });
           store_partial<DP>(tdv + lane_at, c0, Scales<T>::kUnshift, zero, a.d, room, [&](int r) { return r < rows ? pv + (r - lane) * step : nullptr; });
         } else {
-          store_quarter<T, DP>(tdk + lane_at, c0, a.scale_raw / gs, zero, a.d, room, [&](int r) { return r < rows ? rk + (r - lane) * a.dk.sn : nullptr; });
+          store_quarter<T, DP>(tdk + lane_at, c0, undo, zero, a.d, room, [&](int r) { return r < rows ? rk + (r - lane) * a.dk.sn : nullptr; });
           store_quarter<T, DP>(tdv + lane_at, c0, Scales<T>::kUnshift, zero, a.d, room, [&](int r) { return r < rows ? rv + (r - lane) * a.dv.sn : nullptr; });
         }
       } else {
@@ -607,6 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
   auto empty = [&](int s) { return bars + 64 + s * 8; };
   auto sfull = [&](int s) { return bars + 128 + s * 8; };
   const uint32_t own = bars + 144, dpfull = bars + 152, dsfull = bars + 160, done = bars + 168, tmem_at = bars + 176, drained = bars + 184, slots = bars + 256;
+  auto xbar = [&](int q) { return bars + 384 + q * 8; };
   auto wait = [&](uint32_t bar, uint32_t parity) { return wait_bar(bar, parity, t.wait_ns); };
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x < 4) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : threadIdx.x == 2 ? &maps.q : &maps.dout);
@@ -642,6 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     if (elect_one()) {
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       mbar_init(own, 1), mbar_init(sfull(0), 1), mbar_init(sfull(1), 1), mbar_init(dpfull, 1), mbar_init(dsfull, 16), mbar_init(done, 1), mbar_init(drained, 1);
+      if constexpr (Scales<T>::kHalf)
+        for (int q = 0; q < 4; ++q) mbar_init(xbar(q), 4);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -757,9 +830,10 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     const int all_before = lim.row_end(i0, a.causal);
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;
-    const float f = CAP ? a.cap2 : a.scale, gs = Scales<T>::ds(t);
+    const float f = CAP ? a.cap2 : a.scale;
+    RowScale row_scale;
     // a row that sees nothing has no weights, and no delta, which may be NaN there
-    const float add = lse == -INFINITY ? -INFINITY : -lse * kLog2e, nd = lse == -INFINITY ? 0.f : -delta * gs;
+    const float add = lse == -INFINITY ? -INFINITY : -lse * kLog2e, nd = lse == -INFINITY ? 0.f : -delta;
     bool ok = true;
     for (int step = 0; step < steps && ok; ++step) {
       ok = wait(sfull(step & 1), (uint32_t)(step >> 1) & 1);
@@ -799,15 +873,50 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       tc_fence_after();
       uint32_t d[32];
       tmem_read32(tp + lane_at + mine0, d);
+      auto slopes_at = [&](int c, float (&y)[2]) {  // two dS, in the place of the weights
+        tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])),
+                             tc::add2(tc::pack2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), both(nd))),
+                    y[0], y[1]);
+      };
+      if constexpr (Scales<T>::kHalf) {
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float y[2];
+          slopes_at(c, y);
+          top = fmaxf(fmaxf(top, fabsf(y[0])), fabsf(y[1]));
+          s[0][c] = __float_as_uint(y[0]);
+          s[0][c + 1] = __float_as_uint(y[1]);
+        }
+        put_top(base + L::kTops, w, top);
+        __syncwarp();
+        if (elect_one()) mbar_arrive(xbar(warp & 3));
+        __syncwarp();
+        ok = wait(xbar(warp & 3), (uint32_t)step & 1);
+        if (!ok) break;
+        float change;
+        const bool changes = row_scale.follow(largest_top(base + L::kTops), change);
+        if (__any_sync(0xffffffffu, changes) && step > 0) {
+          // dP of this step was issued ahead of dQ of the last one, which gives its keys' place in the ring back when it is done
+          const int n = 2 * (step - 1);
+          ok = wait(empty(n % kStages), (uint32_t)(n / kStages) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          rescale_quarter<DP>(tdq + lane_at + w * (DP / 4), change);
+        }
+      }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         uint32_t o[4], lo[4];
 #pragma unroll
         for (int c = 8 * p; c < 8 * p + 8; c += 2) {
           float y[2];
-          tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])),
-                               tc::fma2(tc::pack2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), both(gs), both(nd))),
-                      y[0], y[1]);
+          if constexpr (Scales<T>::kHalf) {
+            y[0] = __uint_as_float(s[0][c]) * row_scale.now;
+            y[1] = __uint_as_float(s[0][c + 1]) * row_scale.now;
+          } else {
+            slopes_at(c, y);
+          }
           o[c % 8 / 2] = pack16<T>(y[0], y[1]);
           if constexpr (FINE) lo[c % 8 / 2] = left_over<T>(y[0], y[1], o[c % 8 / 2]);
         }
@@ -826,7 +935,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
       T* row = reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)i * a.dq.sn + h * a.dq.sh;
       const int c0 = w * (DP / 4);
       if (ok && steps > 0)
-        store_quarter<T, DP>(tdq + lane_at, c0, a.scale_raw / gs, add == -INFINITY, a.d, base + L::kRing + warp * 4096, [&](int e) {
+        store_quarter<T, DP>(tdq + lane_at, c0, Scales<T>::kHalf ? row_scale.undo(a.scale_raw) : a.scale_raw, add == -INFINITY, a.d, base + L::kRing + warp * 4096, [&](int e) {
           const int rr = r - (int)(threadIdx.x & 31) + e;
           return rr < t.rows ? reinterpret_cast<T*>(a.dq.p) + b * a.dq.sb + (int64_t)(rr >> t.pg_shift) * a.dq.sn + (hp * t.pg + (rr & (t.pg - 1))) * a.dq.sh
                              : nullptr;

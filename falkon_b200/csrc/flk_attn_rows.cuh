@@ -1,4 +1,4 @@
-// Row kernels around attention's products: delta of the backward pass, largest magnitudes, results of rows that see nothing.
+// Row kernels around attention's products: delta of the backward pass, results of rows that see nothing.
 #pragma once
 
 #include "flk_attn.cuh"
@@ -6,43 +6,16 @@
 namespace flk {
 namespace attn {
 
-// Largest |v| of the rows of a sequence that may be seen, as bits; `block` of `blocks`.
-template <typename T>
-__device__ __forceinline__ void largest_value(const Args& a, int b, uint32_t block, uint32_t blocks, uint32_t* amax) {
-  constexpr int kVec = 16 / sizeof(T);
-  const int packs = a.d / kVec, len = limits_of(a, b).len;
-  const int64_t n = (int64_t)len * a.hk * packs;
-  float top = 0.f;
-  for (int64_t e = (int64_t)block * 256 + threadIdx.x; e < n; e += (int64_t)blocks * 256) {
-    const int c = (int)(e % packs) * kVec;
-    const int64_t row = e / packs;
-    const int h = (int)(row % a.hk), j = (int)(row / a.hk);
-    if (a.kdocs != nullptr && a.kdocs[(int64_t)b * a.nk_pad + j] < 0) continue;
-    T u[kVec];
-    *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>((const T*)a.v.p + b * a.v.sb + j * a.v.sn + h * a.v.sh + c);
-#pragma unroll
-    for (int x = 0; x < kVec; ++x) top = fmaxf(top, fabsf(to_f<T>(u[x])));
-  }
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) atomicMax(amax, __float_as_uint(top));
-}
-
-// delta_i = dO_i . O_i, a group of LANES lanes per row of one head (16 bytes of each array per lane), two rows per group at a time,
-// and the largest |dO| of the rows that see something (`amax`, as bits, unless null; a maximum does not depend on the order it
-// is taken in).  Bound by the bytes of dO, O and what rounding took from O.  With `amax`, the blocks from `delta_blocks` on take
-// the largest |v| to amax[1].
+// delta_i = dO_i . O_i, a group of LANES lanes per row of one head (16 bytes of each array per lane), two rows per group at a time.
+// Bound by the bytes of dO, O and what rounding took from O.
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) delta_kernel(const Args a, uint32_t* amax, uint32_t delta_blocks) {
+__global__ void __launch_bounds__(256) delta_kernel(const Args a) {
   constexpr int kVec = 16 / sizeof(T), kGroups = 256 / LANES;
-  if (blockIdx.x >= delta_blocks) {
-    largest_value<T>(a, blockIdx.y, blockIdx.x - delta_blocks, gridDim.x - delta_blocks, amax + 1);
-    return;
-  }
   const uint32_t n = (uint32_t)a.nq * (uint32_t)a.hq;
   const int b = blockIdx.y, c = (threadIdx.x % LANES) * kVec;
   const T *dout = (const T*)a.dout.p + b * a.dout.sb, *o = (const T*)a.o.p + b * a.o.sb;
   const T* lo = a.o_lo == nullptr ? nullptr : (const T*)a.o_lo + b * a.o.sb;
-  float s[2] = {0.f, 0.f}, top[2] = {0.f, 0.f};
+  float s[2] = {0.f, 0.f};
   int64_t at[2];
   bool on[2];
   uint4 u[2], w[2], x[2];
@@ -68,37 +41,19 @@ __global__ void __launch_bounds__(256) delta_kernel(const Args a, uint32_t* amax
       const float g = to_f<T>(p[k]);
       s[e] = fmaf(g, to_f<T>(q[k]), s[e]);
       if (sizeof(T) == 2) s[e] = fmaf(g, to_f<T>(r[k]), s[e]);
-      top[e] = fmaxf(top[e], fabsf(g));
     }
     for (int k = LANES / 2; k > 0; k >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], k);
     if (c == 0 && on[e]) a.delta[at[e]] = s[e];
   }
-  if (amax != nullptr) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (!on[e] || a.lse[at[e]] == -INFINITY) top[e] = 0.f;
-      for (int k = 16; k > 0; k >>= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], k));
-    }
-    const uint32_t bits = __float_as_uint(fmaxf(top[0], top[1]));
-    if ((threadIdx.x & 31) == 0 && bits > *reinterpret_cast<volatile uint32_t*>(amax)) atomicMax(amax, bits);
-  }
 }
 template <typename T>
-inline int launch_delta(const Args& a, uint32_t* amax, cudaStream_t st) {
+inline int launch_delta(const Args& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const int64_t n = (int64_t)a.nq * a.hq;
   const int lanes = a.d <= 8 * kVec ? 8 : a.d <= 16 * kVec ? 16 : 32;
-  const unsigned blocks = (unsigned)ceil_div(n, 2 * 256 / lanes);
-  unsigned more = 0;
-  if (amax != nullptr) {
-    FLK_CUDA_TRY(cudaMemsetAsync(amax, 0, 8, st));
-    const int64_t want = ceil_div((int64_t)a.nk * a.hk * a.d / kVec, 256 * 8), most = ceil_div(8 * kNumSMs, a.b);
-    more = (unsigned)(want < most ? want : most);
-  }
-  const dim3 grid(blocks + more, a.b);
-  if (lanes == 8) delta_kernel<T, 8><<<grid, 256, 0, st>>>(a, amax, blocks);
-  else if (sizeof(T) == 2 || lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a, amax, blocks);
-  else if constexpr (sizeof(T) == 4) delta_kernel<T, 32><<<grid, 256, 0, st>>>(a, amax, blocks);
+  const dim3 grid((unsigned)ceil_div((int64_t)a.nq * a.hq, 2 * 256 / lanes), a.b);
+  if (lanes == 8) delta_kernel<T, 8><<<grid, 256, 0, st>>>(a);
+  else if (sizeof(T) == 2 || lanes == 16) delta_kernel<T, 16><<<grid, 256, 0, st>>>(a);
+  else if constexpr (sizeof(T) == 4) delta_kernel<T, 32><<<grid, 256, 0, st>>>(a);
   count_launch();
   return FLK_OK;
 }

@@ -368,7 +368,6 @@ struct TcArgs {
   Tanh tanh;         // of the cap
   // the order in which the row blocks (backward: the key tiles) of all sequences start: sequence * blocks + block, or null
   const int* order;
-  const uint32_t* amax;  // backward, fp16: largest |dout| and largest |v| as bits; else null
   uint32_t wait_ns;      // limit of a wait; 0: the issuing warp gives up before its first product
 };
 

@@ -74,3 +74,68 @@ def test_capped_rows_beside_a_large_one(cap, size, dtype):
     assert worst(got["lse"][..., small], want["lse"][..., small], bounds["e_lse"][..., small]) <= 2
     token = attention(q[:, 76:79], k, v, softcap=cap)
     assert worst(token[:, ::2], want["out"][:, 76:79:2], bounds["e_out"][:, 76:79:2]) <= 2
+
+
+def bits_of(got, part):
+    return [part(got["dq"]), part(got["dk"]), part(got["dv"])]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,hq,hk,d", [(100, 2, 2, 64), (400, 6, 2, 128), (1000, 4, 1, 64)])
+def test_gradients_owe_nothing_to_other_sequences_and_heads(n, hq, hk, d, dtype):
+    """Upstream gradients and values of another sequence, or of another key head's group, may be 10^5 times larger, or infinite:
+    the gradients stay what they are, bit by bit."""
+    q, k, v, do = make(2, n, n, hq, hk, d, dtype, 3)
+    do = do / 16
+    want = run(q, k, v, do, causal=True)
+    for change in (lambda t: t * 2.0**13, lambda t: t * math.inf):
+        d2, v2 = do.clone(), v.clone()
+        d2[0] = change(do[0])
+        v2[0] = v[0] * 256
+        got = run(q, k, v2, d2, causal=True)
+        for x, y in zip(bits_of(got, lambda t: t[1]), bits_of(want, lambda t: t[1])):
+            assert torch.equal(x, y)
+        if hk > 1:
+            d2 = do.clone()
+            d2[:, :, :hq // hk] = change(do[:, :, :hq // hk])
+            got = run(q, k, v, d2, causal=True)
+            for n_, first in (("dq", hq // hk), ("dk", 1), ("dv", 1)):
+                assert torch.equal(got[n_][:, :, first:], want[n_][:, :, first:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,hq,hk,d", [(200, 2, 2, 64), (500, 4, 2, 128), (900, 4, 1, 64)])
+def test_gradients_owe_nothing_to_other_rows(n, hq, hk, d, dtype):
+    """The same within a sequence: queries of its first part, and documents beside one another in a tile."""
+    q, k, v, do = make(1, n, n, hq, hk, d, dtype, 4)
+    do = do / 16
+    cut = n // 2 + 5
+    large = do.clone()
+    large[:, :cut] *= 2.0**13
+    want, got = run(q, k, v, do, causal=True), run(q, k, v, large, causal=True)
+    for x, y in zip(bits_of(got, lambda t: t[:, cut:]), bits_of(want, lambda t: t[:, cut:])):  # keys that only later queries see
+        assert torch.equal(x, y)
+    docs = torch.arange(n, device=DEV)[None] // 37
+    even = (docs[0] % 2 == 0)
+    large = torch.where(even[None, :, None, None], do * 2.0**13, do)
+    big_v = torch.where(even[None, :, None, None], v * 256, v)
+    want, got = run(q, k, v, do, documents=docs), run(q, k, big_v, large, documents=docs)
+    for x, y in zip(bits_of(got, lambda t: t[:, ~even]), bits_of(want, lambda t: t[:, ~even])):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("growth", [2.0**0.03, 2.0**-0.03])
+def test_fp16_gradients_that_grow_along_a_row(growth, d):
+    """Terms of dK and dV grow, or shrink, by 2^18 from the first query tile to the last, and those of dQ along the keys: the
+    factor that a row is held with follows.  A row keeps the bounds that it has when the smaller terms are not there to be lost:
+    2^-29 of the largest term for each of 600 terms is far below the rounding of the largest one, 2^-11."""
+    n = 600
+    q, k, v, do = make(1, n, n, 2, 1, d, torch.float16, 5)
+    f = growth ** torch.arange(n, device=DEV, dtype=torch.float64)
+    f = (f / f.max() * 2.0**6).to(torch.float32)[None, :, None, None]
+    for do2, v2 in ((do * f, v), (do, v * f), (do * f, v * f)):
+        do2, v2 = do2.half(), v2.half()
+        want, got = reference(q, k, v2, do2, causal=growth < 1), run(q, k, v2, do2, causal=growth < 1)
+        for name in ("out", "dq", "dk", "dv"):
+            assert worst(got[name], want[name], want["e_" + name]) <= 1, name
