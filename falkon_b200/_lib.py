@@ -35,6 +35,7 @@ NVCC_FLAGS = [
 ]
 LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared"]
 PTXAS_REPORT = LIB_PATH + ".ptxas.txt"
+OBJECTS = LIB_PATH + ".objects"
 # The tensor-core sweeps read their accumulators with asynchronous tcgen05.ld: a register that such a load is still
 # to fill must never be spilled, so the resident kernel has to compile without any spill.  It re-partitions
 # registers between its warp roles and relies on being launched with exactly this many per thread:
@@ -77,9 +78,9 @@ def _includes(path: str, seen=None):
 
 
 def _compile(unit: str, flags, force: bool, verbose: bool):
-    """(object file, ptxas report) of one translation unit; both are kept in csrc/ and made again when a source that
-    the unit includes, or the command, has changed."""
-    obj = unit[:-3] + ".o"
+    """(object file, ptxas report) of one translation unit; both are kept beside the library that they go into, under its
+    lock, and made again when a source that the unit includes, or the command, has changed."""
+    obj = os.path.join(OBJECTS, os.path.basename(unit)[:-3] + ".o")
     report = obj + ".ptxas.txt"
     cmd = [os.environ.get("NVCC", "nvcc")] + flags + ["-c", unit]
     head = "# " + " ".join(cmd) + "\n"
@@ -119,6 +120,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         try:
             if not force and _up_to_date():
                 return LIB_PATH
+            os.makedirs(OBJECTS, exist_ok=True)
             tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
             extra = os.environ.get("FALKON_B200_NVCC_EXTRA", "").split()  # e.g. -D tuning macros of the kernels
             units = [s for s in sources() if s.endswith(".cu")]
