@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib
 from .fmmv import _require_cuda
-from .utils import differentiable_once
+from .utils import differentiable_once, refuse_tangents
 
 __all__ = ("attention", "AttentionFn")
 
@@ -69,6 +69,7 @@ def _forward(q, k, v, opts, with_lse, with_lo=False):
 def _backward(ctx, dout, _):
     if dout is None:
         return None, None, None, None
+    refuse_tangents("attention", dout)
     q, k, v, out, out_lo, lse, *kept = ctx.saved_tensors
     kept = iter(kept)
     opts = tuple(next(kept) if held else t for t, held in zip(ctx.opts, ctx.held))
@@ -189,11 +190,12 @@ def attention(
     A query that sees no key gets zeros, and -inf in the log-sum-exp.  What such queries, padding rows, keys behind
     ``kv_lens`` and, with ``causal``, keys that no query reaches hold does not matter, NaN included.  Integer tables are
     read on the device: lengths beyond [0, Nk] count as the nearer end.  At most 65535 sequences, 65535 heads, 2^29 rows.
-    Differentiable once with respect to q, k and v.  Runs on the current stream of the data's device, allocates its output
+    Differentiable once with respect to q, k and v, in reverse mode only (no tangents, no ``torch.func``).  Runs on the current stream of the data's device, allocates its output
     and workspace from torch's allocator, and may be captured into a CUDA graph (a backward pass, as torch has it for every
     operator, only while no graph of the same leaves that was built outside of the capture is alive).  With 16-bit data every wait
     inside a kernel is bounded: rows that a stalled GPU does not finish within a second are NaN, and so are their gradients.
     """
+    refuse_tangents("attention", q, k, v, slopes)
     try:
         fits = q.dtype is k.dtype is v.dtype and q.dtype in _lib._ROW_TYPES and k.shape == v.shape and q.device == k.device == v.device
         b, nq, hq, d = q.shape

@@ -10,7 +10,7 @@ import torch
 
 from .. import _lib
 from .fmmv import _require_cuda
-from .utils import differentiable_once
+from .utils import differentiable_once, refuse_tangents
 
 __all__ = ("layer_norm", "LayerNormFn")
 
@@ -62,6 +62,7 @@ def _forward(x, weight, bias, eps, with_stats):
 
 
 def _backward(ctx, dy):
+    refuse_tangents("layer_norm", dy)
     x, weight, stats = ctx.saved_tensors
     need_x, need_w, need_b, _ = ctx.needs_input_grad
     d, dev = x.shape[-1], x.device
@@ -114,9 +115,10 @@ def layer_norm(
     eps : added to the variance, which is the mean of the squared centred values
 
     Statistics and sums are kept in float32; the result is dense and has x's type.  Differentiable once with respect to
-    x, weight and bias.  Runs on the current stream of x's device, and may be captured into a CUDA graph (a backward pass, as
+    x, weight and bias, in reverse mode only (no tangents, no ``torch.func``).  Runs on the current stream of x's device, and may be captured into a CUDA graph (a backward pass, as
     torch has it for every operator, only while no graph of the same leaves that was built outside of the capture is alive).
     """
+    refuse_tangents("layer_norm", x, weight, bias)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a torch.Tensor, not {type(x).__name__}")
     _lib.row_dtype_code(x.dtype)

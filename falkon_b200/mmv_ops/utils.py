@@ -8,8 +8,9 @@ created on the first CUDA input's device, else on the CPU (pinned), with the mem
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
-__all__ = ("differentiable_once", "is_contig", "is_f_contig", "check_contiguity", "create_output_mat", "create_same_stride")
+__all__ = ("differentiable_once", "refuse_tangents", "is_contig", "is_f_contig", "check_contiguity", "create_output_mat", "create_same_stride")
 
 
 def is_contig(tensor: torch.Tensor) -> bool:
@@ -89,3 +90,12 @@ def differentiable_once(what: str, grads, anchors):
     there = [g for g in grads if g is not None]
     out = iter(_OnceFn.apply(what, len(there), *there, *anchors))
     return tuple(None if g is None else next(out) for g in grads)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises where an operand carries a tangent of forward-mode differentiation, which a kernel would drop."""
+    if forward_ad._current_level < 0:  # outside of every dual level: nothing carries one
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative.")
