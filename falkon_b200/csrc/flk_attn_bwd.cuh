@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           float y[4];
           if constexpr (Scales<T>::kHalf) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) y[q] = __uint_as_float(s[0][c + q]) * row_scale.now;
+            for (int q = 0; q < 4; q += 2)
+              tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c + q]), __uint_as_float(s[0][c + q + 1])), both(row_scale.now)), y[q], y[q + 1]);
           } else {
             slopes_at(c, d, s[0], st, y);
           }
@@ -912,8 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
         for (int c = 8 * p; c < 8 * p + 8; c += 2) {
           float y[2];
           if constexpr (Scales<T>::kHalf) {
-            y[0] = __uint_as_float(s[0][c]) * row_scale.now;
-            y[1] = __uint_as_float(s[0][c + 1]) * row_scale.now;
+            tc::unpack2(tc::mul2(tc::pack2(__uint_as_float(s[0][c]), __uint_as_float(s[0][c + 1])), both(row_scale.now)), y[0], y[1]);
           } else {
             slopes_at(c, y);
           }
