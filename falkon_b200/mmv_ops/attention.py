@@ -111,8 +111,9 @@ class AttentionFn(torch.autograd.Function):
         return differentiable_once("attention", out, [*ctx.saved_tensors[:3], *(g for g in grads if g is not None)])
 
 
-def _table(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[torch.Tensor]:
-    """An integer table on the data's device, as int32 with unit stride over its last dimension."""
+def _table(name: str, t: Optional[torch.Tensor], shape, device, labels: bool = False) -> Optional[torch.Tensor]:
+    """An integer table on the data's device, as int32 with unit stride over its last dimension.  Numbers beyond int32 become
+    its ends; labels, which must not fall together, become negative, that is padding (2^31 wraps)."""
     if t is None:
         return None
     if not isinstance(t, torch.Tensor):
@@ -124,7 +125,7 @@ def _table(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[torc
     if t.dtype != torch.int32:
         if t.dtype != torch.int64:
             raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-        t = t.clamp(-(2**31), 2**31 - 1).to(torch.int32)
+        t = t.clamp(-(2**31), 2**31 if labels else 2**31 - 1).to(torch.int32)
     return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
@@ -180,7 +181,7 @@ def attention(
     slopes : (Hq,) float32, the distance bias of each query head (a constant: it gets no gradient)
     prefix_lens : (B,) integers; with ``causal``, the first keys of a sequence that every query may see
     documents : (B, Nk) integers; a query sees the keys of its own document only.  A negative label marks padding, which
-        sees and shows nothing; labels lie below 2^31
+        sees and shows nothing, and so does one of 2^31 and more
     q_documents : (B, Nq) integers, the queries' documents; default ``documents`` where Nq == Nk
     kv_lens : (B,) integers; keys at or behind this length do not exist (a cache's length), default Nk
     q_starts : (B,) integers, position of the first query of a sequence; by default the last query stands at the last
@@ -226,7 +227,7 @@ def attention(
         q_documents = documents
     opts = (scale, softcap, 1 if causal else 0, slopes, _table("prefix_lens", prefix_lens, (b,), dev),
             _table("kv_lens", kv_lens, (b,), dev), _table("q_starts", q_starts, (b,), dev),
-            _table("q_documents", q_documents, (b, nq), dev), _table("documents", documents, (b, nk), dev))
+            _table("q_documents", q_documents, (b, nq), dev, True), _table("documents", documents, (b, nk), dev, True))
     pad = -d % 8
     if pad:  # the kernels read whole vectors of 16 bytes; zeros change no dot product
         q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))

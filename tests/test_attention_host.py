@@ -3,9 +3,12 @@ import glob
 import os
 import re
 
-import pytest
+import sys
 
-from falkon_b200 import _lib
+import pytest
+import torch
+
+from falkon_b200 import _lib, mmv_ops  # noqa: F401
 
 
 @pytest.fixture(scope="module")
@@ -37,3 +40,12 @@ def test_loads_from_tensor_memory_end_where_they_begin():
                 loads += 1
                 assert "tcgen05.wait::ld" in statement, path
     assert loads > 0
+
+
+def test_labels_beyond_int32_do_not_fall_together():
+    table = sys.modules["falkon_b200.mmv_ops.attention"]._table
+    t = torch.tensor([[0, 2**31 - 1, 2**31, 2**31 + 5, 2**32, 2**62, -1, -(2**31), -(2**40)]])
+    got = table("documents", t, t.shape, t.device, True)
+    assert got.dtype == torch.int32 and got[0, :2].tolist() == [0, 2**31 - 1] and bool((got[0, 2:] < 0).all())
+    got = table("kv_lens", t, t.shape, t.device)
+    assert got[0].tolist() == [0] + [2**31 - 1] * 5 + [-1] + [-(2**31)] * 2

@@ -139,3 +139,15 @@ def test_fp16_gradients_that_grow_along_a_row(growth, d):
         want, got = reference(q, k, v2, do2, causal=growth < 1), run(q, k, v2, do2, causal=growth < 1)
         for name in ("out", "dq", "dk", "dv"):
             assert worst(got[name], want[name], want["e_" + name]) <= 1, name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_labels_beyond_int32(dtype):
+    """They mark padding: two documents never become one, and the largest label that is one stays apart from them."""
+    q, k, v, do = make(1, 200, 200, 2, 1, 64, dtype, 6)
+    docs = torch.tensor([3, 2**31 - 1, 2**31, 2**40], device=DEV).repeat_interleave(50)[None]
+    out = run(q, k, v, do, documents=docs)
+    same = run(q, k, v, do, documents=torch.tensor([0, 1, -1, -1], device=DEV, dtype=torch.int32).repeat_interleave(50)[None])
+    for n in out:
+        assert torch.equal(out[n], same[n]), n
+    assert not bool(out["out"][:, 100:].any()) and bool((out["lse"][..., 100:] == -math.inf).all())
