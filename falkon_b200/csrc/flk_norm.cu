@@ -204,32 +204,37 @@ __global__ void __launch_bounds__(1024 / (V * VEC > 16 ? 2 : 1)) forward_kernel(
   }
 }
 
-// One block per row, rows of any length; the row is read three times (from L2 after the first).
+// One block per row, rows of any length; the row is read three times (from L2 after the first).  A thread adds up d / 1024 values,
+// so a first mean may be off by that many roundings (rows of 2^22 values with a mean of 1000: by 0.01).  The second pass adds up
+// the centred values too, and what their mean says is left of the first mean comes off them.
 template <typename T>
 __global__ void __launch_bounds__(1024) forward_long_kernel(const Args a) {
-  __shared__ float red[2 * 32];
+  __shared__ float red[2 * 32 * 2];
   int flip = 0;
   T* y = reinterpret_cast<T*>(a.y);
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(a.x) + a.xr.at(row);
-    float s[1] = {0.f};
+    float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) s[0] += to_f<T>(x[c]);
-    group_sum<1>(s, blockDim.x, red, flip);
+    group_sum<2>(s, blockDim.x, red, flip);
     const float mu = s[0] * a.inv_d;
-    s[0] = 0.f;
+    s[0] = s[1] = 0.f;
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
       const float v = to_f<T>(x[c]) - mu;
-      s[0] = fmaf(v, v, s[0]);
+      s[0] += v;
+      s[1] = fmaf(v, v, s[1]);
     }
-    group_sum<1>(s, blockDim.x, red, flip);
-    const float r = inverse_root(fmaf(s[0], a.inv_d, a.eps));
+    group_sum<2>(s, blockDim.x, red, flip);
+    const float left = s[0] * a.inv_d;
+    // mean(v^2) - left^2 without a difference of two large numbers: `left` is a rounding error of the mean
+    const float r = inverse_root(fmaxf(fmaf(s[1], a.inv_d, -left * left), 0.f) + a.eps);
     if (threadIdx.x == 0 && a.mean != nullptr) {
-      a.mean[row] = mu;
+      a.mean[row] = mu + left;
       a.rstd[row] = r;
     }
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
       const float w = a.w != nullptr ? load_any(a.w, a.wdtype, c) : 1.f, b = a.b != nullptr ? load_any(a.b, a.wdtype, c) : 0.f;
-      y[row * a.d + c] = from_f<T>(fmaf((to_f<T>(x[c]) - mu) * r, w, b));
+      y[row * a.d + c] = from_f<T>(fmaf((to_f<T>(x[c]) - mu - left) * r, w, b));
     }
   }
 }
