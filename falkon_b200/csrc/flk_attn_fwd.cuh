@@ -9,7 +9,7 @@
 //   !PAIR  one row tile; the groups take the even and the odd key tiles, and end with a partial result each: few
 //          rows over a long key axis (single tokens)
 // Weights are exp2(s - m) with a maximum m that follows the running one only when that has grown by more than 8: weights
-// stay below 2^8, and the accumulator is rescaled a few times in a row's life instead of once per tile.  Weights are rounded to
+// stay below 2^8 (fp16: 2^15, see kLift), and the accumulator is rescaled a few times in a row's life instead of once per tile.  Weights are rounded to
 // the data's 16 bits before they meet V (a relative error of half a step each, which is what the result itself is rounded by).
 // The result is divided by the sum of the rounded weights, so that their common error cancels; the log-sum-exp, which the
 // backward pass makes exact weights from, has the sum of the weights as they were.  Sums, maximum and accumulators are fp32.
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         lr *= f;
         m = mn;
       }
-      const float mb = m == -INFINITY ? 0.f : m;
+      const float mb = (m == -INFINITY ? 0.f : m) - kLift<T>;
       const uint64_t f2v = tc::pack2(f2, f2), mv = tc::pack2(-mb, -mb);
       uint64_t sum = 0, rounded = 0;
 #pragma unroll
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    const float inv = none ? 0.f : 1.0f / lr, lse2 = none ? -INFINITY : m + log2f(l);
+    const float inv = none ? 0.f : 1.0f / lr, lse2 = none ? -INFINITY : m - kLift<T> + log2f(l);
     if (live && ok) {
       // read again instead of held in registers through the loop above
       const int4 at = get_place(place);

@@ -214,6 +214,11 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// Forward, weights are exp2(s - m + kLift) with a maximum m that may be 8 behind.  fp16 ends at 2^-25 and just below 2^16, so there
+// they are lifted to where the largest is 2^15: up to 2^32 times smaller ones count, of which a long row may have many.
+template <typename T>
+constexpr float kLift = std::is_same<T, __nv_bfloat16>::value ? 0.f : 7.f;
+
 // the pair of fp32 values that a packed pair holds
 template <typename T>
 __device__ __forceinline__ uint64_t unpack16(uint32_t v) {

@@ -207,10 +207,11 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float base = m[e / 2] == -INFINITY ? 0.f : m[e / 2];
+        const float base = (m[e / 2] == -INFINITY ? 0.f : m[e / 2]) - kLift<T>;
         p[n][e] = ex2_approx(s[n][e] - base);
         l[e / 2] += p[n][e];
       }
+    // rounded to the data's type, as the prompts' kernel does; the error of a weight, half a step, is what the result is rounded by
     const uint32_t w[4] = {pack16<T>(p[0][0], p[0][1]), pack16<T>(p[0][2], p[0][3]), pack16<T>(p[1][0], p[1][1]), pack16<T>(p[1][2], p[1][3])};
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
     for (int n = 0; n < DP / 8; ++n)
       *reinterpret_cast<float2*>(buf + (warp * kRows + r) * kLd + n * 8 + 2 * (lane % 4)) = make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
     if (warp == 0 && lane % 4 == 0 && r < t.rows)
-      t.part_lse[(((int64_t)split * a.b + b) * a.hk + hk) * t.rows + r] = sum == 0.f ? -INFINITY : top + log2f(sum);
+      t.part_lse[(((int64_t)split * a.b + b) * a.hk + hk) * t.rows + r] = sum == 0.f ? -INFINITY : top - kLift<T> + log2f(sum);
   }
   __syncthreads();
   const int64_t row0 = (((int64_t)split * a.b + b) * a.hk + hk) * t.rows;

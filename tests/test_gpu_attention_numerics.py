@@ -151,3 +151,25 @@ def test_labels_beyond_int32(dtype):
     for n in out:
         assert torch.equal(out[n], same[n]), n
     assert not bool(out["out"][:, 100:].any()) and bool((out["lse"][..., 100:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,nq,nk,hq,hk", [(1, 8192, 1 << 18, 16, 1), (222, 1, 1 << 16, 8, 8)])
+def test_many_small_weights_beside_a_large_one(b, nq, nk, hq, hk, dtype):
+    """One key has most of the weight, and each of very many others a 2^-25th of it, half of fp16's smallest step: held as they are
+    they would be lost, though together they make 2^-7 (or 2^-9) of the sum.  The key axis is in one part here.  The large key's
+    value is zero, so the result is the small ones' share.  Relative error: u for the result, 2^-7 for the weights (which have at
+    least 6 bits), and nk steps of fp32 for a sum of nk equal terms in any order, each addition cut or rounded.
+    """
+    gap = torch.tensor(17.35).to(dtype)
+    q, k, v = (torch.zeros(b, n, h, 8, device=DEV, dtype=dtype) for n, h in ((nq, hq), (nk, hk), (nk, hk)))
+    q[..., 0] = 1
+    k[:, 5, :, 0] = gap
+    v[:] = 1
+    v[:, 5] = 0
+    small = (nk - 1) * math.exp(-float(gap))
+    assert 2.0**-10 < small < 2.0**-6
+    want, lse = small / (small + 1), float(gap) + math.log1p(small)
+    out, got = attention(q, k, v, scale=1.0, return_lse=True)
+    assert float((out.double() - want).abs().max()) <= want * (HALF_STEP[dtype] + 2.0**-7 + nk * 2.0**-23)
+    assert float((got.double() - lse).abs().max()) <= 2.0**-18 + nk / 16 * 2.0**-24
