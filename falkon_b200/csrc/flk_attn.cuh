@@ -44,6 +44,7 @@ struct Args {
 
 struct Limits {  // of one sequence; no query sees keys at or behind `len`
   int len, start, prefix;
+  int at;  // `start` as distances are counted from it
   __device__ __forceinline__ int row_end(int i, int causal) const {
     if (!causal) return len;
     const int e = max(start + i + 1, prefix);
@@ -55,6 +56,9 @@ __device__ __forceinline__ Limits limits_of(const Args& a, int b) {
   l.len = a.kv_lens != nullptr ? min(max(a.kv_lens[b], 0), a.nk) : a.nk;
   // positions stay far from the ends of int, whatever the caller's table holds
   l.start = a.q_starts != nullptr ? min(max(a.q_starts[b], -(1 << 29)), 1 << 29) : l.len - a.nq;
+  // Where all queries stand behind all keys, or before them, the distance between the two is the same for every pair and changes
+  // no weight; fp32 scores would lose their digits to it.  It is left out of the scores, and of the log-sum-exp that is kept.
+  l.at = min(max(l.start, -a.nq), max(l.len, 1) - 1);
   l.prefix = a.prefix != nullptr ? a.prefix[b] : 0;
   // under a causal mask what lies behind the last query (the rest of a cache, say) may hold anything too
   l.len = l.row_end(a.nq - 1, a.causal);

@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_keys(const __grid_constant
           put(kDelta, __float_as_uint(none ? 0.f : -delta[x] * Scales<T>::kUnshift));
           if constexpr (BIAS) {
             put(kSlope, __float_as_uint(-slope[x] * kLog2e));
-            put(kPos, __float_as_uint((float)(lim.start + i - k0)));
+            put(kPos, __float_as_uint((float)(lim.at + i - k0)));
           }
           put(kLabel, (uint32_t)label[x]);
         }
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel_queries(const __grid_const
     const uint32_t lane_at = (uint32_t)(warp & 3) << 21, mine0 = 32 * w;
     const int end = exists ? lim.row_end(i, a.causal) : 0;
     const float slope2 = slope * kLog2e;
-    const int pos = lim.start + i;
+    const int pos = lim.at + i;
     const int all_before = lim.row_end(i0, a.causal);
     int only = -1;
     if (kd && !lab.bad && lab.lo == lab.hi) only = lab.lo;

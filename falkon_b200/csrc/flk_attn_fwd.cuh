@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int s = 0; s < kStages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
       for (int w = 0; w < 2; ++w) mbar_init(sfull(w), 1), mbar_init(pfull(w), 8), mbar_init(odone(w), 1), mbar_init(xbar(w), 8);
       mbar_init(qfull, 1), mbar_init(drained, 1);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place + 16), "r"(lim.len), "r"(lim.start), "r"(lim.prefix), "r"(0) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place + 16), "r"(lim.len), "r"(lim.start), "r"(lim.prefix), "r"(lim.at) : "memory");
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(hp), "r"(b), "r"(split), "r"(row0) : "memory");
       tc::fence_barrier_init();
     }
@@ -280,7 +280,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t mine = halves + (w * 256 + side * 128 + (threadIdx.x & 127)) * 4, other = side == 0 ? mine + 512 : mine - 512;
     const int i = r >> t.pg_shift, h = hp * t.pg + (r & (t.pg - 1));
     const float slope2 = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
-    const int pos = lim.start + i;
     // for the tile of this warpgroup: keys before `x` are visible to every row that exists; `y` is the one label of its queries
     const uint32_t rule = place + 32 + 8 * w;
     {
@@ -332,7 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t at = ts(w) + lane_at + 64 * side;
       tmem_read64(at, s[0], s[1]);
       if constexpr (CAP) to_tanh(s, t.tanh, a.scale);
-      if constexpr (BIAS) add_bias(s, f2, slope2, (float)(pos - k0));
+      if constexpr (BIAS) {  // (read again instead of held in a register)
+        const int r = get_place(place).w + (PAIR ? w * kTile : 0) + (int)(threadIdx.x & 127);
+        add_bias(s, f2, slope2, (float)(get_place(place + 16).w + (r >> t.pg_shift) - k0));
+      }
       if (!whole) {
         uint32_t seen[2];
         const int4 x = get_place(place + 16);

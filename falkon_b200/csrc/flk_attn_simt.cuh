@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) forward_kernel(co
     scores(a, s, tanh);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int pos = lim.start + q0 + 4 * ty + i;
+      const int pos = lim.at + q0 + 4 * ty + i;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) backward_kv_kerne
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = k0 + 4 * ty + i, r = q0 + tx + 16 * j;
-        const float v = biased(s[i][j], slope2, lim.start + r - key);
+        const float v = biased(s[i][j], slope2, lim.at + r - key);
         const bool see = r < a.nq && key < lim.row_end(r, a.causal) && (kd == nullptr || qd[r] == id[i]);
         s[i][j] = see ? ex2_approx(v - lse2[j]) : 0.f;
         dp[i][j] = see ? s[i][j] * (dp[i][j] - dl[j]) * (1.f - t[i][j] * t[i][j]) : 0.f;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads* Smem<DM>::kGroups) backward_q_kernel
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = k0 + tx + 16 * j;
-        const float v = biased(s[i][j], slope2, lim.start + q0 + 4 * ty + i - col);
+        const float v = biased(s[i][j], slope2, lim.at + q0 + 4 * ty + i - col);
         const bool see = col < end[i] && (kd == nullptr || kd[col] == id[i]);
         s[i][j] = see ? ex2_approx(v - lse2[i]) * (dp[i][j] - delta[i]) * (1.f - t[i][j] * t[i][j]) : 0.f;
       }

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
     end[e] = exists ? lim.row_end(i, a.causal) : 0;
     my[e] = qd != nullptr && exists ? qd[i] : -2;
     slope2[e] = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
-    pos[e] = (float)(lim.start + i);
+    pos[e] = (float)(lim.at + i);
   }
   // the queries as A operands: columns 2 (lane % 4) and up of rows lane / 4, lane / 4 + 8
   uint32_t q[DP / 16][4];

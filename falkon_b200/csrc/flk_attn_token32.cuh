@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kWarps * 32, RW * DM <= 64 ? 5 : RW * DM <= 12
     const int r = r0 + threadIdx.x, i = r / a.grp, h = hk * a.grp + r - i * a.grp;
     const bool exists = r < t.rows;
     row_of[threadIdx.x] = make_int4(exists ? lim.row_end(i, a.causal) : 0, a.qdocs != nullptr && exists ? a.qdocs[(int64_t)b * a.nq_pad + i] : -2,
-                                    __float_as_int(a.slopes != nullptr && exists ? a.slopes[h] * kLog2e : 0.f), lim.start + i);
+                                    __float_as_int(a.slopes != nullptr && exists ? a.slopes[h] * kLog2e : 0.f), lim.at + i);
   }
   // columns 4 part + 32 c and up of the rows, in pairs
   uint64_t q[RW][kPairs], acc[RW][kPairs] = {};

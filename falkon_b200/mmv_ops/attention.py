@@ -129,6 +129,13 @@ def _table(name: str, t: Optional[torch.Tensor], shape, device, labels: bool = F
     return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _left_out(opts, nq: int, nk: int) -> torch.Tensor:
+    """The distance, per sequence, that the kernels leave out of every score (include/falkon_b200.h)."""
+    kv_lens, q_starts = opts[5], opts[6].clamp(-(2**29), 2**29)
+    last = max(nk, 1) - 1 if kv_lens is None else kv_lens.clamp(1, max(nk, 1)) - 1
+    return (q_starts - q_starts.clamp(min=-nq).clamp(max=last)).abs()
+
+
 def _refuse(q, k, v):
     """Says what is wrong with operands that do not fit."""
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -238,4 +245,8 @@ def attention(
         out, _, lse = _forward(q, k, v, opts, return_lse)
     if pad:
         out = out[..., :d]
-    return (out, lse) if return_lse else out
+    if not return_lse:
+        return out
+    if slopes is not None and q_starts is not None:
+        lse = lse - slopes[:, None] * _left_out(opts, nq, nk)[:, None, None]
+    return out, lse

@@ -263,7 +263,9 @@ int flk_kgrad(int dtype, int kernel,
  *      and  (no documents  or  q_documents[b][i] == k_documents[b][j] >= 0).
  * A query that sees nothing gets out = 0 and lse = -inf, and passes no gradient.  Such queries (q and dout), keys and values
  * at or behind kv_lens[b] or, with causal, behind the last query's reach, and rows whose document is negative, may hold
- * anything (NaN included).  A value or key that is not finite
+ * anything (NaN included).  With slopes, the lse that is written, and read by backward, leaves out slope_h s_b, where s_b is the distance
+ * that all queries of a sequence have from all of its keys beyond one row: the sum of both is far larger than what its digits are
+ * needed for.  s_b = |q_starts[b] - min(max(q_starts[b], -nq), max(kv_len_b, 1) - 1)|: lse_i is less than what is written by slope_h s_b.  A value or key that is not finite
  * and that some query may see reaches the outputs of the queries that share a tile with that one.
  *
  * Types FLK_F32, FLK_BF16, FLK_F16; 1 <= d <= 128, d a multiple of 8 (of 4 with FLK_F32); hq a multiple of hk (query

@@ -173,3 +173,29 @@ def test_many_small_weights_beside_a_large_one(b, nq, nk, hq, hk, dtype):
     out, got = attention(q, k, v, scale=1.0, return_lse=True)
     assert float((out.double() - want).abs().max()) <= want * (HALF_STEP[dtype] + 2.0**-7 + nk * 2.0**-23)
     assert float((got.double() - lse).abs().max()) <= 2.0**-18 + nk / 16 * 2.0**-24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("nq,nk", [(1, 300), (20, 300), (300, 200)])
+def test_positions_far_from_all_keys(nq, nk, causal, dtype):
+    """A distance that every pair of a sequence has changes no weight and no gradient: queries far behind all keys, or before them,
+    get what queries next to the keys get, within those queries' bounds.  The log-sum-exp has the distance in it, and fp32's step
+    of that."""
+    q, k, v, do = make(5, nq, nk, 4, 2, 64, dtype, 7)
+    lens = torch.tensor([nk, nk, nk - 77, nk, nk - 20], device=DEV)
+    far = torch.tensor([10**6, 2**29, 300000, nk - nq, 2**40], device=DEV)
+    near = torch.tensor([nk - 1, nk - 1, nk - 78, nk - nq, nk - 21], device=DEV)
+    if not causal:
+        far[3], near[3] = -(10**7), -nq
+    slopes = slopes_of(4)
+    opts = dict(causal=causal, kv_lens=lens, slopes=slopes)
+    want = reference(q, k, v, do, q_starts=near, **opts)
+    got = run(q, k, v, do, q_starts=far, **opts)
+    for n in ("out", "dq", "dk", "dv"):
+        assert worst(got[n], want[n], want["e_" + n]) <= 1, n
+    shift = slopes.double()[:, None] * (far.clamp(-(2**29), 2**29) - near).abs()[:, None, None]
+    some = want["lse"].isfinite()  # of queries that see a key
+    assert torch.equal(got["lse"].isfinite(), some)
+    assert worst(got["lse"][some], (want["lse"] - shift)[some], (want["e_lse"] + 2.0**-23 * (want["lse"].abs() + shift))[some]) <= 1
+    assert torch.equal(got["out"], attention(q, k, v, q_starts=far, **opts))
