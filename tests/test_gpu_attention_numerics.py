@@ -199,3 +199,56 @@ def test_positions_far_from_all_keys(nq, nk, causal, dtype):
     assert torch.equal(got["lse"].isfinite(), some)
     assert worst(got["lse"][some], (want["lse"] - shift)[some], (want["e_lse"] + 2.0**-23 * (want["lse"].abs() + shift))[some]) <= 1
     assert torch.equal(got["out"], attention(q, k, v, q_starts=far, **opts))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nq,nk,hq,hk,d", [(300, 300, 4, 2, 128), (300, 300, 3, 3, 64), (40, 900, 2, 1, 64), (16, 5000, 4, 1, 128), (1, 700, 8, 2, 80)])
+def test_what_rounding_takes_from_the_output_is_kept(nq, nk, hq, hk, d, dtype):
+    """Equal scores make the weights exact, and the output a mean of values in fp32: it and what rounding took from it, which the
+    backward pass adds back, together miss it by the rounding of what was taken, u (u |out|), and of nk additions."""
+    q, k, v, do = make(2, nq, nk, hq, hk, d, dtype, 8)
+    q = torch.zeros_like(q).requires_grad_()
+    u = HALF_STEP[dtype]
+    for opts in (dict(), dict(causal=True), dict(documents=(torch.arange(nk, device=DEV) // 50).expand(2, nk),
+                                                 q_documents=(torch.arange(nq, device=DEV) // 50).expand(2, nq))):
+        out = attention(q, k, v, **opts)
+        hi, lo = out.grad_fn.saved_tensors[3:5]
+        hi, lo = hi[..., :d].double(), lo[..., :d].double()
+        want, size = reference(q, k, v, **opts)["out"], reference(q, k, v.abs(), **opts)["out"]
+        assert torch.equal(hi, out.detach().double()) and bool((lo.abs() <= u * hi.abs() + 2.0**-25).all())
+        tiny = 2.0**-25 if dtype == torch.float16 else 0.0  # half of the smallest step, for the remainder too
+        assert bool(((hi + lo - want).abs() <= u * u * want.abs() * 1.01 + nk * 2.0**-23 * size + tiny + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,hq,hk,d", [(2, 2, 2, 64), (8, 4, 2, 128), (64, 3, 1, 64), (256, 2, 1, 128)])
+def test_gradients_of_few_keys_that_cancel(n, hq, hk, d, dtype):
+    """Equal scores of 2^m keys: weights are exact, so what dq and dk miss comes from dS alone.  Its row adds up to zero, and a vector
+    that all keys share, 32 times as large as what tells them apart, leaves nothing but errors of dS, and of dout . out; so do
+    queries that come in pairs of opposite sign with the same upstream gradient.  dS and its remainder miss u u |dS| (twice: the
+    remainder is rounded, and what the product's fp32 sums cut is no more), and the fp32 sums of dP and delta d 2^-24 of their terms.
+    """
+    u = HALF_STEP[dtype]
+    _, k, v, do = make(2, n, n, hq, hk, d, dtype, 9)
+    shift = torch.randn(2, 1, hk, d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(10)).to(dtype) * 32
+    zero = torch.zeros(2, n, hq, d, device=DEV, dtype=dtype)
+    sign = (1 - 2 * (torch.arange(n, device=DEV) % 2)).to(dtype)[None, :, None, None]
+    pairs = torch.randn(2, 1, hq, d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(11)).to(dtype) * 32 * sign
+    same = do[:, ::2].repeat_interleave(2, 1)
+    for which, q2, k2, do2 in (("dq", zero, k + shift, do), ("dk", pairs, torch.zeros_like(k), same)):
+        want, got = reference(q2, k2, v, do2), run(q2, k2, v, do2)
+        D, V = do2.double(), v.double().repeat_interleave(hq // hk, 2)
+        P = 1.0 / n
+        dP = torch.einsum("bihd,bjhd->bhij", D, V)
+        dS = (P * (dP - dP.mean(-1, keepdim=True))).abs()
+        size = torch.einsum("bihd,bjhd->bhij", D.abs(), V.abs())
+        e = (2 * u * u + 2.0**-19) * dS + P * d * 2.0**-23 * (size + size.mean(-1, keepdim=True)) + (n + 4) * 2.0**-23 * dS
+        if dtype == torch.float16:
+            e = e + 2.0**-28 * dS.amax((-1, -2), keepdim=True)  # the lower end of fp16 under a row's factor
+        scale = 1 / math.sqrt(d)
+        if which == "dq":
+            bound = scale * torch.einsum("bhij,bjhd->bihd", e, k2.double().abs().repeat_interleave(hq // hk, 2))
+        else:
+            bound = scale * torch.einsum("bhij,bihd->bjhd", e, q2.double().abs()).unflatten(2, (hk, hq // hk)).sum(3)
+        bound = bound + u * want[which].abs() + (2.0**-25 if dtype == torch.float16 else 0.0) + 1e-30
+        assert worst(got[which], want[which], bound) <= 1, which
