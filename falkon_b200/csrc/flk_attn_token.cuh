@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
   const int first = split * even + min(split, odd), last = first + even + (split < odd ? 1 : 0);
 
   // rows lane / 4 and lane / 4 + 8 of the tile; row r is query r / grp of head r % grp
-  int end[2], my[2];
-  float slope2[2], pos[2];
+  int end[2], my[2], pos[2];
+  float slope2[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = lane / 4 + 8 * e;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
     end[e] = exists ? lim.row_end(i, a.causal) : 0;
     my[e] = qd != nullptr && exists ? qd[i] : -2;
     slope2[e] = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
-    pos[e] = (float)(lim.at + i);
+    pos[e] = lim.at + i;
   }
   // the queries as A operands: columns 2 (lane % 4) and up of rows lane / 4, lane / 4 + 8
   uint32_t q[DP / 16][4];
@@ -168,13 +168,14 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
         }
     }
     float top[2] = {-INFINITY, -INFINITY};
+    const float d0[2] = {(float)(pos[0] - k0), (float)(pos[1] - k0)};  // exact where it matters, however far the row and the key lie
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = e / 2, key = k0 + 8 * n + e % 2;
         float x = s[n][e] * f2;
-        if constexpr (BIAS) x = fmaf(-slope2[row], fabsf(pos[row] - (float)key), x);
+        if constexpr (BIAS) x = fmaf(-slope2[row], fabsf(d0[row] - (float)(8 * n + e % 2)), x);
         const bool see = key < end[row] && (kd == nullptr || __ldg(kd + key) == my[row]);
         s[n][e] = see ? x : -INFINITY;
         top[row] = fmaxf(top[row], s[n][e]);

@@ -252,3 +252,20 @@ def test_gradients_of_few_keys_that_cancel(n, hq, hk, d, dtype):
             bound = scale * torch.einsum("bhij,bihd->bjhd", e, q2.double().abs()).unflatten(2, (hk, hq // hk)).sum(3)
         bound = bound + u * want[which].abs() + (2.0**-25 if dtype == torch.float16 else 0.0) + 1e-30
         assert worst(got[which], want[which], bound) <= 1, which
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,hq", [(1, 2), (3, 4), (30, 2)])
+def test_distances_behind_the_16_millionth_key(nq, hq, dtype):
+    """fp32 has no odd numbers beyond 2^24: distances are taken between whole numbers.  With a slope of one only the last keys have
+    weight (what lies 300 keys back has less than e^-200 of it), so the call on those alone is the reference."""
+    nk, last = 2**24 + 1001, 400
+    g = torch.Generator(device=DEV).manual_seed(12)
+    k, v = (torch.zeros(1, nk, 1, 8, device=DEV, dtype=dtype) for _ in range(2))
+    for t in (k, v):
+        t[:, -last:] = torch.randn(1, last, 1, 8, device=DEV, generator=g, dtype=dtype)
+    q = torch.randn(1, nq, hq, 8, device=DEV, generator=g, dtype=dtype)
+    slopes = torch.ones(hq, device=DEV)
+    out = attention(q, k, v, causal=True, slopes=slopes)
+    want = reference(q, k[:, -last:], v[:, -last:], causal=True, slopes=slopes)
+    assert worst(out, want["out"], want["e_out"]) <= 1
