@@ -43,7 +43,8 @@ def _pack(q, k, v, out, out_lo, lse, opts) -> bytes:
     scale, softcap, causal, slopes, prefix_lens, kv_lens, q_starts, q_docs, k_docs = opts
     b, nq, hq, d = q.shape
     _, nk, hk, _ = k.shape
-    qd, qs, kd, ks = (0, 0, 0, 0) if k_docs is None else (q_docs.data_ptr(), q_docs.stride(0), k_docs.data_ptr(), k_docs.stride(0))
+    # (tables of no entries have no address, and there is nothing for the labels to tell apart)
+    qd, qs, kd, ks = (0, 0, 0, 0) if k_docs is None or nq == 0 or nk == 0 else (q_docs.data_ptr(), q_docs.stride(0), k_docs.data_ptr(), k_docs.stride(0))
     return _lib._ATTENTION_FORWARD.pack(
         _lib._ROW_TYPES[q.dtype], b, nq, nk, hq, hk, d, causal, 0, scale, softcap, *_t4(q), *_t4(k), *_t4(v), *_t4(out),
         _ptr(out_lo), _ptr(lse), _ptr(slopes), _ptr(prefix_lens), _ptr(kv_lens), _ptr(q_starts), qd, qs, kd, ks)

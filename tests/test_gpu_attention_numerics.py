@@ -269,3 +269,13 @@ def test_distances_behind_the_16_millionth_key(nq, hq, dtype):
     out = attention(q, k, v, causal=True, slopes=slopes)
     want = reference(q, k[:, -last:], v[:, -last:], causal=True, slopes=slopes)
     assert worst(out, want["out"], want["e_out"]) <= 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,nq,nk", [(0, 5, 5), (2, 0, 5), (2, 5, 0), (1, 0, 0)])
+def test_documents_of_nothing(b, nq, nk, dtype):
+    q, k, v, do = make(b, nq, nk, 2, 1, 64, dtype, 13)
+    docs, q_docs = (torch.zeros(b, n, device=DEV, dtype=torch.int32) for n in (nk, nq))
+    got = run(q, k, v, do, causal=True, documents=docs, q_documents=q_docs)
+    assert got["out"].shape == q.shape and bool((got["lse"] == -math.inf).all())
+    assert not any(bool(got[n].any()) for n in ("out", "dq", "dk", "dv"))
