@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) kernel(const Tc
         p[n][e] = ex2_approx(s[n][e] - base);
         l[e / 2] += p[n][e];
       }
-    // rounded to the data's type, as the prompts' kernel does; the error of a weight, half a step, is what the result is rounded by
+    // rounded to the data's type, as the prompts' kernel does: half a step of each weight, as much as the result itself is rounded by
+    // (rms error of bf16 results 2.0e-3 to 2.3e-3 of their size; rounding alone 1.6e-3, and with what rounding takes in a second operand
+    // that, but 32 long caches then take 566 us instead of 533, 24 ragged ones 65 instead of 62)
     const uint32_t w[4] = {pack16<T>(p[0][0], p[0][1]), pack16<T>(p[0][2], p[0][3]), pack16<T>(p[1][0], p[1][1]), pack16<T>(p[1][2], p[1][3])};
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
