@@ -17,6 +17,7 @@
 #include <cuda.h>
 #include <string.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "flk_attn.cuh"
@@ -546,9 +547,12 @@ inline int make_map(CUtensorMap* m, const Tensor4& t, int dtype, int d, int h, i
   return FLK_OK;
 }
 
-// The status word of this translation unit's kernels, which goes back to 0; waits for the stream.
+// The status word of this translation unit's kernels, which goes back to 0; waits for the stream.  One query at a time: the word is
+// taken to a place that the next one would overwrite.
+inline std::mutex g_status_lock;
 static __global__ void take_status_kernel() { g_wait_taken = atomicExch(&g_wait_status, 0); }
 static int read_wait_status(cudaStream_t st, int* out) {
+  const std::lock_guard<std::mutex> alone(g_status_lock);
   take_status_kernel<<<1, 1, 0, st>>>();
   count_launch();
   FLK_CUDA_TRY(cudaGetLastError());

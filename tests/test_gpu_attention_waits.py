@@ -1,4 +1,6 @@
 """Waits inside the tensor-core attention kernels that run out, because their limit is short or what they wait for never comes."""
+import concurrent.futures
+
 import pytest
 import torch
 
@@ -72,3 +74,23 @@ def test_some_time(shape, dtype, wait_limit):
             lost = lost or bool(x.isnan().any())
             assert bool((x.isnan() | (x == y)).all()), ns
         assert gave_up or not lost
+
+
+def test_status_queries_side_by_side(wait_limit):
+    """What gave up is told to one of the queries that are made at the same time."""
+    device = torch.device("cuda", torch.cuda.current_device())
+    *_, forward = call((1, 300, 300, 2, 2, 64), torch.bfloat16)
+    forward()
+    _lib.attention_status(device)
+    for _ in range(20):
+        wait_limit(0)
+        forward()
+        torch.cuda.synchronize()
+        wait_limit(1000000000)
+
+        def query(_):
+            with torch.cuda.stream(torch.cuda.Stream(device)):
+                return _lib.attention_status(device)
+
+        with concurrent.futures.ThreadPoolExecutor(4) as pool:
+            assert sum(pool.map(query, range(4))) == 1
