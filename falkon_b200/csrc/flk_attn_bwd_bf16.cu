@@ -1,5 +1,6 @@
 // Backward attention kernels of bf16 data.
 #include "flk_attn_bwd.cuh"
+#include "flk_attn_status.cuh"
 
 namespace flk {
 namespace attn {

@@ -16,9 +16,9 @@
 // backward pass makes exact weights from, has the sum of the weights as they were.  Sums, maximum and accumulators are fp32.
 // Where blocks are fewer than SMs, the key axis is cut into parts, whose normalised fp32 results a second kernel joins.
 //
-// Measured: 2 x 6000 rows, 16 heads of 128 on 8, causal with a prefix: 320 us, 0.95 PFLOP/s of visible pairs; tensor pipe and MUFU
+// Measured: 2 x 6000 rows, 16 heads of 128 on 8, causal with a prefix: 318 us, 0.95 PFLOP/s of visible pairs; tensor pipe and MUFU
 // 50 % busy each.  A step of two tiles takes 3.9 k cycles, 1.5 k of them waiting for scores, whose place in tensor memory the
-// weights still hold.  8192 rows of documents, capped: 116 us; 4 x 2048 rows, heads of 64, distance bias: 82 us.
+// weights still hold.  8192 rows of documents, capped: 115 us; 4 x 2048 rows, heads of 64, distance bias: 83 us.
 #pragma once
 
 #include "flk_attn_tc.cuh"

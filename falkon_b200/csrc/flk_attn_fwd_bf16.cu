@@ -1,5 +1,6 @@
 // Forward attention kernels of bf16 data.
 #include "flk_attn_fwd.cuh"
+#include "flk_attn_status.cuh"
 
 namespace flk {
 namespace attn {

@@ -9,7 +9,10 @@
 // With heads of up to 64 a block has two groups: one takes the even tiles, one the odd, with accumulators of their own that are
 // joined at the end.  Eight warps on an SM would leave its pipes idle for most of the dependent steps (2 x 1000 rows, 4 heads of
 // 64, not causal, capped scores, 128 blocks: forward 93 -> 77 us, dK and dV 170 -> 147 us, dQ 133 -> 108 us).  Larger heads leave no
-// room for a second set of tiles.
+// room for a second set of tiles.  A training pass of 2 x 1000 rows and 4 heads of 128 takes 614 us, as long as elementary torch
+// operations, whose products are a library's.  dK and dV have a block per 64 keys of a key head, whatever the number of query heads
+// that share it: 1000 rows with 8 heads on one take 1270 us (heads of 64) and 2510 (of 128) on 16 blocks, 0.40 and 0.24 of the speed of
+// those elementary operations.
 #pragma once
 
 #include "flk_attn_fwd.cuh"

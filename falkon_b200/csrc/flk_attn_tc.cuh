@@ -17,7 +17,6 @@
 #include <cuda.h>
 #include <string.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "flk_attn.cuh"
@@ -40,8 +39,8 @@ using tc::tmem_relinquish;
 
 constexpr uint32_t kBlockBytes = kTile * 128;  // 128 rows x 64 columns of 16 bits
 
-// Set by a kernel whose bounded wait gave up (one word per translation unit), and what it was when it was last asked for.
-static __device__ int g_wait_status, g_wait_taken;
+// Set by a kernel whose bounded wait gave up (one word per translation unit).
+static __device__ int g_wait_status;
 
 // Whether the barrier has passed the phase, the same answer for all lanes of a warp.  May suspend the warp for a while.
 __device__ __forceinline__ bool passed(uint32_t bar, uint32_t parity) {
@@ -544,20 +543,6 @@ inline int make_map(CUtensorMap* m, const Tensor4& t, int dtype, int d, int h, i
                         unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FLK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return FLK_OK;
-}
-
-// The status word of this translation unit's kernels, which goes back to 0; waits for the stream.  One query at a time: the word is
-// taken to a place that the next one would overwrite.
-inline std::mutex g_status_lock;
-static __global__ void take_status_kernel() { g_wait_taken = atomicExch(&g_wait_status, 0); }
-static int read_wait_status(cudaStream_t st, int* out) {
-  const std::lock_guard<std::mutex> alone(g_status_lock);
-  take_status_kernel<<<1, 1, 0, st>>>();
-  count_launch();
-  FLK_CUDA_TRY(cudaGetLastError());
-  FLK_CUDA_TRY(cudaMemcpyFromSymbolAsync(out, g_wait_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
-  FLK_CUDA_TRY(cudaStreamSynchronize(st));
   return FLK_OK;
 }
 
