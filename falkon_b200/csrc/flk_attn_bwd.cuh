@@ -17,11 +17,12 @@
 // 2.5 k with 64: the chain product - exponentials - product, 16 warps on one tile; a block's start takes 2 to 5 k, its end 3 k.
 //
 // P and dS are rounded to the data's 16 bits before their second product, as P is in the forward pass (rms error of a bf16 training
-// pass 2.4e-3, of its results rounded once 1.7e-3).  In fp16 they would leave its range: weights are held times 2^12, and the dS of a row (a key in the one kernel, a query in the other) times a power
-// of two of its own, which follows what the row has met so far as a running maximum does: the first terms take it to 2^4, and
-// terms beyond 2^15 take the row's accumulator down with it.  So no row, sequence or head costs another one bits, and
-// terms lost to fp16's lower end are 2^-29 of the row's largest.  The exchange of a row's largest term costs fp16 4 to 7% of both kernels
-// (4 x 2048 rows, 12 heads of 128, causal, forward and backward: 340 us, bf16 319).
+// pass 2.4e-3, of its results rounded once 1.7e-3).  In fp16 they would leave its range: weights are held times 2^12, and the dS of
+// a row (a key in the one kernel, a query in the other) times a power of two of its own, which follows what the row has met so far
+// as a running maximum does: the first terms take it to 2^4, and terms beyond 2^15 take the row's accumulator down with it.  So no
+// row, sequence or head costs another one bits, and terms lost to fp16's lower end are 2^-29 of the row's largest.  The exchange of
+// a row's largest term costs fp16 4 to 7% of both kernels (4 x 2048 rows, 12 heads of 128, causal, forward and backward: 340 us,
+// bf16 319).
 //
 // The dS of a row add up to zero, so where a row has few keys the terms of dQ and dK cancel, and the rounding of dS would be the
 // largest error (up to 1.8 times that of rounding the result, for rows of ten keys).  With up to 256 queries and keys, where a

@@ -9,9 +9,10 @@
 //   !PAIR  one row tile; the groups take the even and the odd key tiles, and end with a partial result each: few
 //          rows over a long key axis (single tokens)
 // Weights are exp2(s - m) with a maximum m that follows the running one only when that has grown by more than 8: weights
-// stay below 2^8 (fp16: 2^15, see kLift), and the accumulator is rescaled a few times in a row's life instead of once per tile.  Weights are rounded to
-// the data's 16 bits before they meet V (a relative error of half a step each, which is what the result itself is rounded by: rms error
-// of bf16 results 2.3e-3 of their size, of results rounded once 1.7e-3; a second product with what is left would be half as much again).
+// stay below 2^8 (fp16: 2^15, see kLift), and the accumulator is rescaled a few times in a row's life instead of once per tile.
+// Weights are rounded to the data's 16 bits before they meet V (a relative error of half a step each, which is what the result
+// itself is rounded by: rms error of bf16 results 2.3e-3 of their size, of results rounded once 1.7e-3; a second product with what
+// is left would be half as much work again).
 // The result is divided by the sum of the rounded weights, so that their common error cancels; the log-sum-exp, which the
 // backward pass makes exact weights from, has the sum of the weights as they were.  Sums, maximum and accumulators are fp32.
 // Where blocks are fewer than SMs, the key axis is cut into parts, whose normalised fp32 results a second kernel joins.
