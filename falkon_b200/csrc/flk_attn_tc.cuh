@@ -237,12 +237,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
 
 // The tanh of capped scores.  Where all of a warp's arguments x = scale s lie in [-1/2, 1/2], and scores of up to half the cap do,
 // an odd polynomial on the FMA pipe takes the place of an exponential and a reciprocal: tanh(x) = x p(x^2) with p of degree 4
-// fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32); up to 1/8 degree 2 does (6e-9).  With both on the MUFU unit, the exponential of the
-// weight included, that unit would set the pace: 3 x 16384 operations of a 128 x 128 tile at 16 per cycle are 3072 cycles against
-// 1024 of the two products.  The scale is multiplied into the coefficients once per call (Tanh), which saves a
-// multiplication per score.  Where one of the warp's arguments is larger, every score is scaled first and takes the polynomial or
-// the MUFU unit by its own size: 1 - 2 / (1 + e^2x) is off by 2e-7 whatever x is, and the cap, which may be as large as it likes,
-// multiplies that.
+// fitted to tanh(x) / x at Chebyshev nodes (relative error 6e-8 in fp32); up to 1/8 degree 2 does (6e-9).  With both on the MUFU
+// unit, the exponential of the weight included, that unit would set the pace: three operations for each score of a tile of
+// 128 x 128, 16 per cycle, are three times the 1024 cycles of the two products.  The scale is multiplied into the coefficients once
+// per call (Tanh), which saves a multiplication per score.  Where one of the warp's arguments is larger, every score is scaled first
+// and takes the polynomial or the MUFU unit by its own size: 1 - 2 / (1 + e^2x) is off by 2e-7 whatever x is, and the cap, which may
+// be as large as it likes, multiplies that.
 __device__ __forceinline__ uint64_t both(float x) { return tc::pack2(x, x); }
 constexpr double kTanh4[5] = {1.0, -0.3333306908607483, 0.133247509598732, -0.05298423767089844, 0.017131345346570015};
 constexpr double kTanh2[3] = {0.999999993627153, -0.33332598923104395, 0.1320774045773301};
